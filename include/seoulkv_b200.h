@@ -356,6 +356,96 @@ int skv_shard_gids(void *handle, const int32_t **gids);
 int skv_attention_noalloc(int32_t n_slots, const uint16_t *q, const uint8_t *const *kv8, const int32_t *ids,
                           int32_t context, int32_t sink, int32_t local, uint16_t *out, void *stream);
 
+/* Stand-alone operators around a decode step -- no counterpart in the
+ * reference, whose K, Q and cache arrive ready made.  They work on the
+ * caller's device buffers, allocate nothing, wait for nothing and are ordered
+ * on `stream` (they may be captured into a CUDA graph).  The descriptor is
+ * read during the call.  `device` is the ordinal that holds every buffer; the
+ * calling thread's current device is left as it was.  Strides are counted in
+ * elements (skv_evict: K and V in bytes); the innermost dimension is
+ * contiguous. */
+#define SKV_DTYPE_BF16 0
+#define SKV_DTYPE_FP16 1
+#define SKV_DTYPE_FP32 2
+#define SKV_DTYPE_E4M3 3
+
+/* Rotary positions: q [batch][n][heads][dim] and k [batch][kv_heads][n][dim]
+ * (kv_heads 0: no k) to q_out, k_out, which may be the inputs themselves.
+ * Pair i < rotary_dim / 2 of a head turns by position * phase[i] / 2^64
+ * turns and is multiplied by `factor`; the dimensions from rotary_dim on are
+ * copied.  Pair i is (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1).
+ * Negative positions turn back. */
+#define SKV_ROTARY_HALF 0
+#define SKV_ROTARY_INTERLEAVED 1
+#define SKV_ROTARY_MAX_PAIRS 256
+typedef struct SkvRotary {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void *positions;        /* int32, or int64 with pos64 != 0          */
+  const uint64_t *phase;        /* host memory, [rotary_dim / 2]            */
+  double factor;
+  int64_t device, dtype, layout, pos64;
+  int64_t batch, n, heads, kv_heads, dim, rotary_dim;
+  int64_t q_stride[3];          /* batch, token, head                       */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  int64_t pos_stride[2];        /* batch, token                             */
+} SkvRotary;
+int skv_rotary(const SkvRotary *desc, void *stream);
+
+/* Eviction: of every (sequence, KV head) the `sink` first and `local` last of
+ * lengths[b] tokens (clamped to [0, tokens]) and the best others by weight
+ * (ties: the lowest index; NaN below every number) stay, `keep` in all, and
+ * move to the front in their order.  Outputs are contiguous: k_out, v_out
+ * [batch][kv_heads][keep] rows of row_bytes, weights_out FP32 and ids int32
+ * [batch][kv_heads][keep], lengths_out int32 [batch]; past the kept tokens
+ * rows and weights are zero and ids -1.  No output may overlap an input. */
+typedef struct SkvEvict {
+  const void *k, *v, *weights, *lengths;
+  void *k_out, *v_out, *weights_out, *ids, *lengths_out;
+  int64_t device, batch, kv_heads, tokens, row_bytes, keep, sink, local;
+  int64_t k_stride[3];          /* bytes: sequence, head, token             */
+  int64_t v_stride[3];
+  int64_t weights_stride[3];    /* elements                                 */
+} SkvEvict;
+int skv_evict(const SkvEvict *desc, void *stream);
+
+/* Attention of n drafted tokens (nodes of a tree) of each sequence over its
+ * cache and over their own ancestors.  Node i of sequence b sees the first
+ * lengths[b] (clamped to [0, tokens]) cache rows, itself and its ancestors;
+ * parents[b][i] is the node before it (< i), -1 if it follows the cache, and
+ * anything else marks an unused node.  An unused node, and a node below one,
+ * gets zeros and an lse of -inf, and its K and V are not read into any row.
+ *   q BF16 [batch][n][heads][dim], k, v BF16 [batch][kv_heads][n][dim],
+ *   k_cache, v_cache BF16 or FP8 e4m3 [batch][kv_heads][tokens][dim],
+ *   out BF16 [batch][n][heads][dim] and lse FP32 [batch][n][heads] contiguous;
+ *   workspace: skv_tree_workspace() bytes, not shared by calls that overlap.
+ * dim is 64, 128 or 256, n at most SKV_TREE_MAX_NODES.  Rows start on 16-byte
+ * boundaries.  Sequence and head strides may be 0 (a cache that all share). */
+#define SKV_TREE_MAX_NODES 64
+typedef struct SkvTree {
+  const void *q, *k_cache, *v_cache, *lengths, *k, *v, *parents;
+  void *out, *lse, *workspace;
+  double scale;
+  int64_t device, cache_dtype, workspace_bytes;
+  int64_t batch, n, heads, kv_heads, dim, tokens;
+  int64_t q_stride[3];          /* sequence, node, head                     */
+  int64_t k_cache_stride[3];    /* sequence, head, token                    */
+  int64_t v_cache_stride[3];
+  int64_t k_stride[3];          /* sequence, head, node                     */
+  int64_t v_stride[3];
+  int64_t parents_stride[2];    /* sequence, node                           */
+  int64_t lengths_stride;
+} SkvTree;
+int skv_tree_attention(const SkvTree *desc, void *stream);
+int skv_tree_workspace(const SkvTree *desc, int64_t *bytes);
+
+/* Waits for the device and reads its operators' status word: bits
+ * SKV_STATUS_* of bounded device waits that gave up since the library was
+ * loaded (the results of such a call are NaN). */
+int skv_operator_status(int32_t device, uint32_t *flags);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,7 @@ EXPORTS = (
     "skv_shard_outputs", "skv_shard_merge", "skv_shard_attention", "skv_shard_combine",
     "skv_shard_setup", "skv_shard_connect", "skv_shard_ipc_handle_bytes", "skv_shard_gids",
     "skv_append", "skv_context", "skv_set_l2_residency",
+    "skv_rotary", "skv_tree_attention", "skv_tree_workspace", "skv_evict", "skv_operator_status",
 )
 
 SKV_FLAG_STAGED = 1
@@ -80,6 +81,8 @@ def library_path() -> Path:
 def load() -> ctypes.CDLL:
     """Load (building first if stale and nvcc exists) the CUDA library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -145,6 +148,11 @@ def load() -> ctypes.CDLL:
                                    ctypes.c_int32, ctypes.c_void_p]
         lib.skv_context.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32)]
         lib.skv_set_l2_residency.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]
+        # the stand-alone operators take their descriptors as packed bytes
+        for name in ("skv_rotary", "skv_tree_attention", "skv_evict"):
+            getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        lib.skv_tree_workspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
+        lib.skv_operator_status.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint32)]
         _lib = lib
         return lib
 

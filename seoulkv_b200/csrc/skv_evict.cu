@@ -1,0 +1,312 @@
+// skv_evict.cu -- eviction from a cache by accumulated attention weight.
+//
+// Per (sequence, KV head) with n valid tokens and a budget of `keep`: the
+// first `sink` and the last `local` tokens stay, and of the rest the
+// keep - sink - local of largest weight (equal weights: the lowest index; NaN
+// below every number).  n <= keep keeps everything.  The kept tokens' K, V
+// and weights move to the front in their order; rows past them are zero,
+// their ids -1.
+//
+// Two launches.  k_evict_select, one cluster per (sequence, head): the weights
+// are mapped to integers of the same order, and three histogram passes (11,
+// 11, 10 bits) find the value of the last kept one; the ranks of the tokens
+// above it and of the ties in index order give every kept token its place, so
+// ids come out sorted and the result does not depend on the order of any
+// atomic (they only count).  k_evict_gather then moves the rows at copy
+// bandwidth: every byte is read once and written once.
+#include <cooperative_groups.h>
+
+#include "skv_ops.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace skv {
+namespace {
+
+constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
+constexpr int EV_BINS = 2048;
+// copies of the histogram, one per lane modulo 8: weights share exponents, so
+// a warp's counts fall on few bins and one copy would serialise them
+constexpr int EV_COPIES = 8;
+constexpr int EV_CACHED = 24576;  // keys a CTA holds in shared memory (96 KB); longer segments are read again
+constexpr int EV_CLUSTER = 8;
+constexpr int EV_SMALL = 4096;    // tokens up to which one CTA does a row by itself
+
+struct EvictArgs {
+  const float *weights;
+  int64_t ws[3];  // element strides (sequence, head, token)
+  const int32_t *lengths;
+  int32_t *ids, *out_lengths;
+  float *out_w;
+  int heads, t, keep, sink, local;
+};
+
+struct SelectSmem {
+  uint32_t hist[EV_COPIES][EV_BINS];
+  uint32_t sum[2][EV_BINS];
+  uint32_t scan[EV_WARPS];
+  uint32_t tie[EV_WARPS];
+  uint32_t found[2];   // bin, still wanted inside it
+  uint32_t total[2];   // this CTA's kept-above and tied counts
+  uint32_t key[EV_CACHED];
+};
+
+// Larger weight, larger key; -0 equals +0, NaN is 0 (below -inf).
+__device__ __forceinline__ uint32_t order_key(float w) {
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+__global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  SelectSmem &s = *reinterpret_cast<SelectSmem *>(smem_raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+  const int row = blockIdx.x / ranks;
+  const int b = row / a.heads, h = row - b * a.heads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_release();
+  const int n = max(0, min(a.lengths[b], a.t));
+  const int m = min(n, a.keep);
+  const float *w = a.weights + b * a.ws[0] + h * a.ws[1];
+  int32_t *ids = a.ids + (int64_t)row * a.keep;
+  float *out_w = a.out_w + (int64_t)row * a.keep;
+  if (h == 0 && rank == 0 && tid == 0) a.out_lengths[b] = m;
+  for (int j = m + rank * EV_THREADS + tid; j < a.keep; j += ranks * EV_THREADS) {
+    ids[j] = -1;
+    out_w[j] = 0.0f;
+  }
+  // a warp owns consecutive tokens, so that ballots give places in index order
+  const int warps = ranks * EV_WARPS;
+  const int seg = ((n + warps - 1) / warps + 31) & ~31;
+  const int begin = min(n, (rank * EV_WARPS + warp) * seg), end = min(n, begin + seg);
+  const bool cached = seg * EV_WARPS <= EV_CACHED;
+  uint32_t *mine = s.key + (cached ? warp * seg : 0);
+  const int lo = n <= a.keep ? n : a.sink, hi = n - a.local;  // the middle that competes: [lo, hi)
+  auto key_at = [&](int i) { return cached ? mine[i - begin] : order_key(w[i * a.ws[2]]); };
+  if (cached)
+    for (int i = begin + lane; i < end; i += 32) mine[i - begin] = order_key(w[i * a.ws[2]]);
+  uint32_t want = n <= a.keep ? 0u : (uint32_t)(a.keep - a.sink - a.local);
+  uint32_t edge = 0xffffffffu;  // key of the last kept token: kept above it, ties in index order
+  uint32_t ties = 0;
+  if (want) {
+    uint32_t prefix = 0;
+    int pass = 0;
+    for (int shift : {21, 10, 0}) {
+      const int bits = shift ? 11 : 10;
+      for (int i = tid; i < EV_COPIES * EV_BINS; i += EV_THREADS) (&s.hist[0][0])[i] = 0;
+      __syncthreads();
+      for (int i = begin + lane; i < end; i += 32) {
+        if (i < lo || i >= hi) continue;
+        const uint32_t k = key_at(i);
+        if (pass && (k >> (shift + bits)) != prefix) continue;
+        atomicAdd(&s.hist[lane % EV_COPIES][(k >> shift) & ((1u << bits) - 1)], 1u);
+      }
+      __syncthreads();
+      uint32_t *sum = s.sum[pass & 1];
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int c = 0; c < EV_COPIES; ++c) x += s.hist[c][i];
+        sum[i] = x;
+      }
+      cluster.sync();  // (also keeps the other buffer's remote readers of the pass before apart from its next writes)
+      // thread t: the two bins 2047 - 2t, 2046 - 2t, so that a prefix sum runs from the largest keys down
+      const int top = EV_BINS - 1 - 2 * tid;
+      uint32_t c0 = 0, c1 = 0;
+      for (int r = 0; r < ranks; ++r) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(sum, r) + top - 1);
+        c0 += v.y;
+        c1 += v.x;
+      }
+      const uint32_t inc = warp_inclusive(c0 + c1, lane);
+      if (lane == 31) s.scan[warp] = inc;
+      __syncthreads();
+      if (warp == 0) s.scan[lane] = warp_inclusive(s.scan[lane], lane);
+      __syncthreads();
+      const uint32_t upto = inc + (warp ? s.scan[warp - 1] : 0u), before = upto - c0 - c1;
+      if (before < want && want <= upto) {
+        const bool second = before + c0 < want;
+        s.found[0] = (uint32_t)(top - (second ? 1 : 0));
+        s.found[1] = want - before - (second ? c0 : 0u);
+      }
+      __syncthreads();
+      prefix = (prefix << bits) | s.found[0];
+      want = s.found[1];
+      ++pass;
+    }
+    edge = prefix;
+    ties = want;
+  }
+  // places: tokens kept for certain and tied ones, counted per warp, CTA and cluster
+  auto kinds = [&](int i, bool &above, bool &tied) {
+    above = tied = false;
+    if (i >= end) return;
+    if (i < lo || i >= hi) {
+      above = true;
+    } else {
+      const uint32_t k = key_at(i);
+      above = k > edge;
+      tied = ties && k == edge;
+    }
+  };
+  uint32_t n_above = 0, n_tied = 0;
+  __syncwarp();
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    bool above, tied;
+    kinds(i0 + lane, above, tied);
+    n_above += __popc(__ballot_sync(0xffffffffu, above));
+    n_tied += __popc(__ballot_sync(0xffffffffu, tied));
+  }
+  if (lane == 0) s.scan[warp] = n_above, s.tie[warp] = n_tied;
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t x = warp_inclusive(s.scan[lane], lane), y = warp_inclusive(s.tie[lane], lane);
+    s.scan[lane] = x;
+    s.tie[lane] = y;
+    if (lane == 31) s.total[0] = x, s.total[1] = y;
+  }
+  __syncthreads();
+  if (ranks > 1) cluster.sync();
+  uint32_t at = warp ? s.scan[warp - 1] : 0u, tie = warp ? s.tie[warp - 1] : 0u;
+  for (int r = 0; r < rank; ++r) {
+    const uint32_t *o = cluster.map_shared_rank(s.total, r);
+    at += o[0];
+    tie += o[1];
+  }
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    bool above, tied;
+    const int i = i0 + lane;
+    kinds(i, above, tied);
+    const uint32_t ba = __ballot_sync(0xffffffffu, above), bt = __ballot_sync(0xffffffffu, tied);
+    const uint32_t tie_before = tie + __popc(bt & below);
+    if (above || (tied && tie_before < ties)) {
+      const uint32_t place = at + __popc(ba & below) + min(tie_before, ties);
+      ids[place] = i;
+      out_w[place] = w[i * a.ws[2]];
+    }
+    at += __popc(ba);
+    tie += __popc(bt);
+  }
+  if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its counts
+}
+
+constexpr int EG_THREADS = 256, EG_ROWS = 4;  // rows whose K and V loads one thread has in flight
+
+struct GatherArgs {
+  const uint8_t *x[2];
+  uint8_t *y[2];
+  int64_t xs[2][3];  // byte strides (sequence, head, token)
+  const int32_t *ids;
+  int64_t rows;
+  int heads, keep, row_bytes;
+};
+
+template <typename C>
+__global__ void __launch_bounds__(EG_THREADS) k_evict_gather(GatherArgs a) {
+  const int per_row = a.row_bytes / (int)sizeof(C);
+  const int lanes = min(per_row, EG_THREADS), group = EG_THREADS / lanes;
+  const int mine = threadIdx.x / lanes;
+  if (mine >= group) return;  // (no barrier below)
+  grid_dependency_wait();
+  const int64_t row0 = (int64_t)blockIdx.x * group * EG_ROWS + mine;
+  for (int c = threadIdx.x - mine * lanes; c < per_row; c += lanes) {
+    C v[EG_ROWS][2];
+    int32_t id[EG_ROWS];
+#pragma unroll
+    for (int u = 0; u < EG_ROWS; ++u) {
+      const int64_t r = row0 + u * group;
+      id[u] = r < a.rows ? a.ids[r] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < EG_ROWS; ++u) {
+      v[u][0] = v[u][1] = C{};
+      if (id[u] < 0) continue;
+      const int64_t bh = (row0 + u * group) / a.keep;
+      const int b = (int)(bh / a.heads), h = (int)(bh - (int64_t)b * a.heads);
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        v[u][w] = __ldcs(reinterpret_cast<const C *>(a.x[w] + b * a.xs[w][0] + h * a.xs[w][1] + id[u] * a.xs[w][2]) + c);
+    }
+#pragma unroll
+    for (int u = 0; u < EG_ROWS; ++u) {
+      const int64_t r = row0 + u * group;
+      if (r >= a.rows) break;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) __stcs(reinterpret_cast<C *>(a.y[w] + r * a.row_bytes) + c, v[u][w]);
+    }
+  }
+}
+
+template <typename C>
+cudaError_t launch_gather(const GatherArgs &g, cudaStream_t st) {
+  const int per_row = g.row_bytes / (int)sizeof(C);
+  const int group = EG_THREADS / (per_row < EG_THREADS ? per_row : EG_THREADS);
+  const int64_t blocks = (g.rows + group * EG_ROWS - 1) / (group * EG_ROWS);
+  return op_launch(k_evict_gather<C>, dim3((unsigned)blocks), dim3(EG_THREADS), 0, st, true, 1, g);
+}
+
+}  // namespace
+}  // namespace skv
+
+extern "C" int skv_evict(const SkvEvict *d, void *stream) {
+  using namespace skv;
+  if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
+  if (d->batch < 0 || d->kv_heads < 1 || d->tokens < 1 || d->tokens > INT32_MAX / 2 || d->row_bytes < 1 ||
+      d->row_bytes > 65536 || d->batch * d->kv_heads > (1 << 24))
+    return op_fail(SKV_E_INVALID, "batch, heads, tokens or row_bytes out of range");
+  if (d->keep < 1 || d->keep > d->tokens || d->sink < 0 || d->local < 0 || d->sink + d->local > d->keep)
+    return op_fail(SKV_E_INVALID, "keep must be in [1, tokens] and hold the sink and local tokens");
+  const int64_t rows = d->batch * d->kv_heads * d->keep;
+  if (rows > (int64_t)INT32_MAX * 8) return op_fail(SKV_E_INVALID, "too many kept rows");
+  if (d->batch == 0) return SKV_OK;
+  if (!d->k || !d->v || !d->weights || !d->lengths || !d->k_out || !d->v_out || !d->weights_out || !d->ids || !d->lengths_out)
+    return op_fail(SKV_E_INVALID, "null input or output pointer");
+  DeviceScope scope((int)d->device);
+  if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  EvictArgs a;
+  a.weights = static_cast<const float *>(d->weights);
+  for (int i = 0; i < 3; ++i) a.ws[i] = d->weights_stride[i];
+  a.lengths = static_cast<const int32_t *>(d->lengths);
+  a.ids = static_cast<int32_t *>(d->ids);
+  a.out_lengths = static_cast<int32_t *>(d->lengths_out);
+  a.out_w = static_cast<float *>(d->weights_out);
+  a.heads = (int)d->kv_heads, a.t = (int)d->tokens, a.keep = (int)d->keep;
+  a.sink = (int)d->sink, a.local = (int)d->local;
+  int rc = op_cuda(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)sizeof(SelectSmem)), "k_evict_select shared memory");
+  if (rc) return rc;
+  const int ranks = d->tokens <= EV_SMALL ? 1 : EV_CLUSTER;
+  rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
+                         sizeof(SelectSmem), st, false, (unsigned)ranks, a), "k_evict_select launch");
+  if (rc) return rc;
+  GatherArgs g;
+  g.x[0] = static_cast<const uint8_t *>(d->k), g.x[1] = static_cast<const uint8_t *>(d->v);
+  g.y[0] = static_cast<uint8_t *>(d->k_out), g.y[1] = static_cast<uint8_t *>(d->v_out);
+  uintptr_t all = (uintptr_t)g.x[0] | (uintptr_t)g.x[1] | (uintptr_t)g.y[0] | (uintptr_t)g.y[1] | (uintptr_t)d->row_bytes;
+  for (int i = 0; i < 3; ++i) {
+    g.xs[0][i] = d->k_stride[i], g.xs[1][i] = d->v_stride[i];
+    all |= (uintptr_t)g.xs[0][i] | (uintptr_t)g.xs[1][i];
+  }
+  g.ids = a.ids;
+  g.rows = rows;
+  g.heads = a.heads, g.keep = a.keep, g.row_bytes = (int)d->row_bytes;
+  // the widest access that every row start allows
+  cudaError_t e = all % 16 == 0  ? launch_gather<uint4>(g, st)
+                  : all % 4 == 0 ? launch_gather<uint32_t>(g, st)
+                  : all % 2 == 0 ? launch_gather<uint16_t>(g, st)
+                                 : launch_gather<uint8_t>(g, st);
+  return op_cuda(e, "k_evict_gather launch");
+}

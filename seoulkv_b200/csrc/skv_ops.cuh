@@ -1,0 +1,93 @@
+// skv_ops.cuh -- host side shared by the stand-alone operators (rotary, tree
+// attention, accumulated weights, eviction): errors, the current device and
+// kernel launches that may start before the kernel ahead of them has ended.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <string>
+
+#include "../../include/seoulkv_b200.h"
+
+namespace skv {
+
+void set_last_error(const std::string &msg);
+
+// Sets skv_last_error() and returns `code`; nothing is thrown through the C
+// entries (a message that cannot be stored is dropped).
+inline int op_fail(int code, const char *fmt, ...) noexcept {
+  char buf[320];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  try {
+    set_last_error(buf);
+  } catch (...) {
+  }
+  return code;
+}
+
+inline int op_cuda(cudaError_t e, const char *what) noexcept {
+  return e == cudaSuccess ? SKV_OK : op_fail(SKV_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// Makes `device` current for one call and restores the caller's afterwards.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) noexcept {
+    err_ = cudaGetDevice(&old_);
+    if (err_ == cudaSuccess && device != old_) {
+      err_ = cudaSetDevice(device);
+      changed_ = err_ == cudaSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (changed_) cudaSetDevice(old_);
+  }
+  DeviceScope(const DeviceScope &) = delete;
+  DeviceScope &operator=(const DeviceScope &) = delete;
+  cudaError_t error() const { return err_; }
+
+ private:
+  int old_ = 0;
+  bool changed_ = false;
+  cudaError_t err_;
+};
+
+// Launch; with `early` the kernel's blocks may be placed while the kernel
+// before it on the stream still runs (it calls grid_dependency_wait() before
+// it reads what that kernel wrote), which hides its launch.
+template <typename... P, typename... A>
+inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool early,
+                             unsigned cluster, A &&...args) noexcept {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_release() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+}  // namespace skv

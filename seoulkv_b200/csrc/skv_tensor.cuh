@@ -1,0 +1,206 @@
+// skv_tensor.cuh -- the Blackwell tensor core, tensor memory, TMA and mbarrier
+// instructions that the attention operators use, and waits that end.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/seoulkv_b200.h"
+
+namespace skv {
+
+__device__ __forceinline__ uint32_t s_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- mbarriers -----------------------------------------------------------
+
+// A wait that lasts WAIT_NS gives up: it raises `abort` for its CTA (every
+// later wait then gives up at once, so that all roles run to their end
+// without waiting) and a bit in the device's status word, which the host reads.
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+constexpr int WAIT_FREE_POLLS = 256;
+
+__device__ __forceinline__ unsigned long long timer_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(s_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool bar_wait_long(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status) {
+  const unsigned long long t0 = timer_ns();
+  do {
+    for (int i = 0; i < WAIT_FREE_POLLS; ++i)
+      if (bar_try(bar, parity)) return true;
+    if (*abort) return false;
+  } while (timer_ns() - t0 < WAIT_NS);
+  *abort = 1;
+  atomicOr(status, SKV_STATUS_TIMEOUT);
+  return false;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status) {
+  if (bar_try(bar, parity)) return true;
+  return bar_wait_long(bar, parity, abort, status);
+}
+
+// Writes to shared memory by threads, before the tensor core or TMA reads them.
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- TMA (own memory, no multicast) ---------------------------------------
+
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// Box at (x elements, row, y, z) of a 4-d map; x is a multiple of 64 elements here.
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int row, int y, int z,
+                                         uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(s_addr(dst)),
+      "l"(map), "r"(x), "r"(row), "r"(y), "r"(z), "r"(s_addr(bar))
+      : "memory");
+}
+
+// ---- tensor memory and tcgen05.mma ----------------------------------------
+
+__device__ __forceinline__ void tmem_alloc(uint32_t *where, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(where)), "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Arrives on `bar` when every MMA issued so far by this thread has ended.
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(bar))
+               : "memory");
+}
+
+// Instruction descriptor: FP32 accumulator, BF16 operands, A K-major, B
+// K-major or (b_rows) stored with its N index contiguous.
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_rows) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+// Shared-memory operand in 128-byte-swizzled rows (8-row groups of 1024
+// bytes); `lead` is the stride between 64-element pieces of an operand whose
+// M or N index is contiguous (unused otherwise).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// D (tensor memory) = A (tensor memory) B (shared memory) [+ D], K = 16.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+// D (tensor memory) = A (shared memory) B (shared memory) [+ D], K = 16.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+
+#define SKV_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), \
+                     "=r"(v[i + 6]), "=r"(v[i + 7])
+#define SKV_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), \
+                     "r"(v[i + 6]), "r"(v[i + 7])
+// 32 / 16 consecutive columns of this thread's lane (warp w of four: lanes 32w..32w+31).
+__device__ __forceinline__ void tmem_ld32(uint32_t (&v)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : SKV_R8(v, 0), SKV_R8(v, 8), SKV_R8(v, 16), SKV_R8(v, 24)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&v)[16], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : SKV_R8(v, 0), SKV_R8(v, 8)
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::SKV_W8(v, 0),
+      SKV_W8(v, 8), SKV_W8(v, 16), SKV_W8(v, 24), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::SKV_W8(
+          v, 0),
+      SKV_W8(v, 8), "r"(at)
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// Two FP8 e4m3 codes to two BF16 (exact).
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+  float lo, hi;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(h));
+  return pack_bf16(lo, hi);
+}
+
+// ---- cp.async --------------------------------------------------------------
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---- host: tensor maps and the status word (skv_tree.cu) -------------------
+
+// 4-d map [z][y][rows][dim] of 16-bit elements with element strides
+// {row, y, z}; boxes of box_rows rows x 64 elements, 128-byte swizzle.  A
+// dimension of one element, or of stride 0, is mapped with one element.
+int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
+             const int64_t *stride, int box_rows);
+// The device's status word (set by waits that gave up).
+int status_word(int device, uint32_t **word);
+
+}  // namespace skv

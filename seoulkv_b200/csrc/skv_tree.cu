@@ -1,0 +1,968 @@
+// skv_tree.cu -- exact attention of a tree of drafted tokens over a cache.
+//
+// N <= 64 drafted tokens (nodes) of one sequence see its cache and their own
+// ancestors.  With G query heads per KV head, one KV head has R = N * G rows
+// (row r: node r / G, query head r % G) over one stream of keys: the cache's
+// tiles, then one tile of the N nodes' own keys under the ancestor mask.
+//   s = scale q.k,  out = sum exp(s - m) v / sum exp(s - m),  lse = m + log sum exp(s - m)
+// in one pass with a running maximum; the row statistics and the accumulator
+// are FP32 (the accumulator in tensor memory).
+//
+// Both products run on tcgen05 with the rows as M = 128 lanes: S = Q K^T with
+// Q in tensor memory (loaded once per unit; from shared memory it would be
+// read again for every tile, at 192 bytes a cycle of the 128 there are) and
+// O += P V with P = exp(s - m) written back over S as BF16, rounded once (half
+// a step, 2^-9 of each weight, as the BF16 values it multiplies; the row sum
+// is taken before rounding).  K and V tiles arrive by TMA in a ring that keeps
+// 100 KB and more in flight per SM, which is what carries the HBM bandwidth.
+//
+// The tiles of all units (sequence, KV head, 128 rows) form one list that is
+// cut into equal contiguous ranges, one per CTA (one CTA per SM): ragged
+// lengths balance by themselves.  A unit that one CTA covers is written at
+// once; of a unit cut across CTAs every CTA writes its partial (m, l, O) and
+// k_tree_combine joins them in order, so that results do not depend on timing.
+// The cut is worked out on the device from the lengths: no host wait, and a
+// captured graph follows its caches as they grow.
+#include <cuda_bf16.h>
+
+#include <mutex>
+
+#include "skv_device.cuh"
+#include "skv_ops.cuh"
+#include "skv_tensor.cuh"
+
+namespace skv {
+
+__device__ uint32_t g_op_status;
+
+int status_word(int device, uint32_t **word) {
+  static std::mutex lock;
+  static uint32_t *known[64] = {};
+  if (device < 0 || device >= 64) return op_fail(SKV_E_INVALID, "device ordinal out of range");
+  std::lock_guard<std::mutex> hold(lock);
+  if (!known[device]) {
+    void *p = nullptr;
+    if (int rc = op_cuda(cudaGetSymbolAddress(&p, g_op_status), "cudaGetSymbolAddress(status)")) return rc;
+    known[device] = static_cast<uint32_t *>(p);
+  }
+  *word = known[device];
+  return SKV_OK;
+}
+
+int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
+             const int64_t *stride, int box_rows) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode) return op_fail(SKV_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const int64_t n[3] = {rows, ny, nz};
+  cuuint64_t size[4] = {(cuuint64_t)dim, 1, 1, 1}, step[3];
+  for (int i = 0; i < 3; ++i) {
+    const bool one = n[i] == 1 || stride[i] == 0;
+    size[i + 1] = one ? 1 : (cuuint64_t)n[i];
+    step[i] = one ? (cuuint64_t)dim * 2 : (cuuint64_t)stride[i] * 2;
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, unit[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), size, step, box, unit,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SKV_OK : op_fail(SKV_E_INVALID, "cuTensorMapEncodeTiled: error %d", (int)r);
+}
+
+namespace {
+
+constexpr int TR_NODES = SKV_TREE_MAX_NODES;
+constexpr int TR_BATCH = 512;  // sequences of one launch (their tile counts are kept in shared memory)
+constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
+
+template <int D_, bool F8_>
+struct TreeCfg {
+  static constexpr int D = D_;
+  static constexpr bool F8 = F8_;
+  static constexpr int KT = D == 256 ? 64 : 128;  // keys of a tile: 32 KB of BF16 (16 KB at D = 64)
+  static constexpr int SUB = D / 64;              // 128-byte pieces of a row
+  static constexpr int STAGE = KT * D * 2;
+  static constexpr int RAW = KT * D;              // an FP8 tile before its conversion
+  static constexpr int NRAW = F8 ? 5 : 0;
+  static constexpr int NSTAGE = F8 ? 4 : D == 64 ? 12 : 6;
+  static constexpr int THREADS = F8 ? 512 : 256;
+  // tensor memory columns: O, Q (BF16 pairs), two score tiles (P over S)
+  static constexpr int COL_Q = D, COL_S = D + D / 2;
+  static constexpr int RING = NSTAGE * STAGE + NRAW * RAW;
+  static_assert(COL_S + 2 * KT <= 512, "tensor memory");
+};
+
+struct TreeMaps {
+  CUtensorMap k, v, kn, vn;  // cache and nodes
+};
+
+struct TreeArgs {
+  const uint16_t *q;
+  int64_t qs[3];  // element strides (sequence, node, head)
+  const uint8_t *k8, *v8;
+  int64_t k8s[3], v8s[3];  // FP8 caches: byte strides (sequence, head, token)
+  const CellDev *cells;    // the engine's FP8 records instead (cell = sequence * heads + head)
+  const uint16_t *kn, *vn;
+  int64_t kns[3], vns[3];  // element strides (sequence, head, node)
+  const int32_t *lengths;
+  int64_t len_stride;
+  int32_t context;         // length of every sequence without `lengths`
+  const int32_t *parents;
+  int64_t ps[2];           // element strides (sequence, node)
+  uint16_t *out;           // [sequence][node][query head][D]
+  float *lse;              // [sequence][node][query head]
+  float2 *ml;              // partials: [slot][rows] (m in log2 units, l; l < 0: the row is unused)
+  float *part;             // [slot][rows][D]
+  int32_t batch, n, heads, group, t, mtiles, rows;
+  int32_t along[4][2];     // coordinate steps (head, sequence) of the four maps: 0 where one element stands for all
+  float c2;                // scale * log2(e)
+  uint32_t *status;
+};
+
+template <class C>
+struct TreeSmem {
+  uint64_t full[C::NSTAGE], empty[C::NSTAGE];
+  uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;  // (by tile parity: S(g) follows O(g - 2), so a wait is at most one phase behind)
+  uint64_t anc[TR_NODES];   // nodes that node i sees (0: unused)
+  unsigned long long bad;   // nodes with a value that is not finite
+  int32_t up[TR_NODES];
+  uint32_t tmem;
+  uint32_t abort;
+  int32_t len[TR_BATCH];
+  int32_t pre[TR_BATCH + 1];  // tiles of the sequences before (one unit's worth)
+};
+
+// ---- the list of tiles and a CTA's range of it ------------------------------
+
+struct Plan {
+  long long total;  // tiles of all units
+  int ctas;         // CTAs that have a range
+  __host__ __device__ long long begin(int c) const { return total * c / ctas; }
+  // the CTA whose range holds tile g
+  __host__ __device__ int owner(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
+};
+
+// pre[b] and len[b] by one warp.
+template <int KT>
+__device__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch, int32_t *len,
+                            int32_t *pre) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int b = b0 + lane;
+    int n = 0, tiles = 0;
+    if (b < batch) {
+      n = lengths ? lengths[b * stride] : context;
+      n = max(0, min(n, t));
+      tiles = (n + KT - 1) / KT + 1;
+    }
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (b < batch) {
+      if (len) len[b] = n;
+      pre[b + 1] = base + x;
+    }
+    base += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) pre[0] = 0;
+}
+
+// The segments of [g, end): tiles [tile, tile + count) of one unit.
+struct Walk {
+  long long g, end;
+  const int32_t *pre;
+  int units;  // per sequence
+  int b = 0, unit = 0, tile = 0, count = 0, tiles = 0;
+  __device__ Walk(const int32_t *pre_, int batch, int units_, long long g_, long long end_)
+      : g(g_), end(end_), pre(pre_), units(units_) {
+    int lo = 0, hi = batch - 1;  // the last sequence that starts at or before g
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)pre[mid] * units <= g) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+  }
+  __device__ bool next() {
+    if (g >= end) return false;
+    while ((long long)pre[b + 1] * units <= g) ++b;
+    tiles = pre[b + 1] - pre[b];
+    const long long rel = g - (long long)pre[b] * units;
+    unit = (int)(rel / tiles);
+    tile = (int)(rel - (long long)unit * tiles);
+    count = (int)min((long long)(tiles - tile), end - g);
+    g += count;
+    return true;
+  }
+};
+
+// Order of a segment's 2n operand tiles in the ring: K0, K1, V0, K2, V1, ...,
+// V(n-1), the order in which the MMA thread needs them.
+__device__ __forceinline__ int pos_k(int i) { return i ? 2 * i - 1 : 0; }
+__device__ __forceinline__ int pos_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
+__device__ __forceinline__ void item_at(int p, int n, bool &is_v, int &i) {
+  is_v = p == 2 * n - 1 || (p > 0 && !(p & 1));
+  i = p == 0 ? 0 : p == 2 * n - 1 ? n - 1 : is_v ? (p - 2) / 2 : (p + 1) / 2;
+}
+
+__device__ __forceinline__ bool not_finite_bf16(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
+
+// ---- the attention kernel ----------------------------------------------------
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1)
+    k_tree_attention(const __grid_constant__ TreeMaps maps, const __grid_constant__ TreeArgs a) {
+  constexpr int D = C::D, KT = C::KT;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t *ring = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;
+  uint8_t *raw = ring + C::NSTAGE * C::STAGE;
+  TreeSmem<C> &s = *reinterpret_cast<TreeSmem<C> *>(ring + C::RING);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int units = a.heads * a.mtiles;
+
+  if (warp == 0) {
+    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, s.len, s.pre);
+    if (lane == 0 && !C::F8) {
+      tma_prefetch_map(&maps.k);
+      tma_prefetch_map(&maps.v);
+      tma_prefetch_map(&maps.kn);
+      tma_prefetch_map(&maps.vn);
+    }
+  } else if (warp == 1) {
+    tmem_alloc(&s.tmem, 512);
+  } else if (warp == 2 && lane == 0) {
+    for (int i = 0; i < C::NSTAGE; ++i) {
+      bar_init(&s.full[i], C::F8 ? 8 : 1);
+      bar_init(&s.empty[i], 1);
+    }
+    bar_init(&s.q_ready, 4);
+    bar_init(&s.drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.s_full[i], 1);
+      bar_init(&s.o_done[i], 1);
+      bar_init(&s.p_ready[i], 4);
+    }
+    bar_init_fence();
+    s.abort = 0;
+    s.bad = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dependency_release();
+  const uint32_t tmem = *(volatile uint32_t *)&s.tmem;
+  volatile uint32_t *abort = &s.abort;
+  const Plan plan{(long long)s.pre[a.batch] * units, (int)min((long long)gridDim.x, (long long)s.pre[a.batch] * units)};
+  const int cta = blockIdx.x;
+  const long long g_begin = cta < plan.ctas ? plan.begin(cta) : 0, g_end = cta < plan.ctas ? plan.begin(cta + 1) : 0;
+  auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
+
+  if (warp == 0 && !C::F8) {
+    // ---- loads
+    if (lane == 0) {
+      Walk w(s.pre, a.batch, units, g_begin, g_end);
+      uint32_t seq = 0;
+      bool ok = true;
+      while (ok && w.next()) {
+        const int h = w.unit / a.mtiles;
+        for (int p = 0; p < 2 * w.count; ++p, ++seq) {
+          bool is_v;
+          int i;
+          item_at(p, w.count, is_v, i);
+          const int stage = seq % C::NSTAGE;
+          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
+          const bool nodes = w.tile + i == w.tiles - 1;
+          const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
+          const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
+          const int row = nodes ? 0 : (w.tile + i) * KT;
+          bar_expect(&s.full[stage], C::STAGE);
+#pragma unroll
+          for (int sub = 0; sub < C::SUB; ++sub)
+            tma_load(ring + stage * C::STAGE + sub * KT * 128, map, sub * 64, row, h * a.along[which][0],
+                     w.b * a.along[which][1], &s.full[stage]);
+        }
+      }
+      if (!ok)  // gave up: the copies in flight still land before the CTA ends
+        for (uint32_t back = 1; back <= C::NSTAGE && back <= seq; ++back) {
+          const uint32_t q = seq - back;
+          const unsigned long long t0 = timer_ns();
+          while (!bar_try(&s.full[q % C::NSTAGE], (q / C::NSTAGE) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+          }
+        }
+    }
+  } else if (warp == 1) {
+    // ---- tensor core
+    if (lane == 0) {
+      Walk w(s.pre, a.batch, units, g_begin, g_end);
+      constexpr uint32_t DESC_S = mma_desc(TR_ROWS, KT, false), DESC_O = mma_desc(TR_ROWS, D, true);
+      uint32_t base = 0, gt = 0, seg = 0;
+      while (w.next()) {
+        const int n = w.count;
+        auto scores = [&](int i) {
+          const uint32_t item = base + pos_k(i), stage = item % C::NSTAGE;
+          wait(&s.full[stage], (item / C::NSTAGE) & 1);
+          tc_fence_after();
+          const uint32_t k0 = s_addr(ring + stage * C::STAGE);
+          const uint32_t d = tmem + C::COL_S + ((gt + i) & 1) * KT;
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            mma_ts(d, tmem + C::COL_Q + 8 * ks, smem_desc(k0 + (ks / 4) * KT * 128 + (ks % 4) * 32, 16), DESC_S, ks > 0);
+          mma_commit(&s.empty[stage]);
+          mma_commit(&s.s_full[(gt + i) & 1]);
+        };
+        wait(&s.q_ready, seg & 1);
+        tc_fence_after();
+        scores(0);
+        for (int i = 0; i < n; ++i) {
+          if (i + 1 < n) scores(i + 1);
+          const uint32_t buf = (gt + i) & 1;
+          wait(&s.p_ready[buf], ((gt + i) >> 1) & 1);
+          const uint32_t item = base + pos_v(i, n), stage = item % C::NSTAGE;
+          wait(&s.full[stage], (item / C::NSTAGE) & 1);
+          tc_fence_after();
+          const uint32_t v0 = s_addr(ring + stage * C::STAGE);
+#pragma unroll
+          for (int ks = 0; ks < KT / 16; ++ks)
+            mma_ts(tmem, tmem + C::COL_S + buf * KT + 8 * ks, smem_desc(v0 + ks * 2048, KT * 128), DESC_O, i > 0 || ks > 0);
+          mma_commit(&s.empty[stage]);
+          mma_commit(&s.o_done[buf]);
+        }
+        base += 2 * n;
+        gt += n;
+        ++seg;
+      }
+      if (*abort) {  // what was issued ends before tensor memory is given back
+        mma_commit(&s.drain);
+        const unsigned long long t0 = timer_ns();
+        while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
+        }
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // ---- softmax: one row per thread
+    const int row = tid - 128;
+    const uint32_t lanes = tmem + ((uint32_t)(warp - 4) << 21);  // this warp's 32 lanes (bits 16..)
+    Walk w(s.pre, a.batch, units, g_begin, g_end);
+    uint32_t base = 0, gt = 0;
+    bool first = true;
+    while (w.next()) {
+      const int n = w.count, h = w.unit / a.mtiles, mt = w.unit - h * a.mtiles;
+      const int r = mt * TR_ROWS + row;                 // row of the KV head
+      const int left = a.n * a.group - mt * TR_ROWS;    // rows of this unit
+      const bool warp_on = 32 * (warp - 4) < left, on = row < left;
+      const int node = on ? r / a.group : 0, qh = h * a.group + (on ? r - node * a.group : 0);
+      const int len = s.len[w.b];
+      const bool has_nodes = w.tile + n == w.tiles;
+      // every S of the segment before has been read, so its MMAs are done with Q
+      if (warp_on) {
+        const uint16_t *q = a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t x[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint4 v = on ? __ldg(reinterpret_cast<const uint4 *>(q + c * 64) + j) : make_uint4(0, 0, 0, 0);
+            x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+          }
+          tmem_st32(lanes + C::COL_Q + 32 * c, x);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&s.q_ready);
+      uint64_t see = 0;
+      if (has_nodes) {
+        // ancestors by pointer doubling: after k rounds a node knows 2^k of its line
+        uint64_t mask = 0;
+        int up = -2;
+        if (row < a.n) {
+          up = a.parents[w.b * a.ps[0] + row * a.ps[1]];
+          if (up < -1 || up >= row) up = -2;
+          mask = up == -2 ? 0 : 1ull << row;
+        }
+        for (int step = 1;; step <<= 1) {
+          if (row < TR_NODES) {
+            s.anc[row] = mask;
+            s.up[row] = up;
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (step >= a.n) break;
+          uint64_t over = 0;
+          int next = -1;
+          if (up >= 0) over = s.anc[up], next = s.up[up];
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (up >= 0) {
+            mask = over ? mask | over : 0;  // a node below an unused one is unused
+            up = over ? next : -2;
+          }
+        }
+        if (on) see = s.anc[node];
+      }
+      const bool dead = has_nodes && see == 0;
+      float m = -INFINITY, l = 0.0f;  // running maximum (log2 units) and sum
+      for (int i = 0; i < n; ++i) {
+        const uint32_t buf = (gt + i) & 1;
+        const uint32_t at = lanes + C::COL_S + buf * KT;
+        const bool nodes = w.tile + i == w.tiles - 1;
+        const int valid = nodes ? a.n : min(KT, len - (w.tile + i) * KT);
+        const bool whole = valid == KT && !nodes;
+        uint64_t keep[KT / 64];  // columns this row sees
+#pragma unroll
+        for (int j = 0; j < KT / 64; ++j) {
+          const int v = valid - 64 * j;
+          keep[j] = nodes ? (j ? 0 : see) : v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
+        }
+        wait(&s.s_full[buf], ((gt + i) >> 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        if (warp_on) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) {
+            uint32_t x[32];
+            tmem_ld32(x, at + 32 * c);
+            tmem_wait_ld();
+            const uint32_t bits = (uint32_t)(keep[c / 2] >> (32 * (c & 1)));
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) top = fmaxf(top, bits >> j & 1 ? __uint_as_float(x[j]) : -INFINITY);
+            }
+          }
+          top *= a.c2;
+          // the maximum moves only when it grows by more than 2^8: until then
+          // weights up to 2^8 lose nothing in FP32 sums and BF16 products,
+          // and the accumulator stays where it is
+          const bool move = i == 0 || top > m + 8.0f;
+          if (i > 0 && __any_sync(0xffffffffu, move)) {
+            const float f = move ? exp2_fast(m - top) : 1.0f;
+            wait(&s.o_done[buf ^ 1], ((gt + i - 1) >> 1) & 1);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t x[32];
+              tmem_ld32(x, lanes + 32 * c);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+              tmem_st32(lanes + 32 * c, x);
+            }
+            l *= f;
+          }
+          if (move) m = top;
+          const float base2 = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) {
+            uint32_t x[32], y[16];
+            tmem_ld32(x, at + 32 * c);
+            tmem_wait_ld();
+            const uint32_t bits = (uint32_t)(keep[c / 2] >> (32 * (c & 1)));
+            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float p0 = exp2_fast(fmaf(__uint_as_float(x[j]), a.c2, -base2));
+              float p1 = exp2_fast(fmaf(__uint_as_float(x[j + 1]), a.c2, -base2));
+              if (!whole) {
+                p0 = bits >> j & 1 ? p0 : 0.0f;
+                p1 = bits >> (j + 1) & 1 ? p1 : 0.0f;
+              }
+              sum0 += p0;
+              sum1 += p1;
+              y[j / 2] = pack_bf16(p0, p1);
+            }
+            l += sum0 + sum1;
+            tmem_st16(at + 16 * c, y);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        if (!whole && (nodes || !C::F8)) {
+          // V rows that no row may see are taken out of the product (0 * NaN is
+          // NaN there): tokens behind the cache's length, unused nodes, and
+          // values of a node that are not finite (its siblings do not see
+          // them; the rows that do get them back below)
+          const uint32_t item = base + pos_v(i, n), stage = item % C::NSTAGE;
+          wait(&s.full[stage], (item / C::NSTAGE) & 1);
+          uint8_t *v = ring + stage * C::STAGE;
+          const int from = nodes ? 0 : valid, to = nodes ? a.n : KT;
+          for (int x = from * (D / 8) + row; x < to * (D / 8); x += 128) {
+            const int key = x / (D / 8), c16 = x % (D / 8);
+            uint4 *p = reinterpret_cast<uint4 *>(v + (c16 / 8) * KT * 128 + key * 128 + (c16 % 8) * 16);
+            if (!nodes || s.anc[key] == 0) {
+              *p = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 u = *p;
+            uint32_t *e = reinterpret_cast<uint32_t *>(&u);
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (not_finite_bf16(e[j])) e[j] &= 0xffff0000u, found = true;
+              if (not_finite_bf16(e[j] >> 16)) e[j] &= 0x0000ffffu, found = true;
+            }
+            if (found) {
+              *p = u;
+              atomicOr(&s.bad, 1ull << key);
+            }
+          }
+          async_fence();
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.p_ready[buf]);
+      }
+      // ---- the unit's rows, or this CTA's part of them
+      wait(&s.o_done[(gt + n - 1) & 1], ((gt + n - 1) >> 1) & 1);
+      __syncwarp();
+      tc_fence_after();
+      uint64_t bad = 0;
+      if (has_nodes) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        bad = s.bad & see;
+      }
+      if (*abort) l = __uint_as_float(0x7fffffffu);
+      const bool direct = n == w.tiles;
+      if (warp_on) {
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const int64_t out_row = ((int64_t)w.b * a.n + node) * (a.heads * a.group) + qh;
+        const int64_t part_row = (int64_t)(2 * cta + (first ? 0 : 1)) * a.rows + row;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t x[32];
+          tmem_ld32(x, lanes + 32 * c);
+          tmem_wait_ld();
+          if (bad)
+            for (uint64_t rest = bad; rest; rest &= rest - 1) {
+              const uint16_t *vn = a.vn + w.b * a.vns[0] + h * a.vns[1] + (__ffsll((long long)rest) - 1) * a.vns[2] + 32 * c;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const uint32_t v = vn[j];
+                if (not_finite_bf16(v)) x[j] = __float_as_uint(__uint_as_float(x[j]) + __uint_as_float(v << 16));
+              }
+            }
+          if (!on) {
+          } else if (direct) {
+            uint32_t y[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              y[j] = dead ? 0u : pack_bf16(__uint_as_float(x[2 * j]) * inv, __uint_as_float(x[2 * j + 1]) * inv);
+            uint4 *o = reinterpret_cast<uint4 *>(a.out + out_row * D + 32 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+          } else {
+            uint4 *o = reinterpret_cast<uint4 *>(a.part + part_row * D + 32 * c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+          }
+          __syncwarp();
+        }
+        if (on) {
+          if (direct) a.lse[out_row] = dead ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          else a.ml[part_row] = make_float2(m, dead ? -1.0f : l);
+        }
+        tc_fence_before();
+      }
+      if (has_nodes) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // all have read s.bad and s.anc
+        if (row == 0) s.bad = 0;
+      }
+      base += 2 * n;
+      gt += n;
+      first = false;
+    }
+  } else if (C::F8 && warp >= 8) {
+    // ---- FP8 caches: each thread copies its own 16-code pieces ahead with
+    // cp.async (no barrier between the copy and its use), turns them into
+    // BF16 and puts them where TMA would have put a BF16 tile
+    constexpr int PIECES = C::RAW / 16 / 256;  // of one thread and tile
+    const int ct = tid - 256;
+    struct Items {
+      Walk w;
+      int p = 0;
+      bool live;
+      __device__ Items(const Walk &x) : w(x) { live = w.next(); }
+      __device__ void step() {
+        if (++p == 2 * w.count) {
+          p = 0;
+          live = w.next();
+        }
+      }
+    };
+    Items ahead(Walk(s.pre, a.batch, units, g_begin, g_end)), now = ahead;
+    auto source = [&](const Items &it, bool is_v) {
+      const int h = it.w.unit / a.mtiles;
+      if (a.cells) return a.cells[it.w.b * a.heads + h].kv8 + (is_v ? D : 0);
+      return is_v ? a.v8 + it.w.b * a.v8s[0] + h * a.v8s[1] : a.k8 + it.w.b * a.k8s[0] + h * a.k8s[1];
+    };
+    auto issue = [&](const Items &it, int slot) {
+      if (it.live) {
+        bool is_v;
+        int i;
+        item_at(it.p, it.w.count, is_v, i);
+        if (it.w.tile + i < it.w.tiles - 1) {
+          const uint8_t *src = source(it, is_v);
+          const int64_t st = a.cells ? REC : is_v ? a.v8s[2] : a.k8s[2];
+          const int t0 = (it.w.tile + i) * KT, len = s.len[it.w.b];
+#pragma unroll
+          for (int j = 0; j < PIECES; ++j) {
+            const int c = ct + j * 256, key = c / (D / 16);
+            if (t0 + key < len) cp_async16(raw + slot * C::RAW + c * 16, src + (t0 + key) * st + (c % (D / 16)) * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    constexpr int AHEAD = C::F8 ? C::NRAW : 1;
+    for (int i = 0; i < AHEAD; ++i) {
+      issue(ahead, i);
+      if (ahead.live) ahead.step();
+    }
+    uint32_t seq = 0;
+    while (now.live) {
+      const int stage = seq % C::NSTAGE, slot = seq % AHEAD;
+      bool is_v;
+      int i;
+      item_at(now.p, now.w.count, is_v, i);
+      const bool nodes = now.w.tile + i == now.w.tiles - 1;
+      uint8_t *to = ring + stage * C::STAGE;
+      cp_async_wait<AHEAD - 1>();
+      if (!nodes) {
+        const int left = s.len[now.w.b] - (now.w.tile + i) * KT;
+        uint4 v[PIECES];
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int c = ct + j * 256;
+          v[j] = c / (D / 16) < left ? *reinterpret_cast<const uint4 *>(raw + slot * C::RAW + c * 16) : make_uint4(0, 0, 0, 0);
+        }
+        issue(ahead, slot);
+        if (ahead.live) ahead.step();
+        if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int c = ct + j * 256, key = c / (D / 16), c16 = 2 * (c % (D / 16));
+          const uint32_t *x = reinterpret_cast<const uint32_t *>(&v[j]);
+          uint4 y[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            y[u] = make_uint4(e4m3x2_to_bf16x2((uint16_t)x[2 * u]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u] >> 16)),
+                              e4m3x2_to_bf16x2((uint16_t)x[2 * u + 1]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u + 1] >> 16)));
+          // neighbouring threads write the two halves in opposite order where
+          // they would meet in the same banks (pieces of different subtiles)
+          uint8_t *line = to + (c16 / 8) * KT * 128 + key * 128;
+          const int flip = (c16 >> 3) & 1;
+          *reinterpret_cast<uint4 *>(line + (((c16 + flip) % 8) ^ (key & 7)) * 16) = flip ? y[1] : y[0];
+          *reinterpret_cast<uint4 *>(line + (((c16 + 1 - flip) % 8) ^ (key & 7)) * 16) = flip ? y[0] : y[1];
+        }
+      } else {
+        issue(ahead, slot);
+        if (ahead.live) ahead.step();
+        if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
+        const int h = now.w.unit / a.mtiles;
+        const uint16_t *src = is_v ? a.vn + now.w.b * a.vns[0] + h * a.vns[1] : a.kn + now.w.b * a.kns[0] + h * a.kns[1];
+        const int64_t st = is_v ? a.vns[2] : a.kns[2];
+#pragma unroll
+        for (int j = 0; j < 2 * PIECES; ++j) {
+          const int c = ct + j * 256, key = c / (D / 8), c16 = c % (D / 8);
+          const uint4 y = key < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + key * st) + c16) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(to + (c16 / 8) * KT * 128 + key * 128 + ((c16 % 8) ^ (key & 7)) * 16) = y;
+        }
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&s.full[stage]);
+      now.step();
+      ++seq;
+    }
+    cp_async_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// ---- joining the parts of a unit ---------------------------------------------
+
+constexpr int TC_THREADS = 256, TC_MAX = 512;  // most CTAs of the attention kernel
+
+// One row per block: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over
+// the CTAs c of the row's unit, in their order.  D / 4 threads hold the row;
+// the groups of them take every TC_THREADS / (D / 4)-th part.
+template <int D, int KT>
+__global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int ctas) {
+  constexpr int LANES = D / 4, GROUPS = TC_THREADS / LANES;
+  __shared__ int32_t s_pre[TR_BATCH + 1];
+  __shared__ float s_w[TC_MAX];
+  __shared__ float s_red[2][TC_THREADS / 32];
+  __shared__ float4 s_o[GROUPS][LANES];
+  __shared__ int s_dead;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, nullptr, s_pre);
+  if (tid == 0) s_dead = 0;
+  __syncthreads();
+  const int rows = a.n * a.group;
+  const int r = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % a.heads, b = bh / a.heads;
+  const int units = a.heads * a.mtiles, mt = r / TR_ROWS;
+  const long long total = (long long)s_pre[a.batch] * units;
+  const Plan plan{total, (int)min((long long)ctas, total)};
+  const int tiles = s_pre[b + 1] - s_pre[b];
+  const long long g0 = (long long)s_pre[b] * units + (long long)(h * a.mtiles + mt) * tiles;
+  const int c0 = plan.owner(g0), c1 = plan.owner(g0 + tiles - 1);
+  if (c0 == c1) return;  // written by its one CTA
+  const int shift = plan.begin(c0) < g0 ? 1 : 0;  // only its first CTA may have had a unit before
+  grid_dependency_wait();
+  const int parts = c1 - c0 + 1, prow = r - mt * TR_ROWS;
+  auto slot = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0 ? shift : 0)) * a.rows + prow; };
+  float m = -INFINITY, l = 0.0f;
+  for (int i = tid; i < parts; i += TC_THREADS) {
+    const float2 x = __ldcg(a.ml + slot(i));
+    if (x.y < 0.0f) s_dead = 1;
+    s_w[i] = x.x;
+    m = fmaxf(m, x.x);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) s_red[0][warp] = m;
+  __syncthreads();
+  m = s_red[0][0];
+#pragma unroll
+  for (int i = 1; i < TC_THREADS / 32; ++i) m = fmaxf(m, s_red[0][i]);
+  const float base = m == -INFINITY ? 0.0f : m;
+  for (int i = tid; i < parts; i += TC_THREADS) {
+    const float w = exp2_fast(s_w[i] - base);
+    s_w[i] = w;
+    l += w * __ldcg(a.ml + slot(i)).y;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) s_red[1][warp] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < TC_THREADS / 32; ++i) l += s_red[1][i];
+  const int group = tid / LANES, d4 = tid % LANES;
+  float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int i = group; i < parts; i += GROUPS) {
+    const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.part + slot(i) * D) + d4);
+    const float w = s_w[i];
+    // (a part without a visible key has weight 0 and zeros or, for an unused row, anything)
+    if (w != 0.0f) {
+      o.x = fmaf(w, x.x, o.x);
+      o.y = fmaf(w, x.y, o.y);
+      o.z = fmaf(w, x.z, o.z);
+      o.w = fmaf(w, x.w, o.w);
+    }
+  }
+  s_o[group][d4] = o;
+  __syncthreads();
+  if (group) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    const float4 x = s_o[i][d4];
+    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+  }
+  const int node = r / a.group;
+  const int64_t row = ((int64_t)b * a.n + node) * (a.heads * a.group) + h * a.group + (r - node * a.group);
+  const bool dead = s_dead;
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const uint2 y = dead ? make_uint2(0, 0) : make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  reinterpret_cast<uint2 *>(a.out + row * D)[d4] = y;
+  if (d4 == 0) a.lse[row] = dead ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <class C>
+int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t st) {
+  constexpr int smem = 1024 + C::RING + (int)sizeof(TreeSmem<C>);
+  static_assert(smem <= 232448, "shared memory");
+  auto *kernel = &k_tree_attention<C>;
+  if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                       "k_tree_attention shared memory"))
+    return rc;
+  if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, false, 1, maps, a),
+                       "k_tree_attention launch"))
+    return rc;
+  const unsigned rows = (unsigned)(a.batch * a.heads * a.n * a.group);
+  return op_cuda(op_launch(k_tree_combine<C::D, C::KT>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas),
+                 "k_tree_combine launch");
+}
+
+template <bool F8>
+int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t st) {
+  if (d == 64) return launch_tree<TreeCfg<64, F8>>(maps, a, ctas, st);
+  if (d == 128) return launch_tree<TreeCfg<128, F8>>(maps, a, ctas, st);
+  return launch_tree<TreeCfg<256, F8>>(maps, a, ctas, st);
+}
+
+// CTAs of a launch: one per SM, or the most tiles that there can be.
+int tree_ctas(int sms, int64_t batch, int64_t units, int64_t t, int64_t dim) {
+  const int64_t kt = dim == 256 ? 64 : 128, most = batch * units * ((t + kt - 1) / kt + 1);
+  const int64_t c = sms < TC_MAX ? sms : TC_MAX;
+  return (int)(most < c ? most : c);
+}
+
+int sm_count(int device, int *sms) {
+  return op_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device), "device attribute");
+}
+
+int64_t tree_workspace(int sms, const SkvTree *d) {
+  const int64_t rows = d->n * (d->heads / d->kv_heads), per = rows < TR_ROWS ? rows : TR_ROWS;
+  const int64_t units = d->kv_heads * ((rows + TR_ROWS - 1) / TR_ROWS);
+  const int64_t batch = d->batch < TR_BATCH ? d->batch : TR_BATCH;
+  const int64_t slots = 2 * (int64_t)tree_ctas(sms, batch, units, d->tokens, d->dim);
+  return slots * per * (d->dim + 2) * 4;
+}
+
+int check_tree(const SkvTree *d) {
+  if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
+  if (d->dim != 64 && d->dim != 128 && d->dim != 256) return op_fail(SKV_E_INVALID, "head size must be 64, 128 or 256");
+  if (d->n < 1 || d->n > TR_NODES) return op_fail(SKV_E_INVALID, "nodes must be in [1, %d]", TR_NODES);
+  if (d->batch < 0 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096 ||
+      d->batch * d->heads * d->n > INT32_MAX)
+    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, counts in range");
+  if (d->tokens < 1 || d->tokens > (1 << 26)) return op_fail(SKV_E_INVALID, "tokens must be in [1, 2^26]");
+  if (!(d->scale > 0.0) || !(d->scale < 1e30)) return op_fail(SKV_E_INVALID, "scale must be positive and finite");
+  if (d->cache_dtype != SKV_DTYPE_BF16 && d->cache_dtype != SKV_DTYPE_E4M3)
+    return op_fail(SKV_E_INVALID, "the cache is BF16 or FP8 e4m3");
+  return SKV_OK;
+}
+
+}  // namespace
+
+// Attention over a cache given by `d`, or (cells != null) over the engine's
+// FP8 records with the context at `tlen` (null: `context`).
+int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
+  if (int rc = check_tree(d)) return rc;
+  if (d->batch == 0) return SKV_OK;
+  if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse || !d->workspace ||
+      (!cells && (!d->k_cache || !d->v_cache || !d->lengths)))
+    return op_fail(SKV_E_INVALID, "null input, output or workspace pointer");
+  const bool f8 = d->cache_dtype == SKV_DTYPE_E4M3;
+  const int align = f8 ? 16 : 8;  // elements of 16 bytes
+  auto aligned = [&](const void *p, const int64_t *s, int64_t unit) {
+    if ((uintptr_t)p % 16) return false;
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || s[i] % unit) return false;
+    return true;
+  };
+  if (!aligned(d->q, d->q_stride, 8) || !aligned(d->k, d->k_stride, 8) || !aligned(d->v, d->v_stride, 8) ||
+      (!cells && (!aligned(d->k_cache, d->k_cache_stride, align) || !aligned(d->v_cache, d->v_cache_stride, align))) ||
+      (uintptr_t)d->out % 16 || (uintptr_t)d->workspace % 16)
+    return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
+  if ((!cells && d->tokens > 1 && (!d->k_cache_stride[2] || !d->v_cache_stride[2])) ||
+      (d->n > 1 && (!d->k_stride[2] || !d->v_stride[2])))
+    return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  DeviceScope scope((int)d->device);
+  if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
+  int sms = 0;
+  if (int rc = sm_count((int)d->device, &sms)) return rc;
+  if (d->workspace_bytes < tree_workspace(sms, d))
+    return op_fail(SKV_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
+                   (long long)tree_workspace(sms, d));
+  TreeArgs a{};
+  if (int rc = status_word((int)d->device, &a.status)) return rc;
+  const int group = (int)(d->heads / d->kv_heads), rows = (int)d->n * group;
+  a.heads = (int)d->kv_heads, a.group = group, a.n = (int)d->n, a.t = (int)d->tokens;
+  a.mtiles = (rows + TR_ROWS - 1) / TR_ROWS;
+  a.rows = rows < TR_ROWS ? rows : TR_ROWS;
+  a.c2 = (float)(d->scale * 1.4426950408889634);
+  a.cells = cells;
+  a.context = context;
+  a.len_stride = cells ? 0 : d->lengths_stride;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = d->q_stride[i];
+    a.kns[i] = d->k_stride[i], a.vns[i] = d->v_stride[i];
+    a.k8s[i] = d->k_cache_stride[i], a.v8s[i] = d->v_cache_stride[i];
+  }
+  a.ps[0] = d->parents_stride[0], a.ps[1] = d->parents_stride[1];
+  for (int64_t b0 = 0; b0 < d->batch; b0 += TR_BATCH) {
+    const int64_t nb = d->batch - b0 < TR_BATCH ? d->batch - b0 : TR_BATCH;
+    a.batch = (int)nb;
+    a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0];
+    a.kn = static_cast<const uint16_t *>(d->k) + b0 * a.kns[0];
+    a.vn = static_cast<const uint16_t *>(d->v) + b0 * a.vns[0];
+    a.cells = cells ? cells + b0 * d->kv_heads : nullptr;
+    a.lengths = cells ? tlen : static_cast<const int32_t *>(d->lengths) + b0 * a.len_stride;
+    a.parents = static_cast<const int32_t *>(d->parents) + b0 * a.ps[0];
+    a.out = static_cast<uint16_t *>(d->out) + b0 * d->n * d->heads * d->dim;
+    a.lse = static_cast<float *>(d->lse) + b0 * d->n * d->heads;
+    const int ctas = tree_ctas(sms, nb, (int64_t)a.heads * a.mtiles, d->tokens, d->dim);
+    a.part = static_cast<float *>(d->workspace);
+    a.ml = reinterpret_cast<float2 *>(a.part + 2 * (int64_t)ctas * a.rows * d->dim);
+    TreeMaps maps{};
+    int rc = SKV_OK;
+    if (!f8) {
+      const int kt = d->dim == 256 ? 64 : 128;
+      const struct {
+        CUtensorMap *map;
+        const void *base;
+        const int64_t *s;
+        int64_t rows;
+      } four[4] = {{&maps.k, static_cast<const uint16_t *>(d->k_cache) + b0 * d->k_cache_stride[0], d->k_cache_stride, d->tokens},
+                   {&maps.v, static_cast<const uint16_t *>(d->v_cache) + b0 * d->v_cache_stride[0], d->v_cache_stride, d->tokens},
+                   {&maps.kn, a.kn, d->k_stride, d->n},
+                   {&maps.vn, a.vn, d->v_stride, d->n}};
+      for (int i = 0; i < 4 && !rc; ++i) {
+        const int64_t step[3] = {four[i].s[2], four[i].s[1], four[i].s[0]};
+        rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step, kt);
+        a.along[i][0] = d->kv_heads > 1 && four[i].s[1] ? 1 : 0;
+        a.along[i][1] = nb > 1 && four[i].s[0] ? 1 : 0;
+      }
+    } else if (!cells) {
+      a.k8 = static_cast<const uint8_t *>(d->k_cache) + b0 * a.k8s[0];
+      a.v8 = static_cast<const uint8_t *>(d->v_cache) + b0 * a.v8s[0];
+    }
+    if (!rc) rc = f8 ? launch_tree_d<true>((int)d->dim, maps, a, ctas, st) : launch_tree_d<false>((int)d->dim, maps, a, ctas, st);
+    if (rc) return rc;
+  }
+  return SKV_OK;
+}
+
+}  // namespace skv
+
+extern "C" {
+
+int skv_tree_attention(const SkvTree *d, void *stream) {
+  return skv::tree_attention(d, nullptr, nullptr, 0, static_cast<cudaStream_t>(stream));
+}
+
+int skv_tree_workspace(const SkvTree *d, int64_t *bytes) {
+  using namespace skv;
+  if (!bytes) return op_fail(SKV_E_INVALID, "null result pointer");
+  if (int rc = check_tree(d)) return rc;
+  int sms = 0;
+  if (int rc = sm_count((int)d->device, &sms)) return rc;
+  *bytes = tree_workspace(sms, d);
+  return SKV_OK;
+}
+
+int skv_operator_status(int32_t device, uint32_t *flags) {
+  using namespace skv;
+  if (!flags) return op_fail(SKV_E_INVALID, "null result pointer");
+  DeviceScope scope(device);
+  if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
+  uint32_t *word = nullptr, got = 0;
+  if (int rc = status_word(device, &word)) return rc;
+  if (int rc = op_cuda(cudaDeviceSynchronize(), "waiting for the device")) return rc;
+  if (int rc = op_cuda(cudaMemcpy(&got, word, sizeof got, cudaMemcpyDeviceToHost), "reading the status word")) return rc;
+  *flags = got;
+  return SKV_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,379 @@
+"""Operators around a decode step: rotary positions, attention of a tree of
+drafted tokens over a cache, attention weights accumulated per cached key, and
+eviction from the cache by those weights.
+
+The reference takes rotated K and Q, decodes one token per step and never
+drops one; these are what a decode loop that drafts several tokens ahead, or
+that has to stay inside a memory budget, needs next to it::
+
+    q, k = rotary(q, k, positions)                                     # drafted tokens
+    y, lse = tree_attention(q, k_cache, v_cache, lengths, k, v, parents)
+    weights = accumulate_weights(q, k_cache, lengths, lse, weights, rows=accepted)
+    k_cache, v_cache, weights, ids, lengths = evict(k_cache, v_cache, weights, lengths, keep=budget)
+
+Every operator is a function of CUDA tensors of one device and returns new
+ones (``rotary`` and ``accumulate_weights`` also write into given ones).  The
+work is enqueued on the current PyTorch stream of that device; nothing waits,
+and every call may be captured into a CUDA graph.  Tensors may have any
+strides as long as the innermost dimension is contiguous and, for the
+attention operators, rows start on 16-byte boundaries; ValueError otherwise.
+They are for inference: a tensor that requires a gradient is refused while
+gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+import struct
+
+import torch
+
+from seoulkv_b200 import _native
+from seoulkv_b200.api import _current_stream
+
+TREE_MAX_NODES = 64
+ROTARY_MAX_DIM = 512
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
+_NAMES = {torch.bfloat16: "BF16", torch.float16: "FP16", torch.float32: "FP32", torch.float8_e4m3fn: "FP8 e4m3"}
+
+
+def _check(name: str, t, shape, dtypes, device=None) -> None:
+    """A CUDA tensor of one of the dtypes; ``shape`` entries of None are free."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        raise ValueError(f"{name}: expected a {' or '.join(_NAMES.get(x, str(x)) for x in dtypes)} tensor")
+    got = t.shape
+    if len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
+        raise ValueError(f"{name}: expected shape [{','.join('*' if w is None else str(w) for w in shape)}], "
+                         f"got {list(got)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the operators have no backward pass (detach it, or use no_grad)")
+
+
+def _rows(name: str, t: torch.Tensor) -> None:
+    """Contiguous innermost dimension, rows on 16-byte boundaries, no two tokens in one row."""
+    st, unit = t.stride(), 16 // t.element_size()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the innermost dimension must be contiguous")
+    if t.data_ptr() % 16 or any(s % unit and n > 1 for s, n in zip(st[:-1], t.shape)):
+        raise ValueError(f"{name}: rows must start on 16-byte boundaries")
+
+
+def _steps(t: torch.Tensor, axes, unit: int = 1) -> list[int]:
+    """Strides of the axes; 0 for an axis of one element (its own stride means nothing)."""
+    st, n = t.stride(), t.shape
+    return [st[x] * unit if n[x] > 1 else 0 for x in axes]
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and last byte address (exclusive) that a tensor reaches."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _run(entry, packed: bytes, device: torch.device, what: str) -> None:
+    rc = entry(packed, _current_stream(device.index))
+    if rc:
+        message = _native.load().skv_last_error().decode(errors="replace")
+        if rc == -1:
+            raise ValueError(f"{what}: {message}")
+        raise _native.NativeError(rc, f"{what}: {message}")
+
+
+def check_operators(device) -> None:
+    """Wait for the device; RuntimeError if a bounded wait of an operator's kernel gave up on it
+    (the outputs of that call are NaN).  Not for the inner loop."""
+    from seoulkv_b200.api import _cuda_index
+
+    flags = ctypes.c_uint32()
+    _native.check(_native.load().skv_operator_status(_cuda_index(device), ctypes.byref(flags)), "skv_operator_status")
+    if flags.value:
+        raise RuntimeError(f"an operator's kernel gave up waiting (status {flags.value:#x}); its results are invalid")
+
+
+# ---------------------------------------------------------------- rotary positions
+
+
+@functools.lru_cache(maxsize=64)
+def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
+    """(turns per position * 2^64 of each pair as packed uint64, factor on the rotated part)."""
+    if not theta > 0.0 or not math.isfinite(theta) or theta == 1.0:
+        raise ValueError("theta must be positive, finite and not 1")
+    if not factor > 0.0 or not math.isfinite(factor):
+        raise ValueError("factor must be positive and finite")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise ValueError("scaling must be 'none', 'linear', 'ntk' or 'yarn'")
+    pairs, r = rotary_dim // 2, float(rotary_dim)
+    base = theta
+    if scaling == "ntk" and rotary_dim > 2:
+        base = theta * factor ** (r / (r - 2.0))
+    freq = [base ** (-2.0 * i / r) for i in range(pairs)]
+    m = 1.0
+    if scaling == "linear":
+        freq = [f / factor for f in freq]
+    elif scaling == "yarn":
+        if original_context is None or original_context < 1:
+            raise ValueError("yarn scaling needs original_context >= 1")
+        if not beta_fast > beta_slow > 0.0:
+            raise ValueError("yarn scaling needs beta_fast > beta_slow > 0")
+
+        def pair_of(turns):  # the (real) pair that turns so often in the original context
+            return r * math.log(original_context / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))
+
+        low = max(math.floor(pair_of(beta_fast)), 0)
+        high = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+        for i in range(pairs):
+            part = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
+            freq[i] = freq[i] * (1.0 - part) + freq[i] / factor * part
+        m = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    if attention_factor is not None:
+        m = float(attention_factor)
+    if not math.isfinite(m):
+        raise ValueError("attention_factor must be finite")
+    turns = [int(round(f / (2.0 * math.pi) * 2.0 ** 64)) & (2 ** 64 - 1) for f in freq]
+    table = ctypes.create_string_buffer(struct.pack(f"{pairs}Q", *turns))
+    return table, ctypes.addressof(table), m
+
+
+_ROTARY = struct.Struct("6Qd" + 10 * "q" + 14 * "q")
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, rotary_dim: int | None = None,
+           theta: float = 10000.0, layout: str = "half", scaling: str = "none", factor: float = 1.0,
+           original_context: int | None = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+           attention_factor: float | None = None, out=None):
+    """Rotary positions on queries [B, N, Hq, D] and keys [B, Hkv, N, D] (or None).
+
+    BF16, FP16 or FP32, both alike, on one device.  ``positions`` int32 or
+    int64, [N] or [B, N]; angles are exact to an FP32 rounding at any position
+    (2^-65 turns each), negative ones turn back (the inverse rotation, and the
+    gradient's, for a factor of 1).  The first ``rotary_dim`` (even, at most
+    512; all of D by default) dimensions turn, the others are copied.
+    ``layout``: "half" pairs dimension i with i + rotary_dim/2,
+    "interleaved" 2i with 2i + 1.
+
+    ``scaling`` for contexts beyond the trained one: "linear" divides every
+    frequency by ``factor``; "ntk" raises theta so that the slowest pair is
+    divided by it; "yarn" (Peng et al., 2023) divides the pairs that turn less
+    than ``beta_slow`` times in ``original_context`` tokens, keeps those above
+    ``beta_fast``, goes linearly between, and multiplies the rotated part by
+    0.1 ln(factor) + 1 (``attention_factor`` sets another multiplier).
+
+    Returns (q, k) in new tensors, or in ``out=(q_out, k_out)``, which may be
+    the inputs themselves (otherwise they must not overlap them).
+    """
+    if not isinstance(q, torch.Tensor) or q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("q: expected a BF16 or FP16 or FP32 tensor")
+    _check("q", q, (None,) * 4, (q.dtype,))
+    b, n, hq, d = q.shape
+    dev = q.device
+    hkv = 0
+    if k is not None:
+        _check("k", k, (b, None, n, d), (q.dtype,), dev)
+        hkv = k.shape[1]
+    if hq < 1 or (k is not None and hkv < 1):
+        raise ValueError("q and k need at least one head")
+    if not isinstance(positions, torch.Tensor) or positions.ndim not in (1, 2):
+        raise ValueError("positions: expected an int32 or int64 tensor [N] or [B,N]")
+    _check("positions", positions, (n,) if positions.ndim == 1 else (b, n), (torch.int32, torch.int64), dev)
+    r = d if rotary_dim is None else rotary_dim
+    if type(r) is not int or r < 2 or r % 2 or r > d or r > ROTARY_MAX_DIM:
+        raise ValueError(f"rotary_dim must be an even integer in [2, min(D, {ROTARY_MAX_DIM})]")
+    if layout not in ("half", "interleaved"):
+        raise ValueError("layout must be 'half' or 'interleaved'")
+    _, phase, m = _rotary_table(r, float(theta), scaling, float(factor), original_context, float(beta_fast),
+                                float(beta_slow), attention_factor)
+    if out is None:
+        qo = torch.empty((b, n, hq, d), dtype=q.dtype, device=dev)
+        ko = None if k is None else torch.empty((b, hkv, n, d), dtype=q.dtype, device=dev)
+    else:
+        qo, ko = out
+        _check("out[0]", qo, (b, n, hq, d), (q.dtype,), dev)
+        pairs = [("out[0]", qo, q)]
+        if k is None:
+            if ko is not None:
+                raise ValueError("out[1]: there is no k")
+        else:
+            _check("out[1]", ko, (b, hkv, n, d), (q.dtype,), dev)
+            pairs.append(("out[1]", ko, k))
+        for name, y, x in pairs:
+            if any(s == 0 and size > 1 for s, size in zip(y.stride(), y.shape)):
+                raise ValueError(f"{name}: two elements share one place")
+            same = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
+            if not same and _overlap(y, x):
+                raise ValueError(f"{name} overlaps its input without being it")
+        if k is not None and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
+            # (in place, q and k may be interleaved parts of one projection)
+            for name, y, x in (("out[0]", qo, k), ("out[1]", ko, q), ("out[1]", ko, qo)):
+                if _overlap(y, x):
+                    raise ValueError(f"{name} overlaps another tensor of the call")
+    for name, t in (("q", q), ("k", k), ("out[0]", qo), ("out[1]", ko)):
+        if t is not None and t.stride(3) != 1 and d > 1:
+            raise ValueError(f"{name}: the innermost dimension must be contiguous")
+    if not b or not n:
+        return qo, ko
+    kk, kko = (q, qo) if k is None else (k, ko)
+    pos = _steps(positions, (0, 1)) if positions.ndim == 2 else [0, *_steps(positions, (0,))]
+    packed = _ROTARY.pack(
+        q.data_ptr(), kk.data_ptr(), qo.data_ptr(), kko.data_ptr(), positions.data_ptr(), phase, m,
+        dev.index, _DTYPE[q.dtype], layout == "interleaved", positions.dtype == torch.int64, b, n, hq, hkv, d, r,
+        *_steps(q, (0, 1, 2)), *_steps(kk, (0, 2, 1)), *_steps(qo, (0, 1, 2)), *_steps(kko, (0, 2, 1)), *pos)
+    _run(_native.load().skv_rotary, packed, dev, "rotary")
+    return qo, ko
+
+
+# ---------------------------------------------------------------- attention of drafted trees
+
+
+_TREE = struct.Struct("10Qd" + 9 * "q" + 18 * "q")
+
+
+def _check_cache(k_cache, v_cache, lengths, hkv=None):
+    _check("k_cache", k_cache, (None, hkv, None, None), (torch.bfloat16, torch.float8_e4m3fn))
+    b, h, t, d = k_cache.shape
+    if d not in (64, 128, 256):
+        raise ValueError("head size must be 64, 128 or 256")
+    if t < 1 or h < 1:
+        raise ValueError("k_cache: expected at least one head and one token of room")
+    tensors = [("k_cache", k_cache)]
+    if v_cache is not None:
+        _check("v_cache", v_cache, (b, h, t, d), (k_cache.dtype,), k_cache.device)
+        tensors.append(("v_cache", v_cache))
+    _check("lengths", lengths, (b,), (torch.int32,), k_cache.device)
+    for name, x in tensors:
+        _rows(name, x)
+        if t > 1 and x.stride(2) == 0:
+            raise ValueError(f"{name}: tokens must not share one row")
+
+
+def _scale(scale, d: int) -> float:
+    s = d ** -0.5 if scale is None else float(scale)
+    if not (s > 0.0 and math.isfinite(s)):
+        raise ValueError("scale must be positive and finite")
+    return s
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                   k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, *, scale: float | None = None):
+    """Exact attention of N drafted tokens per sequence over a cache and their own ancestors.
+
+    ``q`` BF16 [B, N, Hq, D] with N <= 64 and D 64, 128 or 256; ``k_cache``
+    and ``v_cache`` BF16 or FP8 e4m3 [B, Hkv, T, D] with Hq a multiple of Hkv;
+    ``lengths`` int32 [B], the valid tokens (clamped to [0, T]; what lies
+    behind them is not read into any result); ``k`` and ``v`` BF16
+    [B, Hkv, N, D], the drafted tokens' own; ``parents`` int32 [B, N]: the
+    node before node i (below i), -1 for a node that follows the cache.  Any
+    other value marks an unused node (padding of a smaller tree): it and the
+    nodes below it get zeros and an lse of -inf, and nothing sees them.
+
+    Returns the attention output, BF16 [B, N, Hq, D], and the natural
+    log-sum-exp of each row's scaled scores, FP32 [B, N, Hq].  ``scale``
+    defaults to D**-0.5.  N = 1 with parent -1 is exact decode of one token.
+    """
+    _check_cache(k_cache, v_cache, lengths)
+    b, hkv, t, d = k_cache.shape
+    dev = k_cache.device
+    _check("q", q, (b, None, None, d), (torch.bfloat16,), dev)
+    n, hq = q.shape[1], q.shape[2]
+    if not 1 <= n <= TREE_MAX_NODES:
+        raise ValueError(f"the tree must have 1 to {TREE_MAX_NODES} nodes")
+    if hq < 1 or hq % hkv:
+        raise ValueError("query heads must be a multiple of the KV heads")
+    _check("k", k, (b, hkv, n, d), (torch.bfloat16,), dev)
+    _check("v", v, (b, hkv, n, d), (torch.bfloat16,), dev)
+    _check("parents", parents, (b, n), (torch.int32,), dev)
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        _rows(name, x)
+    if n > 1 and (k.stride(2) == 0 or v.stride(2) == 0):
+        raise ValueError("k and v: nodes must not share one row")
+    s = _scale(scale, d)
+    out = torch.empty((b, n, hq, d), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((b, n, hq), dtype=torch.float32, device=dev)
+    if not b:
+        return out, lse
+    lib = _native.load()
+    size = _tree_workspace(dev.index, min(b, 512), n, hq, hkv, d, t)
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    packed = _TREE.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
+        parents.data_ptr(), out.data_ptr(), lse.data_ptr(), work.data_ptr(), s, dev.index, _DTYPE[k_cache.dtype], size,
+        b, n, hq, hkv, d, t, *_steps(q, (0, 1, 2)), *_steps(k_cache, (0, 1, 2)), *_steps(v_cache, (0, 1, 2)),
+        *_steps(k, (0, 1, 2)), *_steps(v, (0, 1, 2)), *_steps(parents, (0, 1)), *_steps(lengths, (0,)))
+    _run(lib.skv_tree_attention, packed, dev, "tree_attention")
+    return out, lse
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: int) -> int:
+    """Bytes of scratch that one call needs (a function of the sizes)."""
+    size = ctypes.c_int64()
+    packed = _TREE.pack(*(10 * (0,)), 1.0, device, 0, 0, b, n, hq, hkv, d, t, *(18 * (0,)))
+    _native.check(_native.load().skv_tree_workspace(packed, ctypes.byref(size)), "skv_tree_workspace")
+    return max(16, size.value)
+
+
+# ---------------------------------------------------------------- eviction
+
+
+_EVICT = struct.Struct("9Q" + 8 * "q" + 9 * "q")
+
+
+def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, lengths: torch.Tensor, *, keep: int,
+          sink: int = 128, local: int = 256):
+    """Shrink caches to ``keep`` tokens per head by accumulated attention weight.
+
+    ``k_cache`` and ``v_cache`` [B, Hkv, T, D] (BF16, FP16, FP32 or FP8),
+    ``weights`` FP32 [B, Hkv, T], ``lengths`` int32 [B] (clamped to [0, T]).
+    Per head the first ``sink`` and the last ``local`` tokens stay and, of the
+    others, the keep - sink - local heaviest (equal weights: the lowest index;
+    NaN counts below every number); a cache of at most ``keep`` tokens stays
+    whole.  Kept tokens keep their order.
+
+    Returns new tensors (k, v, weights, ids, lengths): K and V
+    [B, Hkv, keep, D], FP32 weights and int32 ids (indices into the old cache)
+    [B, Hkv, keep], lengths int32 [B]; past the kept tokens K, V and weights
+    are zero and ids -1.
+    """
+    kinds = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn)
+    _check("k_cache", k_cache, (None,) * 4, kinds)
+    b, h, t, d = k_cache.shape
+    dev = k_cache.device
+    if h < 1 or t < 1 or d < 1:
+        raise ValueError("k_cache: expected at least one head, token and dimension")
+    _check("v_cache", v_cache, (b, h, t, d), (k_cache.dtype,), dev)
+    _check("weights", weights, (b, h, t), (torch.float32,), dev)
+    _check("lengths", lengths, (b,), (torch.int32,), dev)
+    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if x.stride(3) != 1 and d > 1:
+            raise ValueError(f"{name}: the innermost dimension must be contiguous")
+    if any(type(x) is not int for x in (keep, sink, local)) or not 1 <= keep <= t or sink < 0 or local < 0 \
+            or sink + local > keep:
+        raise ValueError(f"keep must be in [1, {t}] and hold the sink and local tokens")
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    ko = torch.empty((b, h, keep, d), dtype=k_cache.dtype, device=dev)
+    vo = torch.empty((b, h, keep, d), dtype=k_cache.dtype, device=dev)
+    wo = torch.empty((b, h, keep), dtype=torch.float32, device=dev)
+    ids = torch.empty((b, h, keep), dtype=torch.int32, device=dev)
+    left = torch.empty((b,), dtype=torch.int32, device=dev)
+    if not b:
+        return ko, vo, wo, ids, left
+    e = k_cache.element_size()
+    packed = _EVICT.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lengths.data_ptr(), ko.data_ptr(), vo.data_ptr(),
+        wo.data_ptr(), ids.data_ptr(), left.data_ptr(), dev.index, b, h, t, d * e, keep, sink, local,
+        *_steps(k_cache, (0, 1, 2), e), *_steps(v_cache, (0, 1, 2), e), *_steps(weights, (0, 1, 2)))
+    _run(_native.load().skv_evict, packed, dev, "evict")
+    return ko, vo, wo, ids, left
