@@ -441,6 +441,30 @@ typedef struct SkvTree {
 int skv_tree_attention(const SkvTree *desc, void *stream);
 int skv_tree_workspace(const SkvTree *desc, int64_t *bytes);
 
+/* Attention weights accumulated per cached key:
+ *   weights_out[b][h][t] = weights[b][h][t] + sum of exp(scale q_r.k_t - lse_r)
+ * over the rows r (nodes i with rows[b][i] != 0, or all of them with rows
+ * null, and the query heads of KV head h) for t < lengths[b]; the weights of
+ * later tokens are copied.  Rows whose lse is -inf do not count.  q, k_cache
+ * and lengths as skv_tree_attention (n is not limited), lse FP32
+ * [batch][n][heads], weights FP32 [batch][kv_heads][tokens]; weights_out may
+ * be weights itself. */
+typedef struct SkvWeights {
+  const void *q, *k_cache, *lengths, *lse, *rows, *weights;
+  void *weights_out;
+  double scale;
+  int64_t device, cache_dtype;
+  int64_t batch, n, heads, kv_heads, dim, tokens;
+  int64_t q_stride[3];          /* sequence, node, head                     */
+  int64_t k_cache_stride[3];    /* sequence, head, token                    */
+  int64_t lse_stride[3];        /* sequence, node, head                     */
+  int64_t rows_stride[2];       /* sequence, node                           */
+  int64_t weights_stride[3];    /* sequence, head, token                    */
+  int64_t weights_out_stride[3];
+  int64_t lengths_stride;
+} SkvWeights;
+int skv_accumulate_weights(const SkvWeights *desc, void *stream);
+
 /* Waits for the device and reads its operators' status word: bits
  * SKV_STATUS_* of bounded device waits that gave up since the library was
  * loaded (the results of such a call are NaN). */

@@ -13,8 +13,8 @@ from seoulkv_b200.api import SeoulKV4
 from seoulkv_b200.batched import BatchResult, SeoulKV4Batch
 from seoulkv_b200.config import SeoulKV4Config
 from seoulkv_b200.index import SeoulKV4Index
-from seoulkv_b200.operators import check_operators, evict, rotary, tree_attention
+from seoulkv_b200.operators import accumulate_weights, check_operators, evict, rotary, tree_attention
 from seoulkv_b200.result import DecodeResult
 
 __all__ = ["BatchResult", "DecodeResult", "SeoulKV4", "SeoulKV4Batch", "SeoulKV4Config", "SeoulKV4Index",
-           "check_operators", "evict", "rotary", "tree_attention"]
+           "accumulate_weights", "check_operators", "evict", "rotary", "tree_attention"]

@@ -18,7 +18,8 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libseoulkv_b200.so"
 SOURCES = ("skv_kernels.cu", "skv_fused.cu", "skv_shard.cu", "skv_append.cu", "skv_engine.cu", "skv_noalloc.cu",
-           "skv_rotary.cu", "skv_evict.cu", "skv_tree.cu")
+           "skv_rotary.cu", "skv_evict.cu", "skv_tree.cu",
+           "skv_weights.cu")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 

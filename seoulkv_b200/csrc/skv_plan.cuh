@@ -1,0 +1,75 @@
+// skv_plan.cuh -- the list of key tiles that the attention operators work
+// through, cut into one contiguous range per CTA.
+#pragma once
+#include <cstdint>
+
+namespace skv {
+
+constexpr int PLAN_BATCH = 512;  // sequences of one launch (their tile counts are kept in shared memory)
+
+struct Plan {
+  long long total;  // tiles of all units
+  int ctas;         // CTAs that have a range
+  __host__ __device__ long long begin(int c) const { return total * c / ctas; }
+  // the CTA whose range holds tile g
+  __host__ __device__ int owner(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
+};
+
+// pre[b] and len[b] by one warp: KT cached tokens a tile, and `extra` tiles more.
+template <int KT>
+__device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch, int extra,
+                                            int32_t *len, int32_t *pre) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int b = b0 + lane;
+    int n = 0, tiles = 0;
+    if (b < batch) {
+      n = lengths ? lengths[b * stride] : context;
+      n = max(0, min(n, t));
+      tiles = (n + KT - 1) / KT + extra;
+    }
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (b < batch) {
+      if (len) len[b] = n;
+      pre[b + 1] = base + x;
+    }
+    base += __shfl_sync(0xffffffffu, x, 31);
+  }
+  if (lane == 0) pre[0] = 0;
+}
+
+// The segments of [g, end): tiles [tile, tile + count) of one unit.
+struct Walk {
+  long long g, end;
+  const int32_t *pre;
+  int units;  // per sequence
+  int b = 0, unit = 0, tile = 0, count = 0, tiles = 0;
+  __device__ Walk(const int32_t *pre_, int batch, int units_, long long g_, long long end_)
+      : g(g_), end(end_), pre(pre_), units(units_) {
+    int lo = 0, hi = batch - 1;  // the last sequence that starts at or before g
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((long long)pre[mid] * units <= g) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+  }
+  __device__ bool next() {
+    if (g >= end) return false;
+    while ((long long)pre[b + 1] * units <= g) ++b;
+    tiles = pre[b + 1] - pre[b];
+    const long long rel = g - (long long)pre[b] * units;
+    unit = (int)(rel / tiles);
+    tile = (int)(rel - (long long)unit * tiles);
+    count = (int)min((long long)(tiles - tile), end - g);
+    g += count;
+    return true;
+  }
+};
+
+}  // namespace skv

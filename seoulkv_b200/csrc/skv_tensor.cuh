@@ -44,7 +44,7 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __noinline__ bool bar_wait_long(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status) {
+static __device__ __noinline__ bool bar_wait_long(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status) {
   const unsigned long long t0 = timer_ns();
   do {
     for (int i = 0; i < WAIT_FREE_POLLS; ++i)

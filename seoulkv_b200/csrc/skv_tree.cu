@@ -29,6 +29,7 @@
 
 #include "skv_device.cuh"
 #include "skv_ops.cuh"
+#include "skv_plan.cuh"
 #include "skv_tensor.cuh"
 
 namespace skv {
@@ -80,7 +81,6 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
 namespace {
 
 constexpr int TR_NODES = SKV_TREE_MAX_NODES;
-constexpr int TR_BATCH = 512;  // sequences of one launch (their tile counts are kept in shared memory)
 constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
 
 template <int D_, bool F8_>
@@ -136,75 +136,8 @@ struct TreeSmem {
   int32_t up[TR_NODES];
   uint32_t tmem;
   uint32_t abort;
-  int32_t len[TR_BATCH];
-  int32_t pre[TR_BATCH + 1];  // tiles of the sequences before (one unit's worth)
-};
-
-// ---- the list of tiles and a CTA's range of it ------------------------------
-
-struct Plan {
-  long long total;  // tiles of all units
-  int ctas;         // CTAs that have a range
-  __host__ __device__ long long begin(int c) const { return total * c / ctas; }
-  // the CTA whose range holds tile g
-  __host__ __device__ int owner(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
-};
-
-// pre[b] and len[b] by one warp.
-template <int KT>
-__device__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch, int32_t *len,
-                            int32_t *pre) {
-  const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int b0 = 0; b0 < batch; b0 += 32) {
-    const int b = b0 + lane;
-    int n = 0, tiles = 0;
-    if (b < batch) {
-      n = lengths ? lengths[b * stride] : context;
-      n = max(0, min(n, t));
-      tiles = (n + KT - 1) / KT + 1;
-    }
-    int x = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (b < batch) {
-      if (len) len[b] = n;
-      pre[b + 1] = base + x;
-    }
-    base += __shfl_sync(0xffffffffu, x, 31);
-  }
-  if (lane == 0) pre[0] = 0;
-}
-
-// The segments of [g, end): tiles [tile, tile + count) of one unit.
-struct Walk {
-  long long g, end;
-  const int32_t *pre;
-  int units;  // per sequence
-  int b = 0, unit = 0, tile = 0, count = 0, tiles = 0;
-  __device__ Walk(const int32_t *pre_, int batch, int units_, long long g_, long long end_)
-      : g(g_), end(end_), pre(pre_), units(units_) {
-    int lo = 0, hi = batch - 1;  // the last sequence that starts at or before g
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((long long)pre[mid] * units <= g) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
-  }
-  __device__ bool next() {
-    if (g >= end) return false;
-    while ((long long)pre[b + 1] * units <= g) ++b;
-    tiles = pre[b + 1] - pre[b];
-    const long long rel = g - (long long)pre[b] * units;
-    unit = (int)(rel / tiles);
-    tile = (int)(rel - (long long)unit * tiles);
-    count = (int)min((long long)(tiles - tile), end - g);
-    g += count;
-    return true;
-  }
+  int32_t len[PLAN_BATCH];
+  int32_t pre[PLAN_BATCH + 1];  // tiles of the sequences before (one unit's worth)
 };
 
 // Order of a segment's 2n operand tiles in the ring: K0, K1, V0, K2, V1, ...,
@@ -232,7 +165,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   const int units = a.heads * a.mtiles;
 
   if (warp == 0) {
-    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, s.len, s.pre);
+    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1, s.len, s.pre);
     if (lane == 0 && !C::F8) {
       tma_prefetch_map(&maps.k);
       tma_prefetch_map(&maps.v);
@@ -707,13 +640,13 @@ constexpr int TC_THREADS = 256, TC_MAX = 512;  // most CTAs of the attention ker
 template <int D, int KT>
 __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int ctas) {
   constexpr int LANES = D / 4, GROUPS = TC_THREADS / LANES;
-  __shared__ int32_t s_pre[TR_BATCH + 1];
+  __shared__ int32_t s_pre[PLAN_BATCH + 1];
   __shared__ float s_w[TC_MAX];
   __shared__ float s_red[2][TC_THREADS / 32];
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ int s_dead;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, nullptr, s_pre);
+  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1, nullptr, s_pre);
   if (tid == 0) s_dead = 0;
   __syncthreads();
   const int rows = a.n * a.group;
@@ -824,7 +757,7 @@ int sm_count(int device, int *sms) {
 int64_t tree_workspace(int sms, const SkvTree *d) {
   const int64_t rows = d->n * (d->heads / d->kv_heads), per = rows < TR_ROWS ? rows : TR_ROWS;
   const int64_t units = d->kv_heads * ((rows + TR_ROWS - 1) / TR_ROWS);
-  const int64_t batch = d->batch < TR_BATCH ? d->batch : TR_BATCH;
+  const int64_t batch = d->batch < PLAN_BATCH ? d->batch : PLAN_BATCH;
   const int64_t slots = 2 * (int64_t)tree_ctas(sms, batch, units, d->tokens, d->dim);
   return slots * per * (d->dim + 2) * 4;
 }
@@ -891,8 +824,8 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
     a.k8s[i] = d->k_cache_stride[i], a.v8s[i] = d->v_cache_stride[i];
   }
   a.ps[0] = d->parents_stride[0], a.ps[1] = d->parents_stride[1];
-  for (int64_t b0 = 0; b0 < d->batch; b0 += TR_BATCH) {
-    const int64_t nb = d->batch - b0 < TR_BATCH ? d->batch - b0 : TR_BATCH;
+  for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
+    const int64_t nb = d->batch - b0 < PLAN_BATCH ? d->batch - b0 : PLAN_BATCH;
     a.batch = (int)nb;
     a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0];
     a.kn = static_cast<const uint16_t *>(d->k) + b0 * a.kns[0];

@@ -1,0 +1,425 @@
+// skv_weights.cu -- attention weights accumulated per cached key.
+//
+//   out[t] = w[t] + sum over the rows r of a KV head of exp(scale q_r.k_t - lse_r)
+//
+// for t below the sequence's length; elsewhere out[t] = w[t].  With the rows'
+// log-sum-exp known, a key's sum needs no other key: one pass over K.
+//
+// The product runs on tcgen05 with the keys as M = 128 lanes and the rows as
+// N: every thread of the epilogue then holds one key's scores in its own lane
+// and sums their exponentials without a word to its neighbours, in a fixed
+// order.  A tile's K arrives as pieces of 128 keys x 64 dimensions (16 KB), so
+// that the ring stays deep beside up to 128 KB of queries in shared memory;
+// the accumulator (FP32, tensor memory) is double-buffered against two
+// epilogue groups.  CTAs take contiguous ranges of the list of all tiles.
+#include <cuda_bf16.h>
+
+#include "skv_ops.cuh"
+#include "skv_plan.cuh"
+#include "skv_tensor.cuh"
+
+namespace skv {
+namespace {
+
+constexpr int WT_KEYS = 128, WT_PIECE = WT_KEYS * 128;  // bytes of a piece
+constexpr int WT_ROWS = 256;                            // rows of one launch: the MMA's largest N
+constexpr int WT_STAGES = 12;
+constexpr int WT_RAW = 6;                               // FP8 pieces in flight
+constexpr int WT_THREADS = 384, WT_THREADS_F8 = 640;
+
+struct WeightsArgs {
+  const uint16_t *q;
+  int64_t qs[3];  // element strides (sequence, node, head)
+  const uint8_t *k8;
+  int64_t k8s[3];  // FP8 cache: byte strides (sequence, head, token)
+  const int32_t *lengths;
+  int64_t len_stride;
+  const float *lse;
+  int64_t ls[3];  // (sequence, node, head)
+  const uint8_t *take;  // [sequence][node]: rows that count (null: all)
+  int64_t ts[2];
+  const float *w;
+  float *out;
+  int64_t ws[3], os[3];  // (sequence, head, token)
+  int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head; cols: rows up to 16s
+  int32_t along[2];
+  int32_t stages;
+  float c2;
+  uint32_t *status;
+};
+
+struct WeightsSmem {
+  uint64_t full[WT_STAGES], empty[WT_STAGES];
+  uint64_t q_ready, q_free, acc_full[2], acc_free[2], drain;
+  uint32_t tmem, abort;
+  alignas(16) float lse2[2][WT_ROWS];  // log2(e) * lse, +inf for rows that do not count
+  int32_t len[PLAN_BATCH];
+  int32_t pre[PLAN_BATCH + 1];
+};
+
+template <int D, bool F8>
+__global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
+    k_weights(const __grid_constant__ CUtensorMap map, const __grid_constant__ WeightsArgs a) {
+  constexpr int SUB = D / 64;
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t *queries = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;  // [SUB][cols][128 bytes], swizzled
+  uint8_t *ring = queries + SUB * a.cols * 128;
+  uint8_t *raw = ring + a.stages * WT_PIECE;
+  WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(raw + (F8 ? WT_RAW * WT_PIECE / 2 : 0));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int stages = a.stages;
+  if (warp == 0) {
+    tile_prefix<WT_KEYS>(a.lengths, a.len_stride, 0, a.t, a.batch, 0, s.len, s.pre);
+    if (lane == 0 && !F8) tma_prefetch_map(&map);
+  } else if (warp == 1) {
+    tmem_alloc(&s.tmem, 512);
+  } else if (warp == 2 && lane == 0) {
+    for (int i = 0; i < stages; ++i) {
+      bar_init(&s.full[i], F8 ? 8 : 1);
+      bar_init(&s.empty[i], 1);
+    }
+    bar_init(&s.q_ready, 8);
+    bar_init(&s.q_free, 1);
+    bar_init(&s.drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.acc_full[i], 1);
+      bar_init(&s.acc_free[i], 4);
+    }
+    bar_init_fence();
+    s.abort = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *(volatile uint32_t *)&s.tmem;
+  volatile uint32_t *abort = &s.abort;
+  const long long total = (long long)s.pre[a.batch] * a.heads;
+  const Plan plan{total, (int)min((long long)gridDim.x, total)};
+  const int cta = blockIdx.x;
+  const long long g_begin = cta < plan.ctas ? plan.begin(cta) : 0, g_end = cta < plan.ctas ? plan.begin(cta + 1) : 0;
+  auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
+
+  if (warp == 0 && !F8) {
+    // ---- loads
+    if (lane == 0) {
+      Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+      uint32_t seq = 0;
+      int stage = 0;
+      uint32_t turn = 0;
+      bool ok = true;
+      while (ok && w.next())
+        for (int i = 0; i < w.count && ok; ++i)
+          for (int sub = 0; sub < SUB; ++sub) {
+            if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
+            bar_expect(&s.full[stage], WT_PIECE);
+            tma_load(ring + stage * WT_PIECE, &map, sub * 64, (w.tile + i) * WT_KEYS, w.unit * a.along[0],
+                     w.b * a.along[1], &s.full[stage]);
+            ++seq;
+            if (++stage == stages) stage = 0, turn ^= 1;
+          }
+      if (!ok)  // gave up: the copies in flight still land before the CTA ends
+        for (uint32_t back = 1; back <= (uint32_t)stages && back <= seq; ++back) {
+          const uint32_t q = seq - back;
+          const unsigned long long t0 = timer_ns();
+          while (!bar_try(&s.full[q % stages], (q / stages) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+          }
+        }
+    }
+  } else if (warp == 1) {
+    // ---- tensor core
+    if (lane == 0) {
+      Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+      const uint32_t desc = mma_desc(WT_KEYS, a.cols, false);
+      const uint32_t q0 = s_addr(queries);
+      int stage = 0;
+      uint32_t turn = 0, gt = 0, seg = 0;
+      while (w.next()) {
+        wait(&s.q_ready, seg & 1);
+        for (int i = 0; i < w.count; ++i, ++gt) {
+          const uint32_t buf = gt & 1;
+          wait(&s.acc_free[buf], ((gt >> 1) & 1) ^ 1);
+          for (int sub = 0; sub < SUB; ++sub) {
+            wait(&s.full[stage], turn);
+            tc_fence_after();
+            const uint32_t k0 = s_addr(ring + stage * WT_PIECE), qs = q0 + sub * a.cols * 128;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma_ss(tmem + buf * WT_ROWS, smem_desc(k0 + ks * 32, 16), smem_desc(qs + ks * 32, 16), desc, sub + ks > 0);
+            mma_commit(&s.empty[stage]);
+            if (++stage == stages) stage = 0, turn ^= 1;
+          }
+          mma_commit(&s.acc_full[buf]);
+        }
+        mma_commit(&s.q_free);
+        ++seg;
+      }
+      if (*abort) {  // what was issued ends before tensor memory is given back
+        mma_commit(&s.drain);
+        const unsigned long long t0 = timer_ns();
+        while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
+        }
+      }
+    }
+  } else if (warp < 4) {
+    // ---- tokens behind the lengths keep their weights
+    if (a.w != a.out) {
+      const int pairs = a.batch * a.heads, ctas = (int)gridDim.x;
+      const int share = ctas > pairs ? ctas / pairs : 1;  // CTAs of one (sequence, head)
+      for (int p = cta / share; p < pairs; p += (ctas + share - 1) / share) {
+        const int b = p / a.heads, h = p - b * a.heads;
+        const float *w = a.w + b * a.ws[0] + h * a.ws[1];
+        float *o = a.out + b * a.os[0] + h * a.os[1];
+        for (int t = s.len[b] + (cta % share) * 64 + tid - 64; t < a.t; t += share * 64) o[t * a.os[2]] = w[t * a.ws[2]];
+      }
+    }
+  } else if (warp < 12) {
+    // ---- epilogue: one key per thread, tiles in turn between the two groups
+    const int et = tid - 128, half = (warp - 4) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)((warp - 4) & 3) << 21) + half * WT_ROWS;
+    Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+    uint32_t gt = 0, seg = 0;
+    while (w.next()) {
+      const int h = w.unit;
+      // the head's rows, once the tensor core is done with the ones before
+      if (seg) wait(&s.q_free, (seg - 1) & 1);
+      for (int x = et; x < a.cols * (D / 8); x += 256) {
+        const int r = x / (D / 8), c16 = x % (D / 8), row = a.row0 + r;
+        const int node = row / a.group, qh = h * a.group + row - node * a.group;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]]) &&
+            a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]] != -INFINITY)
+          v = __ldg(reinterpret_cast<const uint4 *>(a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2]) + c16);
+        *reinterpret_cast<uint4 *>(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16) = v;
+      }
+      if (et < a.cols) {
+        float l2 = INFINITY;
+        const int row = a.row0 + et, node = row / a.group, qh = h * a.group + row - node * a.group;
+        if (et < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]])) {
+          const float l = a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]];
+          if (l != -INFINITY) l2 = l * 1.4426950408889634f;  // (-inf: a row that saw nothing)
+        }
+        s.lse2[seg & 1][et] = l2;
+      }
+      async_fence();
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (lane == 0) bar_arrive(&s.q_ready);
+      const float4 *lse2 = reinterpret_cast<const float4 *>(s.lse2[seg & 1]);
+      const float *wrow = a.w + w.b * a.ws[0] + h * a.ws[1];
+      float *orow = a.out + w.b * a.os[0] + h * a.os[1];
+      for (int i = 0; i < w.count; ++i, ++gt) {
+        if ((gt & 1) != (uint32_t)half) continue;
+        const int t = (w.tile + i) * WT_KEYS + (et & 127);
+        const bool on = t < s.len[w.b];
+        const float before = on ? wrow[t * a.ws[2]] : 0.0f;
+        wait(&s.acc_full[half], (gt >> 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        float sum[4] = {0, 0, 0, 0};
+        for (int c = 0; c < a.cols; c += 16) {
+          uint32_t x[16];
+          tmem_ld16(x, lanes + c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 l = lse2[c / 4 + j];
+            sum[0] += exp2_fast(fmaf(__uint_as_float(x[4 * j]), a.c2, -l.x));
+            sum[1] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 1]), a.c2, -l.y));
+            sum[2] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 2]), a.c2, -l.z));
+            sum[3] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 3]), a.c2, -l.w));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.acc_free[half]);
+        float add = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (*abort) add = __uint_as_float(0x7fffffffu);
+        if (on) orow[t * a.os[2]] = before + add;
+      }
+      ++seg;
+    }
+  } else if (F8) {
+    // ---- FP8 caches: pieces copied ahead with cp.async, each thread its own
+    // 16 codes, turned into BF16 where TMA would have put a BF16 piece
+    constexpr int CHUNKS = WT_PIECE / 2 / 16 / 256;  // of one thread and piece
+    const int ct = tid - 384;
+    struct Items {
+      Walk w;
+      int tile = 0, sub = 0;
+      bool live;
+      __device__ Items(const Walk &x) : w(x) { live = w.next(); }
+      __device__ void step() {
+        if (++sub < SUB) return;
+        sub = 0;
+        if (++tile < w.count) return;
+        tile = 0;
+        live = w.next();
+      }
+    };
+    Items ahead(Walk(s.pre, a.batch, a.heads, g_begin, g_end)), now = ahead;
+    auto issue = [&](const Items &it, int slot) {
+      if (it.live) {
+        const uint8_t *src = a.k8 + it.w.b * a.k8s[0] + it.w.unit * a.k8s[1] + it.sub * 64;
+        const int t0 = (it.w.tile + it.tile) * WT_KEYS, len = s.len[it.w.b];
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) {
+          const int c = ct + j * 256, key = c / 4;
+          if (t0 + key < len) cp_async16(raw + slot * (WT_PIECE / 2) + c * 16, src + (t0 + key) * a.k8s[2] + (c % 4) * 16);
+        }
+      }
+      cp_async_commit();
+    };
+    for (int i = 0; i < WT_RAW; ++i) {
+      issue(ahead, i);
+      if (ahead.live) ahead.step();
+    }
+    int stage = 0, slot = 0;
+    uint32_t turn = 0;
+    while (now.live) {
+      const int left = s.len[now.w.b] - (now.w.tile + now.tile) * WT_KEYS;
+      uint4 v[CHUNKS];
+      cp_async_wait<WT_RAW - 1>();
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        const int c = ct + j * 256;
+        v[j] = c / 4 < left ? *reinterpret_cast<const uint4 *>(raw + slot * (WT_PIECE / 2) + c * 16) : make_uint4(0, 0, 0, 0);
+      }
+      issue(ahead, slot);
+      if (ahead.live) ahead.step();
+      if (!wait(&s.empty[stage], turn ^ 1)) break;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        const int c = ct + j * 256, key = c / 4, c16 = 2 * (c % 4);
+        const uint32_t *x = reinterpret_cast<const uint32_t *>(&v[j]);
+        uint4 y[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          y[u] = make_uint4(e4m3x2_to_bf16x2((uint16_t)x[2 * u]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u] >> 16)),
+                            e4m3x2_to_bf16x2((uint16_t)x[2 * u + 1]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u + 1] >> 16)));
+        // (eight neighbouring threads are two keys, whose swizzles differ: all banks differ)
+        uint8_t *line = ring + stage * WT_PIECE + key * 128;
+        *reinterpret_cast<uint4 *>(line + (c16 ^ (key & 7)) * 16) = y[0];
+        *reinterpret_cast<uint4 *>(line + ((c16 + 1) ^ (key & 7)) * 16) = y[1];
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&s.full[stage]);
+      now.step();
+      if (++stage == stages) stage = 0, turn ^= 1;
+      if (++slot == WT_RAW) slot = 0;
+    }
+    cp_async_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+template <int D, bool F8>
+int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, cudaStream_t st) {
+  constexpr int most = 232448, fixed = 1024 + (int)sizeof(WeightsSmem) + (F8 ? WT_RAW * WT_PIECE / 2 : 0);
+  const int rows = (D / 64) * a.cols * 128;
+  int stages = (most - fixed - rows) / WT_PIECE;
+  a.stages = stages < WT_STAGES ? stages : WT_STAGES;
+  const int smem = fixed + rows + a.stages * WT_PIECE;
+  auto *kernel = &k_weights<D, F8>;
+  if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
+                       "k_weights shared memory"))
+    return rc;
+  const int64_t tiles = (int64_t)a.batch * a.heads * ((a.t + WT_KEYS - 1) / WT_KEYS);
+  const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
+  return op_cuda(op_launch(kernel, dim3(grid), dim3(F8 ? WT_THREADS_F8 : WT_THREADS), smem, st, false, 1, map, a),
+                 "k_weights launch");
+}
+
+template <bool F8>
+int launch_weights_d(int d, const CUtensorMap &map, WeightsArgs &a, int sms, cudaStream_t st) {
+  if (d == 64) return launch_weights<64, F8>(map, a, sms, st);
+  if (d == 128) return launch_weights<128, F8>(map, a, sms, st);
+  return launch_weights<256, F8>(map, a, sms, st);
+}
+
+}  // namespace
+}  // namespace skv
+
+extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
+  using namespace skv;
+  if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
+  if (d->dim != 64 && d->dim != 128 && d->dim != 256) return op_fail(SKV_E_INVALID, "head size must be 64, 128 or 256");
+  if (d->batch < 0 || d->n < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096 ||
+      d->n > (1 << 20) || d->batch > (1 << 20))
+    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, counts in range");
+  if (d->tokens < 1 || d->tokens > (1 << 26)) return op_fail(SKV_E_INVALID, "tokens must be in [1, 2^26]");
+  if (!(d->scale > 0.0) || !(d->scale < 1e30)) return op_fail(SKV_E_INVALID, "scale must be positive and finite");
+  if (d->cache_dtype != SKV_DTYPE_BF16 && d->cache_dtype != SKV_DTYPE_E4M3)
+    return op_fail(SKV_E_INVALID, "the cache is BF16 or FP8 e4m3");
+  if (d->batch == 0) return SKV_OK;
+  if (!d->q || !d->k_cache || !d->lengths || !d->lse || !d->weights || !d->weights_out)
+    return op_fail(SKV_E_INVALID, "null input or output pointer");
+  const bool f8 = d->cache_dtype == SKV_DTYPE_E4M3;
+  auto aligned = [&](const void *p, const int64_t *s, int64_t unit) {
+    if ((uintptr_t)p % 16) return false;
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || s[i] % unit) return false;
+    return true;
+  };
+  if (!aligned(d->q, d->q_stride, 8) || !aligned(d->k_cache, d->k_cache_stride, f8 ? 16 : 8))
+    return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
+  if (d->tokens > 1 && !d->k_cache_stride[2]) return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  DeviceScope scope((int)d->device);
+  if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
+  int sms = 0;
+  if (int rc = op_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, (int)d->device), "device attribute"))
+    return rc;
+  WeightsArgs a{};
+  if (int rc = status_word((int)d->device, &a.status)) return rc;
+  const int group = (int)(d->heads / d->kv_heads);
+  a.heads = (int)d->kv_heads, a.group = group, a.t = (int)d->tokens;
+  a.c2 = (float)(d->scale * 1.4426950408889634);
+  a.len_stride = d->lengths_stride;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = d->q_stride[i], a.k8s[i] = d->k_cache_stride[i], a.ls[i] = d->lse_stride[i];
+    a.os[i] = d->weights_out_stride[i];
+  }
+  a.ts[0] = d->rows_stride[0], a.ts[1] = d->rows_stride[1];
+  const int64_t rows = d->n * group;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
+    const int64_t nb = d->batch - b0 < PLAN_BATCH ? d->batch - b0 : PLAN_BATCH;
+    a.batch = (int)nb;
+    a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0];
+    a.lengths = static_cast<const int32_t *>(d->lengths) + b0 * a.len_stride;
+    a.lse = static_cast<const float *>(d->lse) + b0 * a.ls[0];
+    a.take = d->rows ? static_cast<const uint8_t *>(d->rows) + b0 * a.ts[0] : nullptr;
+    a.out = static_cast<float *>(d->weights_out) + b0 * a.os[0];
+    CUtensorMap map{};
+    if (f8) {
+      a.k8 = static_cast<const uint8_t *>(d->k_cache) + b0 * a.k8s[0];
+    } else {
+      const int64_t step[3] = {d->k_cache_stride[2], d->k_cache_stride[1], d->k_cache_stride[0]};
+      if (int rc = make_map(&map, static_cast<const uint16_t *>(d->k_cache) + b0 * d->k_cache_stride[0], d->dim, d->tokens,
+                            d->kv_heads, nb, step, WT_KEYS))
+        return rc;
+      a.along[0] = d->kv_heads > 1 && d->k_cache_stride[1] ? 1 : 0;
+      a.along[1] = nb > 1 && d->k_cache_stride[0] ? 1 : 0;
+    }
+    // more rows than the MMA's N: further launches add to what the first wrote
+    for (int64_t r0 = 0; r0 < rows; r0 += WT_ROWS) {
+      a.row0 = (int)r0;
+      a.rows = (int)(rows - r0 < WT_ROWS ? rows - r0 : WT_ROWS);
+      a.cols = (a.rows + 15) & ~15;
+      if (r0 == 0) {
+        a.w = static_cast<const float *>(d->weights) + b0 * d->weights_stride[0];
+        for (int i = 0; i < 3; ++i) a.ws[i] = d->weights_stride[i];
+      } else {
+        a.w = a.out;
+        for (int i = 0; i < 3; ++i) a.ws[i] = a.os[i];
+      }
+      const int rc = f8 ? launch_weights_d<true>((int)d->dim, map, a, sms, st) : launch_weights_d<false>((int)d->dim, map, a, sms, st);
+      if (rc) return rc;
+    }
+  }
+  return SKV_OK;
+}

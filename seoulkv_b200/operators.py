@@ -324,6 +324,61 @@ def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: i
     return max(16, size.value)
 
 
+# ---------------------------------------------------------------- accumulated weights
+
+
+_WEIGHTS = struct.Struct("7Qd" + 8 * "q" + 18 * "q")
+
+
+def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Tensor, lse: torch.Tensor,
+                       weights: torch.Tensor, *, rows: torch.Tensor | None = None, scale: float | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Add the attention that rows of queries pay to each cached key to the keys' weights.
+
+    weights[b, h, t] + sum over nodes and the query heads of KV head h of
+    exp(scale q.k_t - lse) for t < lengths[b]; later tokens keep their weight.
+    ``q`` BF16 [B, N, Hq, D] and ``lse`` FP32 [B, N, Hq] as given to and
+    returned by ``tree_attention`` (N is not limited here: a window of prompt
+    tokens with their log-sum-exp works as well), ``k_cache`` and ``lengths``
+    as there, ``weights`` FP32 [B, Hkv, T].  ``rows`` (bool [B, N]) names the
+    nodes that count, the accepted ones; a row whose lse is -inf never counts.
+
+    Returns a new tensor, or ``out``, which may be ``weights`` itself
+    (otherwise it must not overlap it).
+    """
+    _check_cache(k_cache, None, lengths)
+    b, hkv, t, d = k_cache.shape
+    dev = k_cache.device
+    _check("q", q, (b, None, None, d), (torch.bfloat16,), dev)
+    n, hq = q.shape[1], q.shape[2]
+    if n < 1 or hq < 1 or hq % hkv:
+        raise ValueError("q: expected at least one node, and query heads a multiple of the KV heads")
+    _rows("q", q)
+    _check("lse", lse, (b, n, hq), (torch.float32,), dev)
+    _check("weights", weights, (b, hkv, t), (torch.float32,), dev)
+    if rows is not None:
+        _check("rows", rows, (b, n), (torch.bool,), dev)
+    s = _scale(scale, d)
+    if out is None:
+        out = torch.empty((b, hkv, t), dtype=torch.float32, device=dev)
+    else:
+        _check("out", out, (b, hkv, t), (torch.float32,), dev)
+        if any(x == 0 and size > 1 for x, size in zip(out.stride(), out.shape)):
+            raise ValueError("out: two elements share one place")
+        if not (out.data_ptr() == weights.data_ptr() and out.stride() == weights.stride()) and _overlap(out, weights):
+            raise ValueError("out overlaps weights without being it")
+    if not b:
+        return out
+    packed = _WEIGHTS.pack(
+        q.data_ptr(), k_cache.data_ptr(), lengths.data_ptr(), lse.data_ptr(), 0 if rows is None else rows.data_ptr(),
+        weights.data_ptr(), out.data_ptr(), s, dev.index, _DTYPE[k_cache.dtype], b, n, hq, hkv, d, t,
+        *_steps(q, (0, 1, 2)), *_steps(k_cache, (0, 1, 2)), *_steps(lse, (0, 1, 2)),
+        *((0, 0) if rows is None else _steps(rows, (0, 1))), *_steps(weights, (0, 1, 2)), *_steps(out, (0, 1, 2)),
+        *_steps(lengths, (0,)))
+    _run(_native.load().skv_accumulate_weights, packed, dev, "accumulate_weights")
+    return out
+
+
 # ---------------------------------------------------------------- eviction
 
 
