@@ -1,5 +1,5 @@
 // skv_plan.cuh -- the list of key tiles that the attention operators work
-// through, cut into one contiguous range per CTA.
+// through, cut into contiguous ranges (items).
 #pragma once
 #include <cstdint>
 
@@ -7,18 +7,22 @@ namespace skv {
 
 constexpr int PLAN_BATCH = 512;  // sequences of one launch (their tile counts are kept in shared memory)
 
+// The list: sequence after sequence, unit (KV head) after unit, tile after
+// tile; every unit ends with `idle` places that stand for its fixed cost.
 struct Plan {
-  long long total;  // tiles of all units
-  int ctas;         // CTAs that have a range
-  __host__ __device__ long long begin(int c) const { return total * c / ctas; }
-  // the CTA whose range holds tile g
-  __host__ __device__ int owner(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
+  long long total;  // places in the list
+  int items;        // ranges that are not empty
+  __device__ Plan(long long total_, int items_) : total(total_), items((int)min((long long)items_, total_)) {}
+  __device__ long long begin(int i) const { return i < items ? total * i / items : total; }
+  // the item whose range holds place g
+  __device__ int owner(long long g) const { return (int)(((g + 1) * items - 1) / total); }
 };
 
-// pre[b] and len[b] by one warp: KT cached tokens a tile, and `extra` tiles more.
+// pre[b] (places of the sequences before b, one unit's worth) and len[b], by
+// one warp: KT cached tokens a tile, and `extra` places more.
 template <int KT>
-__device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch, int extra,
-                                            int32_t *len, int32_t *pre) {
+__device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch,
+                                            int extra, int32_t *len, int32_t *pre) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   for (int b0 = 0; b0 < batch; b0 += 32) {
@@ -44,14 +48,15 @@ __device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stri
   if (lane == 0) pre[0] = 0;
 }
 
-// The segments of [g, end): tiles [tile, tile + count) of one unit.
+// The segments of places [g, end): tiles [tile, tile + count) of one unit of
+// `tiles`, at place `start`.
 struct Walk {
-  long long g, end;
+  long long g, end, start = 0;
   const int32_t *pre;
-  int units;  // per sequence
+  int units, idle;  // units per sequence
   int b = 0, unit = 0, tile = 0, count = 0, tiles = 0;
-  __device__ Walk(const int32_t *pre_, int batch, int units_, long long g_, long long end_)
-      : g(g_), end(end_), pre(pre_), units(units_) {
+  __device__ Walk(const int32_t *pre_, int batch, int units_, int idle_, long long g_, long long end_)
+      : g(g_), end(end_), pre(pre_), units(units_), idle(idle_) {
     int lo = 0, hi = batch - 1;  // the last sequence that starts at or before g
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -60,15 +65,19 @@ struct Walk {
     b = lo;
   }
   __device__ bool next() {
-    if (g >= end) return false;
-    while ((long long)pre[b + 1] * units <= g) ++b;
-    tiles = pre[b + 1] - pre[b];
-    const long long rel = g - (long long)pre[b] * units;
-    unit = (int)(rel / tiles);
-    tile = (int)(rel - (long long)unit * tiles);
-    count = (int)min((long long)(tiles - tile), end - g);
-    g += count;
-    return true;
+    while (g < end) {
+      while ((long long)pre[b + 1] * units <= g) ++b;
+      const int places = pre[b + 1] - pre[b];
+      const long long rel = g - (long long)pre[b] * units;
+      unit = (int)(rel / places);
+      tile = (int)(rel - (long long)unit * places);
+      start = g - tile;
+      tiles = places - idle;
+      g = min(end, start + places);
+      count = min(tiles, (int)(g - start)) - tile;
+      if (count > 0) return true;
+    }
+    return false;
   }
 };
 

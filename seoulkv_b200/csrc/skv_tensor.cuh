@@ -68,13 +68,13 @@ __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// Box at (x elements, row, y, z) of a 4-d map; x is a multiple of 64 elements here.
-__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int row, int y, int z,
+// Box at (row, piece, y, z) of a make_map() map.
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int row, int piece, int y, int z,
                                          uint64_t *bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(s_addr(dst)),
-      "l"(map), "r"(x), "r"(row), "r"(y), "r"(z), "r"(s_addr(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(s_addr(dst)),
+      "l"(map), "r"(0), "r"(row), "r"(piece), "r"(y), "r"(z), "r"(s_addr(bar))
       : "memory");
 }
 
@@ -195,11 +195,13 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // ---- host: tensor maps and the status word (skv_tree.cu) -------------------
 
-// 4-d map [z][y][rows][dim] of 16-bit elements with element strides
-// {row, y, z}; boxes of box_rows rows x 64 elements, 128-byte swizzle.  A
-// dimension of one element, or of stride 0, is mapped with one element.
+// Map of [z][y][rows][dim] 16-bit elements with element strides {row, y, z},
+// taken as pieces of 64 elements: a box is `box_rows` rows of `pieces` pieces,
+// in shared memory piece after piece, each a stack of 128-byte rows with the
+// 128-byte swizzle.  A dimension of one element, or of stride 0, is mapped
+// with one element.
 int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
-             const int64_t *stride, int box_rows);
+             const int64_t *stride, int box_rows, int pieces);
 // The device's status word (set by waits that gave up).
 int status_word(int device, uint32_t **word);
 

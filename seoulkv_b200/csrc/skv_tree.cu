@@ -51,7 +51,7 @@ int status_word(int device, uint32_t **word) {
 }
 
 int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
-             const int64_t *stride, int box_rows) {
+             const int64_t *stride, int box_rows, int pieces) {
   using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -65,14 +65,15 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
   }();
   if (!encode) return op_fail(SKV_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
   const int64_t n[3] = {rows, ny, nz};
-  cuuint64_t size[4] = {(cuuint64_t)dim, 1, 1, 1}, step[3];
+  cuuint64_t size[5] = {64, 1, (cuuint64_t)dim / 64, 1, 1}, step[4] = {0, 128, 0, 0};
   for (int i = 0; i < 3; ++i) {
     const bool one = n[i] == 1 || stride[i] == 0;
-    size[i + 1] = one ? 1 : (cuuint64_t)n[i];
-    step[i] = one ? (cuuint64_t)dim * 2 : (cuuint64_t)stride[i] * 2;
+    const int at = i ? i + 2 : 1;
+    size[at] = one ? 1 : (cuuint64_t)n[i];
+    step[at - 1] = one ? (cuuint64_t)dim * 2 : (cuuint64_t)stride[i] * 2;
   }
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, unit[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), size, step, box, unit,
+  const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)pieces, 1, 1}, unit[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void *>(base), size, step, box, unit,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SKV_OK : op_fail(SKV_E_INVALID, "cuTensorMapEncodeTiled: error %d", (int)r);
@@ -82,6 +83,7 @@ namespace {
 
 constexpr int TR_NODES = SKV_TREE_MAX_NODES;
 constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
+constexpr int TR_IDLE = 2;     // what starting and ending a unit costs, in tiles
 
 template <int D_, bool F8_>
 struct TreeCfg {
@@ -130,7 +132,7 @@ struct TreeArgs {
 template <class C>
 struct TreeSmem {
   uint64_t full[C::NSTAGE], empty[C::NSTAGE];
-  uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;  // (by tile parity: S(g) follows O(g - 2), so a wait is at most one phase behind)
+  uint64_t q_ready, p_ready[2], drain;
   uint64_t anc[TR_NODES];   // nodes that node i sees (0: unused)
   unsigned long long bad;   // nodes with a value that is not finite
   int32_t up[TR_NODES];
@@ -162,10 +164,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   uint8_t *raw = ring + C::NSTAGE * C::STAGE;
   TreeSmem<C> &s = *reinterpret_cast<TreeSmem<C> *>(ring + C::RING);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int units = a.heads * a.mtiles;
 
   if (warp == 0) {
-    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1, s.len, s.pre);
+    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, s.len, s.pre);
     if (lane == 0 && !C::F8) {
       tma_prefetch_map(&maps.k);
       tma_prefetch_map(&maps.v);
@@ -181,11 +182,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
     bar_init(&s.q_ready, 4);
     bar_init(&s.drain, 1);
-    for (int i = 0; i < 2; ++i) {
-      bar_init(&s.s_full[i], 1);
-      bar_init(&s.o_done[i], 1);
-      bar_init(&s.p_ready[i], 4);
-    }
+    for (int i = 0; i < 2; ++i) bar_init(&s.p_ready[i], 4);
     bar_init_fence();
     s.abort = 0;
     s.bad = 0;
@@ -196,19 +193,21 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   grid_dependency_release();
   const uint32_t tmem = *(volatile uint32_t *)&s.tmem;
   volatile uint32_t *abort = &s.abort;
-  const Plan plan{(long long)s.pre[a.batch] * units, (int)min((long long)gridDim.x, (long long)s.pre[a.batch] * units)};
-  const int cta = blockIdx.x;
-  const long long g_begin = cta < plan.ctas ? plan.begin(cta) : 0, g_end = cta < plan.ctas ? plan.begin(cta + 1) : 0;
+  // CTA: item (blockIdx / mtiles) of the list for one 128-row part of its
+  // units; the parts of an item are neighbours, so that they read the same
+  // keys at the same time and HBM delivers them once
+  const Plan plan((long long)s.pre[a.batch] * a.heads, (int)gridDim.x / a.mtiles);
+  const int item = blockIdx.x / a.mtiles, mt = blockIdx.x % a.mtiles;
+  const Walk walk(s.pre, a.batch, a.heads, TR_IDLE, plan.begin(item), plan.begin(item + 1));
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
 
   if (warp == 0 && !C::F8) {
     // ---- loads
     if (lane == 0) {
-      Walk w(s.pre, a.batch, units, g_begin, g_end);
+      Walk w = walk;
       uint32_t seq = 0;
       bool ok = true;
       while (ok && w.next()) {
-        const int h = w.unit / a.mtiles;
         for (int p = 0; p < 2 * w.count; ++p, ++seq) {
           bool is_v;
           int i;
@@ -220,10 +219,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
           const int row = nodes ? 0 : (w.tile + i) * KT;
           bar_expect(&s.full[stage], C::STAGE);
-#pragma unroll
-          for (int sub = 0; sub < C::SUB; ++sub)
-            tma_load(ring + stage * C::STAGE + sub * KT * 128, map, sub * 64, row, h * a.along[which][0],
-                     w.b * a.along[which][1], &s.full[stage]);
+          tma_load(ring + stage * C::STAGE, map, row, 0, w.unit * a.along[which][0], w.b * a.along[which][1],
+                   &s.full[stage]);
         }
       }
       if (!ok)  // gave up: the copies in flight still land before the CTA ends
@@ -237,7 +234,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   } else if (warp == 1) {
     // ---- tensor core
     if (lane == 0) {
-      Walk w(s.pre, a.batch, units, g_begin, g_end);
+      Walk w = walk;
       constexpr uint32_t DESC_S = mma_desc(TR_ROWS, KT, false), DESC_O = mma_desc(TR_ROWS, D, true);
       uint32_t base = 0, gt = 0, seg = 0;
       while (w.next()) {
@@ -252,7 +249,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           for (int ks = 0; ks < D / 16; ++ks)
             mma_ts(d, tmem + C::COL_Q + 8 * ks, smem_desc(k0 + (ks / 4) * KT * 128 + (ks % 4) * 32, 16), DESC_S, ks > 0);
           mma_commit(&s.empty[stage]);
-          mma_commit(&s.s_full[(gt + i) & 1]);
         };
         wait(&s.q_ready, seg & 1);
         tc_fence_after();
@@ -269,7 +265,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           for (int ks = 0; ks < KT / 16; ++ks)
             mma_ts(tmem, tmem + C::COL_S + buf * KT + 8 * ks, smem_desc(v0 + ks * 2048, KT * 128), DESC_O, i > 0 || ks > 0);
           mma_commit(&s.empty[stage]);
-          mma_commit(&s.o_done[buf]);
         }
         base += 2 * n;
         gt += n;
@@ -286,11 +281,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // ---- softmax: one row per thread
     const int row = tid - 128;
     const uint32_t lanes = tmem + ((uint32_t)(warp - 4) << 21);  // this warp's 32 lanes (bits 16..)
-    Walk w(s.pre, a.batch, units, g_begin, g_end);
+    Walk w = walk;
     uint32_t base = 0, gt = 0;
-    bool first = true;
+    // The product that used an operand tile is done: S(i) with K(i), O(i) with
+    // V(i).  The stage's use before is older than what this thread has seen
+    // done, so that the parity names this use.
+    auto used = [&](uint32_t at) { wait(&s.empty[at % C::NSTAGE], (at / C::NSTAGE) & 1); };
     while (w.next()) {
-      const int n = w.count, h = w.unit / a.mtiles, mt = w.unit - h * a.mtiles;
+      const int n = w.count, h = w.unit;
       const int r = mt * TR_ROWS + row;                 // row of the KV head
       const int left = a.n * a.group - mt * TR_ROWS;    // rows of this unit
       const bool warp_on = 32 * (warp - 4) < left, on = row < left;
@@ -357,7 +355,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const int v = valid - 64 * j;
           keep[j] = nodes ? (j ? 0 : see) : v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
         }
-        wait(&s.s_full[buf], ((gt + i) >> 1) & 1);
+        used(base + pos_k(i));
         __syncwarp();
         tc_fence_after();
         if (warp_on) {
@@ -383,7 +381,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const bool move = i == 0 || top > m + 8.0f;
           if (i > 0 && __any_sync(0xffffffffu, move)) {
             const float f = move ? exp2_fast(m - top) : 1.0f;
-            wait(&s.o_done[buf ^ 1], ((gt + i - 1) >> 1) & 1);
+            used(base + pos_v(i - 1, n));
             __syncwarp();
             tc_fence_after();
 #pragma unroll 1
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (lane == 0) bar_arrive(&s.p_ready[buf]);
       }
       // ---- the unit's rows, or this CTA's part of them
-      wait(&s.o_done[(gt + n - 1) & 1], ((gt + n - 1) >> 1) & 1);
+      used(base + pos_v(n - 1, n));
       __syncwarp();
       tc_fence_after();
       uint64_t bad = 0;
@@ -472,7 +470,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       if (warp_on) {
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const int64_t out_row = ((int64_t)w.b * a.n + node) * (a.heads * a.group) + qh;
-        const int64_t part_row = (int64_t)(2 * cta + (first ? 0 : 1)) * a.rows + row;
+        const int64_t part_row = (int64_t)(2 * blockIdx.x + (walk.g < w.start ? 1 : 0)) * a.rows + row;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t x[32];
@@ -515,7 +513,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       }
       base += 2 * n;
       gt += n;
-      first = false;
     }
   } else if (C::F8 && warp >= 8) {
     // ---- FP8 caches: each thread copies its own 16-code pieces ahead with
@@ -535,9 +532,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         }
       }
     };
-    Items ahead(Walk(s.pre, a.batch, units, g_begin, g_end)), now = ahead;
+    Items ahead(walk), now = ahead;
     auto source = [&](const Items &it, bool is_v) {
-      const int h = it.w.unit / a.mtiles;
+      const int h = it.w.unit;
       if (a.cells) return a.cells[it.w.b * a.heads + h].kv8 + (is_v ? D : 0);
       return is_v ? a.v8 + it.w.b * a.v8s[0] + h * a.v8s[1] : a.k8 + it.w.b * a.k8s[0] + h * a.k8s[1];
     };
@@ -604,7 +601,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         issue(ahead, slot);
         if (ahead.live) ahead.step();
         if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
-        const int h = now.w.unit / a.mtiles;
+        const int h = now.w.unit;
         const uint16_t *src = is_v ? a.vn + now.w.b * a.vns[0] + h * a.vns[1] : a.kn + now.w.b * a.kns[0] + h * a.kns[1];
         const int64_t st = is_v ? a.vns[2] : a.kns[2];
 #pragma unroll
@@ -632,13 +629,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 
 // ---- joining the parts of a unit ---------------------------------------------
 
-constexpr int TC_THREADS = 256, TC_MAX = 512;  // most CTAs of the attention kernel
+constexpr int TC_THREADS = 256, TC_MAX = 512;  // most items of a launch
 
 // One row per block: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over
 // the CTAs c of the row's unit, in their order.  D / 4 threads hold the row;
 // the groups of them take every TC_THREADS / (D / 4)-th part.
 template <int D, int KT>
-__global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int groups) {
   constexpr int LANES = D / 4, GROUPS = TC_THREADS / LANES;
   __shared__ int32_t s_pre[PLAN_BATCH + 1];
   __shared__ float s_w[TC_MAX];
@@ -646,22 +643,20 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ int s_dead;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1, nullptr, s_pre);
+  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
   if (tid == 0) s_dead = 0;
   __syncthreads();
   const int rows = a.n * a.group;
   const int r = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % a.heads, b = bh / a.heads;
-  const int units = a.heads * a.mtiles, mt = r / TR_ROWS;
-  const long long total = (long long)s_pre[a.batch] * units;
-  const Plan plan{total, (int)min((long long)ctas, total)};
-  const int tiles = s_pre[b + 1] - s_pre[b];
-  const long long g0 = (long long)s_pre[b] * units + (long long)(h * a.mtiles + mt) * tiles;
-  const int c0 = plan.owner(g0), c1 = plan.owner(g0 + tiles - 1);
+  const int mt = r / TR_ROWS, places = s_pre[b + 1] - s_pre[b];
+  const Plan plan((long long)s_pre[a.batch] * a.heads, groups);
+  const long long g0 = (long long)s_pre[b] * a.heads + (long long)h * places;
+  const int c0 = plan.owner(g0), c1 = plan.owner(g0 + places - TR_IDLE - 1);
   if (c0 == c1) return;  // written by its one CTA
-  const int shift = plan.begin(c0) < g0 ? 1 : 0;  // only its first CTA may have had a unit before
+  const int shift = plan.begin(c0) < g0 ? 1 : 0;  // only its first item may hold a part of a unit before
   grid_dependency_wait();
   const int parts = c1 - c0 + 1, prow = r - mt * TR_ROWS;
-  auto slot = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0 ? shift : 0)) * a.rows + prow; };
+  auto slot = [&](int i) { return (int64_t)(2 * ((c0 + i) * a.mtiles + mt) + (i == 0 ? shift : 0)) * a.rows + prow; };
   float m = -INFINITY, l = 0.0f;
   for (int i = tid; i < parts; i += TC_THREADS) {
     const float2 x = __ldcg(a.ml + slot(i));
@@ -732,7 +727,7 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t 
                        "k_tree_attention launch"))
     return rc;
   const unsigned rows = (unsigned)(a.batch * a.heads * a.n * a.group);
-  return op_cuda(op_launch(k_tree_combine<C::D, C::KT>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas),
+  return op_cuda(op_launch(k_tree_combine<C::D, C::KT>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas / a.mtiles),
                  "k_tree_combine launch");
 }
 
@@ -743,11 +738,11 @@ int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, cuda
   return launch_tree<TreeCfg<256, F8>>(maps, a, ctas, st);
 }
 
-// CTAs of a launch: one per SM, or the most tiles that there can be.
-int tree_ctas(int sms, int64_t batch, int64_t units, int64_t t, int64_t dim) {
-  const int64_t kt = dim == 256 ? 64 : 128, most = batch * units * ((t + kt - 1) / kt + 1);
-  const int64_t c = sms < TC_MAX ? sms : TC_MAX;
-  return (int)(most < c ? most : c);
+// CTAs of a launch: one per SM, whole items (or fewer, the most places that the list can have).
+int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t t, int64_t dim) {
+  const int64_t kt = dim == 256 ? 64 : 128, most = batch * heads * ((t + kt - 1) / kt + 1 + TR_IDLE);
+  const int64_t c = sms > mtiles ? (sms / mtiles < TC_MAX ? sms / mtiles : TC_MAX) : 1;
+  return (most < c ? most : c) * mtiles;
 }
 
 int sm_count(int device, int *sms) {
@@ -756,9 +751,8 @@ int sm_count(int device, int *sms) {
 
 int64_t tree_workspace(int sms, const SkvTree *d) {
   const int64_t rows = d->n * (d->heads / d->kv_heads), per = rows < TR_ROWS ? rows : TR_ROWS;
-  const int64_t units = d->kv_heads * ((rows + TR_ROWS - 1) / TR_ROWS);
   const int64_t batch = d->batch < PLAN_BATCH ? d->batch : PLAN_BATCH;
-  const int64_t slots = 2 * (int64_t)tree_ctas(sms, batch, units, d->tokens, d->dim);
+  const int64_t slots = 2 * tree_ctas(sms, batch, d->kv_heads, (rows + TR_ROWS - 1) / TR_ROWS, d->tokens, d->dim);
   return slots * per * (d->dim + 2) * 4;
 }
 
@@ -835,7 +829,7 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
     a.parents = static_cast<const int32_t *>(d->parents) + b0 * a.ps[0];
     a.out = static_cast<uint16_t *>(d->out) + b0 * d->n * d->heads * d->dim;
     a.lse = static_cast<float *>(d->lse) + b0 * d->n * d->heads;
-    const int ctas = tree_ctas(sms, nb, (int64_t)a.heads * a.mtiles, d->tokens, d->dim);
+    const int ctas = (int)tree_ctas(sms, nb, a.heads, a.mtiles, d->tokens, d->dim);
     a.part = static_cast<float *>(d->workspace);
     a.ml = reinterpret_cast<float2 *>(a.part + 2 * (int64_t)ctas * a.rows * d->dim);
     TreeMaps maps{};
@@ -853,7 +847,7 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
                    {&maps.vn, a.vn, d->v_stride, d->n}};
       for (int i = 0; i < 4 && !rc; ++i) {
         const int64_t step[3] = {four[i].s[2], four[i].s[1], four[i].s[0]};
-        rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step, kt);
+        rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step, kt, (int)d->dim / 64);
         a.along[i][0] = d->kv_heads > 1 && four[i].s[1] ? 1 : 0;
         a.along[i][1] = nb > 1 && four[i].s[0] ? 1 : 0;
       }

@@ -94,15 +94,15 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   const uint32_t tmem = *(volatile uint32_t *)&s.tmem;
   volatile uint32_t *abort = &s.abort;
   const long long total = (long long)s.pre[a.batch] * a.heads;
-  const Plan plan{total, (int)min((long long)gridDim.x, total)};
+  const Plan plan(total, (int)gridDim.x);
   const int cta = blockIdx.x;
-  const long long g_begin = cta < plan.ctas ? plan.begin(cta) : 0, g_end = cta < plan.ctas ? plan.begin(cta + 1) : 0;
+  const long long g_begin = plan.begin(cta), g_end = plan.begin(cta + 1);
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
 
   if (warp == 0 && !F8) {
     // ---- loads
     if (lane == 0) {
-      Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+      Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
       uint32_t seq = 0;
       int stage = 0;
       uint32_t turn = 0;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
           for (int sub = 0; sub < SUB; ++sub) {
             if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
             bar_expect(&s.full[stage], WT_PIECE);
-            tma_load(ring + stage * WT_PIECE, &map, sub * 64, (w.tile + i) * WT_KEYS, w.unit * a.along[0],
+            tma_load(ring + stage * WT_PIECE, &map, (w.tile + i) * WT_KEYS, sub, w.unit * a.along[0],
                      w.b * a.along[1], &s.full[stage]);
             ++seq;
             if (++stage == stages) stage = 0, turn ^= 1;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   } else if (warp == 1) {
     // ---- tensor core
     if (lane == 0) {
-      Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+      Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
       const uint32_t desc = mma_desc(WT_KEYS, a.cols, false);
       const uint32_t q0 = s_addr(queries);
       int stage = 0;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
     // ---- epilogue: one key per thread, tiles in turn between the two groups
     const int et = tid - 128, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)((warp - 4) & 3) << 21) + half * WT_ROWS;
-    Walk w(s.pre, a.batch, a.heads, g_begin, g_end);
+    Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
     uint32_t gt = 0, seg = 0;
     while (w.next()) {
       const int h = w.unit;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
         live = w.next();
       }
     };
-    Items ahead(Walk(s.pre, a.batch, a.heads, g_begin, g_end)), now = ahead;
+    Items ahead(Walk(s.pre, a.batch, a.heads, 0, g_begin, g_end)), now = ahead;
     auto issue = [&](const Items &it, int slot) {
       if (it.live) {
         const uint8_t *src = a.k8 + it.w.b * a.k8s[0] + it.w.unit * a.k8s[1] + it.sub * 64;
@@ -400,7 +400,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
     } else {
       const int64_t step[3] = {d->k_cache_stride[2], d->k_cache_stride[1], d->k_cache_stride[0]};
       if (int rc = make_map(&map, static_cast<const uint16_t *>(d->k_cache) + b0 * d->k_cache_stride[0], d->dim, d->tokens,
-                            d->kv_heads, nb, step, WT_KEYS))
+                            d->kv_heads, nb, step, WT_KEYS, 1))
         return rc;
       a.along[0] = d->kv_heads > 1 && d->k_cache_stride[1] ? 1 : 0;
       a.along[1] = nb > 1 && d->k_cache_stride[0] ? 1 : 0;
