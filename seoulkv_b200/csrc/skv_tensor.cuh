@@ -12,6 +12,18 @@ namespace skv {
 
 __device__ __forceinline__ uint32_t s_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// The loading and the tensor-core warp run their loops as whole warps, and
+// only their instructions are predicated on one elected lane: descriptors and
+// addresses then stay in uniform registers.  In a branch that one lane takes,
+// every instruction moves its operands there first, and the issue alone takes
+// longer than the tensor core (2990 cycles against 2100 for a tile of 128 keys
+// at D = 256, and 4200 beside busy warps).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
+}
+
 // ---- mbarriers -----------------------------------------------------------
 
 // A wait that lasts WAIT_NS gives up: it raises `abort` for its CTA (every
@@ -31,9 +43,6 @@ __device__ __forceinline__ void bar_init(uint64_t *bar, uint32_t count) {
 __device__ __forceinline__ void bar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_addr(bar)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
   uint32_t ok;
@@ -68,13 +77,16 @@ __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// Box at (row, piece, y, z) of a make_map() map.
-__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int row, int piece, int y, int z,
-                                         uint64_t *bar) {
+// The elected lane announces `bytes` on `bar` and loads the box at (row,
+// piece, y, z) of a make_map() map.
+__device__ __forceinline__ void tma_load(uint32_t one, void *dst, const CUtensorMap *map, int row, int piece, int y,
+                                         int z, uint64_t *bar, uint32_t bytes) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-      "%6}], [%7];" ::"r"(s_addr(dst)),
-      "l"(map), "r"(0), "r"(row), "r"(piece), "r"(y), "r"(z), "r"(s_addr(bar))
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %8, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%7], %9;\n\t"
+      "@q cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];\n\t}" ::"r"(s_addr(dst)),
+      "l"(map), "r"(0), "r"(row), "r"(piece), "r"(y), "r"(z), "r"(s_addr(bar)), "r"(one), "r"(bytes)
       : "memory");
 }
 
@@ -92,10 +104,13 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Arrives on `bar` when every MMA issued so far by this thread has ended.
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(bar))
-               : "memory");
+// Arrives on `bar` when every MMA issued so far by the elected lane has ended.
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(s_addr(bar)),
+      "r"(one)
+      : "memory");
 }
 
 // Instruction descriptor: FP32 accumulator, BF16 operands, A K-major, B
@@ -111,20 +126,20 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
-// D (tensor memory) = A (tensor memory) B (shared memory) [+ D], K = 16.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+// By the elected lane: D (tensor memory) = A (tensor memory) B (shared memory) [+ D], K = 16.
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(one)
       : "memory");
 }
-// D (tensor memory) = A (shared memory) B (shared memory) [+ D], K = 16.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+// By the elected lane: D (tensor memory) = A (shared memory) B (shared memory) [+ D], K = 16.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(one)
       : "memory");
 }
 

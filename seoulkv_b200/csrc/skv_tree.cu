@@ -82,24 +82,25 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
 namespace {
 
 constexpr int TR_NODES = SKV_TREE_MAX_NODES;
+constexpr int TR_KEYS = 128;   // keys of a tile
 constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
-constexpr int TR_IDLE = 2;     // what starting and ending a unit costs, in tiles
+constexpr int TR_IDLE = 1;     // what starting and ending a unit costs, in tiles
 
 template <int D_, bool F8_>
 struct TreeCfg {
   static constexpr int D = D_;
   static constexpr bool F8 = F8_;
-  static constexpr int KT = D == 256 ? 64 : 128;  // keys of a tile: 32 KB of BF16 (16 KB at D = 64)
-  static constexpr int SUB = D / 64;              // 128-byte pieces of a row
-  static constexpr int STAGE = KT * D * 2;
-  static constexpr int RAW = KT * D;              // an FP8 tile before its conversion
-  static constexpr int NRAW = F8 ? 5 : 0;
-  static constexpr int NSTAGE = F8 ? 4 : D == 64 ? 12 : 6;
-  static constexpr int THREADS = F8 ? 512 : 256;
-  // tensor memory columns: O, Q (BF16 pairs), two score tiles (P over S)
-  static constexpr int COL_Q = D, COL_S = D + D / 2;
-  static constexpr int RING = NSTAGE * STAGE + NRAW * RAW;
-  static_assert(COL_S + 2 * KT <= 512, "tensor memory");
+  static constexpr int KT = TR_KEYS;
+  static constexpr int PIECES = D / 64;   // ring stages of a tile's K, and of its V
+  static constexpr int VROWS = KT / PIECES;  // keys of a V stage
+  static constexpr int STAGE = KT * 128;  // bytes: K 128 keys x 64 dimensions, V VROWS keys x D
+  static constexpr int RAW = STAGE / 2;   // an FP8 stage before its conversion
+  static constexpr int NRAW = F8 ? 8 : 0;
+  static constexpr int NSTAGE = F8 ? 6 : D == 256 ? 10 : D == 128 ? 11 : 12;
+  static constexpr int THREADS = F8 ? 640 : 384;
+  static constexpr int COL_S = 256;       // tensor memory columns: O, then two score tiles (P over S)
+  static constexpr int QBYTES = TR_ROWS * D * 2;
+  static constexpr int RING = QBYTES + NSTAGE * STAGE + NRAW * RAW;
 };
 
 struct TreeMaps {
@@ -132,21 +133,21 @@ struct TreeArgs {
 template <class C>
 struct TreeSmem {
   uint64_t full[C::NSTAGE], empty[C::NSTAGE];
-  uint64_t q_ready, p_ready[2], drain;
-  uint64_t anc[TR_NODES];   // nodes that node i sees (0: unused)
-  unsigned long long bad;   // nodes with a value that is not finite
+  uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;
+  uint64_t anc[TR_NODES];      // nodes that node i sees (0: unused)
+  unsigned long long bad;      // nodes with a value that is not finite
+  float share[2][TR_ROWS];     // maxima and sums that the two threads of a row exchange
   int32_t up[TR_NODES];
   uint32_t tmem;
   uint32_t abort;
-  int32_t len[PLAN_BATCH];
-  int32_t pre[PLAN_BATCH + 1];  // tiles of the sequences before (one unit's worth)
+  int32_t pre[PLAN_BATCH + 1];  // places of the sequences before (one unit's worth)
 };
 
 // Order of a segment's 2n operand tiles in the ring: K0, K1, V0, K2, V1, ...,
 // V(n-1), the order in which the MMA thread needs them.
 __device__ __forceinline__ int pos_k(int i) { return i ? 2 * i - 1 : 0; }
 __device__ __forceinline__ int pos_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
-__device__ __forceinline__ void item_at(int p, int n, bool &is_v, int &i) {
+__device__ __forceinline__ void tile_at(int p, int n, bool &is_v, int &i) {
   is_v = p == 2 * n - 1 || (p > 0 && !(p & 1));
   i = p == 0 ? 0 : p == 2 * n - 1 ? n - 1 : is_v ? (p - 2) / 2 : (p + 1) / 2;
 }
@@ -159,14 +160,15 @@ template <class C>
 __global__ void __launch_bounds__(C::THREADS, 1)
     k_tree_attention(const __grid_constant__ TreeMaps maps, const __grid_constant__ TreeArgs a) {
   constexpr int D = C::D, KT = C::KT;
-  extern __shared__ uint8_t smem_dyn[];
-  uint8_t *ring = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;
+  extern __shared__ __align__(1024) uint8_t smem_dyn[];
+  uint8_t *queries = smem_dyn;  // [D / 64][128 rows][128 bytes], swizzled
+  uint8_t *ring = queries + C::QBYTES;
   uint8_t *raw = ring + C::NSTAGE * C::STAGE;
-  TreeSmem<C> &s = *reinterpret_cast<TreeSmem<C> *>(ring + C::RING);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  TreeSmem<C> &s = *reinterpret_cast<TreeSmem<C> *>(smem_dyn + C::RING);
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (warp == 0) {
-    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, s.len, s.pre);
+    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
     if (lane == 0 && !C::F8) {
       tma_prefetch_map(&maps.k);
       tma_prefetch_map(&maps.v);
@@ -177,12 +179,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::NSTAGE; ++i) {
-      bar_init(&s.full[i], C::F8 ? 8 : 1);
+      bar_init(&s.full[i], C::F8 ? 4 : 1);
       bar_init(&s.empty[i], 1);
     }
-    bar_init(&s.q_ready, 4);
+    bar_init(&s.q_ready, 8);
     bar_init(&s.drain, 1);
-    for (int i = 0; i < 2; ++i) bar_init(&s.p_ready[i], 4);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&s.s_full[i], 1);
+      bar_init(&s.p_ready[i], 8);
+      bar_init(&s.o_done[i], 1);
+    }
     bar_init_fence();
     s.abort = 0;
     s.bad = 0;
@@ -200,117 +206,128 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   const int item = blockIdx.x / a.mtiles, mt = blockIdx.x % a.mtiles;
   const Walk walk(s.pre, a.batch, a.heads, TR_IDLE, plan.begin(item), plan.begin(item + 1));
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
+  auto length = [&](int b) {
+    const int n = a.lengths ? a.lengths[b * a.len_stride] : a.context;
+    return max(0, min(n, a.t));
+  };
 
   if (warp == 0 && !C::F8) {
     // ---- loads
-    if (lane == 0) {
-      Walk w = walk;
-      uint32_t seq = 0;
-      bool ok = true;
-      while (ok && w.next()) {
-        for (int p = 0; p < 2 * w.count; ++p, ++seq) {
-          bool is_v;
-          int i;
-          item_at(p, w.count, is_v, i);
+    const uint32_t one = elect_lane();
+    Walk w = walk;
+    uint32_t seq = 0;
+    bool ok = true;
+    while (ok && w.next()) {
+      for (int p = 0; ok && p < 2 * w.count; ++p) {
+        bool is_v;
+        int i;
+        tile_at(p, w.count, is_v, i);
+        const bool nodes = w.tile + i == w.tiles - 1;
+        const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
+        const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
+        const int row = nodes ? 0 : (w.tile + i) * KT;
+        const int y = w.unit * a.along[which][0], z = w.b * a.along[which][1];
+        for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
           const int stage = seq % C::NSTAGE;
           if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
-          const bool nodes = w.tile + i == w.tiles - 1;
-          const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
-          const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
-          const int row = nodes ? 0 : (w.tile + i) * KT;
-          bar_expect(&s.full[stage], C::STAGE);
-          tma_load(ring + stage * C::STAGE, map, row, 0, w.unit * a.along[which][0], w.b * a.along[which][1],
-                   &s.full[stage]);
+          tma_load(one, ring + stage * C::STAGE, map, row + (is_v ? piece * C::VROWS : 0), is_v ? 0 : piece, y, z,
+                   &s.full[stage], C::STAGE);
         }
       }
-      if (!ok)  // gave up: the copies in flight still land before the CTA ends
-        for (uint32_t back = 1; back <= C::NSTAGE && back <= seq; ++back) {
-          const uint32_t q = seq - back;
-          const unsigned long long t0 = timer_ns();
-          while (!bar_try(&s.full[q % C::NSTAGE], (q / C::NSTAGE) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
-          }
-        }
     }
+    if (!ok)  // gave up: the copies in flight still land before the CTA ends
+      for (uint32_t back = 1; back <= C::NSTAGE && back <= seq; ++back) {
+        const uint32_t q = seq - back;
+        const unsigned long long t0 = timer_ns();
+        while (!bar_try(&s.full[q % C::NSTAGE], (q / C::NSTAGE) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+        }
+      }
   } else if (warp == 1) {
     // ---- tensor core
-    if (lane == 0) {
-      Walk w = walk;
-      constexpr uint32_t DESC_S = mma_desc(TR_ROWS, KT, false), DESC_O = mma_desc(TR_ROWS, D, true);
-      uint32_t base = 0, gt = 0, seg = 0;
-      while (w.next()) {
-        const int n = w.count;
-        auto scores = [&](int i) {
-          const uint32_t item = base + pos_k(i), stage = item % C::NSTAGE;
-          wait(&s.full[stage], (item / C::NSTAGE) & 1);
-          tc_fence_after();
-          const uint32_t k0 = s_addr(ring + stage * C::STAGE);
-          const uint32_t d = tmem + C::COL_S + ((gt + i) & 1) * KT;
+    const uint32_t one = elect_lane();
+    Walk w = walk;
+    constexpr uint32_t DESC_S = mma_desc(TR_ROWS, KT, false), DESC_O = mma_desc(TR_ROWS, D, true);
+    const uint32_t q0 = s_addr(queries), ring0 = s_addr(ring);
+    uint32_t seq = 0, gt = 0, seg = 0;
+    while (w.next()) {
+      const int n = w.count;
+      auto scores = [&](uint32_t buf) {
+        const uint32_t d = tmem + C::COL_S + buf * KT;
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            mma_ts(d, tmem + C::COL_Q + 8 * ks, smem_desc(k0 + (ks / 4) * KT * 128 + (ks % 4) * 32, 16), DESC_S, ks > 0);
-          mma_commit(&s.empty[stage]);
-        };
-        wait(&s.q_ready, seg & 1);
+        for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
+          const uint32_t stage = seq % C::NSTAGE;
+          wait(&s.full[stage], (seq / C::NSTAGE) & 1);
+          const uint32_t k0 = ring0 + stage * C::STAGE, qp = q0 + piece * TR_ROWS * 128;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            mma_ss(one, d, smem_desc(qp + ks * 32, 16), smem_desc(k0 + ks * 32, 16), DESC_S, piece + ks > 0);
+          mma_commit(one, &s.empty[stage]);
+        }
+        mma_commit(one, &s.s_full[buf]);
+      };
+      wait(&s.q_ready, seg & 1);
+      scores(gt & 1);
+      for (int i = 0; i < n; ++i, ++gt) {
+        const uint32_t buf = gt & 1;
+        if (i + 1 < n) scores(buf ^ 1);
+        wait(&s.p_ready[buf], (gt >> 1) & 1);
         tc_fence_after();
-        scores(0);
-        for (int i = 0; i < n; ++i) {
-          if (i + 1 < n) scores(i + 1);
-          const uint32_t buf = (gt + i) & 1;
-          wait(&s.p_ready[buf], ((gt + i) >> 1) & 1);
-          const uint32_t item = base + pos_v(i, n), stage = item % C::NSTAGE;
-          wait(&s.full[stage], (item / C::NSTAGE) & 1);
-          tc_fence_after();
-          const uint32_t v0 = s_addr(ring + stage * C::STAGE);
 #pragma unroll
-          for (int ks = 0; ks < KT / 16; ++ks)
-            mma_ts(tmem, tmem + C::COL_S + buf * KT + 8 * ks, smem_desc(v0 + ks * 2048, KT * 128), DESC_O, i > 0 || ks > 0);
-          mma_commit(&s.empty[stage]);
+        for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
+          const uint32_t stage = seq % C::NSTAGE;
+          wait(&s.full[stage], (seq / C::NSTAGE) & 1);
+          const uint32_t v0 = ring0 + stage * C::STAGE, p0 = tmem + C::COL_S + buf * KT + piece * (C::VROWS / 2);
+#pragma unroll
+          for (int ks = 0; ks < C::VROWS / 16; ++ks)
+            mma_ts(one, tmem, p0 + 8 * ks, smem_desc(v0 + ks * 2048, C::VROWS * 128), DESC_O, i > 0 || piece + ks > 0);
+          mma_commit(one, &s.empty[stage]);
         }
-        base += 2 * n;
-        gt += n;
-        ++seg;
+        mma_commit(one, &s.o_done[buf]);
       }
-      if (*abort) {  // what was issued ends before tensor memory is given back
-        mma_commit(&s.drain);
-        const unsigned long long t0 = timer_ns();
-        while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
-        }
+      ++seg;
+    }
+    if (*abort) {  // what was issued ends before tensor memory is given back
+      mma_commit(one, &s.drain);
+      const unsigned long long t0 = timer_ns();
+      while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
       }
     }
-  } else if (warp >= 4 && warp < 8) {
-    // ---- softmax: one row per thread
-    const int row = tid - 128;
-    const uint32_t lanes = tmem + ((uint32_t)(warp - 4) << 21);  // this warp's 32 lanes (bits 16..)
+  } else if (warp >= 4 && warp < 12) {
+    // ---- softmax: two threads per row, each half of a tile's columns and of O's
+    const int st = tid - 128, half = st >> 7, row = st & 127;
+    const int pair = 2 + ((warp - 4) & 3);  // barrier of the two warps that share 32 rows
+    const uint32_t lanes = tmem + ((uint32_t)((warp - 4) & 3) << 21);  // these 32 lanes (bits 16..)
+    const int left = a.n * a.group - mt * TR_ROWS;  // rows of this part
+    const bool warp_on = (row & ~31) < left, on = row < left;
+    const int r = mt * TR_ROWS + row;  // row of the KV head
+    const int node = on ? r / a.group : 0, qg = on ? r - node * a.group : 0;
+    // rows that do not exist are zeros: a product of zeros draws no power,
+    // and power is what the clock follows
+    for (int x = st; x < (TR_ROWS - min(left, TR_ROWS)) * (D / 8); x += 256) {
+      const int at = min(left, TR_ROWS) + x / (D / 8), c16 = x % (D / 8);
+      *reinterpret_cast<uint4 *>(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + (c16 % 8) * 16) = make_uint4(0, 0, 0, 0);
+    }
     Walk w = walk;
     uint32_t base = 0, gt = 0;
-    // The product that used an operand tile is done: S(i) with K(i), O(i) with
-    // V(i).  The stage's use before is older than what this thread has seen
-    // done, so that the parity names this use.
-    auto used = [&](uint32_t at) { wait(&s.empty[at % C::NSTAGE], (at / C::NSTAGE) & 1); };
+    // Tile g's S and O.  Both alternate between two barriers, and S(g) follows
+    // O(g - 2): a wait is never two phases behind, so its parity names one.
+    auto done = [&](uint64_t *two, uint32_t g) {
+      wait(&two[g & 1], (g >> 1) & 1);
+      __syncwarp();
+      tc_fence_after();
+    };
     while (w.next()) {
       const int n = w.count, h = w.unit;
-      const int r = mt * TR_ROWS + row;                 // row of the KV head
-      const int left = a.n * a.group - mt * TR_ROWS;    // rows of this unit
-      const bool warp_on = 32 * (warp - 4) < left, on = row < left;
-      const int node = on ? r / a.group : 0, qh = h * a.group + (on ? r - node * a.group : 0);
-      const int len = s.len[w.b];
+      const int len = length(w.b);
       const bool has_nodes = w.tile + n == w.tiles;
       // every S of the segment before has been read, so its MMAs are done with Q
-      if (warp_on) {
-        const uint16_t *q = a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2];
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t x[32];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint4 v = on ? __ldg(reinterpret_cast<const uint4 *>(q + c * 64) + j) : make_uint4(0, 0, 0, 0);
-            x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
-          }
-          tmem_st32(lanes + C::COL_Q + 32 * c, x);
-        }
-        tmem_wait_st();
-        tc_fence_before();
+      for (int x = st; x < min(left, TR_ROWS) * (D / 8); x += 256) {
+        const int at = x / (D / 8), c16 = x % (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
+        const uint16_t *q = a.q + w.b * a.qs[0] + nd * a.qs[1] + (h * a.group + rr - nd * a.group) * a.qs[2];
+        *reinterpret_cast<uint4 *>(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16) =
+            __ldg(reinterpret_cast<const uint4 *>(q) + c16);
       }
+      async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
       uint64_t see = 0;
@@ -318,22 +335,22 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         // ancestors by pointer doubling: after k rounds a node knows 2^k of its line
         uint64_t mask = 0;
         int up = -2;
-        if (row < a.n) {
-          up = a.parents[w.b * a.ps[0] + row * a.ps[1]];
-          if (up < -1 || up >= row) up = -2;
-          mask = up == -2 ? 0 : 1ull << row;
+        if (st < a.n) {
+          up = a.parents[w.b * a.ps[0] + st * a.ps[1]];
+          if (up < -1 || up >= st) up = -2;
+          mask = up == -2 ? 0 : 1ull << st;
         }
         for (int step = 1;; step <<= 1) {
-          if (row < TR_NODES) {
-            s.anc[row] = mask;
-            s.up[row] = up;
+          if (st < TR_NODES) {
+            s.anc[st] = mask;
+            s.up[st] = up;
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           if (step >= a.n) break;
           uint64_t over = 0;
           int next = -1;
           if (up >= 0) over = s.anc[up], next = s.up[up];
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
           if (up >= 0) {
             mask = over ? mask | over : 0;  // a node below an unused one is unused
             up = over ? next : -2;
@@ -342,30 +359,24 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (on) see = s.anc[node];
       }
       const bool dead = has_nodes && see == 0;
-      float m = -INFINITY, l = 0.0f;  // running maximum (log2 units) and sum
+      float m = -INFINITY, l = 0.0f;  // the row's running maximum (log2 units), this thread's part of the sum
       for (int i = 0; i < n; ++i) {
         const uint32_t buf = (gt + i) & 1;
         const uint32_t at = lanes + C::COL_S + buf * KT;
         const bool nodes = w.tile + i == w.tiles - 1;
         const int valid = nodes ? a.n : min(KT, len - (w.tile + i) * KT);
         const bool whole = valid == KT && !nodes;
-        uint64_t keep[KT / 64];  // columns this row sees
-#pragma unroll
-        for (int j = 0; j < KT / 64; ++j) {
-          const int v = valid - 64 * j;
-          keep[j] = nodes ? (j ? 0 : see) : v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
-        }
-        used(base + pos_k(i));
-        __syncwarp();
-        tc_fence_after();
+        const int v64 = valid - 64 * half;
+        const uint64_t keep = nodes ? (half ? 0 : see) : v64 >= 64 ? ~0ull : v64 > 0 ? (1ull << v64) - 1 : 0;
+        done(s.s_full, gt + i);
         if (warp_on) {
           float top = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < KT / 32; ++c) {
+          for (int c = 0; c < 2; ++c) {
             uint32_t x[32];
-            tmem_ld32(x, at + 32 * c);
+            tmem_ld32(x, at + 64 * half + 32 * c);
             tmem_wait_ld();
-            const uint32_t bits = (uint32_t)(keep[c / 2] >> (32 * (c & 1)));
+            const uint32_t bits = (uint32_t)(keep >> (32 * c));
             if (whole) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
@@ -374,18 +385,18 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               for (int j = 0; j < 32; ++j) top = fmaxf(top, bits >> j & 1 ? __uint_as_float(x[j]) : -INFINITY);
             }
           }
-          top *= a.c2;
+          s.share[half][row] = top;
+          asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+          top = fmaxf(top, s.share[half ^ 1][row]) * a.c2;
           // the maximum moves only when it grows by more than 2^8: until then
           // weights up to 2^8 lose nothing in FP32 sums and BF16 products,
           // and the accumulator stays where it is
           const bool move = i == 0 || top > m + 8.0f;
           if (i > 0 && __any_sync(0xffffffffu, move)) {
             const float f = move ? exp2_fast(m - top) : 1.0f;
-            used(base + pos_v(i - 1, n));
-            __syncwarp();
-            tc_fence_after();
+            done(s.o_done, gt + i - 1);
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
               uint32_t x[32];
               tmem_ld32(x, lanes + 32 * c);
               tmem_wait_ld();
@@ -397,12 +408,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
           if (move) m = top;
           const float base2 = m == -INFINITY ? 0.0f : m;
+          uint32_t y[32];
 #pragma unroll
-          for (int c = 0; c < KT / 32; ++c) {
-            uint32_t x[32], y[16];
-            tmem_ld32(x, at + 32 * c);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t x[32];
+            tmem_ld32(x, at + 64 * half + 32 * c);
             tmem_wait_ld();
-            const uint32_t bits = (uint32_t)(keep[c / 2] >> (32 * (c & 1)));
+            const uint32_t bits = (uint32_t)(keep >> (32 * c));
             float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -414,11 +426,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               }
               sum0 += p0;
               sum1 += p1;
-              y[j / 2] = pack_bf16(p0, p1);
+              y[16 * c + j / 2] = pack_bf16(p0, p1);
             }
             l += sum0 + sum1;
-            tmem_st16(at + 16 * c, y);
           }
+          // P goes over the first half of S: only when both threads have read theirs
+          tc_fence_before();
+          asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+          tc_fence_after();
+          tmem_st32(at + 32 * half, y);
           tmem_wait_st();
           tc_fence_before();
         }
@@ -427,28 +443,34 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           // NaN there): tokens behind the cache's length, unused nodes, and
           // values of a node that are not finite (its siblings do not see
           // them; the rows that do get them back below)
-          const uint32_t item = base + pos_v(i, n), stage = item % C::NSTAGE;
-          wait(&s.full[stage], (item / C::NSTAGE) & 1);
-          uint8_t *v = ring + stage * C::STAGE;
+          // (the tile before is waited for so that a stage's parity names V(i)'s use of it)
+          if (i > 0) done(s.o_done, gt + i - 1);
+          const uint32_t v0 = base + pos_v(i, n) * C::PIECES;
           const int from = nodes ? 0 : valid, to = nodes ? a.n : KT;
-          for (int x = from * (D / 8) + row; x < to * (D / 8); x += 128) {
-            const int key = x / (D / 8), c16 = x % (D / 8);
-            uint4 *p = reinterpret_cast<uint4 *>(v + (c16 / 8) * KT * 128 + key * 128 + (c16 % 8) * 16);
-            if (!nodes || s.anc[key] == 0) {
-              *p = make_uint4(0, 0, 0, 0);
-              continue;
-            }
-            uint4 u = *p;
-            uint32_t *e = reinterpret_cast<uint32_t *>(&u);
-            bool found = false;
+          for (int piece = from / C::VROWS; piece * C::VROWS < to; ++piece) {
+            const uint32_t stage = (v0 + piece) % C::NSTAGE;
+            wait(&s.full[stage], ((v0 + piece) / C::NSTAGE) & 1);
+            uint8_t *v = ring + stage * C::STAGE;
+            const int first = max(from - piece * C::VROWS, 0), last = min(to - piece * C::VROWS, C::VROWS);
+            for (int x = first * (D / 8) + st; x < last * (D / 8); x += 256) {
+              const int key = x / (D / 8), c16 = x % (D / 8);
+              uint4 *p = reinterpret_cast<uint4 *>(v + (c16 / 8) * C::VROWS * 128 + key * 128 + (c16 % 8) * 16);
+              if (!nodes || s.anc[piece * C::VROWS + key] == 0) {
+                *p = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              uint4 u = *p;
+              uint32_t *e = reinterpret_cast<uint32_t *>(&u);
+              bool found = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (not_finite_bf16(e[j])) e[j] &= 0xffff0000u, found = true;
-              if (not_finite_bf16(e[j] >> 16)) e[j] &= 0x0000ffffu, found = true;
-            }
-            if (found) {
-              *p = u;
-              atomicOr(&s.bad, 1ull << key);
+              for (int j = 0; j < 4; ++j) {
+                if (not_finite_bf16(e[j])) e[j] &= 0xffff0000u, found = true;
+                if (not_finite_bf16(e[j] >> 16)) e[j] &= 0x0000ffffu, found = true;
+              }
+              if (found) {
+                *p = u;
+                atomicOr(&s.bad, 1ull << (piece * C::VROWS + key));
+              }
             }
           }
           async_fence();
@@ -456,23 +478,24 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(&s.p_ready[buf]);
       }
-      // ---- the unit's rows, or this CTA's part of them
-      used(base + pos_v(n - 1, n));
-      __syncwarp();
-      tc_fence_after();
+      // ---- the unit's rows, or this item's part of them
+      done(s.o_done, gt + n - 1);
       uint64_t bad = 0;
       if (has_nodes) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         bad = s.bad & see;
       }
-      if (*abort) l = __uint_as_float(0x7fffffffu);
       const bool direct = n == w.tiles;
       if (warp_on) {
+        s.share[half][row] = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        l = s.share[0][row] + s.share[1][row];
+        if (*abort) l = __uint_as_float(0x7fffffffu);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const int64_t out_row = ((int64_t)w.b * a.n + node) * (a.heads * a.group) + qh;
+        const int64_t out_row = ((int64_t)w.b * a.n + node) * (a.heads * a.group) + h * a.group + qg;
         const int64_t part_row = (int64_t)(2 * blockIdx.x + (walk.g < w.start ? 1 : 0)) * a.rows + row;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
           uint32_t x[32];
           tmem_ld32(x, lanes + 32 * c);
           tmem_wait_ld();
@@ -501,89 +524,111 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
           __syncwarp();
         }
-        if (on) {
+        if (on && half == 0) {
           if (direct) a.lse[out_row] = dead ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           else a.ml[part_row] = make_float2(m, dead ? -1.0f : l);
         }
         tc_fence_before();
       }
-      if (has_nodes) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // all have read s.bad and s.anc
-        if (row == 0) s.bad = 0;
-      }
-      base += 2 * n;
+      // all have read O, s.bad and s.anc before the next segment's products and nodes
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (has_nodes && st == 0) s.bad = 0;
+      base += 2 * n * C::PIECES;
       gt += n;
     }
-  } else if (C::F8 && warp >= 8) {
+  } else if (C::F8 && warp >= 12) {
     // ---- FP8 caches: each thread copies its own 16-code pieces ahead with
     // cp.async (no barrier between the copy and its use), turns them into
-    // BF16 and puts them where TMA would have put a BF16 tile
-    constexpr int PIECES = C::RAW / 16 / 256;  // of one thread and tile
-    const int ct = tid - 256;
-    struct Items {
+    // BF16 and puts them where TMA would have put a BF16 stage.  Two groups of
+    // four warps take the stages in turn.
+    constexpr int CHUNKS = C::F8 ? C::RAW / 16 / 128 : 1;  // of one thread and stage
+    constexpr int AHEAD = C::F8 ? C::NRAW / 2 : 1;         // stages of a group in flight
+    const int ct = (tid - 384) & 127, grp = (tid - 384) >> 7;
+    struct Stages {
       Walk w;
-      int p = 0;
+      int p = 0, piece = 0, len = 0;
       bool live;
-      __device__ Items(const Walk &x) : w(x) { live = w.next(); }
-      __device__ void step() {
-        if (++p == 2 * w.count) {
-          p = 0;
-          live = w.next();
-        }
-      }
     };
-    Items ahead(walk), now = ahead;
-    auto source = [&](const Items &it, bool is_v) {
-      const int h = it.w.unit;
-      if (a.cells) return a.cells[it.w.b * a.heads + h].kv8 + (is_v ? D : 0);
-      return is_v ? a.v8 + it.w.b * a.v8s[0] + h * a.v8s[1] : a.k8 + it.w.b * a.k8s[0] + h * a.k8s[1];
+    auto start = [&](Stages &x) {
+      x.live = x.w.next();
+      if (x.live) x.len = length(x.w.b);
     };
-    auto issue = [&](const Items &it, int slot) {
-      if (it.live) {
+    auto step = [&](Stages &x) {
+      if (++x.piece < C::PIECES) return;
+      x.piece = 0;
+      if (++x.p < 2 * x.w.count) return;
+      x.p = 0;
+      start(x);
+    };
+    auto skip = [&](Stages &x) {  // to this group's next stage
+      if (x.live) step(x);
+      if (x.live) step(x);
+    };
+    Stages ahead{walk}, now{walk};
+    start(ahead);
+    if (grp && ahead.live) step(ahead);
+    now = ahead;
+    // a stage's 16-byte pieces: K 4 a key (64 dimensions), V D / 16 a key
+    auto place = [&](int c, bool is_v, int piece, int &key, int &dim) {
+      key = is_v ? piece * C::VROWS + c / (D / 16) : c / 4;
+      dim = is_v ? (c % (D / 16)) * 16 : piece * 64 + (c % 4) * 16;
+    };
+    auto issue = [&](const Stages &x, int slot) {
+      if (x.live) {
         bool is_v;
         int i;
-        item_at(it.p, it.w.count, is_v, i);
-        if (it.w.tile + i < it.w.tiles - 1) {
-          const uint8_t *src = source(it, is_v);
-          const int64_t st = a.cells ? REC : is_v ? a.v8s[2] : a.k8s[2];
-          const int t0 = (it.w.tile + i) * KT, len = s.len[it.w.b];
+        tile_at(x.p, x.w.count, is_v, i);
+        if (x.w.tile + i < x.w.tiles - 1) {
+          const uint8_t *src;
+          int64_t st;
+          if (a.cells) {
+            src = a.cells[x.w.b * a.heads + x.w.unit].kv8 + (is_v ? D : 0);
+            st = REC;
+          } else {
+            src = is_v ? a.v8 + x.w.b * a.v8s[0] + x.w.unit * a.v8s[1] : a.k8 + x.w.b * a.k8s[0] + x.w.unit * a.k8s[1];
+            st = is_v ? a.v8s[2] : a.k8s[2];
+          }
+          const int t0 = (x.w.tile + i) * KT;
 #pragma unroll
-          for (int j = 0; j < PIECES; ++j) {
-            const int c = ct + j * 256, key = c / (D / 16);
-            if (t0 + key < len) cp_async16(raw + slot * C::RAW + c * 16, src + (t0 + key) * st + (c % (D / 16)) * 16);
+          for (int j = 0; j < CHUNKS; ++j) {
+            int key, dim;
+            place(ct + j * 128, is_v, x.piece, key, dim);
+            if (t0 + key < x.len) cp_async16(raw + slot * C::RAW + (ct + j * 128) * 16, src + (t0 + key) * st + dim);
           }
         }
       }
       cp_async_commit();
     };
-    constexpr int AHEAD = C::F8 ? C::NRAW : 1;
     for (int i = 0; i < AHEAD; ++i) {
-      issue(ahead, i);
-      if (ahead.live) ahead.step();
+      issue(ahead, grp * AHEAD + i);
+      skip(ahead);
     }
-    uint32_t seq = 0;
+    uint32_t seq = grp, turn = 0;
     while (now.live) {
-      const int stage = seq % C::NSTAGE, slot = seq % AHEAD;
+      const int stage = seq % C::NSTAGE, slot = grp * AHEAD + (int)(turn % AHEAD);
       bool is_v;
       int i;
-      item_at(now.p, now.w.count, is_v, i);
+      tile_at(now.p, now.w.count, is_v, i);
       const bool nodes = now.w.tile + i == now.w.tiles - 1;
       uint8_t *to = ring + stage * C::STAGE;
+      const int rows = is_v ? C::VROWS : KT;  // of a 64-dimension piece in the stage
       cp_async_wait<AHEAD - 1>();
       if (!nodes) {
-        const int left = s.len[now.w.b] - (now.w.tile + i) * KT;
-        uint4 v[PIECES];
+        const int left = now.len - (now.w.tile + i) * KT;
+        uint4 v[CHUNKS];
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-          const int c = ct + j * 256;
-          v[j] = c / (D / 16) < left ? *reinterpret_cast<const uint4 *>(raw + slot * C::RAW + c * 16) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < CHUNKS; ++j) {
+          int key, dim;
+          place(ct + j * 128, is_v, now.piece, key, dim);
+          v[j] = key < left ? *reinterpret_cast<const uint4 *>(raw + slot * C::RAW + (ct + j * 128) * 16) : make_uint4(0, 0, 0, 0);
         }
         issue(ahead, slot);
-        if (ahead.live) ahead.step();
+        skip(ahead);
         if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-          const int c = ct + j * 256, key = c / (D / 16), c16 = 2 * (c % (D / 16));
+        for (int j = 0; j < CHUNKS; ++j) {
+          const int c = ct + j * 128;
+          const int key = is_v ? c / (D / 16) : c / 4, c16 = 2 * (is_v ? c % (D / 16) : c % 4);
           const uint32_t *x = reinterpret_cast<const uint32_t *>(&v[j]);
           uint4 y[2];
 #pragma unroll
@@ -592,30 +637,33 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                               e4m3x2_to_bf16x2((uint16_t)x[2 * u + 1]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u + 1] >> 16)));
           // neighbouring threads write the two halves in opposite order where
           // they would meet in the same banks (pieces of different subtiles)
-          uint8_t *line = to + (c16 / 8) * KT * 128 + key * 128;
+          uint8_t *line = to + (c16 / 8) * rows * 128 + key * 128;
           const int flip = (c16 >> 3) & 1;
           *reinterpret_cast<uint4 *>(line + (((c16 + flip) % 8) ^ (key & 7)) * 16) = flip ? y[1] : y[0];
           *reinterpret_cast<uint4 *>(line + (((c16 + 1 - flip) % 8) ^ (key & 7)) * 16) = flip ? y[0] : y[1];
         }
       } else {
         issue(ahead, slot);
-        if (ahead.live) ahead.step();
+        skip(ahead);
         if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
-        const int h = now.w.unit;
-        const uint16_t *src = is_v ? a.vn + now.w.b * a.vns[0] + h * a.vns[1] : a.kn + now.w.b * a.kns[0] + h * a.kns[1];
+        const uint16_t *src = is_v ? a.vn + now.w.b * a.vns[0] + now.w.unit * a.vns[1]
+                                   : a.kn + now.w.b * a.kns[0] + now.w.unit * a.kns[1];
         const int64_t st = is_v ? a.vns[2] : a.kns[2];
+        const int per = is_v ? D / 8 : 8;  // 16-byte pieces of a key in this stage
 #pragma unroll
-        for (int j = 0; j < 2 * PIECES; ++j) {
-          const int c = ct + j * 256, key = c / (D / 8), c16 = c % (D / 8);
-          const uint4 y = key < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + key * st) + c16) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(to + (c16 / 8) * KT * 128 + key * 128 + ((c16 % 8) ^ (key & 7)) * 16) = y;
+        for (int j = 0; j < 2 * CHUNKS; ++j) {
+          const int c = ct + j * 128, key = c / per, c16 = c % per;
+          const int nd = is_v ? now.piece * C::VROWS + key : key, off = is_v ? c16 : now.piece * 8 + c16;
+          const uint4 y = nd < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + nd * st) + off) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4 *>(to + (c16 / 8) * rows * 128 + key * 128 + ((c16 % 8) ^ (key & 7)) * 16) = y;
         }
       }
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.full[stage]);
-      now.step();
-      ++seq;
+      skip(now);
+      seq += 2;
+      ++turn;
     }
     cp_async_wait<0>();
   }
@@ -634,7 +682,7 @@ constexpr int TC_THREADS = 256, TC_MAX = 512;  // most items of a launch
 // One row per block: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over
 // the CTAs c of the row's unit, in their order.  D / 4 threads hold the row;
 // the groups of them take every TC_THREADS / (D / 4)-th part.
-template <int D, int KT>
+template <int D>
 __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int groups) {
   constexpr int LANES = D / 4, GROUPS = TC_THREADS / LANES;
   __shared__ int32_t s_pre[PLAN_BATCH + 1];
@@ -643,7 +691,7 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   __shared__ float4 s_o[GROUPS][LANES];
   __shared__ int s_dead;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 0) tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
+  if (warp == 0) tile_prefix<TR_KEYS>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
   if (tid == 0) s_dead = 0;
   __syncthreads();
   const int rows = a.n * a.group;
@@ -717,7 +765,7 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
 
 template <class C>
 int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t st) {
-  constexpr int smem = 1024 + C::RING + (int)sizeof(TreeSmem<C>);
+  constexpr int smem = C::RING + (int)sizeof(TreeSmem<C>);
   static_assert(smem <= 232448, "shared memory");
   auto *kernel = &k_tree_attention<C>;
   if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
@@ -727,7 +775,7 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t 
                        "k_tree_attention launch"))
     return rc;
   const unsigned rows = (unsigned)(a.batch * a.heads * a.n * a.group);
-  return op_cuda(op_launch(k_tree_combine<C::D, C::KT>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas / a.mtiles),
+  return op_cuda(op_launch(k_tree_combine<C::D>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas / a.mtiles),
                  "k_tree_combine launch");
 }
 
@@ -739,8 +787,8 @@ int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, cuda
 }
 
 // CTAs of a launch: one per SM, whole items (or fewer, the most places that the list can have).
-int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t t, int64_t dim) {
-  const int64_t kt = dim == 256 ? 64 : 128, most = batch * heads * ((t + kt - 1) / kt + 1 + TR_IDLE);
+int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t t) {
+  const int64_t most = batch * heads * ((t + TR_KEYS - 1) / TR_KEYS + 1 + TR_IDLE);
   const int64_t c = sms > mtiles ? (sms / mtiles < TC_MAX ? sms / mtiles : TC_MAX) : 1;
   return (most < c ? most : c) * mtiles;
 }
@@ -752,7 +800,7 @@ int sm_count(int device, int *sms) {
 int64_t tree_workspace(int sms, const SkvTree *d) {
   const int64_t rows = d->n * (d->heads / d->kv_heads), per = rows < TR_ROWS ? rows : TR_ROWS;
   const int64_t batch = d->batch < PLAN_BATCH ? d->batch : PLAN_BATCH;
-  const int64_t slots = 2 * tree_ctas(sms, batch, d->kv_heads, (rows + TR_ROWS - 1) / TR_ROWS, d->tokens, d->dim);
+  const int64_t slots = 2 * tree_ctas(sms, batch, d->kv_heads, (rows + TR_ROWS - 1) / TR_ROWS, d->tokens);
   return slots * per * (d->dim + 2) * 4;
 }
 
@@ -829,13 +877,13 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
     a.parents = static_cast<const int32_t *>(d->parents) + b0 * a.ps[0];
     a.out = static_cast<uint16_t *>(d->out) + b0 * d->n * d->heads * d->dim;
     a.lse = static_cast<float *>(d->lse) + b0 * d->n * d->heads;
-    const int ctas = (int)tree_ctas(sms, nb, a.heads, a.mtiles, d->tokens, d->dim);
+    const int ctas = (int)tree_ctas(sms, nb, a.heads, a.mtiles, d->tokens);
     a.part = static_cast<float *>(d->workspace);
     a.ml = reinterpret_cast<float2 *>(a.part + 2 * (int64_t)ctas * a.rows * d->dim);
     TreeMaps maps{};
     int rc = SKV_OK;
     if (!f8) {
-      const int kt = d->dim == 256 ? 64 : 128;
+      const int pieces = (int)d->dim / 64;
       const struct {
         CUtensorMap *map;
         const void *base;
@@ -847,7 +895,8 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
                    {&maps.vn, a.vn, d->v_stride, d->n}};
       for (int i = 0; i < 4 && !rc; ++i) {
         const int64_t step[3] = {four[i].s[2], four[i].s[1], four[i].s[0]};
-        rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step, kt, (int)d->dim / 64);
+        rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step,
+                      i % 2 ? TR_KEYS / pieces : TR_KEYS, i % 2 ? pieces : 1);  // K: one piece, V: all of a row
         a.along[i][0] = d->kv_heads > 1 && four[i].s[1] ? 1 : 0;
         a.along[i][1] = nb > 1 && four[i].s[0] ? 1 : 0;
       }

@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   uint8_t *ring = queries + SUB * a.cols * 128;
   uint8_t *raw = ring + a.stages * WT_PIECE;
   WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(raw + (F8 ? WT_RAW * WT_PIECE / 2 : 0));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int stages = a.stages;
   if (warp == 0) {
     tile_prefix<WT_KEYS>(a.lengths, a.len_stride, 0, a.t, a.batch, 0, s.len, s.pre);
@@ -101,63 +101,61 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 
   if (warp == 0 && !F8) {
     // ---- loads
-    if (lane == 0) {
-      Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
-      uint32_t seq = 0;
-      int stage = 0;
-      uint32_t turn = 0;
-      bool ok = true;
-      while (ok && w.next())
-        for (int i = 0; i < w.count && ok; ++i)
-          for (int sub = 0; sub < SUB; ++sub) {
-            if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
-            bar_expect(&s.full[stage], WT_PIECE);
-            tma_load(ring + stage * WT_PIECE, &map, (w.tile + i) * WT_KEYS, sub, w.unit * a.along[0],
-                     w.b * a.along[1], &s.full[stage]);
-            ++seq;
-            if (++stage == stages) stage = 0, turn ^= 1;
-          }
-      if (!ok)  // gave up: the copies in flight still land before the CTA ends
-        for (uint32_t back = 1; back <= (uint32_t)stages && back <= seq; ++back) {
-          const uint32_t q = seq - back;
-          const unsigned long long t0 = timer_ns();
-          while (!bar_try(&s.full[q % stages], (q / stages) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
-          }
+    const uint32_t one = elect_lane();
+    Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
+    uint32_t seq = 0;
+    int stage = 0;
+    uint32_t turn = 0;
+    bool ok = true;
+    while (ok && w.next())
+      for (int i = 0; i < w.count && ok; ++i)
+        for (int sub = 0; sub < SUB; ++sub) {
+          if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
+          tma_load(one, ring + stage * WT_PIECE, &map, (w.tile + i) * WT_KEYS, sub, w.unit * a.along[0],
+                   w.b * a.along[1], &s.full[stage], WT_PIECE);
+          ++seq;
+          if (++stage == stages) stage = 0, turn ^= 1;
         }
-    }
+    if (!ok)  // gave up: the copies in flight still land before the CTA ends
+      for (uint32_t back = 1; back <= (uint32_t)stages && back <= seq; ++back) {
+        const uint32_t q = seq - back;
+        const unsigned long long t0 = timer_ns();
+        while (!bar_try(&s.full[q % stages], (q / stages) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+        }
+      }
   } else if (warp == 1) {
     // ---- tensor core
-    if (lane == 0) {
-      Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
-      const uint32_t desc = mma_desc(WT_KEYS, a.cols, false);
-      const uint32_t q0 = s_addr(queries);
-      int stage = 0;
-      uint32_t turn = 0, gt = 0, seg = 0;
-      while (w.next()) {
-        wait(&s.q_ready, seg & 1);
-        for (int i = 0; i < w.count; ++i, ++gt) {
-          const uint32_t buf = gt & 1;
-          wait(&s.acc_free[buf], ((gt >> 1) & 1) ^ 1);
-          for (int sub = 0; sub < SUB; ++sub) {
-            wait(&s.full[stage], turn);
-            tc_fence_after();
-            const uint32_t k0 = s_addr(ring + stage * WT_PIECE), qs = q0 + sub * a.cols * 128;
+    const uint32_t one = elect_lane();
+    Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
+    const uint32_t desc = mma_desc(WT_KEYS, a.cols, false);
+    const uint32_t q0 = s_addr(queries), ring0 = s_addr(ring);
+    int stage = 0;
+    uint32_t turn = 0, gt = 0, seg = 0;
+    while (w.next()) {
+      wait(&s.q_ready, seg & 1);
+      for (int i = 0; i < w.count; ++i, ++gt) {
+        const uint32_t buf = gt & 1;
+        wait(&s.acc_free[buf], ((gt >> 1) & 1) ^ 1);
+        tc_fence_after();
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              mma_ss(tmem + buf * WT_ROWS, smem_desc(k0 + ks * 32, 16), smem_desc(qs + ks * 32, 16), desc, sub + ks > 0);
-            mma_commit(&s.empty[stage]);
-            if (++stage == stages) stage = 0, turn ^= 1;
-          }
-          mma_commit(&s.acc_full[buf]);
+        for (int sub = 0; sub < SUB; ++sub) {
+          wait(&s.full[stage], turn);
+          const uint32_t k0 = ring0 + stage * WT_PIECE, qs = q0 + sub * a.cols * 128;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            mma_ss(one, tmem + buf * WT_ROWS, smem_desc(k0 + ks * 32, 16), smem_desc(qs + ks * 32, 16), desc, sub + ks > 0);
+          mma_commit(one, &s.empty[stage]);
+          if (++stage == stages) stage = 0, turn ^= 1;
         }
-        mma_commit(&s.q_free);
-        ++seg;
+        mma_commit(one, &s.acc_full[buf]);
       }
-      if (*abort) {  // what was issued ends before tensor memory is given back
-        mma_commit(&s.drain);
-        const unsigned long long t0 = timer_ns();
-        while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
-        }
+      mma_commit(one, &s.q_free);
+      ++seg;
+    }
+    if (*abort) {  // what was issued ends before tensor memory is given back
+      mma_commit(one, &s.drain);
+      const unsigned long long t0 = timer_ns();
+      while (!bar_try(&s.drain, 0) && timer_ns() - t0 < WAIT_NS / 4) {
       }
     }
   } else if (warp < 4) {

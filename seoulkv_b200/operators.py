@@ -304,7 +304,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if not b:
         return out, lse
     lib = _native.load()
-    size = _tree_workspace(dev.index, min(b, 512), n, hq, hkv, d, t)
+    size = _tree_workspace(dev.index, b, n, hq, hkv, d, t)
     work = torch.empty(size, dtype=torch.uint8, device=dev)
     packed = _TREE.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
