@@ -90,6 +90,19 @@ __device__ __forceinline__ void tma_load(uint32_t one, void *dst, const CUtensor
       : "memory");
 }
 
+// The elected lane announces `bytes` on `bar` and loads the box at (byte, row,
+// y, z) of a make_byte_map() map.
+__device__ __forceinline__ void tma_load_bytes(uint32_t one, void *dst, const CUtensorMap *map, int byte, int row, int y,
+                                               int z, uint64_t *bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %7, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%6], %8;\n\t"
+      "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];\n\t}" ::"r"(s_addr(dst)),
+      "l"(map), "r"(byte), "r"(row), "r"(y), "r"(z), "r"(s_addr(bar)), "r"(one), "r"(bytes)
+      : "memory");
+}
+
 // ---- tensor memory and tcgen05.mma ----------------------------------------
 
 __device__ __forceinline__ void tmem_alloc(uint32_t *where, uint32_t columns) {
@@ -186,15 +199,55 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
   return y;
 }
-// Two FP8 e4m3 codes to two BF16 (exact).
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint16_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
-  float lo, hi;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
-      : "=f"(lo), "=f"(hi)
-      : "r"(h));
-  return pack_bf16(lo, hi);
+// 16 FP8 e4m3 codes to BF16, exactly.  The conversion instructions run at 16
+// lanes a cycle and would take longer than the product that follows (8192
+// codes: 1024 cycles of an SM), so the bits are moved instead: sign, exponent
+// and mantissa of a code, put at a BF16's places, are its value times 2^-120
+// (subnormal codes are subnormal there too), and the product with 2^120 is
+// exact.  The one code that is not a number comes out as 480 and is put right
+// where a piece has one.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t x, uint32_t pick) {
+  // (pick: two bytes, each with its sign spread over the byte above)
+  uint32_t bits, y;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(bits) : "r"(x), "r"(pick));
+  bits = (bits << 4) & 0x87f087f0u;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(bits), "r"(0x7b807b80u));
+  return y;
+}
+// (nan: bits 7, 15, 23, 31 are raised where a code is not a number)
+__device__ __forceinline__ void e4m3_to_bf16(const uint4 &x, uint4 &lo, uint4 &hi, uint32_t &nan) {
+  lo = make_uint4(e4m3_pair(x.x, 0x9180), e4m3_pair(x.x, 0xb3a2), e4m3_pair(x.y, 0x9180), e4m3_pair(x.y, 0xb3a2));
+  hi = make_uint4(e4m3_pair(x.z, 0x9180), e4m3_pair(x.z, 0xb3a2), e4m3_pair(x.w, 0x9180), e4m3_pair(x.w, 0xb3a2));
+  nan |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u);
+  nan |= ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+}
+constexpr uint32_t E4M3_NAN = 0x80808080u;
+// 480 to NaN, in 16 bytes that e4m3_to_bf16 wrote.
+static __device__ __noinline__ void e4m3_put_nan(uint4 *at) {
+  uint32_t *y = reinterpret_cast<uint32_t *>(at);
+  for (int i = 0; i < 4; ++i) {
+    if ((y[i] & 0x7fffu) == 0x43f0u) y[i] |= 0x7fffu;
+    if ((y[i] & 0x7fff0000u) == 0x43f00000u) y[i] |= 0x7fff0000u;
+  }
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
+  return y;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
 }
 
 // ---- cp.async --------------------------------------------------------------
@@ -217,6 +270,10 @@ __device__ __forceinline__ void cp_async_wait() {
 // with one element.
 int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
              const int64_t *stride, int box_rows, int pieces);
+// Map of [z][y][rows][bytes] with byte strides {row, y, z}, boxes of box_rows
+// rows of box_bytes bytes one after the other.
+int make_byte_map(CUtensorMap *map, const void *base, int64_t bytes, int64_t rows, int64_t ny, int64_t nz,
+                  const int64_t *stride, int box_rows, int box_bytes);
 // The device's status word (set by waits that gave up).
 int status_word(int device, uint32_t **word);
 

@@ -50,11 +50,13 @@ int status_word(int device, uint32_t **word) {
   return SKV_OK;
 }
 
-int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
-             const int64_t *stride, int box_rows, int pieces) {
-  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+namespace {
+
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                            const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
   static const Encode encode = [] {
     void *fn = nullptr;
     cudaDriverEntryPointQueryResult found;
@@ -63,6 +65,14 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
       fn = nullptr;
     return reinterpret_cast<Encode>(fn);
   }();
+  return encode;
+}
+
+}  // namespace
+
+int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
+             const int64_t *stride, int box_rows, int pieces) {
+  const Encode encode = encoder();
   if (!encode) return op_fail(SKV_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
   const int64_t n[3] = {rows, ny, nz};
   cuuint64_t size[5] = {64, 1, (cuuint64_t)dim / 64, 1, 1}, step[4] = {0, 128, 0, 0};
@@ -79,11 +89,30 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
   return r == CUDA_SUCCESS ? SKV_OK : op_fail(SKV_E_INVALID, "cuTensorMapEncodeTiled: error %d", (int)r);
 }
 
+int make_byte_map(CUtensorMap *map, const void *base, int64_t bytes, int64_t rows, int64_t ny, int64_t nz,
+                  const int64_t *stride, int box_rows, int box_bytes) {
+  const Encode encode = encoder();
+  if (!encode) return op_fail(SKV_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const int64_t n[3] = {rows, ny, nz};
+  cuuint64_t size[4] = {(cuuint64_t)bytes, 1, 1, 1}, step[3];
+  for (int i = 0; i < 3; ++i) {
+    const bool one = n[i] == 1 || stride[i] == 0;
+    size[i + 1] = one ? 1 : (cuuint64_t)n[i];
+    step[i] = one ? (cuuint64_t)bytes : (cuuint64_t)stride[i];
+  }
+  const cuuint32_t box[4] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, 1, 1}, unit[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), size, step, box, unit,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SKV_OK : op_fail(SKV_E_INVALID, "cuTensorMapEncodeTiled: error %d", (int)r);
+}
+
 namespace {
 
 constexpr int TR_NODES = SKV_TREE_MAX_NODES;
 constexpr int TR_KEYS = 128;   // keys of a tile
 constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
+constexpr int TR_GROUP = 64;   // threads that turn an FP8 stage into BF16
 constexpr int TR_IDLE = 1;     // what starting and ending a unit costs, in tiles
 
 template <int D_, bool F8_>
@@ -97,7 +126,7 @@ struct TreeCfg {
   static constexpr int RAW = STAGE / 2;   // an FP8 stage before its conversion
   static constexpr int NRAW = F8 ? 8 : 0;
   static constexpr int NSTAGE = F8 ? 6 : D == 256 ? 10 : D == 128 ? 11 : 12;
-  static constexpr int THREADS = F8 ? 640 : 384;
+  static constexpr int THREADS = F8 ? 576 : 384;  // FP8: warps 2, 3 and 12.. convert
   static constexpr int COL_S = 256;       // tensor memory columns: O, then two score tiles (P over S)
   static constexpr int QBYTES = TR_ROWS * D * 2;
   static constexpr int RING = QBYTES + NSTAGE * STAGE + NRAW * RAW;
@@ -110,9 +139,7 @@ struct TreeMaps {
 struct TreeArgs {
   const uint16_t *q;
   int64_t qs[3];  // element strides (sequence, node, head)
-  const uint8_t *k8, *v8;
-  int64_t k8s[3], v8s[3];  // FP8 caches: byte strides (sequence, head, token)
-  const CellDev *cells;    // the engine's FP8 records instead (cell = sequence * heads + head)
+  const CUtensorMap *cell_maps;  // FP8 caches in separate buffers: K and V maps of cell = sequence * heads + head
   const uint16_t *kn, *vn;
   int64_t kns[3], vns[3];  // element strides (sequence, head, node)
   const int32_t *lengths;
@@ -133,11 +160,12 @@ struct TreeArgs {
 template <class C>
 struct TreeSmem {
   uint64_t full[C::NSTAGE], empty[C::NSTAGE];
+  uint64_t raw_full[C::NRAW + 1], raw_empty[C::NRAW + 1];  // (+ 1: no empty arrays without FP8)
   uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;
   uint64_t anc[TR_NODES];      // nodes that node i sees (0: unused)
   unsigned long long bad;      // nodes with a value that is not finite
   float share[2][TR_ROWS];     // maxima and sums that the two threads of a row exchange
-  int32_t up[TR_NODES];
+  int8_t up[TR_NODES];         // the node before (-1: the cache, -2: none, unused)
   uint32_t tmem;
   uint32_t abort;
   int32_t pre[PLAN_BATCH + 1];  // places of the sequences before (one unit's worth)
@@ -169,18 +197,26 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 
   if (warp == 0) {
     tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
-    if (lane == 0 && !C::F8) {
-      tma_prefetch_map(&maps.k);
-      tma_prefetch_map(&maps.v);
-      tma_prefetch_map(&maps.kn);
-      tma_prefetch_map(&maps.vn);
+    if (lane == 0) {
+      if (!a.cell_maps) {
+        tma_prefetch_map(&maps.k);
+        tma_prefetch_map(&maps.v);
+      }
+      if (!C::F8) {
+        tma_prefetch_map(&maps.kn);
+        tma_prefetch_map(&maps.vn);
+      }
     }
   } else if (warp == 1) {
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
     for (int i = 0; i < C::NSTAGE; ++i) {
-      bar_init(&s.full[i], C::F8 ? 4 : 1);
+      bar_init(&s.full[i], C::F8 ? TR_GROUP / 32 : 1);
       bar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < C::NRAW; ++i) {
+      bar_init(&s.raw_full[i], 1);
+      bar_init(&s.raw_empty[i], TR_GROUP / 32);
     }
     bar_init(&s.q_ready, 8);
     bar_init(&s.drain, 1);
@@ -211,9 +247,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     return max(0, min(n, a.t));
   };
 
-  if (warp == 0 && !C::F8) {
-    // ---- loads
+  if (warp == 0) {
+    // ---- loads: BF16 stages into the ring, FP8 stages (cache tiles alone) beside it
     const uint32_t one = elect_lane();
+    constexpr int SLOTS = C::F8 ? C::NRAW : C::NSTAGE;
+    uint64_t *const landed = C::F8 ? s.raw_full : s.full, *const freed = C::F8 ? s.raw_empty : s.empty;
     Walk w = walk;
     uint32_t seq = 0;
     bool ok = true;
@@ -223,23 +261,29 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         int i;
         tile_at(p, w.count, is_v, i);
         const bool nodes = w.tile + i == w.tiles - 1;
+        if (C::F8 && nodes) continue;
         const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
         const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
+        if (C::F8 && a.cell_maps) map = a.cell_maps + 2 * ((int64_t)w.b * a.heads + w.unit) + is_v;
         const int row = nodes ? 0 : (w.tile + i) * KT;
         const int y = w.unit * a.along[which][0], z = w.b * a.along[which][1];
         for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
-          const int stage = seq % C::NSTAGE;
-          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
-          tma_load(one, ring + stage * C::STAGE, map, row + (is_v ? piece * C::VROWS : 0), is_v ? 0 : piece, y, z,
-                   &s.full[stage], C::STAGE);
+          const int slot = seq % SLOTS;
+          if (!(ok = wait(&freed[slot], ((seq / SLOTS) & 1) ^ 1))) break;
+          if (C::F8)
+            tma_load_bytes(one, raw + slot * C::RAW, map, is_v ? 0 : piece * 64, row + (is_v ? piece * C::VROWS : 0), y,
+                           z, &landed[slot], C::RAW);
+          else
+            tma_load(one, ring + slot * C::STAGE, map, row + (is_v ? piece * C::VROWS : 0), is_v ? 0 : piece, y, z,
+                     &landed[slot], C::STAGE);
         }
       }
     }
     if (!ok)  // gave up: the copies in flight still land before the CTA ends
-      for (uint32_t back = 1; back <= C::NSTAGE && back <= seq; ++back) {
+      for (uint32_t back = 1; back <= SLOTS && back <= seq; ++back) {
         const uint32_t q = seq - back;
         const unsigned long long t0 = timer_ns();
-        while (!bar_try(&s.full[q % C::NSTAGE], (q / C::NSTAGE) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+        while (!bar_try(&landed[q % SLOTS], (q / SLOTS) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
         }
       }
   } else if (warp == 1) {
@@ -276,10 +320,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
           const uint32_t stage = seq % C::NSTAGE;
           wait(&s.full[stage], (seq / C::NSTAGE) & 1);
-          const uint32_t v0 = ring0 + stage * C::STAGE, p0 = tmem + C::COL_S + buf * KT + piece * (C::VROWS / 2);
+          const uint32_t v0 = ring0 + stage * C::STAGE, p0 = tmem + C::COL_S + buf * KT;
 #pragma unroll
-          for (int ks = 0; ks < C::VROWS / 16; ++ks)
-            mma_ts(one, tmem, p0 + 8 * ks, smem_desc(v0 + ks * 2048, C::VROWS * 128), DESC_O, i > 0 || piece + ks > 0);
+          for (int ks = 0; ks < C::VROWS / 16; ++ks) {
+            const int key = piece * C::VROWS + 16 * ks;  // P of keys 64.. starts at column 64
+            mma_ts(one, tmem, p0 + key / 64 * 64 + key % 64 / 2, smem_desc(v0 + ks * 2048, C::VROWS * 128), DESC_O,
+                   i > 0 || key > 0);
+          }
           mma_commit(one, &s.empty[stage]);
         }
         mma_commit(one, &s.o_done[buf]);
@@ -343,7 +390,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         for (int step = 1;; step <<= 1) {
           if (st < TR_NODES) {
             s.anc[st] = mask;
-            s.up[st] = up;
+            s.up[st] = (int8_t)up;
           }
           asm volatile("bar.sync 1, 256;" ::: "memory");
           if (step >= a.n) break;
@@ -370,19 +417,37 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const uint64_t keep = nodes ? (half ? 0 : see) : v64 >= 64 ? ~0ull : v64 > 0 ? (1ull << v64) - 1 : 0;
         done(s.s_full, gt + i);
         if (warp_on) {
+          // S stays in registers between the maximum and the exponentials
+          // where there are enough of them, and is read again where not (FP8)
+          constexpr int HELD = C::F8 ? 32 : 64;
+          uint32_t x[HELD];
           float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(x, at + 64 * half + 32 * c);
-            tmem_wait_ld();
-            const uint32_t bits = (uint32_t)(keep >> (32 * c));
+          auto load = [&](int c) {
+            uint32_t(&z)[32] = *reinterpret_cast<uint32_t(*)[32]>(x + (C::F8 ? 0 : 32 * c));
+            tmem_ld32(z, at + 64 * half + 32 * c);
+          };
+          auto maximum = [&](int c) {
+            const uint32_t *z = x + (C::F8 ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
             if (whole) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+              for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(z[j]));
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) top = fmaxf(top, bits >> j & 1 ? __uint_as_float(x[j]) : -INFINITY);
+              for (int j = 0; j < 32; ++j) top = fmaxf(top, bits >> j & 1 ? __uint_as_float(z[j]) : -INFINITY);
+            }
+          };
+          if (!C::F8) {
+            load(0);
+            load(1);
+            tmem_wait_ld();
+            maximum(0);
+            maximum(1);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              load(c);
+              tmem_wait_ld();
+              maximum(c);
             }
           }
           s.share[half][row] = top;
@@ -396,45 +461,47 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             const float f = move ? exp2_fast(m - top) : 1.0f;
             done(s.o_done, gt + i - 1);
 #pragma unroll 1
-            for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
-              uint32_t x[32];
-              tmem_ld32(x, lanes + 32 * c);
+            for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
+              uint32_t o[16];
+              tmem_ld16(o, lanes + 16 * c);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
-              tmem_st32(lanes + 32 * c, x);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(lanes + 16 * c, o);
             }
             l *= f;
           }
           if (move) m = top;
           const float base2 = m == -INFINITY ? 0.0f : m;
-          uint32_t y[32];
+          const uint64_t scale2 = pack2(a.c2, a.c2), minus2 = pack2(-base2, -base2);
+          uint64_t sum = 0;  // two sums
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(x, at + 64 * half + 32 * c);
-            tmem_wait_ld();
-            const uint32_t bits = (uint32_t)(keep >> (32 * c));
-            float sum0 = 0.0f, sum1 = 0.0f;
+            if (C::F8) {
+              load(c);
+              tmem_wait_ld();
+            }
+            const uint32_t *z = x + (C::F8 ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
+            uint32_t y[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              float p0 = exp2_fast(fmaf(__uint_as_float(x[j]), a.c2, -base2));
-              float p1 = exp2_fast(fmaf(__uint_as_float(x[j + 1]), a.c2, -base2));
+              float p0, p1;
+              unpack2(fma2(pack2(__uint_as_float(z[j]), __uint_as_float(z[j + 1])), scale2, minus2), p0, p1);
+              p0 = exp2_fast(p0);
+              p1 = exp2_fast(p1);
               if (!whole) {
                 p0 = bits >> j & 1 ? p0 : 0.0f;
                 p1 = bits >> (j + 1) & 1 ? p1 : 0.0f;
               }
-              sum0 += p0;
-              sum1 += p1;
-              y[16 * c + j / 2] = pack_bf16(p0, p1);
+              sum = add2(sum, pack2(p0, p1));
+              y[j / 2] = pack_bf16(p0, p1);
             }
-            l += sum0 + sum1;
+            // (over this thread's own, already read scores)
+            tmem_st16(at + 64 * half + 16 * c, y);
           }
-          // P goes over the first half of S: only when both threads have read theirs
-          tc_fence_before();
-          asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-          tc_fence_after();
-          tmem_st32(at + 32 * half, y);
+          float s0, s1;
+          unpack2(sum, s0, s1);
+          l += s0 + s1;
           tmem_wait_st();
           tc_fence_before();
         }
@@ -536,136 +603,104 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       base += 2 * n * C::PIECES;
       gt += n;
     }
-  } else if (C::F8 && warp >= 12) {
-    // ---- FP8 caches: each thread copies its own 16-code pieces ahead with
-    // cp.async (no barrier between the copy and its use), turns them into
-    // BF16 and puts them where TMA would have put a BF16 stage.  Two groups of
-    // four warps take the stages in turn.
-    constexpr int CHUNKS = C::F8 ? C::RAW / 16 / 128 : 1;  // of one thread and stage
-    constexpr int AHEAD = C::F8 ? C::NRAW / 2 : 1;         // stages of a group in flight
-    const int ct = (tid - 384) & 127, grp = (tid - 384) >> 7;
-    struct Stages {
-      Walk w;
-      int p = 0, piece = 0, len = 0;
-      bool live;
-    };
-    auto start = [&](Stages &x) {
-      x.live = x.w.next();
-      if (x.live) x.len = length(x.w.b);
-    };
-    auto step = [&](Stages &x) {
-      if (++x.piece < C::PIECES) return;
-      x.piece = 0;
-      if (++x.p < 2 * x.w.count) return;
-      x.p = 0;
-      start(x);
-    };
-    auto skip = [&](Stages &x) {  // to this group's next stage
-      if (x.live) step(x);
-      if (x.live) step(x);
-    };
-    Stages ahead{walk}, now{walk};
-    start(ahead);
-    if (grp && ahead.live) step(ahead);
-    now = ahead;
-    // a stage's 16-byte pieces: K 4 a key (64 dimensions), V D / 16 a key
-    auto place = [&](int c, bool is_v, int piece, int &key, int &dim) {
-      key = is_v ? piece * C::VROWS + c / (D / 16) : c / 4;
-      dim = is_v ? (c % (D / 16)) * 16 : piece * 64 + (c % 4) * 16;
-    };
-    auto issue = [&](const Stages &x, int slot) {
-      if (x.live) {
+  } else if (C::F8 && (warp >= 12 || warp == 2 || warp == 3)) {
+    // ---- FP8 caches: groups of TR_GROUP threads take the stages in turn, turn
+    // their codes into BF16 and put them where TMA puts a BF16 stage.  The
+    // nodes' own K and V are BF16 and are copied.
+    constexpr int GROUPS = 4, CHUNKS = C::RAW / 16 / TR_GROUP;  // 16-code pieces of one thread and stage
+    const int ct = tid % TR_GROUP, grp = warp < 4 ? 0 : (warp - 10) / 2;
+    static_assert(TR_GROUP == 64 && GROUPS % C::PIECES == 0, "groups of two warps, one stage each");
+    // Piece j of this thread: K key ct / 4 + KSTEP j, dimensions 16 (ct % 4)..
+    // of the stage's 64 (KSTEP is a multiple of 8: one swizzle for all j); V
+    // key CHUNKS (ct / VPER) + j of the stage's, dimensions 16 (ct % VPER)...
+    constexpr int VPER = D / 16, KSTEP = TR_GROUP / 4;
+    static_assert(KSTEP % 8 == 0 && CHUNKS == 8, "swizzle of an FP8 stage's pieces");
+    const int key_k = ct / 4, key_v = ct / VPER * CHUNKS;
+    const int unit_k = 2 * (ct % 4), unit_v = 2 * (ct % VPER);  // the first of its two 16-byte places in a row
+    // neighbouring pieces of different 64-dimension parts would meet in the
+    // same banks: every other part writes its halves in opposite order
+    const int flip = (unit_v >> 3) & 1;
+    const int raw_k = ct * 16, raw_v = key_v * D + ct % VPER * 16;
+    const int to_k0 = key_k * 128 + ((unit_k ^ key_k) & 7) * 16, to_k1 = key_k * 128 + (((unit_k + 1) ^ key_k) & 7) * 16;
+    const int to_v = (unit_v / 8) * C::VROWS * 128 + key_v * 128;
+    constexpr uint32_t SLOTS = C::F8 ? C::NRAW : 1;
+    const int piece = grp % C::PIECES;
+    Walk w = walk;
+    uint32_t base = 0, raw_base = 0;  // stages, and FP8 stages, of the segments before
+    bool ok = true;
+    while (ok && w.next()) {
+      const int n = w.count, len = length(w.b);
+      const int k_nodes = w.tile + n == w.tiles ? pos_k(n - 1) : 2 * n;  // place of the nodes' K (they are in the last tile)
+      for (int p = grp / C::PIECES; p < 2 * n; p += GROUPS / C::PIECES) {
         bool is_v;
         int i;
-        tile_at(x.p, x.w.count, is_v, i);
-        if (x.w.tile + i < x.w.tiles - 1) {
-          const uint8_t *src;
-          int64_t st;
-          if (a.cells) {
-            src = a.cells[x.w.b * a.heads + x.w.unit].kv8 + (is_v ? D : 0);
-            st = REC;
+        tile_at(p, n, is_v, i);
+        const uint32_t seq = base + p * C::PIECES + piece, stage = seq % C::NSTAGE;
+        uint8_t *to = ring + stage * C::STAGE;
+        if (w.tile + i < w.tiles - 1) {
+          const uint32_t raw_at = raw_base + (p - (p > k_nodes)) * C::PIECES + piece, slot = raw_at % SLOTS;
+          if (!(ok = wait(&s.raw_full[slot], (raw_at / SLOTS) & 1))) break;
+          uint4 v[CHUNKS];
+          {
+            const uint8_t *from = raw + slot * C::RAW + (is_v ? raw_v : raw_k);
+            const int gap = is_v ? D : KSTEP * 64;
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) v[j] = *reinterpret_cast<const uint4 *>(from + j * gap);
+          }
+          __syncwarp();
+          if (lane == 0) bar_arrive(&s.raw_empty[slot]);
+          const int left = len - (w.tile + i) * KT - (is_v ? piece * C::VROWS + key_v : key_k);  // keys from this thread's first
+          const int gap = is_v ? 1 : KSTEP;
+          if (left < CHUNKS * gap) {  // behind the length: zeros
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j)
+              if (gap * j >= left) v[j] = make_uint4(0, 0, 0, 0);
+          }
+          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
+          uint32_t nan = 0;
+          if (is_v) {
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) {
+              uint4 y0, y1;
+              e4m3_to_bf16(v[j], y0, y1, nan);
+              uint8_t *at = to + to_v + j * 128;
+              *reinterpret_cast<uint4 *>(at + (((unit_v + flip) & 7) ^ j) * 16) = flip ? y1 : y0;
+              *reinterpret_cast<uint4 *>(at + (((unit_v + 1 - flip) & 7) ^ j) * 16) = flip ? y0 : y1;
+            }
           } else {
-            src = is_v ? a.v8 + x.w.b * a.v8s[0] + x.w.unit * a.v8s[1] : a.k8 + x.w.b * a.k8s[0] + x.w.unit * a.k8s[1];
-            st = is_v ? a.v8s[2] : a.k8s[2];
+#pragma unroll
+            for (int j = 0; j < CHUNKS; ++j) {
+              uint4 y0, y1;
+              e4m3_to_bf16(v[j], y0, y1, nan);
+              *reinterpret_cast<uint4 *>(to + to_k0 + j * KSTEP * 128) = y0;
+              *reinterpret_cast<uint4 *>(to + to_k1 + j * KSTEP * 128) = y1;
+            }
           }
-          const int t0 = (x.w.tile + i) * KT;
-#pragma unroll
-          for (int j = 0; j < CHUNKS; ++j) {
-            int key, dim;
-            place(ct + j * 128, is_v, x.piece, key, dim);
-            if (t0 + key < x.len) cp_async16(raw + slot * C::RAW + (ct + j * 128) * 16, src + (t0 + key) * st + dim);
+          if (nan & E4M3_NAN)
+            for (int j = 0; j < CHUNKS; ++j)
+              for (int u = 0; u < 2; ++u)
+                e4m3_put_nan(reinterpret_cast<uint4 *>(
+                    to + (is_v ? to_v + j * 128 + (((unit_v + u) & 7) ^ j) * 16 : (u ? to_k1 : to_k0) + j * KSTEP * 128)));
+        } else {
+          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
+          const uint16_t *src = is_v ? a.vn + w.b * a.vns[0] + w.unit * a.vns[1] : a.kn + w.b * a.kns[0] + w.unit * a.kns[1];
+          const int64_t st = is_v ? a.vns[2] : a.kns[2];
+          const int rows = is_v ? C::VROWS : KT, per = is_v ? D / 8 : 8;  // 16-byte units of a key in this stage
+#pragma unroll 4
+          for (int c = ct; c < C::STAGE / 16; c += TR_GROUP) {
+            const int key = c / per, c16 = c % per;
+            const int nd = is_v ? piece * C::VROWS + key : key, off = is_v ? c16 : piece * 8 + c16;
+            const uint4 y = nd < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + nd * st) + off) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(to + (c16 / 8) * rows * 128 + key * 128 + ((c16 ^ key) & 7) * 16) = y;
           }
         }
+        async_fence();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.full[stage]);
       }
-      cp_async_commit();
-    };
-    for (int i = 0; i < AHEAD; ++i) {
-      issue(ahead, grp * AHEAD + i);
-      skip(ahead);
+      base += 2 * n * C::PIECES;
+      raw_base += (2 * n - (k_nodes < 2 * n ? 2 : 0)) * C::PIECES;
     }
-    uint32_t seq = grp, turn = 0;
-    while (now.live) {
-      const int stage = seq % C::NSTAGE, slot = grp * AHEAD + (int)(turn % AHEAD);
-      bool is_v;
-      int i;
-      tile_at(now.p, now.w.count, is_v, i);
-      const bool nodes = now.w.tile + i == now.w.tiles - 1;
-      uint8_t *to = ring + stage * C::STAGE;
-      const int rows = is_v ? C::VROWS : KT;  // of a 64-dimension piece in the stage
-      cp_async_wait<AHEAD - 1>();
-      if (!nodes) {
-        const int left = now.len - (now.w.tile + i) * KT;
-        uint4 v[CHUNKS];
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-          int key, dim;
-          place(ct + j * 128, is_v, now.piece, key, dim);
-          v[j] = key < left ? *reinterpret_cast<const uint4 *>(raw + slot * C::RAW + (ct + j * 128) * 16) : make_uint4(0, 0, 0, 0);
-        }
-        issue(ahead, slot);
-        skip(ahead);
-        if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-          const int c = ct + j * 128;
-          const int key = is_v ? c / (D / 16) : c / 4, c16 = 2 * (is_v ? c % (D / 16) : c % 4);
-          const uint32_t *x = reinterpret_cast<const uint32_t *>(&v[j]);
-          uint4 y[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            y[u] = make_uint4(e4m3x2_to_bf16x2((uint16_t)x[2 * u]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u] >> 16)),
-                              e4m3x2_to_bf16x2((uint16_t)x[2 * u + 1]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u + 1] >> 16)));
-          // neighbouring threads write the two halves in opposite order where
-          // they would meet in the same banks (pieces of different subtiles)
-          uint8_t *line = to + (c16 / 8) * rows * 128 + key * 128;
-          const int flip = (c16 >> 3) & 1;
-          *reinterpret_cast<uint4 *>(line + (((c16 + flip) % 8) ^ (key & 7)) * 16) = flip ? y[1] : y[0];
-          *reinterpret_cast<uint4 *>(line + (((c16 + 1 - flip) % 8) ^ (key & 7)) * 16) = flip ? y[0] : y[1];
-        }
-      } else {
-        issue(ahead, slot);
-        skip(ahead);
-        if (!wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1)) break;
-        const uint16_t *src = is_v ? a.vn + now.w.b * a.vns[0] + now.w.unit * a.vns[1]
-                                   : a.kn + now.w.b * a.kns[0] + now.w.unit * a.kns[1];
-        const int64_t st = is_v ? a.vns[2] : a.kns[2];
-        const int per = is_v ? D / 8 : 8;  // 16-byte pieces of a key in this stage
-#pragma unroll
-        for (int j = 0; j < 2 * CHUNKS; ++j) {
-          const int c = ct + j * 128, key = c / per, c16 = c % per;
-          const int nd = is_v ? now.piece * C::VROWS + key : key, off = is_v ? c16 : now.piece * 8 + c16;
-          const uint4 y = nd < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + nd * st) + off) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4 *>(to + (c16 / 8) * rows * 128 + key * 128 + ((c16 % 8) ^ (key & 7)) * 16) = y;
-        }
-      }
-      async_fence();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&s.full[stage]);
-      skip(now);
-      seq += 2;
-      ++turn;
-    }
-    cp_async_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -820,9 +855,10 @@ int check_tree(const SkvTree *d) {
 
 }  // namespace
 
-// Attention over a cache given by `d`, or (cells != null) over the engine's
-// FP8 records with the context at `tlen` (null: `context`).
-int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
+// Attention over a cache given by `d`, or (cells != null: device array of the K
+// and V maps of every cell) over FP8 records with the context at `tlen` (null:
+// `context`).
+int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
   if (int rc = check_tree(d)) return rc;
   if (d->batch == 0) return SKV_OK;
   if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse || !d->workspace ||
@@ -857,13 +893,11 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
   a.mtiles = (rows + TR_ROWS - 1) / TR_ROWS;
   a.rows = rows < TR_ROWS ? rows : TR_ROWS;
   a.c2 = (float)(d->scale * 1.4426950408889634);
-  a.cells = cells;
   a.context = context;
   a.len_stride = cells ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = d->q_stride[i];
     a.kns[i] = d->k_stride[i], a.vns[i] = d->v_stride[i];
-    a.k8s[i] = d->k_cache_stride[i], a.v8s[i] = d->v_cache_stride[i];
   }
   a.ps[0] = d->parents_stride[0], a.ps[1] = d->parents_stride[1];
   for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
@@ -872,7 +906,7 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
     a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0];
     a.kn = static_cast<const uint16_t *>(d->k) + b0 * a.kns[0];
     a.vn = static_cast<const uint16_t *>(d->v) + b0 * a.vns[0];
-    a.cells = cells ? cells + b0 * d->kv_heads : nullptr;
+    a.cell_maps = cells ? cells + 2 * b0 * d->kv_heads : nullptr;
     a.lengths = cells ? tlen : static_cast<const int32_t *>(d->lengths) + b0 * a.len_stride;
     a.parents = static_cast<const int32_t *>(d->parents) + b0 * a.ps[0];
     a.out = static_cast<uint16_t *>(d->out) + b0 * d->n * d->heads * d->dim;
@@ -901,8 +935,14 @@ int tree_attention(const SkvTree *d, const CellDev *cells, const int32_t *tlen, 
         a.along[i][1] = nb > 1 && four[i].s[0] ? 1 : 0;
       }
     } else if (!cells) {
-      a.k8 = static_cast<const uint8_t *>(d->k_cache) + b0 * a.k8s[0];
-      a.v8 = static_cast<const uint8_t *>(d->v_cache) + b0 * a.v8s[0];
+      for (int i = 0; i < 2 && !rc; ++i) {
+        const int64_t *at = i ? d->v_cache_stride : d->k_cache_stride, step[3] = {at[2], at[1], at[0]};
+        const void *base = static_cast<const uint8_t *>(i ? d->v_cache : d->k_cache) + b0 * at[0];
+        rc = make_byte_map(i ? &maps.v : &maps.k, base, d->dim, d->tokens, d->kv_heads, nb, step,
+                           i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : 64);
+        a.along[i][0] = d->kv_heads > 1 && at[1] ? 1 : 0;
+        a.along[i][1] = nb > 1 && at[0] ? 1 : 0;
+      }
     }
     if (!rc) rc = f8 ? launch_tree_d<true>((int)d->dim, maps, a, ctas, st) : launch_tree_d<false>((int)d->dim, maps, a, ctas, st);
     if (rc) return rc;

@@ -287,16 +287,17 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 #pragma unroll
       for (int j = 0; j < CHUNKS; ++j) {
         const int c = ct + j * 256, key = c / 4, c16 = 2 * (c % 4);
-        const uint32_t *x = reinterpret_cast<const uint32_t *>(&v[j]);
         uint4 y[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          y[u] = make_uint4(e4m3x2_to_bf16x2((uint16_t)x[2 * u]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u] >> 16)),
-                            e4m3x2_to_bf16x2((uint16_t)x[2 * u + 1]), e4m3x2_to_bf16x2((uint16_t)(x[2 * u + 1] >> 16)));
+        uint32_t nan = 0;
+        e4m3_to_bf16(v[j], y[0], y[1], nan);
         // (eight neighbouring threads are two keys, whose swizzles differ: all banks differ)
         uint8_t *line = ring + stage * WT_PIECE + key * 128;
         *reinterpret_cast<uint4 *>(line + (c16 ^ (key & 7)) * 16) = y[0];
         *reinterpret_cast<uint4 *>(line + ((c16 + 1) ^ (key & 7)) * 16) = y[1];
+        if (nan & E4M3_NAN) {
+          e4m3_put_nan(reinterpret_cast<uint4 *>(line + (c16 ^ (key & 7)) * 16));
+          e4m3_put_nan(reinterpret_cast<uint4 *>(line + ((c16 + 1) ^ (key & 7)) * 16));
+        }
       }
       async_fence();
       __syncwarp();
