@@ -617,11 +617,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     static_assert(KSTEP % 8 == 0 && CHUNKS == 8, "swizzle of an FP8 stage's pieces");
     const int key_k = ct / 4, key_v = ct / VPER * CHUNKS;
     const int unit_k = 2 * (ct % 4), unit_v = 2 * (ct % VPER);  // the first of its two 16-byte places in a row
-    // neighbouring pieces of different 64-dimension parts would meet in the
-    // same banks: every other part writes its halves in opposite order
-    const int flip = (unit_v >> 3) & 1;
     const int raw_k = ct * 16, raw_v = key_v * D + ct % VPER * 16;
-    const int to_k0 = key_k * 128 + ((unit_k ^ key_k) & 7) * 16, to_k1 = key_k * 128 + (((unit_k + 1) ^ key_k) & 7) * 16;
     const int to_v = (unit_v / 8) * C::VROWS * 128 + key_v * 128;
     constexpr uint32_t SLOTS = C::F8 ? C::NRAW : 1;
     const int piece = grp % C::PIECES;
@@ -640,47 +636,29 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (w.tile + i < w.tiles - 1) {
           const uint32_t raw_at = raw_base + (p - (p > k_nodes)) * C::PIECES + piece, slot = raw_at % SLOTS;
           if (!(ok = wait(&s.raw_full[slot], (raw_at / SLOTS) & 1))) break;
-          uint4 v[CHUNKS];
-          {
-            const uint8_t *from = raw + slot * C::RAW + (is_v ? raw_v : raw_k);
-            const int gap = is_v ? D : KSTEP * 64;
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) v[j] = *reinterpret_cast<const uint4 *>(from + j * gap);
+          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
+          const int left = len - (w.tile + i) * KT - (is_v ? piece * C::VROWS + key_v : key_k);  // keys from this thread's first
+          const int gap = is_v ? 1 : KSTEP, turn = is_v ? 7 : 0;
+          const uint8_t *from = raw + slot * C::RAW + (is_v ? raw_v : raw_k);
+          uint8_t *at = to + (is_v ? to_v : key_k * 128);
+          const uint32_t first = is_v ? unit_v & 7 : (unit_k ^ key_k) & 7;
+          uint32_t nan = 0;
+          // (a short body: straight-line code for all pieces would wait for its instructions)
+#pragma unroll 2
+          for (int j = 0; j < CHUNKS; ++j) {
+            uint4 x = *reinterpret_cast<const uint4 *>(from + j * (is_v ? D : KSTEP * 64)), y0, y1;
+            if (gap * j >= left) x = make_uint4(0, 0, 0, 0);  // behind the length
+            e4m3_to_bf16(x, y0, y1, nan);
+            const uint32_t place = first ^ (j & turn);
+            *reinterpret_cast<uint4 *>(at + j * gap * 128 + place * 16) = y0;
+            *reinterpret_cast<uint4 *>(at + j * gap * 128 + (place ^ 1) * 16) = y1;
           }
           __syncwarp();
           if (lane == 0) bar_arrive(&s.raw_empty[slot]);
-          const int left = len - (w.tile + i) * KT - (is_v ? piece * C::VROWS + key_v : key_k);  // keys from this thread's first
-          const int gap = is_v ? 1 : KSTEP;
-          if (left < CHUNKS * gap) {  // behind the length: zeros
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j)
-              if (gap * j >= left) v[j] = make_uint4(0, 0, 0, 0);
-          }
-          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
-          uint32_t nan = 0;
-          if (is_v) {
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) {
-              uint4 y0, y1;
-              e4m3_to_bf16(v[j], y0, y1, nan);
-              uint8_t *at = to + to_v + j * 128;
-              *reinterpret_cast<uint4 *>(at + (((unit_v + flip) & 7) ^ j) * 16) = flip ? y1 : y0;
-              *reinterpret_cast<uint4 *>(at + (((unit_v + 1 - flip) & 7) ^ j) * 16) = flip ? y0 : y1;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < CHUNKS; ++j) {
-              uint4 y0, y1;
-              e4m3_to_bf16(v[j], y0, y1, nan);
-              *reinterpret_cast<uint4 *>(to + to_k0 + j * KSTEP * 128) = y0;
-              *reinterpret_cast<uint4 *>(to + to_k1 + j * KSTEP * 128) = y1;
-            }
-          }
           if (nan & E4M3_NAN)
             for (int j = 0; j < CHUNKS; ++j)
               for (int u = 0; u < 2; ++u)
-                e4m3_put_nan(reinterpret_cast<uint4 *>(
-                    to + (is_v ? to_v + j * 128 + (((unit_v + u) & 7) ^ j) * 16 : (u ? to_k1 : to_k0) + j * KSTEP * 128)));
+                e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * gap * 128 + ((first ^ (j & turn)) ^ u) * 16));
         } else {
           if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
           const uint16_t *src = is_v ? a.vn + w.b * a.vns[0] + w.unit * a.vns[1] : a.kn + w.b * a.kns[0] + w.unit * a.kns[1];
