@@ -362,8 +362,9 @@ int skv_attention_noalloc(int32_t n_slots, const uint16_t *q, const uint8_t *con
  * on `stream` (they may be captured into a CUDA graph).  The descriptor is
  * read during the call.  `device` is the ordinal that holds every buffer; the
  * calling thread's current device is left as it was.  Strides are counted in
- * elements (skv_evict: K and V in bytes); the innermost dimension is
- * contiguous. */
+ * elements, one per dimension in the order of the shapes given below; the
+ * innermost dimension of q, k, v and caches must be contiguous (stride 1, or
+ * one element).  The stride of a dimension of one element is not looked at. */
 #define SKV_DTYPE_BF16 0
 #define SKV_DTYPE_FP16 1
 #define SKV_DTYPE_FP32 2
@@ -386,28 +387,26 @@ typedef struct SkvRotary {
   double factor;
   int64_t device, dtype, layout, pos64;
   int64_t batch, n, heads, kv_heads, dim, rotary_dim;
-  int64_t q_stride[3];          /* batch, token, head                       */
-  int64_t k_stride[3];
-  int64_t q_out_stride[3];
-  int64_t k_out_stride[3];
-  int64_t pos_stride[2];        /* batch, token                             */
+  int64_t q_stride[4], k_stride[4], q_out_stride[4], k_out_stride[4];
+  int64_t pos_stride[2];        /* batch (0: one row for all), token        */
 } SkvRotary;
 int skv_rotary(const SkvRotary *desc, void *stream);
 
 /* Eviction: of every (sequence, KV head) the `sink` first and `local` last of
  * lengths[b] tokens (clamped to [0, tokens]) and the best others by weight
  * (ties: the lowest index; NaN below every number) stay, `keep` in all, and
- * move to the front in their order.  Outputs are contiguous: k_out, v_out
- * [batch][kv_heads][keep] rows of row_bytes, weights_out FP32 and ids int32
+ * move to the front in their order.  k and v are [batch][kv_heads][tokens]
+ * rows of dim elements of element_bytes, weights FP32 [batch][kv_heads]
+ * [tokens].  Outputs are contiguous: k_out, v_out [batch][kv_heads][keep]
+ * rows, weights_out FP32 and ids int32
  * [batch][kv_heads][keep], lengths_out int32 [batch]; past the kept tokens
  * rows and weights are zero and ids -1.  No output may overlap an input. */
 typedef struct SkvEvict {
   const void *k, *v, *weights, *lengths;
   void *k_out, *v_out, *weights_out, *ids, *lengths_out;
-  int64_t device, batch, kv_heads, tokens, row_bytes, keep, sink, local;
-  int64_t k_stride[3];          /* bytes: sequence, head, token             */
-  int64_t v_stride[3];
-  int64_t weights_stride[3];    /* elements                                 */
+  int64_t device, batch, kv_heads, tokens, dim, element_bytes, keep, sink, local;
+  int64_t k_stride[4], v_stride[4], weights_stride[3];
+  int64_t lengths_stride;
 } SkvEvict;
 int skv_evict(const SkvEvict *desc, void *stream);
 
@@ -430,13 +429,8 @@ typedef struct SkvTree {
   double scale;
   int64_t device, cache_dtype, workspace_bytes;
   int64_t batch, n, heads, kv_heads, dim, tokens;
-  int64_t q_stride[3];          /* sequence, node, head                     */
-  int64_t k_cache_stride[3];    /* sequence, head, token                    */
-  int64_t v_cache_stride[3];
-  int64_t k_stride[3];          /* sequence, head, node                     */
-  int64_t v_stride[3];
-  int64_t parents_stride[2];    /* sequence, node                           */
-  int64_t lengths_stride;
+  int64_t q_stride[4], k_cache_stride[4], v_cache_stride[4], k_stride[4], v_stride[4];
+  int64_t parents_stride[2], lengths_stride;
 } SkvTree;
 int skv_tree_attention(const SkvTree *desc, void *stream);
 int skv_tree_workspace(const SkvTree *desc, int64_t *bytes);
@@ -455,13 +449,8 @@ typedef struct SkvWeights {
   double scale;
   int64_t device, cache_dtype;
   int64_t batch, n, heads, kv_heads, dim, tokens;
-  int64_t q_stride[3];          /* sequence, node, head                     */
-  int64_t k_cache_stride[3];    /* sequence, head, token                    */
-  int64_t lse_stride[3];        /* sequence, node, head                     */
-  int64_t rows_stride[2];       /* sequence, node                           */
-  int64_t weights_stride[3];    /* sequence, head, token                    */
-  int64_t weights_out_stride[3];
-  int64_t lengths_stride;
+  int64_t q_stride[4], k_cache_stride[4], lse_stride[3], rows_stride[2];
+  int64_t weights_stride[3], weights_out_stride[3], lengths_stride;
 } SkvWeights;
 int skv_accumulate_weights(const SkvWeights *desc, void *stream);
 

@@ -36,6 +36,7 @@ struct EvictArgs {
   const float *weights;
   int64_t ws[3];  // element strides (sequence, head, token)
   const int32_t *lengths;
+  int64_t len_stride;
   int32_t *ids, *out_lengths;
   float *out_w;
   int heads, t, keep, sink, local;
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
   const int b = row / a.heads, h = row - b * a.heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dependency_release();
-  const int n = max(0, min(a.lengths[b], a.t));
+  const int n = max(0, min(a.lengths[b * a.len_stride], a.t));
   const int m = min(n, a.keep);
   const float *w = a.weights + b * a.ws[0] + h * a.ws[1];
   int32_t *ids = a.ids + (int64_t)row * a.keep;
@@ -263,9 +264,10 @@ cudaError_t launch_gather(const GatherArgs &g, cudaStream_t st) {
 extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   using namespace skv;
   if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
-  if (d->batch < 0 || d->kv_heads < 1 || d->tokens < 1 || d->tokens > INT32_MAX / 2 || d->row_bytes < 1 ||
-      d->row_bytes > 65536 || d->batch * d->kv_heads > (1 << 24))
-    return op_fail(SKV_E_INVALID, "batch, heads, tokens or row_bytes out of range");
+  if (d->batch < 0 || d->kv_heads < 1 || d->tokens < 1 || d->tokens > INT32_MAX / 2 || d->dim < 1 || d->dim > 65536 ||
+      (d->element_bytes != 1 && d->element_bytes != 2 && d->element_bytes != 4) || d->batch > (1 << 24) ||
+      d->batch * d->kv_heads > (1 << 24))
+    return op_fail(SKV_E_INVALID, "batch, heads, tokens, dim or element_bytes out of range");
   if (d->keep < 1 || d->keep > d->tokens || d->sink < 0 || d->local < 0 || d->sink + d->local > d->keep)
     return op_fail(SKV_E_INVALID, "keep must be in [1, tokens] and hold the sink and local tokens");
   const int64_t rows = d->batch * d->kv_heads * d->keep;
@@ -273,20 +275,25 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   if (d->batch == 0) return SKV_OK;
   if (!d->k || !d->v || !d->weights || !d->lengths || !d->k_out || !d->v_out || !d->weights_out || !d->ids || !d->lengths_out)
     return op_fail(SKV_E_INVALID, "null input or output pointer");
+  if (d->dim > 1 && (d->k_stride[3] != 1 || d->v_stride[3] != 1))
+    return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   EvictArgs a;
   a.weights = static_cast<const float *>(d->weights);
-  for (int i = 0; i < 3; ++i) a.ws[i] = d->weights_stride[i];
+  const int64_t size[3] = {d->batch, d->kv_heads, d->tokens};
+  op_strides(a.ws, d->weights_stride, size, 3);
+  op_strides(&a.len_stride, &d->lengths_stride, size, 1);
   a.lengths = static_cast<const int32_t *>(d->lengths);
   a.ids = static_cast<int32_t *>(d->ids);
   a.out_lengths = static_cast<int32_t *>(d->lengths_out);
   a.out_w = static_cast<float *>(d->weights_out);
   a.heads = (int)d->kv_heads, a.t = (int)d->tokens, a.keep = (int)d->keep;
   a.sink = (int)d->sink, a.local = (int)d->local;
-  int rc = op_cuda(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)sizeof(SelectSmem)), "k_evict_select shared memory");
+  static bool set[64];
+  int sms = 0, rc = sm_count((int)d->device, &sms);  // (checks the ordinal)
+  if (!rc) rc = op_shared_memory(reinterpret_cast<const void *>(&k_evict_select), (int)sizeof(SelectSmem), (int)d->device, set);
   if (rc) return rc;
   const int ranks = d->tokens <= EV_SMALL ? 1 : EV_CLUSTER;
   rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
@@ -295,14 +302,17 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   GatherArgs g;
   g.x[0] = static_cast<const uint8_t *>(d->k), g.x[1] = static_cast<const uint8_t *>(d->v);
   g.y[0] = static_cast<uint8_t *>(d->k_out), g.y[1] = static_cast<uint8_t *>(d->v_out);
-  uintptr_t all = (uintptr_t)g.x[0] | (uintptr_t)g.x[1] | (uintptr_t)g.y[0] | (uintptr_t)g.y[1] | (uintptr_t)d->row_bytes;
+  g.row_bytes = (int)(d->dim * d->element_bytes);
+  uintptr_t all = (uintptr_t)g.x[0] | (uintptr_t)g.x[1] | (uintptr_t)g.y[0] | (uintptr_t)g.y[1] | (uintptr_t)g.row_bytes;
+  op_strides(g.xs[0], d->k_stride, size, 3);
+  op_strides(g.xs[1], d->v_stride, size, 3);
   for (int i = 0; i < 3; ++i) {
-    g.xs[0][i] = d->k_stride[i], g.xs[1][i] = d->v_stride[i];
+    g.xs[0][i] *= d->element_bytes, g.xs[1][i] *= d->element_bytes;
     all |= (uintptr_t)g.xs[0][i] | (uintptr_t)g.xs[1][i];
   }
   g.ids = a.ids;
   g.rows = rows;
-  g.heads = a.heads, g.keep = a.keep, g.row_bytes = (int)d->row_bytes;
+  g.heads = a.heads, g.keep = a.keep;
   // the widest access that every row start allows
   cudaError_t e = all % 16 == 0  ? launch_gather<uint4>(g, st)
                   : all % 4 == 0 ? launch_gather<uint32_t>(g, st)

@@ -57,6 +57,34 @@ class DeviceScope {
   cudaError_t err_;
 };
 
+// Strides as the kernels take them: 0 for a dimension of one element (its own
+// stride means nothing).
+inline void op_strides(int64_t *to, const int64_t *from, const int64_t *size, int n) noexcept {
+  for (int i = 0; i < n; ++i) to[i] = size[i] == 1 ? 0 : from[i];
+}
+
+// SMs of a device, asked once.
+inline int sm_count(int device, int *sms) noexcept {
+  static int known[64];
+  if (device < 0 || device >= 64) return op_fail(SKV_E_INVALID, "device ordinal out of range");
+  int n = __atomic_load_n(&known[device], __ATOMIC_RELAXED);
+  if (!n) {
+    if (int rc = op_cuda(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device attribute")) return rc;
+    __atomic_store_n(&known[device], n, __ATOMIC_RELAXED);
+  }
+  *sms = n;
+  return SKV_OK;
+}
+
+// Dynamic shared memory of a kernel (`set`: one flag per device and kernel), raised once.
+inline int op_shared_memory(const void *kernel, int bytes, int device, bool *set) noexcept {
+  if (__atomic_load_n(&set[device], __ATOMIC_RELAXED)) return SKV_OK;
+  if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory size"))
+    return rc;
+  __atomic_store_n(&set[device], true, __ATOMIC_RELAXED);
+  return SKV_OK;
+}
+
 // Launch; with `early` the kernel's blocks may be placed while the kernel
 // before it on the stream still runs (it calls grid_dependency_wait() before
 // it reads what that kernel wrote), which hides its launch.

@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 
 #include <cstring>
+#include <utility>
 
 #include "skv_ops.cuh"
 
@@ -178,6 +179,8 @@ extern "C" int skv_rotary(const SkvRotary *d, void *stream) {
   if (d->layout != SKV_ROTARY_HALF && d->layout != SKV_ROTARY_INTERLEAVED)
     return op_fail(SKV_E_INVALID, "unknown rotary layout");
   if (d->batch == 0 || d->n == 0) return SKV_OK;
+  if (d->q_stride[3] != 1 || d->q_out_stride[3] != 1 || (has_k && (d->k_stride[3] != 1 || d->k_out_stride[3] != 1)))
+    return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
   if (!d->q || !d->q_out || (has_k && (!d->k || !d->k_out)) || !d->positions || !d->phase)
     return op_fail(SKV_E_INVALID, "null input or output pointer");
   DeviceScope scope((int)d->device);
@@ -186,13 +189,16 @@ extern "C" int skv_rotary(const SkvRotary *d, void *stream) {
   const int size = d->dtype == SKV_DTYPE_FP32 ? 4 : 2;
   RotaryArgs a;
   a.x[0] = d->q, a.x[1] = d->k, a.y[0] = d->q_out, a.y[1] = d->k_out;
-  memcpy(a.xs[0], d->q_stride, sizeof a.xs[0]);
-  memcpy(a.xs[1], d->k_stride, sizeof a.xs[1]);
-  memcpy(a.ys[0], d->q_out_stride, sizeof a.ys[0]);
-  memcpy(a.ys[1], d->k_out_stride, sizeof a.ys[1]);
+  const int64_t nq[3] = {d->batch, d->n, d->heads}, nk[3] = {d->batch, d->kv_heads, d->n};
+  op_strides(a.xs[0], d->q_stride, nq, 3);
+  op_strides(a.ys[0], d->q_out_stride, nq, 3);
+  op_strides(a.xs[1], d->k_stride, nk, 3);
+  op_strides(a.ys[1], d->k_out_stride, nk, 3);
+  std::swap(a.xs[1][1], a.xs[1][2]);  // (batch, token, head) as q's
+  std::swap(a.ys[1][1], a.ys[1][2]);
   a.positions = d->positions;
   a.pos64 = d->pos64 != 0;
-  a.pos_stride[0] = d->pos_stride[0], a.pos_stride[1] = d->pos_stride[1];
+  op_strides(a.pos_stride, d->pos_stride, nq, 2);
   a.tokens = d->batch * d->n;
   a.n = (int)d->n;
   a.heads[0] = (int)d->heads, a.heads[1] = (int)d->kv_heads;
@@ -225,8 +231,7 @@ extern "C" int skv_rotary(const SkvRotary *d, void *stream) {
     a.chunks = a.dim / v;
   }
   int sms = 0;
-  if (int rc = op_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, (int)d->device), "device attribute"))
-    return rc;
+  if (int rc = sm_count((int)d->device, &sms)) return rc;
   // few tokens: more threads share a token's heads (each computes its own
   // sines); many tokens: one thread per token and chunk, sines computed once
   const int total = a.heads[0] + a.heads[1];

@@ -777,13 +777,12 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
 }
 
 template <class C>
-int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t st) {
+int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, cudaStream_t st) {
   constexpr int smem = C::RING + (int)sizeof(TreeSmem<C>);
   static_assert(smem <= 232448, "shared memory");
   auto *kernel = &k_tree_attention<C>;
-  if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                       "k_tree_attention shared memory"))
-    return rc;
+  static bool set[64];
+  if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), smem, device, set)) return rc;
   if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, false, 1, maps, a),
                        "k_tree_attention launch"))
     return rc;
@@ -793,10 +792,10 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t 
 }
 
 template <bool F8>
-int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, cudaStream_t st) {
-  if (d == 64) return launch_tree<TreeCfg<64, F8>>(maps, a, ctas, st);
-  if (d == 128) return launch_tree<TreeCfg<128, F8>>(maps, a, ctas, st);
-  return launch_tree<TreeCfg<256, F8>>(maps, a, ctas, st);
+int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, int device, cudaStream_t st) {
+  if (d == 64) return launch_tree<TreeCfg<64, F8>>(maps, a, ctas, device, st);
+  if (d == 128) return launch_tree<TreeCfg<128, F8>>(maps, a, ctas, device, st);
+  return launch_tree<TreeCfg<256, F8>>(maps, a, ctas, device, st);
 }
 
 // CTAs of a launch: one per SM, whole items (or fewer, the most places that the list can have).
@@ -804,10 +803,6 @@ int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t
   const int64_t most = batch * heads * ((t + TR_KEYS - 1) / TR_KEYS + 1 + TR_IDLE);
   const int64_t c = sms > mtiles ? (sms / mtiles < TC_MAX ? sms / mtiles : TC_MAX) : 1;
   return (most < c ? most : c) * mtiles;
-}
-
-int sm_count(int device, int *sms) {
-  return op_cuda(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device), "device attribute");
 }
 
 int64_t tree_workspace(int sms, const SkvTree *d) {
@@ -843,20 +838,30 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
       (!cells && (!d->k_cache || !d->v_cache || !d->lengths)))
     return op_fail(SKV_E_INVALID, "null input, output or workspace pointer");
   const bool f8 = d->cache_dtype == SKV_DTYPE_E4M3;
-  const int align = f8 ? 16 : 8;  // elements of 16 bytes
-  auto aligned = [&](const void *p, const int64_t *s, int64_t unit) {
-    if ((uintptr_t)p % 16) return false;
-    for (int i = 0; i < 3; ++i)
-      if (s[i] < 0 || s[i] % unit) return false;
-    return true;
-  };
-  if (!aligned(d->q, d->q_stride, 8) || !aligned(d->k, d->k_stride, 8) || !aligned(d->v, d->v_stride, 8) ||
-      (!cells && (!aligned(d->k_cache, d->k_cache_stride, align) || !aligned(d->v_cache, d->v_cache_stride, align))) ||
-      (uintptr_t)d->out % 16 || (uintptr_t)d->workspace % 16)
-    return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
-  if ((!cells && d->tokens > 1 && (!d->k_cache_stride[2] || !d->v_cache_stride[2])) ||
-      (d->n > 1 && (!d->k_stride[2] || !d->v_stride[2])))
-    return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  const int64_t of_q[3] = {d->batch, d->n, d->heads}, of_cache[3] = {d->batch, d->kv_heads, d->tokens},
+                of_nodes[3] = {d->batch, d->kv_heads, d->n};
+  struct Rows {
+    const void *base;
+    const int64_t *given, *size;
+    int64_t unit, stride[3];
+  } rows_of[5] = {{d->q, d->q_stride, of_q, 8, {}},
+                  {d->k, d->k_stride, of_nodes, 8, {}},
+                  {d->v, d->v_stride, of_nodes, 8, {}},
+                  {d->k_cache, d->k_cache_stride, of_cache, f8 ? 16 : 8, {}},
+                  {d->v_cache, d->v_cache_stride, of_cache, f8 ? 16 : 8, {}}};
+  for (int i = 0; i < (cells ? 3 : 5); ++i) {
+    Rows &x = rows_of[i];
+    op_strides(x.stride, x.given, x.size, 3);
+    if (x.given[3] != 1) return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
+    bool ok = (uintptr_t)x.base % 16 == 0;
+    for (int j = 0; j < 3; ++j) ok = ok && x.stride[j] >= 0 && x.stride[j] % x.unit == 0;
+    if (!ok) return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
+    if (i && x.size[2] > 1 && x.stride[2] == 0) return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  }
+  if ((uintptr_t)d->out % 16 || (uintptr_t)d->workspace % 16)
+    return op_fail(SKV_E_INVALID, "outputs must start on 16-byte boundaries");
+  const int64_t *const qs = rows_of[0].stride, *const ks = rows_of[1].stride, *const vs = rows_of[2].stride,
+                *const kcs = rows_of[3].stride, *const vcs = rows_of[4].stride;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
   int sms = 0;
@@ -872,12 +877,12 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
   a.rows = rows < TR_ROWS ? rows : TR_ROWS;
   a.c2 = (float)(d->scale * 1.4426950408889634);
   a.context = context;
-  a.len_stride = cells ? 0 : d->lengths_stride;
+  a.len_stride = cells || d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
-    a.qs[i] = d->q_stride[i];
-    a.kns[i] = d->k_stride[i], a.vns[i] = d->v_stride[i];
+    a.qs[i] = qs[i];
+    a.kns[i] = ks[i], a.vns[i] = vs[i];
   }
-  a.ps[0] = d->parents_stride[0], a.ps[1] = d->parents_stride[1];
+  op_strides(a.ps, d->parents_stride, of_q, 2);
   for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
     const int64_t nb = d->batch - b0 < PLAN_BATCH ? d->batch - b0 : PLAN_BATCH;
     a.batch = (int)nb;
@@ -901,10 +906,10 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
         const void *base;
         const int64_t *s;
         int64_t rows;
-      } four[4] = {{&maps.k, static_cast<const uint16_t *>(d->k_cache) + b0 * d->k_cache_stride[0], d->k_cache_stride, d->tokens},
-                   {&maps.v, static_cast<const uint16_t *>(d->v_cache) + b0 * d->v_cache_stride[0], d->v_cache_stride, d->tokens},
-                   {&maps.kn, a.kn, d->k_stride, d->n},
-                   {&maps.vn, a.vn, d->v_stride, d->n}};
+      } four[4] = {{&maps.k, static_cast<const uint16_t *>(d->k_cache) + b0 * kcs[0], kcs, d->tokens},
+                   {&maps.v, static_cast<const uint16_t *>(d->v_cache) + b0 * vcs[0], vcs, d->tokens},
+                   {&maps.kn, a.kn, ks, d->n},
+                   {&maps.vn, a.vn, vs, d->n}};
       for (int i = 0; i < 4 && !rc; ++i) {
         const int64_t step[3] = {four[i].s[2], four[i].s[1], four[i].s[0]};
         rc = make_map(four[i].map, four[i].base, d->dim, four[i].rows, d->kv_heads, nb, step,
@@ -914,7 +919,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
       }
     } else if (!cells) {
       for (int i = 0; i < 2 && !rc; ++i) {
-        const int64_t *at = i ? d->v_cache_stride : d->k_cache_stride, step[3] = {at[2], at[1], at[0]};
+        const int64_t *at = i ? vcs : kcs, step[3] = {at[2], at[1], at[0]};
         const void *base = static_cast<const uint8_t *>(i ? d->v_cache : d->k_cache) + b0 * at[0];
         rc = make_byte_map(i ? &maps.v : &maps.k, base, d->dim, d->tokens, d->kv_heads, nb, step,
                            i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : 64);
@@ -922,7 +927,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
         a.along[i][1] = nb > 1 && at[0] ? 1 : 0;
       }
     }
-    if (!rc) rc = f8 ? launch_tree_d<true>((int)d->dim, maps, a, ctas, st) : launch_tree_d<false>((int)d->dim, maps, a, ctas, st);
+    if (!rc) rc = f8 ? launch_tree_d<true>((int)d->dim, maps, a, ctas, (int)d->device, st) : launch_tree_d<false>((int)d->dim, maps, a, ctas, (int)d->device, st);
     if (rc) return rc;
   }
   return SKV_OK;

@@ -317,16 +317,15 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 }
 
 template <int D, bool F8>
-int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, cudaStream_t st) {
+int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, int device, cudaStream_t st) {
   constexpr int most = 232448, fixed = 1024 + (int)sizeof(WeightsSmem) + (F8 ? WT_RAW * WT_PIECE / 2 : 0);
   const int rows = (D / 64) * a.cols * 128;
   int stages = (most - fixed - rows) / WT_PIECE;
   a.stages = stages < WT_STAGES ? stages : WT_STAGES;
   const int smem = fixed + rows + a.stages * WT_PIECE;
   auto *kernel = &k_weights<D, F8>;
-  if (int rc = op_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
-                       "k_weights shared memory"))
-    return rc;
+  static bool set[64];
+  if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), most, device, set)) return rc;
   const int64_t tiles = (int64_t)a.batch * a.heads * ((a.t + WT_KEYS - 1) / WT_KEYS);
   const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
   return op_cuda(op_launch(kernel, dim3(grid), dim3(F8 ? WT_THREADS_F8 : WT_THREADS), smem, st, false, 1, map, a),
@@ -334,10 +333,10 @@ int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, cudaStream_t
 }
 
 template <bool F8>
-int launch_weights_d(int d, const CUtensorMap &map, WeightsArgs &a, int sms, cudaStream_t st) {
-  if (d == 64) return launch_weights<64, F8>(map, a, sms, st);
-  if (d == 128) return launch_weights<128, F8>(map, a, sms, st);
-  return launch_weights<256, F8>(map, a, sms, st);
+int launch_weights_d(int d, const CUtensorMap &map, WeightsArgs &a, int sms, int device, cudaStream_t st) {
+  if (d == 64) return launch_weights<64, F8>(map, a, sms, device, st);
+  if (d == 128) return launch_weights<128, F8>(map, a, sms, device, st);
+  return launch_weights<256, F8>(map, a, sms, device, st);
 }
 
 }  // namespace
@@ -358,31 +357,34 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   if (!d->q || !d->k_cache || !d->lengths || !d->lse || !d->weights || !d->weights_out)
     return op_fail(SKV_E_INVALID, "null input or output pointer");
   const bool f8 = d->cache_dtype == SKV_DTYPE_E4M3;
-  auto aligned = [&](const void *p, const int64_t *s, int64_t unit) {
-    if ((uintptr_t)p % 16) return false;
-    for (int i = 0; i < 3; ++i)
-      if (s[i] < 0 || s[i] % unit) return false;
-    return true;
-  };
-  if (!aligned(d->q, d->q_stride, 8) || !aligned(d->k_cache, d->k_cache_stride, f8 ? 16 : 8))
-    return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
-  if (d->tokens > 1 && !d->k_cache_stride[2]) return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  const int64_t of_q[3] = {d->batch, d->n, d->heads}, of_cache[3] = {d->batch, d->kv_heads, d->tokens};
+  int64_t qs[3], kcs[3], ws[3], os[3], ls[3];
+  op_strides(qs, d->q_stride, of_q, 3);
+  op_strides(kcs, d->k_cache_stride, of_cache, 3);
+  op_strides(ws, d->weights_stride, of_cache, 3);
+  op_strides(os, d->weights_out_stride, of_cache, 3);
+  op_strides(ls, d->lse_stride, of_q, 3);
+  if (d->q_stride[3] != 1 || d->k_cache_stride[3] != 1)
+    return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
+  bool ok = (uintptr_t)d->q % 16 == 0 && (uintptr_t)d->k_cache % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && qs[i] >= 0 && qs[i] % 8 == 0 && kcs[i] >= 0 && kcs[i] % (f8 ? 16 : 8) == 0;
+  if (!ok) return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
+  if (d->tokens > 1 && !kcs[2]) return op_fail(SKV_E_INVALID, "tokens must not share one row");
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
   int sms = 0;
-  if (int rc = op_cuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, (int)d->device), "device attribute"))
-    return rc;
+  if (int rc = sm_count((int)d->device, &sms)) return rc;
   WeightsArgs a{};
   if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads);
   a.heads = (int)d->kv_heads, a.group = group, a.t = (int)d->tokens;
   a.c2 = (float)(d->scale * 1.4426950408889634);
-  a.len_stride = d->lengths_stride;
+  a.len_stride = d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
-    a.qs[i] = d->q_stride[i], a.k8s[i] = d->k_cache_stride[i], a.ls[i] = d->lse_stride[i];
-    a.os[i] = d->weights_out_stride[i];
+    a.qs[i] = qs[i], a.k8s[i] = kcs[i], a.ls[i] = ls[i];
+    a.os[i] = os[i];
   }
-  a.ts[0] = d->rows_stride[0], a.ts[1] = d->rows_stride[1];
+  op_strides(a.ts, d->rows_stride, of_q, 2);
   const int64_t rows = d->n * group;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
@@ -397,12 +399,12 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
     if (f8) {
       a.k8 = static_cast<const uint8_t *>(d->k_cache) + b0 * a.k8s[0];
     } else {
-      const int64_t step[3] = {d->k_cache_stride[2], d->k_cache_stride[1], d->k_cache_stride[0]};
-      if (int rc = make_map(&map, static_cast<const uint16_t *>(d->k_cache) + b0 * d->k_cache_stride[0], d->dim, d->tokens,
+      const int64_t step[3] = {kcs[2], kcs[1], kcs[0]};
+      if (int rc = make_map(&map, static_cast<const uint16_t *>(d->k_cache) + b0 * kcs[0], d->dim, d->tokens,
                             d->kv_heads, nb, step, WT_KEYS, 1))
         return rc;
-      a.along[0] = d->kv_heads > 1 && d->k_cache_stride[1] ? 1 : 0;
-      a.along[1] = nb > 1 && d->k_cache_stride[0] ? 1 : 0;
+      a.along[0] = kcs[1] ? 1 : 0;
+      a.along[1] = nb > 1 && kcs[0] ? 1 : 0;
     }
     // more rows than the MMA's N: further launches add to what the first wrote
     for (int64_t r0 = 0; r0 < rows; r0 += WT_ROWS) {
@@ -410,13 +412,13 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
       a.rows = (int)(rows - r0 < WT_ROWS ? rows - r0 : WT_ROWS);
       a.cols = (a.rows + 15) & ~15;
       if (r0 == 0) {
-        a.w = static_cast<const float *>(d->weights) + b0 * d->weights_stride[0];
-        for (int i = 0; i < 3; ++i) a.ws[i] = d->weights_stride[i];
+        a.w = static_cast<const float *>(d->weights) + b0 * ws[0];
+        for (int i = 0; i < 3; ++i) a.ws[i] = ws[i];
       } else {
         a.w = a.out;
         for (int i = 0; i < 3; ++i) a.ws[i] = a.os[i];
       }
-      const int rc = f8 ? launch_weights_d<true>((int)d->dim, map, a, sms, st) : launch_weights_d<false>((int)d->dim, map, a, sms, st);
+      const int rc = f8 ? launch_weights_d<true>((int)d->dim, map, a, sms, (int)d->device, st) : launch_weights_d<false>((int)d->dim, map, a, sms, (int)d->device, st);
       if (rc) return rc;
     }
   }

@@ -35,11 +35,17 @@ from seoulkv_b200.api import _current_stream
 
 TREE_MAX_NODES = 64
 ROTARY_MAX_DIM = 512
+_BF16, _F32, _I32, _FP8 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
-_NAMES = {torch.bfloat16: "BF16", torch.float16: "FP16", torch.float32: "FP32", torch.float8_e4m3fn: "FP8 e4m3"}
+_NAMES = {torch.bfloat16: "BF16", torch.float16: "FP16", torch.float32: "FP32", torch.float8_e4m3fn: "FP8 e4m3",
+          torch.int32: "int32", torch.int64: "int64", torch.bool: "bool"}
+
+# Arguments are checked twice over: one expression that holds for every good
+# call (these functions run once per decode step), and, where it does not
+# hold, _check() on each argument, which says what is wrong.
 
 
-def _check(name: str, t, shape, dtypes, device=None) -> None:
+def _check(name: str, t, shape, dtypes, device: int | None = None) -> None:
     """A CUDA tensor of one of the dtypes; ``shape`` entries of None are free."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise ValueError(f"{name}: expected a {' or '.join(_NAMES.get(x, str(x)) for x in dtypes)} tensor")
@@ -49,25 +55,14 @@ def _check(name: str, t, shape, dtypes, device=None) -> None:
                          f"got {list(got)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators have no backward pass (detach it, or use no_grad)")
 
 
-def _rows(name: str, t: torch.Tensor) -> None:
-    """Contiguous innermost dimension, rows on 16-byte boundaries, no two tokens in one row."""
-    st, unit = t.stride(), 16 // t.element_size()
-    if st[-1] != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the innermost dimension must be contiguous")
-    if t.data_ptr() % 16 or any(s % unit and n > 1 for s, n in zip(st[:-1], t.shape)):
-        raise ValueError(f"{name}: rows must start on 16-byte boundaries")
-
-
-def _steps(t: torch.Tensor, axes, unit: int = 1) -> list[int]:
-    """Strides of the axes; 0 for an axis of one element (its own stride means nothing)."""
-    st, n = t.stride(), t.shape
-    return [st[x] * unit if n[x] > 1 else 0 for x in axes]
+def _recorded(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -83,8 +78,8 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _run(entry, packed: bytes, device: torch.device, what: str) -> None:
-    rc = entry(packed, _current_stream(device.index))
+def _run(entry, packed: bytes, device: int, what: str) -> None:
+    rc = entry(packed, _current_stream(device))
     if rc:
         message = _native.load().skv_last_error().decode(errors="replace")
         if rc == -1:
@@ -108,7 +103,8 @@ def check_operators(device) -> None:
 
 @functools.lru_cache(maxsize=64)
 def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
-    """(turns per position * 2^64 of each pair as packed uint64, factor on the rotated part)."""
+    """(turns per position * 2^64 of each pair as packed uint64, its address, factor on the rotated part)."""
+    theta, factor, beta_fast, beta_slow = (float(x) for x in (theta, factor, beta_fast, beta_slow))
     if not theta > 0.0 or not math.isfinite(theta) or theta == 1.0:
         raise ValueError("theta must be positive, finite and not 1")
     if not factor > 0.0 or not math.isfinite(factor):
@@ -147,7 +143,7 @@ def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fas
     return table, ctypes.addressof(table), m
 
 
-_ROTARY = struct.Struct("6Qd" + 10 * "q" + 14 * "q")
+_ROTARY = struct.Struct("6Qd" + 10 * "q" + 18 * "q")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, rotary_dim: int | None = None,
@@ -176,93 +172,101 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
     """
     if not isinstance(q, torch.Tensor) or q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("q: expected a BF16 or FP16 or FP32 tensor")
-    _check("q", q, (None,) * 4, (q.dtype,))
+    dtype, dev = q.dtype, q.get_device()
+    if q.ndim != 4 or dev < 0:
+        _check("q", q, (None,) * 4, (dtype,))
     b, n, hq, d = q.shape
-    dev = q.device
     hkv = 0
     if k is not None:
-        _check("k", k, (b, None, n, d), (q.dtype,), dev)
+        if not (isinstance(k, torch.Tensor) and k.ndim == 4 and k.dtype is dtype and k.get_device() == dev):
+            _check("k", k, (b, None, n, d), (dtype,), dev)
         hkv = k.shape[1]
+        if k.shape != (b, hkv, n, d):
+            _check("k", k, (b, None, n, d), (dtype,), dev)
     if hq < 1 or (k is not None and hkv < 1):
         raise ValueError("q and k need at least one head")
     if not isinstance(positions, torch.Tensor) or positions.ndim not in (1, 2):
         raise ValueError("positions: expected an int32 or int64 tensor [N] or [B,N]")
-    _check("positions", positions, (n,) if positions.ndim == 1 else (b, n), (torch.int32, torch.int64), dev)
+    if not (positions.dtype in (torch.int64, _I32) and positions.get_device() == dev
+            and positions.shape == ((n,) if positions.ndim == 1 else (b, n))):
+        _check("positions", positions, (n,) if positions.ndim == 1 else (b, n), (_I32, torch.int64), dev)
+    if _recorded(q, q if k is None else k):
+        _check("q", q, (None,) * 4, (dtype,))
+        _check("k", k, (None,) * 4, (dtype,))
     r = d if rotary_dim is None else rotary_dim
     if type(r) is not int or r < 2 or r % 2 or r > d or r > ROTARY_MAX_DIM:
         raise ValueError(f"rotary_dim must be an even integer in [2, min(D, {ROTARY_MAX_DIM})]")
     if layout not in ("half", "interleaved"):
         raise ValueError("layout must be 'half' or 'interleaved'")
-    _, phase, m = _rotary_table(r, float(theta), scaling, float(factor), original_context, float(beta_fast),
-                                float(beta_slow), attention_factor)
+    _, phase, m = _rotary_table(r, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor)
     if out is None:
-        qo = torch.empty((b, n, hq, d), dtype=q.dtype, device=dev)
-        ko = None if k is None else torch.empty((b, hkv, n, d), dtype=q.dtype, device=dev)
+        qo = q.new_empty((b, n, hq, d))
+        ko = None if k is None else k.new_empty((b, hkv, n, d))
     else:
         qo, ko = out
-        _check("out[0]", qo, (b, n, hq, d), (q.dtype,), dev)
-        pairs = [("out[0]", qo, q)]
-        if k is None:
-            if ko is not None:
-                raise ValueError("out[1]: there is no k")
-        else:
-            _check("out[1]", ko, (b, hkv, n, d), (q.dtype,), dev)
-            pairs.append(("out[1]", ko, k))
-        for name, y, x in pairs:
-            if any(s == 0 and size > 1 for s, size in zip(y.stride(), y.shape)):
-                raise ValueError(f"{name}: two elements share one place")
-            same = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
-            if not same and _overlap(y, x):
-                raise ValueError(f"{name} overlaps its input without being it")
-        if k is not None and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
-            # (in place, q and k may be interleaved parts of one projection)
-            for name, y, x in (("out[0]", qo, k), ("out[1]", ko, q), ("out[1]", ko, qo)):
-                if _overlap(y, x):
-                    raise ValueError(f"{name} overlaps another tensor of the call")
-    for name, t in (("q", q), ("k", k), ("out[0]", qo), ("out[1]", ko)):
-        if t is not None and t.stride(3) != 1 and d > 1:
-            raise ValueError(f"{name}: the innermost dimension must be contiguous")
+        _check_rotary_out(q, k, qo, ko, dev)
     if not b or not n:
         return qo, ko
     kk, kko = (q, qo) if k is None else (k, ko)
-    pos = _steps(positions, (0, 1)) if positions.ndim == 2 else [0, *_steps(positions, (0,))]
+    pos = positions.stride()
     packed = _ROTARY.pack(
         q.data_ptr(), kk.data_ptr(), qo.data_ptr(), kko.data_ptr(), positions.data_ptr(), phase, m,
-        dev.index, _DTYPE[q.dtype], layout == "interleaved", positions.dtype == torch.int64, b, n, hq, hkv, d, r,
-        *_steps(q, (0, 1, 2)), *_steps(kk, (0, 2, 1)), *_steps(qo, (0, 1, 2)), *_steps(kko, (0, 2, 1)), *pos)
+        dev, _DTYPE[dtype], layout == "interleaved", positions.dtype is torch.int64, b, n, hq, hkv, d, r,
+        *q.stride(), *kk.stride(), *qo.stride(), *kko.stride(), *((0, *pos) if len(pos) == 1 else pos))
     _run(_native.load().skv_rotary, packed, dev, "rotary")
     return qo, ko
+
+
+def _check_rotary_out(q, k, qo, ko, dev: int) -> None:
+    _check("out[0]", qo, tuple(q.shape), (q.dtype,), dev)
+    pairs = [("out[0]", qo, q)]
+    if k is None:
+        if ko is not None:
+            raise ValueError("out[1]: there is no k")
+    else:
+        _check("out[1]", ko, tuple(k.shape), (q.dtype,), dev)
+        pairs.append(("out[1]", ko, k))
+    for name, y, x in pairs:
+        if any(s == 0 and size > 1 for s, size in zip(y.stride(), y.shape)):
+            raise ValueError(f"{name}: two elements share one place")
+        same = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
+        if not same and _overlap(y, x):
+            raise ValueError(f"{name} overlaps its input without being it")
+    if k is not None and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
+        # (in place, q and k may be interleaved parts of one projection)
+        for name, y, x in (("out[0]", qo, k), ("out[1]", ko, q), ("out[1]", ko, qo)):
+            if _overlap(y, x):
+                raise ValueError(f"{name} overlaps another tensor of the call")
 
 
 # ---------------------------------------------------------------- attention of drafted trees
 
 
-_TREE = struct.Struct("10Qd" + 9 * "q" + 18 * "q")
+_TREE = struct.Struct("10Qd" + 9 * "q" + 23 * "q")
 
 
-def _check_cache(k_cache, v_cache, lengths, hkv=None):
-    _check("k_cache", k_cache, (None, hkv, None, None), (torch.bfloat16, torch.float8_e4m3fn))
+def _check_cache(k_cache, v_cache, lengths) -> None:
+    """Says what is wrong with a cache."""
+    _check("k_cache", k_cache, (None,) * 4, (_BF16, _FP8))
     b, h, t, d = k_cache.shape
+    dev = k_cache.get_device()
     if d not in (64, 128, 256):
         raise ValueError("head size must be 64, 128 or 256")
     if t < 1 or h < 1:
         raise ValueError("k_cache: expected at least one head and one token of room")
-    tensors = [("k_cache", k_cache)]
     if v_cache is not None:
-        _check("v_cache", v_cache, (b, h, t, d), (k_cache.dtype,), k_cache.device)
-        tensors.append(("v_cache", v_cache))
-    _check("lengths", lengths, (b,), (torch.int32,), k_cache.device)
-    for name, x in tensors:
-        _rows(name, x)
-        if t > 1 and x.stride(2) == 0:
-            raise ValueError(f"{name}: tokens must not share one row")
+        _check("v_cache", v_cache, (b, h, t, d), (k_cache.dtype,), dev)
+    _check("lengths", lengths, (b,), (_I32,), dev)
 
 
-def _scale(scale, d: int) -> float:
-    s = d ** -0.5 if scale is None else float(scale)
+def _scale(scale) -> float:
+    s = float(scale)
     if not (s > 0.0 and math.isfinite(s)):
         raise ValueError("scale must be positive and finite")
     return s
+
+
+_ROOT = {64: 0.125, 128: 128 ** -0.5, 256: 0.0625}
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -282,36 +286,46 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     log-sum-exp of each row's scaled scores, FP32 [B, N, Hq].  ``scale``
     defaults to D**-0.5.  N = 1 with parent -1 is exact decode of one token.
     """
-    _check_cache(k_cache, v_cache, lengths)
-    b, hkv, t, d = k_cache.shape
-    dev = k_cache.device
-    _check("q", q, (b, None, None, d), (torch.bfloat16,), dev)
-    n, hq = q.shape[1], q.shape[2]
-    if not 1 <= n <= TREE_MAX_NODES:
-        raise ValueError(f"the tree must have 1 to {TREE_MAX_NODES} nodes")
-    if hq < 1 or hq % hkv:
-        raise ValueError("query heads must be a multiple of the KV heads")
-    _check("k", k, (b, hkv, n, d), (torch.bfloat16,), dev)
-    _check("v", v, (b, hkv, n, d), (torch.bfloat16,), dev)
-    _check("parents", parents, (b, n), (torch.int32,), dev)
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        _rows(name, x)
-    if n > 1 and (k.stride(2) == 0 or v.stride(2) == 0):
-        raise ValueError("k and v: nodes must not share one row")
-    s = _scale(scale, d)
-    out = torch.empty((b, n, hq, d), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((b, n, hq), dtype=torch.float32, device=dev)
+    if not (isinstance(k_cache, torch.Tensor) and k_cache.ndim == 4 and isinstance(q, torch.Tensor) and q.ndim == 4):
+        _check("k_cache", k_cache, (None,) * 4, (_BF16, _FP8))
+        _check("q", q, (None,) * 4, (_BF16,))
+    b, hkv, t, d = shape = k_cache.shape
+    _, n, hq, _ = q.shape
+    dev, kind = k_cache.get_device(), k_cache.dtype
+    node = (b, hkv, n, d)
+    try:
+        good = (dev >= 0 and (kind is _BF16 or kind is _FP8) and v_cache.dtype is kind and v_cache.shape == shape
+                and q.dtype is _BF16 and q.shape == (b, n, hq, d) and k.dtype is _BF16 and k.shape == node
+                and v.dtype is _BF16 and v.shape == node and lengths.dtype is _I32 and lengths.shape == (b,)
+                and parents.dtype is _I32 and parents.shape == (b, n) and v_cache.get_device() == dev
+                and q.get_device() == dev and k.get_device() == dev and v.get_device() == dev
+                and lengths.get_device() == dev and parents.get_device() == dev
+                and d in _ROOT and t and hkv and 0 < n <= TREE_MAX_NODES and hq and not hq % hkv
+                and not _recorded(q, k_cache, v_cache, k, v))
+    except AttributeError:  # not a tensor
+        good = False
+    if not good:
+        _check_cache(k_cache, v_cache, lengths)
+        _check("q", q, (b, None, None, d), (_BF16,), dev)
+        if not 1 <= n <= TREE_MAX_NODES:
+            raise ValueError(f"the tree must have 1 to {TREE_MAX_NODES} nodes")
+        if hq < 1 or hq % hkv:
+            raise ValueError("query heads must be a multiple of the KV heads")
+        _check("k", k, node, (_BF16,), dev)
+        _check("v", v, node, (_BF16,), dev)
+        _check("parents", parents, (b, n), (_I32,), dev)
+    out = q.new_empty((b, n, hq, d))
+    lse = q.new_empty((b, n, hq), dtype=_F32)
     if not b:
         return out, lse
-    lib = _native.load()
-    size = _tree_workspace(dev.index, b, n, hq, hkv, d, t)
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    size = _tree_workspace(dev, b, n, hq, hkv, d, t)
+    work = q.new_empty(size, dtype=torch.uint8)
     packed = _TREE.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
-        parents.data_ptr(), out.data_ptr(), lse.data_ptr(), work.data_ptr(), s, dev.index, _DTYPE[k_cache.dtype], size,
-        b, n, hq, hkv, d, t, *_steps(q, (0, 1, 2)), *_steps(k_cache, (0, 1, 2)), *_steps(v_cache, (0, 1, 2)),
-        *_steps(k, (0, 1, 2)), *_steps(v, (0, 1, 2)), *_steps(parents, (0, 1)), *_steps(lengths, (0,)))
-    _run(lib.skv_tree_attention, packed, dev, "tree_attention")
+        parents.data_ptr(), out.data_ptr(), lse.data_ptr(), work.data_ptr(),
+        _ROOT[d] if scale is None else _scale(scale), dev, _DTYPE[kind], size, b, n, hq, hkv, d, t,
+        *q.stride(), *k_cache.stride(), *v_cache.stride(), *k.stride(), *v.stride(), *parents.stride(), *lengths.stride())
+    _run(_native.load().skv_tree_attention, packed, dev, "tree_attention")
     return out, lse
 
 
@@ -319,7 +333,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: int) -> int:
     """Bytes of scratch that one call needs (a function of the sizes)."""
     size = ctypes.c_int64()
-    packed = _TREE.pack(*(10 * (0,)), 1.0, device, 0, 0, b, n, hq, hkv, d, t, *(18 * (0,)))
+    packed = _TREE.pack(*(10 * (0,)), 1.0, device, 0, 0, b, n, hq, hkv, d, t, *(23 * (0,)))
     _native.check(_native.load().skv_tree_workspace(packed, ctypes.byref(size)), "skv_tree_workspace")
     return max(16, size.value)
 
@@ -327,7 +341,7 @@ def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: i
 # ---------------------------------------------------------------- accumulated weights
 
 
-_WEIGHTS = struct.Struct("7Qd" + 8 * "q" + 18 * "q")
+_WEIGHTS = struct.Struct("7Qd" + 8 * "q" + 20 * "q")
 
 
 def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Tensor, lse: torch.Tensor,
@@ -346,23 +360,36 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
     Returns a new tensor, or ``out``, which may be ``weights`` itself
     (otherwise it must not overlap it).
     """
-    _check_cache(k_cache, None, lengths)
+    if not (isinstance(k_cache, torch.Tensor) and k_cache.ndim == 4 and isinstance(q, torch.Tensor) and q.ndim == 4):
+        _check("k_cache", k_cache, (None,) * 4, (_BF16, _FP8))
+        _check("q", q, (None,) * 4, (_BF16,))
     b, hkv, t, d = k_cache.shape
-    dev = k_cache.device
-    _check("q", q, (b, None, None, d), (torch.bfloat16,), dev)
-    n, hq = q.shape[1], q.shape[2]
-    if n < 1 or hq < 1 or hq % hkv:
-        raise ValueError("q: expected at least one node, and query heads a multiple of the KV heads")
-    _rows("q", q)
-    _check("lse", lse, (b, n, hq), (torch.float32,), dev)
-    _check("weights", weights, (b, hkv, t), (torch.float32,), dev)
-    if rows is not None:
+    _, n, hq, _ = q.shape
+    dev, kind = k_cache.get_device(), k_cache.dtype
+    held = (b, hkv, t)
+    try:
+        good = (dev >= 0 and (kind is _BF16 or kind is _FP8) and q.dtype is _BF16 and q.shape == (b, n, hq, d)
+                and lse.dtype is _F32 and lse.shape == (b, n, hq) and weights.dtype is _F32 and weights.shape == held
+                and lengths.dtype is _I32 and lengths.shape == (b,) and q.get_device() == dev
+                and lse.get_device() == dev and weights.get_device() == dev and lengths.get_device() == dev
+                and d in _ROOT and t and hkv and n and hq and not hq % hkv
+                and not _recorded(q, k_cache, lse, weights))
+    except AttributeError:  # not a tensor
+        good = False
+    if not good:
+        _check_cache(k_cache, None, lengths)
+        _check("q", q, (b, None, None, d), (_BF16,), dev)
+        if n < 1 or hq < 1 or hq % hkv:
+            raise ValueError("q: expected at least one node, and query heads a multiple of the KV heads")
+        _check("lse", lse, (b, n, hq), (_F32,), dev)
+        _check("weights", weights, held, (_F32,), dev)
+    if rows is not None and not (isinstance(rows, torch.Tensor) and rows.dtype is torch.bool and rows.shape == (b, n)
+                                 and rows.get_device() == dev):
         _check("rows", rows, (b, n), (torch.bool,), dev)
-    s = _scale(scale, d)
     if out is None:
-        out = torch.empty((b, hkv, t), dtype=torch.float32, device=dev)
+        out = weights.new_empty(held)
     else:
-        _check("out", out, (b, hkv, t), (torch.float32,), dev)
+        _check("out", out, held, (_F32,), dev)
         if any(x == 0 and size > 1 for x, size in zip(out.stride(), out.shape)):
             raise ValueError("out: two elements share one place")
         if not (out.data_ptr() == weights.data_ptr() and out.stride() == weights.stride()) and _overlap(out, weights):
@@ -371,10 +398,9 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
         return out
     packed = _WEIGHTS.pack(
         q.data_ptr(), k_cache.data_ptr(), lengths.data_ptr(), lse.data_ptr(), 0 if rows is None else rows.data_ptr(),
-        weights.data_ptr(), out.data_ptr(), s, dev.index, _DTYPE[k_cache.dtype], b, n, hq, hkv, d, t,
-        *_steps(q, (0, 1, 2)), *_steps(k_cache, (0, 1, 2)), *_steps(lse, (0, 1, 2)),
-        *((0, 0) if rows is None else _steps(rows, (0, 1))), *_steps(weights, (0, 1, 2)), *_steps(out, (0, 1, 2)),
-        *_steps(lengths, (0,)))
+        weights.data_ptr(), out.data_ptr(), _ROOT[d] if scale is None else _scale(scale), dev, _DTYPE[kind], b, n, hq,
+        hkv, d, t, *q.stride(), *k_cache.stride(), *lse.stride(), *((0, 0) if rows is None else rows.stride()),
+        *weights.stride(), *out.stride(), *lengths.stride())
     _run(_native.load().skv_accumulate_weights, packed, dev, "accumulate_weights")
     return out
 
@@ -382,7 +408,8 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
 # ---------------------------------------------------------------- eviction
 
 
-_EVICT = struct.Struct("9Q" + 8 * "q" + 9 * "q")
+_EVICT = struct.Struct("9Q" + 9 * "q" + 12 * "q")
+_EVICTED = frozenset(_DTYPE)
 
 
 def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, lengths: torch.Tensor, *, keep: int,
@@ -401,34 +428,37 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, l
     [B, Hkv, keep], lengths int32 [B]; past the kept tokens K, V and weights
     are zero and ids -1.
     """
-    kinds = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn)
-    _check("k_cache", k_cache, (None,) * 4, kinds)
-    b, h, t, d = k_cache.shape
-    dev = k_cache.device
-    if h < 1 or t < 1 or d < 1:
-        raise ValueError("k_cache: expected at least one head, token and dimension")
-    _check("v_cache", v_cache, (b, h, t, d), (k_cache.dtype,), dev)
-    _check("weights", weights, (b, h, t), (torch.float32,), dev)
-    _check("lengths", lengths, (b,), (torch.int32,), dev)
-    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if x.stride(3) != 1 and d > 1:
-            raise ValueError(f"{name}: the innermost dimension must be contiguous")
-    if any(type(x) is not int for x in (keep, sink, local)) or not 1 <= keep <= t or sink < 0 or local < 0 \
-            or sink + local > keep:
+    if not (isinstance(k_cache, torch.Tensor) and k_cache.ndim == 4):
+        _check("k_cache", k_cache, (None,) * 4, tuple(_DTYPE))
+    b, h, t, d = shape = k_cache.shape
+    dev, kind = k_cache.get_device(), k_cache.dtype
+    try:
+        good = (dev >= 0 and kind in _EVICTED and v_cache.dtype is kind and v_cache.shape == shape
+                and weights.dtype is _F32 and weights.shape == (b, h, t) and lengths.dtype is _I32
+                and lengths.shape == (b,) and v_cache.get_device() == dev and weights.get_device() == dev
+                and lengths.get_device() == dev and t and h and d and not _recorded(k_cache, v_cache, weights))
+    except AttributeError:  # not a tensor
+        good = False
+    if not good:
+        _check("k_cache", k_cache, (None,) * 4, tuple(_DTYPE))
+        if h < 1 or t < 1 or d < 1:
+            raise ValueError("k_cache: expected at least one head, token and dimension")
+        _check("v_cache", v_cache, (b, h, t, d), (kind,), dev)
+        _check("weights", weights, (b, h, t), (_F32,), dev)
+        _check("lengths", lengths, (b,), (_I32,), dev)
+    if type(keep) is not int or type(sink) is not int or type(local) is not int or not 1 <= keep <= t \
+            or sink < 0 or local < 0 or sink + local > keep:
         raise ValueError(f"keep must be in [1, {t}] and hold the sink and local tokens")
-    if not lengths.is_contiguous():
-        lengths = lengths.contiguous()
-    ko = torch.empty((b, h, keep, d), dtype=k_cache.dtype, device=dev)
-    vo = torch.empty((b, h, keep, d), dtype=k_cache.dtype, device=dev)
-    wo = torch.empty((b, h, keep), dtype=torch.float32, device=dev)
-    ids = torch.empty((b, h, keep), dtype=torch.int32, device=dev)
-    left = torch.empty((b,), dtype=torch.int32, device=dev)
+    ko = k_cache.new_empty((b, h, keep, d))
+    vo = torch.empty_like(ko)
+    wo = weights.new_empty((b, h, keep))
+    ids = torch.empty_like(wo, dtype=_I32)
+    left = lengths.new_empty(b)
     if not b:
         return ko, vo, wo, ids, left
-    e = k_cache.element_size()
     packed = _EVICT.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), lengths.data_ptr(), ko.data_ptr(), vo.data_ptr(),
-        wo.data_ptr(), ids.data_ptr(), left.data_ptr(), dev.index, b, h, t, d * e, keep, sink, local,
-        *_steps(k_cache, (0, 1, 2), e), *_steps(v_cache, (0, 1, 2), e), *_steps(weights, (0, 1, 2)))
+        wo.data_ptr(), ids.data_ptr(), left.data_ptr(), dev, b, h, t, d, k_cache.element_size(), keep, sink, local,
+        *k_cache.stride(), *v_cache.stride(), *weights.stride(), *lengths.stride())
     _run(_native.load().skv_evict, packed, dev, "evict")
     return ko, vo, wo, ids, left

@@ -90,12 +90,13 @@ def _tree(**kw):
     f = dict(scale=0.1, device=0, dtype=0, bytes=0, b=1, n=2, hq=4, hkv=2, d=64, t=9, ptr=P)
     f.update(kw)
     return operators._TREE.pack(*([f["ptr"]] * 10), f["scale"], f["device"], f["dtype"], f["bytes"], f["b"], f["n"],
-                                f["hq"], f["hkv"], f["d"], f["t"], *([f.get("stride", 64)] * 18))
+                                f["hq"], f["hkv"], f["d"], f["t"], *([*([f.get("stride", 64)] * 3), f.get("inner", 1)] * 5), 64, 64, 1)
 
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(n=65), dict(d=96), dict(hq=5), dict(hkv=0), dict(t=0), dict(t=1 << 30),
                                  dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(dtype=2),
-                                 dict(b=-1), dict(ptr=0), dict(ptr=P + 2), dict(stride=4), dict(stride=-64)])
+                                 dict(b=-1), dict(ptr=0), dict(ptr=P + 2), dict(stride=4), dict(stride=-64),
+                                 dict(inner=2)])
 def test_c_tree_attention_refuses(bad):
     rc, message = _refused("skv_tree_attention", _tree(**bad))
     assert rc == -1 and message
@@ -105,25 +106,25 @@ def _weights(**kw):
     f = dict(scale=0.1, device=0, dtype=0, b=1, n=2, hq=4, hkv=2, d=64, t=9, ptr=P)
     f.update(kw)
     return operators._WEIGHTS.pack(*([f["ptr"]] * 7), f["scale"], f["device"], f["dtype"], f["b"], f["n"], f["hq"],
-                                   f["hkv"], f["d"], f["t"], *([f.get("stride", 64)] * 18))
+                                   f["hkv"], f["d"], f["t"], *([*([f.get("stride", 64)] * 3), f.get("inner", 1)] * 2), *([64] * 12))
 
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(d=63), dict(hq=5), dict(t=0), dict(scale=-1.0), dict(dtype=1), dict(ptr=0),
-                                 dict(ptr=P + 8), dict(stride=12)])
+                                 dict(ptr=P + 8), dict(stride=12), dict(inner=0)])
 def test_c_accumulate_weights_refuses(bad):
     rc, message = _refused("skv_accumulate_weights", _weights(**bad))
     assert rc == -1 and message
 
 
 def _evict(**kw):
-    f = dict(device=0, b=1, hkv=2, t=9, row=128, keep=4, sink=1, local=1, ptr=P)
+    f = dict(device=0, b=1, hkv=2, t=9, d=64, size=2, keep=4, sink=1, local=1, ptr=P)
     f.update(kw)
-    return operators._EVICT.pack(*([f["ptr"]] * 9), f["device"], f["b"], f["hkv"], f["t"], f["row"], f["keep"], f["sink"],
-                                 f["local"], *([128] * 9))
+    return operators._EVICT.pack(*([f["ptr"]] * 9), f["device"], f["b"], f["hkv"], f["t"], f["d"], f["size"], f["keep"],
+                                 f["sink"], f["local"], *([64, 64, 64, f.get("inner", 1)] * 2), *([64] * 4))
 
 
 @pytest.mark.parametrize("bad", [dict(keep=0), dict(keep=10), dict(sink=4), dict(sink=-1), dict(local=-1), dict(hkv=0),
-                                 dict(t=0), dict(row=0), dict(row=1 << 20), dict(ptr=0), dict(b=-1)])
+                                 dict(t=0), dict(d=0), dict(d=1 << 20), dict(size=3), dict(ptr=0), dict(b=-1), dict(inner=2)])
 def test_c_evict_refuses(bad):
     rc, message = _refused("skv_evict", _evict(**bad))
     assert rc == -1 and message
@@ -133,11 +134,11 @@ def _rotary(**kw):
     f = dict(device=0, dtype=0, layout=0, b=1, n=2, hq=4, hkv=2, d=64, r=64, ptr=P, stride=64)
     f.update(kw)
     return operators._ROTARY.pack(*([f["ptr"]] * 6), 1.0, f["device"], f["dtype"], f["layout"], 0, f["b"], f["n"], f["hq"],
-                                  f["hkv"], f["d"], f["r"], *([f["stride"]] * 14))
+                                  f["hkv"], f["d"], f["r"], *([*([f["stride"]] * 3), f.get("inner", 1)] * 4), 64, 1)
 
 
 @pytest.mark.parametrize("bad", [dict(r=0), dict(r=63), dict(r=66), dict(d=1), dict(hq=0), dict(hkv=-1), dict(dtype=3),
-                                 dict(layout=2), dict(ptr=0), dict(b=-1), dict(d=1026, r=514)])
+                                 dict(layout=2), dict(ptr=0), dict(b=-1), dict(d=1026, r=514), dict(inner=2)])
 def test_c_rotary_refuses(bad):
     rc, message = _refused("skv_rotary", _rotary(**bad))
     assert rc == -1 and message
