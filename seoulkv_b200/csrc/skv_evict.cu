@@ -8,12 +8,15 @@
 // their ids -1.
 //
 // Two launches.  k_evict_select, one cluster per (sequence, head): the weights
-// are mapped to integers of the same order, and three histogram passes (11,
-// 11, 10 bits) find the value of the last kept one; the ranks of the tokens
-// above it and of the ties in index order give every kept token its place, so
-// ids come out sorted and the result does not depend on the order of any
-// atomic (they only count).  k_evict_gather then moves the rows at copy
-// bandwidth: every byte is read once and written once.
+// are mapped to integers of the same order, and up to four histogram passes of
+// 8 bits find the value of the last kept one (fewer when a bin is kept whole);
+// the ranks of the tokens above it and of the ties in index order give every
+// kept token its place, so ids come out sorted and the result does not depend
+// on the order of any atomic (they only count).  A pass is a few
+// synchronisations of the cluster and one exchange of 1 KB per CTA: 256 bins,
+// since an exchange of 2048 (three passes of 11 bits) took 3600 cycles each.
+// k_evict_gather then moves the rows at copy bandwidth: every byte is read
+// once and written once.
 #include <cooperative_groups.h>
 
 #include "skv_ops.cuh"
@@ -24,13 +27,13 @@ namespace skv {
 namespace {
 
 constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
-constexpr int EV_BINS = 2048;
+constexpr int EV_BINS = 256;
 // copies of the histogram, one per lane modulo 8: weights share exponents, so
 // a warp's counts fall on few bins and one copy would serialise them
 constexpr int EV_COPIES = 8;
 constexpr int EV_CACHED = 24576;  // keys a CTA holds in shared memory (96 KB); longer segments are read again
-constexpr int EV_CLUSTER = 8;
-constexpr int EV_SMALL = 4096;    // tokens up to which one CTA does a row by itself
+constexpr int EV_CLUSTER = 16;    // most CTAs of a row
+constexpr int EV_ROW = 8192;      // tokens of a row up to which one CTA is enough, and per CTA beyond
 
 struct EvictArgs {
   const float *weights;
@@ -47,7 +50,7 @@ struct SelectSmem {
   uint32_t sum[2][EV_BINS];
   uint32_t scan[EV_WARPS];
   uint32_t tie[EV_WARPS];
-  uint32_t found[2];   // bin, still wanted inside it
+  uint32_t found[3];   // bin, still wanted inside it, its count
   uint32_t total[2];   // this CTA's kept-above and tied counts
   uint32_t key[EV_CACHED];
 };
@@ -95,59 +98,62 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
   uint32_t *mine = s.key + (cached ? warp * seg : 0);
   const int lo = n <= a.keep ? n : a.sink, hi = n - a.local;  // the middle that competes: [lo, hi)
   auto key_at = [&](int i) { return cached ? mine[i - begin] : order_key(w[i * a.ws[2]]); };
-  if (cached)
+  if (cached) {
+#pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) mine[i - begin] = order_key(w[i * a.ws[2]]);
+  }
   uint32_t want = n <= a.keep ? 0u : (uint32_t)(a.keep - a.sink - a.local);
-  uint32_t edge = 0xffffffffu;  // key of the last kept token: kept above it, ties in index order
+  uint32_t edge = 0xffffffffu;  // kept above it, ties in index order
   uint32_t ties = 0;
   if (want) {
     uint32_t prefix = 0;
-    int pass = 0;
-    for (int shift : {21, 10, 0}) {
-      const int bits = shift ? 11 : 10;
+    for (int shift = 24; shift >= 0; shift -= 8) {
       for (int i = tid; i < EV_COPIES * EV_BINS; i += EV_THREADS) (&s.hist[0][0])[i] = 0;
       __syncthreads();
+      uint32_t *hist = s.hist[lane % EV_COPIES];
+#pragma unroll 4
       for (int i = begin + lane; i < end; i += 32) {
-        if (i < lo || i >= hi) continue;
         const uint32_t k = key_at(i);
-        if (pass && (k >> (shift + bits)) != prefix) continue;
-        atomicAdd(&s.hist[lane % EV_COPIES][(k >> shift) & ((1u << bits) - 1)], 1u);
+        if (i >= lo && i < hi && (shift == 24 || k >> (shift + 8) == prefix)) atomicAdd(hist + (k >> shift & 255u), 1u);
       }
       __syncthreads();
-      uint32_t *sum = s.sum[pass & 1];
-      for (int i = tid; i < EV_BINS; i += EV_THREADS) {
+      uint32_t *sum = s.sum[shift >> 3 & 1];
+      if (tid < EV_BINS) {
         uint32_t x = 0;
 #pragma unroll
-        for (int c = 0; c < EV_COPIES; ++c) x += s.hist[c][i];
-        sum[i] = x;
+        for (int c = 0; c < EV_COPIES; ++c) x += s.hist[c][tid];
+        sum[tid] = x;
       }
-      cluster.sync();  // (also keeps the other buffer's remote readers of the pass before apart from its next writes)
-      // thread t: the two bins 2047 - 2t, 2046 - 2t, so that a prefix sum runs from the largest keys down
-      const int top = EV_BINS - 1 - 2 * tid;
-      uint32_t c0 = 0, c1 = 0;
-      for (int r = 0; r < ranks; ++r) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(sum, r) + top - 1);
-        c0 += v.y;
-        c1 += v.x;
-      }
-      const uint32_t inc = warp_inclusive(c0 + c1, lane);
-      if (lane == 31) s.scan[warp] = inc;
-      __syncthreads();
-      if (warp == 0) s.scan[lane] = warp_inclusive(s.scan[lane], lane);
-      __syncthreads();
-      const uint32_t upto = inc + (warp ? s.scan[warp - 1] : 0u), before = upto - c0 - c1;
-      if (before < want && want <= upto) {
-        const bool second = before + c0 < want;
-        s.found[0] = (uint32_t)(top - (second ? 1 : 0));
-        s.found[1] = want - before - (second ? c0 : 0u);
+      // (also keeps the other buffer's remote readers of the pass before apart from its next writes)
+      if (ranks > 1) cluster.sync(); else __syncthreads();
+      // thread t: bin 255 - t, so that a prefix sum runs from the largest keys down
+      uint32_t count = 0, inc = 0;
+      if (tid < EV_BINS) {
+        const int bin = EV_BINS - 1 - tid;
+        for (int r = 0; r < ranks; ++r) count += ranks > 1 ? cluster.map_shared_rank(sum, r)[bin] : sum[bin];
+        inc = warp_inclusive(count, lane);
+        if (lane == 31) s.scan[warp] = inc;
       }
       __syncthreads();
-      prefix = (prefix << bits) | s.found[0];
+      if (tid < EV_BINS) {
+        for (int x = 0; x < warp; ++x) inc += s.scan[x];
+        if (inc - count < want && want <= inc) {
+          s.found[0] = (uint32_t)(EV_BINS - 1 - tid);
+          s.found[1] = want - (inc - count);
+          s.found[2] = count;
+        }
+      }
+      __syncthreads();
+      prefix = prefix << 8 | s.found[0];
       want = s.found[1];
-      ++pass;
+      edge = prefix;
+      ties = want;
+      if (want == s.found[2] && prefix) {  // the bin is kept whole: everything from its first key on
+        edge = (prefix << shift) - 1;
+        ties = 0;
+        break;
+      }
     }
-    edge = prefix;
-    ties = want;
   }
   // places: tokens kept for certain and tied ones, counted per warp, CTA and cluster
   auto kinds = [&](int i, bool &above, bool &tied) {
@@ -163,6 +169,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
   };
   uint32_t n_above = 0, n_tied = 0;
   __syncwarp();
+#pragma unroll 4
   for (int i0 = begin; i0 < end; i0 += 32) {
     bool above, tied;
     kinds(i0 + lane, above, tied);
@@ -186,19 +193,29 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
     tie += o[1];
   }
   const uint32_t below = (1u << lane) - 1u;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    bool above, tied;
-    const int i = i0 + lane;
-    kinds(i, above, tied);
-    const uint32_t ba = __ballot_sync(0xffffffffu, above), bt = __ballot_sync(0xffffffffu, tied);
-    const uint32_t tie_before = tie + __popc(bt & below);
-    if (above || (tied && tie_before < ties)) {
-      const uint32_t place = at + __popc(ba & below) + min(tie_before, ties);
-      ids[place] = i;
-      out_w[place] = w[i * a.ws[2]];
+  constexpr int BLOCKS = 4;  // of 32 tokens, whose weights are loaded together
+  for (int i0 = begin; i0 < end; i0 += 32 * BLOCKS) {
+    float x[BLOCKS];
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const int i = i0 + 32 * u + lane;
+      x[u] = i < end ? w[i * a.ws[2]] : 0.0f;
     }
-    at += __popc(ba);
-    tie += __popc(bt);
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      bool above, tied;
+      const int i = i0 + 32 * u + lane;
+      kinds(i, above, tied);
+      const uint32_t ba = __ballot_sync(0xffffffffu, above), bt = __ballot_sync(0xffffffffu, tied);
+      const uint32_t tie_before = tie + __popc(bt & below);
+      if (above || (tied && tie_before < ties)) {
+        const uint32_t place = at + __popc(ba & below) + min(tie_before, ties);
+        ids[place] = i;
+        out_w[place] = x[u];
+      }
+      at += __popc(ba);
+      tie += __popc(bt);
+    }
   }
   if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
@@ -293,9 +310,17 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   a.sink = (int)d->sink, a.local = (int)d->local;
   static bool set[64];
   int sms = 0, rc = sm_count((int)d->device, &sms);  // (checks the ordinal)
+  static bool wide[64];
+  if (!rc && !__atomic_load_n(&wide[d->device], __ATOMIC_RELAXED)) {  // clusters of 16 are not portable
+    rc = op_cuda(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
+    if (!rc) __atomic_store_n(&wide[d->device], true, __ATOMIC_RELAXED);
+  }
   if (!rc) rc = op_shared_memory(reinterpret_cast<const void *>(&k_evict_select), (int)sizeof(SelectSmem), (int)d->device, set);
   if (rc) return rc;
-  const int ranks = d->tokens <= EV_SMALL ? 1 : EV_CLUSTER;
+  // CTAs of a row: as many as its length gives work to, while all rows fit on
+  // the device together (a 128K row: one CTA 60 us, sixteen 10 us)
+  int ranks = 1;
+  while (ranks < EV_CLUSTER && d->tokens > (int64_t)EV_ROW * ranks && d->batch * d->kv_heads * ranks * 2 <= sms) ranks *= 2;
   rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
                          sizeof(SelectSmem), st, false, (unsigned)ranks, a), "k_evict_select launch");
   if (rc) return rc;
