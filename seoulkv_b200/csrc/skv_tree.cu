@@ -691,24 +691,27 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 // ---- joining the parts of a unit ---------------------------------------------
 
 constexpr int TC_THREADS = 256, TC_MAX = 512;  // most items of a launch
+constexpr int TC_BATCH = 8;                    // parts whose O a thread has in flight
 
-// One row per block: out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over
-// the CTAs c of the row's unit, in their order.  D / 4 threads hold the row;
-// the groups of them take every TC_THREADS / (D / 4)-th part.
-template <int D>
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the items c of a
+// row's unit, in their order.  D / 4 threads hold a row's O.  With many items
+// a unit a block has one row and its groups of threads share the parts; with
+// few every group has a row of its own.  What bounds it is latency: the parts
+// are in L2, and all loads of a thread are issued before the first is used.
+template <int D, bool FEW>
 __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_constant__ TreeArgs a, int groups) {
   constexpr int LANES = D / 4, GROUPS = TC_THREADS / LANES;
   __shared__ int32_t s_pre[PLAN_BATCH + 1];
-  __shared__ float s_w[TC_MAX];
-  __shared__ float s_red[2][TC_THREADS / 32];
-  __shared__ float4 s_o[GROUPS][LANES];
-  __shared__ int s_dead;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ float2 s_ml[FEW ? 1 : TC_MAX];
+  __shared__ float s_red[1][TC_THREADS / 32];
+  __shared__ float4 s_o[FEW ? 1 : GROUPS][LANES];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = tid / LANES, d4 = tid % LANES;
   if (warp == 0) tile_prefix<TR_KEYS>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
-  if (tid == 0) s_dead = 0;
   __syncthreads();
-  const int rows = a.n * a.group;
-  const int r = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % a.heads, b = bh / a.heads;
+  const int rows = a.n * a.group, all = rows * a.heads * a.batch;
+  const int index = FEW ? blockIdx.x * GROUPS + group : blockIdx.x;
+  if (index >= all) return;  // (no barrier of the block below where FEW)
+  const int r = index % rows, bh = index / rows, h = bh % a.heads, b = bh / a.heads;
   const int mt = r / TR_ROWS, places = s_pre[b + 1] - s_pre[b];
   const Plan plan((long long)s_pre[a.batch] * a.heads, groups);
   const long long g0 = (long long)s_pre[b] * a.heads + (long long)h * places;
@@ -718,58 +721,72 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   grid_dependency_wait();
   const int parts = c1 - c0 + 1, prow = r - mt * TR_ROWS;
   auto slot = [&](int i) { return (int64_t)(2 * ((c0 + i) * a.mtiles + mt) + (i == 0 ? shift : 0)) * a.rows + prow; };
+  auto o_of = [&](int i) { return __ldcg(reinterpret_cast<const float4 *>(a.part + slot(i) * D) + d4); };
+  const int first = FEW ? 0 : group, gap = FEW ? 1 : GROUPS;
+  float4 x[TC_BATCH];
+#pragma unroll
+  for (int k = 0; k < TC_BATCH; ++k)
+    if (first + k * gap < parts) x[k] = o_of(first + k * gap);
+  // the row's maximum, its sum, and whether it is unused (l < 0 in a part)
   float m = -INFINITY, l = 0.0f;
-  for (int i = tid; i < parts; i += TC_THREADS) {
-    const float2 x = __ldcg(a.ml + slot(i));
-    if (x.y < 0.0f) s_dead = 1;
-    s_w[i] = x.x;
-    m = fmaxf(m, x.x);
+  bool dead = false;
+  if (FEW) {
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, __ldcg(a.ml + slot(i)).x);
+  } else {
+    for (int i = tid; i < parts; i += TC_THREADS) {
+      s_ml[i] = __ldcg(a.ml + slot(i));
+      m = fmaxf(m, s_ml[i].x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_red[0][warp] = m;
+    __syncthreads();
+    m = s_red[0][0];
+#pragma unroll
+    for (int i = 1; i < TC_THREADS / 32; ++i) m = fmaxf(m, s_red[0][i]);
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) s_red[0][warp] = m;
-  __syncthreads();
-  m = s_red[0][0];
-#pragma unroll
-  for (int i = 1; i < TC_THREADS / 32; ++i) m = fmaxf(m, s_red[0][i]);
   const float base = m == -INFINITY ? 0.0f : m;
-  for (int i = tid; i < parts; i += TC_THREADS) {
-    const float w = exp2_fast(s_w[i] - base);
-    s_w[i] = w;
-    l += w * __ldcg(a.ml + slot(i)).y;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) s_red[1][warp] = l;
-  __syncthreads();
-  l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < TC_THREADS / 32; ++i) l += s_red[1][i];
-  const int group = tid / LANES, d4 = tid % LANES;
   float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int i = group; i < parts; i += GROUPS) {
-    const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.part + slot(i) * D) + d4);
-    const float w = s_w[i];
+  auto ml_of = [&](int i) { return FEW ? __ldcg(a.ml + slot(i)) : s_ml[i]; };
+  auto add = [&](const float4 &v, int i) {
+    const float2 ml = ml_of(i);
+    const float w = exp2_fast(ml.x - base);
+    dead = dead || ml.y < 0.0f;
+    l += w * ml.y;
     // (a part without a visible key has weight 0 and zeros or, for an unused row, anything)
     if (w != 0.0f) {
-      o.x = fmaf(w, x.x, o.x);
-      o.y = fmaf(w, x.y, o.y);
-      o.z = fmaf(w, x.z, o.z);
-      o.w = fmaf(w, x.w, o.w);
+      o.x = fmaf(w, v.x, o.x);
+      o.y = fmaf(w, v.y, o.y);
+      o.z = fmaf(w, v.z, o.z);
+      o.w = fmaf(w, v.w, o.w);
     }
-  }
-  s_o[group][d4] = o;
-  __syncthreads();
-  if (group) return;
+  };
 #pragma unroll
-  for (int i = 1; i < GROUPS; ++i) {
-    const float4 x = s_o[i][d4];
-    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+  for (int k = 0; k < TC_BATCH; ++k)
+    if (first + k * gap < parts) add(x[k], first + k * gap);
+  for (int i = first + TC_BATCH * gap; i < parts; i += gap) add(o_of(i), i);
+  if (!FEW) {
+    // the groups' parts, in order
+    s_o[group][d4] = o;
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(s_pre);  // (its last use is above)
+    if (d4 == 0) sums[group] = dead ? -INFINITY : l;
+    __syncthreads();
+    if (group) return;
+    l = 0.0f;
+    dead = false;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      dead = dead || sums[i] == -INFINITY;
+      l += sums[i];
+      if (i) {
+        const float4 v = s_o[i][d4];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+      }
+    }
   }
   const int node = r / a.group;
   const int64_t row = ((int64_t)b * a.n + node) * (a.heads * a.group) + h * a.group + (r - node * a.group);
-  const bool dead = s_dead;
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   const uint2 y = dead ? make_uint2(0, 0) : make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   reinterpret_cast<uint2 *>(a.out + row * D)[d4] = y;
@@ -787,7 +804,12 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, c
                        "k_tree_attention launch"))
     return rc;
   const unsigned rows = (unsigned)(a.batch * a.heads * a.n * a.group);
-  return op_cuda(op_launch(k_tree_combine<C::D>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, ctas / a.mtiles),
+  const int items = ctas / a.mtiles;
+  constexpr unsigned per = TC_THREADS / (C::D / 4);
+  // (a unit has about items / units parts: more than one thread group's batch of them is shared)
+  const bool few = items <= (TC_BATCH - 2) * a.batch * a.heads;
+  return op_cuda(few ? op_launch(k_tree_combine<C::D, true>, dim3((rows + per - 1) / per), dim3(TC_THREADS), 0, st, true, 1, a, items)
+                     : op_launch(k_tree_combine<C::D, false>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, items),
                  "k_tree_combine launch");
 }
 
