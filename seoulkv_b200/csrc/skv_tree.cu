@@ -363,30 +363,45 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       __syncwarp();
       tc_fence_after();
     };
-    while (w.next()) {
-      const int n = w.count, h = w.unit;
-      const int len = length(w.b);
-      const bool has_nodes = w.tile + n == w.tiles;
-      // every S of the segment before has been read, so its MMAs are done with Q
-      for (int x = st; x < min(left, TR_ROWS) * (D / 8); x += 256) {
-        const int at = x / (D / 8), c16 = x % (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
-        const uint16_t *q = a.q + w.b * a.qs[0] + nd * a.qs[1] + (h * a.group + rr - nd * a.group) * a.qs[2];
-        *reinterpret_cast<uint4 *>(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16) =
-            __ldg(reinterpret_cast<const uint4 *>(q) + c16);
+    auto load_queries = [&](const Walk &x) {
+      // (several loads in flight per thread: one after the other a segment
+      // would wait 4000 cycles for its queries)
+      constexpr int BATCH = 4;
+      const int total = min(left, TR_ROWS) * (D / 8);
+      for (int c0 = st; c0 < total; c0 += 256 * BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int c = c0 + 256 * j, at = c / (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
+          const uint16_t *q = a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2];
+          if (c < total) v[j] = __ldg(reinterpret_cast<const uint4 *>(q) + c % (D / 8));
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int c = c0 + 256 * j, at = c / (D / 8), c16 = c % (D / 8);
+          if (c < total)
+            *reinterpret_cast<uint4 *>(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16) = v[j];
+        }
       }
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
-      uint64_t see = 0;
-      if (has_nodes) {
-        // ancestors by pointer doubling: after k rounds a node knows 2^k of its line
-        uint64_t mask = 0;
-        int up = -2;
-        if (st < a.n) {
-          up = a.parents[w.b * a.ps[0] + st * a.ps[1]];
-          if (up < -1 || up >= st) up = -2;
-          mask = up == -2 ? 0 : 1ull << st;
-        }
+    };
+    bool live = w.next();
+    if (live) load_queries(w);
+    while (live) {
+      const Walk cur = w;
+      live = w.next();
+      const int n = cur.count, h = cur.unit;
+      const int len = length(cur.b);
+      const bool has_nodes = cur.tile + n == cur.tiles;
+      int up = -2;  // the parent of node st, wanted at the segment's last tile
+      if (has_nodes && st < a.n) up = a.parents[cur.b * a.ps[0] + st * a.ps[1]];
+      uint64_t see = 0;  // the nodes that this row sees
+      auto ancestors = [&] {
+        // by pointer doubling: after k rounds a node knows 2^k of its line
+        if (up < -1 || up >= st) up = -2;
+        uint64_t mask = up == -2 ? 0 : 1ull << (st & 63);
         for (int step = 1;; step <<= 1) {
           if (st < TR_NODES) {
             s.anc[st] = mask;
@@ -404,14 +419,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
         }
         if (on) see = s.anc[node];
-      }
-      const bool dead = has_nodes && see == 0;
+      };
       float m = -INFINITY, l = 0.0f;  // the row's running maximum (log2 units), this thread's part of the sum
       for (int i = 0; i < n; ++i) {
         const uint32_t buf = (gt + i) & 1;
         const uint32_t at = lanes + C::COL_S + buf * KT;
-        const bool nodes = w.tile + i == w.tiles - 1;
-        const int valid = nodes ? a.n : min(KT, len - (w.tile + i) * KT);
+        const bool nodes = cur.tile + i == cur.tiles - 1;
+        if (nodes) ancestors();
+        // (the length is first looked at where it matters: its load is long done by then)
+        const int valid = nodes ? a.n : cur.tile + i < cur.tiles - 2 ? KT : min(KT, len - (cur.tile + i) * KT);
         const bool whole = valid == KT && !nodes;
         const int v64 = valid - 64 * half;
         const uint64_t keep = nodes ? (half ? 0 : see) : v64 >= 64 ? ~0ull : v64 > 0 ? (1ull << v64) - 1 : 0;
@@ -545,30 +561,34 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         __syncwarp();
         if (lane == 0) bar_arrive(&s.p_ready[buf]);
       }
+      // this segment's scores have all been read, so the tensor core is done
+      // with its queries: the next segment's scores start beside the last product
+      if (live) load_queries(w);
       // ---- the unit's rows, or this item's part of them
+      const bool dead = has_nodes && see == 0;
       done(s.o_done, gt + n - 1);
       uint64_t bad = 0;
       if (has_nodes) {
         asm volatile("bar.sync 1, 256;" ::: "memory");
         bad = s.bad & see;
       }
-      const bool direct = n == w.tiles;
+      const bool direct = n == cur.tiles;
       if (warp_on) {
         s.share[half][row] = l;
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
         l = s.share[0][row] + s.share[1][row];
         if (*abort) l = __uint_as_float(0x7fffffffu);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const int64_t out_row = ((int64_t)w.b * a.n + node) * (a.heads * a.group) + h * a.group + qg;
-        const int64_t part_row = (int64_t)(2 * blockIdx.x + (walk.g < w.start ? 1 : 0)) * a.rows + row;
-#pragma unroll 1
+        const int64_t out_row = ((int64_t)cur.b * a.n + node) * (a.heads * a.group) + h * a.group + qg;
+        const int64_t part_row = (int64_t)(2 * blockIdx.x + (walk.g < cur.start ? 1 : 0)) * a.rows + row;
+#pragma unroll(C::F8 ? 1 : 2)
         for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
           uint32_t x[32];
           tmem_ld32(x, lanes + 32 * c);
           tmem_wait_ld();
           if (bad)
             for (uint64_t rest = bad; rest; rest &= rest - 1) {
-              const uint16_t *vn = a.vn + w.b * a.vns[0] + h * a.vns[1] + (__ffsll((long long)rest) - 1) * a.vns[2] + 32 * c;
+              const uint16_t *vn = a.vn + cur.b * a.vns[0] + h * a.vns[1] + (__ffsll((long long)rest) - 1) * a.vns[2] + 32 * c;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const uint32_t v = vn[j];

@@ -180,14 +180,24 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
       const int h = w.unit;
       // the head's rows, once the tensor core is done with the ones before
       if (seg) wait(&s.q_free, (seg - 1) & 1);
-      for (int x = et; x < a.cols * (D / 8); x += 256) {
-        const int r = x / (D / 8), c16 = x % (D / 8), row = a.row0 + r;
-        const int node = row / a.group, qh = h * a.group + row - node * a.group;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]]) &&
-            a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]] != -INFINITY)
-          v = __ldg(reinterpret_cast<const uint4 *>(a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2]) + c16);
-        *reinterpret_cast<uint4 *>(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16) = v;
+      constexpr int BATCH = 4;  // loads in flight per thread
+      for (int x0 = et; x0 < a.cols * (D / 8); x0 += 256 * BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int x = x0 + 256 * j, r = x / (D / 8), row = a.row0 + r;
+          const int node = row / a.group, qh = h * a.group + row - node * a.group;
+          v[j] = make_uint4(0, 0, 0, 0);
+          if (r < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]]) &&
+              a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]] != -INFINITY)
+            v[j] = __ldg(reinterpret_cast<const uint4 *>(a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2]) + x % (D / 8));
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int x = x0 + 256 * j, r = x / (D / 8), c16 = x % (D / 8);
+          if (r < a.cols)
+            *reinterpret_cast<uint4 *>(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16) = v[j];
+        }
       }
       if (et < a.cols) {
         float l2 = INFINITY;
