@@ -124,8 +124,10 @@ struct TreeCfg {
   static constexpr int VROWS = KT / PIECES;  // keys of a V stage
   static constexpr int STAGE = KT * 128;  // bytes: K 128 keys x 64 dimensions, V VROWS keys x D
   static constexpr int RAW = STAGE / 2;   // an FP8 stage before its conversion
-  static constexpr int NRAW = F8 ? 8 : 0;
-  static constexpr int NSTAGE = F8 ? 6 : D == 256 ? 10 : D == 128 ? 11 : 12;
+  // (FP8: multiples of the converting groups, so that a place in either ring
+  // belongs to one group, which sees its phases in turn)
+  static constexpr int NRAW = F8 ? (D == 256 ? 4 : 8) : 0;
+  static constexpr int NSTAGE = F8 ? 8 : D == 256 ? 10 : D == 128 ? 11 : 12;
   static constexpr int THREADS = F8 ? 576 : 384;  // FP8: warps 2, 3 and 12.. convert
   static constexpr int COL_S = 256;       // tensor memory columns: O, then two score tiles (P over S)
   static constexpr int QBYTES = TR_ROWS * D * 2;
@@ -261,7 +263,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         int i;
         tile_at(p, w.count, is_v, i);
         const bool nodes = w.tile + i == w.tiles - 1;
-        if (C::F8 && nodes) continue;
         const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
         const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
         if (C::F8 && a.cell_maps) map = a.cell_maps + 2 * ((int64_t)w.b * a.heads + w.unit) + is_v;
@@ -270,7 +271,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
           const int slot = seq % SLOTS;
           if (!(ok = wait(&freed[slot], ((seq / SLOTS) & 1) ^ 1))) break;
-          if (C::F8)
+          if (C::F8 && nodes) {  // (not FP8: copied by the converting warps; the place in the ring passes)
+            if (one) bar_arrive(&landed[slot]);
+          } else if (C::F8)
             tma_load_bytes(one, raw + slot * C::RAW, map, is_v ? 0 : piece * 64, row + (is_v ? piece * C::VROWS : 0), y,
                            z, &landed[slot], C::RAW);
           else
@@ -364,25 +367,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       tc_fence_after();
     };
     auto load_queries = [&](const Walk &x) {
-      // (several loads in flight per thread: one after the other a segment
-      // would wait 4000 cycles for its queries)
-      constexpr int BATCH = 4;
+      // asynchronous copies in a short loop: code that runs once per segment
+      // waits for its instructions when it is unrolled
       const int total = min(left, TR_ROWS) * (D / 8);
-      for (int c0 = st; c0 < total; c0 += 256 * BATCH) {
-        uint4 v[BATCH];
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const int c = c0 + 256 * j, at = c / (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
-          const uint16_t *q = a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2];
-          if (c < total) v[j] = __ldg(reinterpret_cast<const uint4 *>(q) + c % (D / 8));
-        }
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const int c = c0 + 256 * j, at = c / (D / 8), c16 = c % (D / 8);
-          if (c < total)
-            *reinterpret_cast<uint4 *>(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16) = v[j];
-        }
+#pragma unroll 1
+      for (int c = st; c < total; c += 256) {
+        const int at = c / (D / 8), c16 = c % (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
+        cp_async16(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16,
+                   a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2] + c16 * 8, true);
       }
+      cp_async_wait();
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
@@ -581,7 +575,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const int64_t out_row = ((int64_t)cur.b * a.n + node) * (a.heads * a.group) + h * a.group + qg;
         const int64_t part_row = (int64_t)(2 * blockIdx.x + (walk.g < cur.start ? 1 : 0)) * a.rows + row;
-#pragma unroll(C::F8 ? 1 : 2)
+#pragma unroll 1
         for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
           uint32_t x[32];
           tmem_ld32(x, lanes + 32 * c);
@@ -630,6 +624,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     constexpr int GROUPS = 4, CHUNKS = C::RAW / 16 / TR_GROUP;  // 16-code pieces of one thread and stage
     const int ct = tid % TR_GROUP, grp = warp < 4 ? 0 : (warp - 10) / 2;
     static_assert(TR_GROUP == 64 && GROUPS % C::PIECES == 0, "groups of two warps, one stage each");
+    static_assert(!C::F8 || (C::NRAW % GROUPS == 0 && C::NSTAGE % GROUPS == 0), "places of one group");
     // Piece j of this thread: K key ct / 4 + KSTEP j, dimensions 16 (ct % 4)..
     // of the stage's 64 (KSTEP is a multiple of 8: one swizzle for all j); V
     // key CHUNKS (ct / VPER) + j of the stage's, dimensions 16 (ct % VPER)...
@@ -642,20 +637,18 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     constexpr uint32_t SLOTS = C::F8 ? C::NRAW : 1;
     const int piece = grp % C::PIECES;
     Walk w = walk;
-    uint32_t base = 0, raw_base = 0;  // stages, and FP8 stages, of the segments before
+    uint32_t base = 0;  // stages of the segments before
     bool ok = true;
     while (ok && w.next()) {
       const int n = w.count, len = length(w.b);
-      const int k_nodes = w.tile + n == w.tiles ? pos_k(n - 1) : 2 * n;  // place of the nodes' K (they are in the last tile)
-      for (int p = grp / C::PIECES; p < 2 * n; p += GROUPS / C::PIECES) {
+      for (int p = (grp - base % GROUPS + GROUPS) % GROUPS / C::PIECES; p < 2 * n; p += GROUPS / C::PIECES) {
         bool is_v;
         int i;
         tile_at(p, n, is_v, i);
-        const uint32_t seq = base + p * C::PIECES + piece, stage = seq % C::NSTAGE;
+        const uint32_t seq = base + p * C::PIECES + piece, stage = seq % C::NSTAGE, slot = seq % SLOTS;
         uint8_t *to = ring + stage * C::STAGE;
         if (w.tile + i < w.tiles - 1) {
-          const uint32_t raw_at = raw_base + (p - (p > k_nodes)) * C::PIECES + piece, slot = raw_at % SLOTS;
-          if (!(ok = wait(&s.raw_full[slot], (raw_at / SLOTS) & 1))) break;
+          if (!(ok = wait(&s.raw_full[slot], (seq / SLOTS) & 1))) break;
           if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
           const int left = len - (w.tile + i) * KT - (is_v ? piece * C::VROWS + key_v : key_k);  // keys from this thread's first
           const int gap = is_v ? 1 : KSTEP, turn = is_v ? 7 : 0;
@@ -680,6 +673,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               for (int u = 0; u < 2; ++u)
                 e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * gap * 128 + ((first ^ (j & turn)) ^ u) * 16));
         } else {
+          if (!(ok = wait(&s.raw_full[slot], (seq / SLOTS) & 1))) break;
+          if (lane == 0) bar_arrive(&s.raw_empty[slot]);
           if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
           const uint16_t *src = is_v ? a.vn + w.b * a.vns[0] + w.unit * a.vns[1] : a.kn + w.b * a.kns[0] + w.unit * a.kns[1];
           const int64_t st = is_v ? a.vns[2] : a.kns[2];
@@ -697,7 +692,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (lane == 0) bar_arrive(&s.full[stage]);
       }
       base += 2 * n * C::PIECES;
-      raw_base += (2 * n - (k_nodes < 2 * n ? 2 : 0)) * C::PIECES;
     }
   }
   tc_fence_before();

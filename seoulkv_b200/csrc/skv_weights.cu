@@ -24,14 +24,14 @@ namespace {
 constexpr int WT_KEYS = 128, WT_PIECE = WT_KEYS * 128;  // bytes of a piece
 constexpr int WT_ROWS = 256;                            // rows of one launch: the MMA's largest N
 constexpr int WT_STAGES = 12;
-constexpr int WT_RAW = 6;                               // FP8 pieces in flight
+constexpr int WT_RAW = 8;                               // FP8 pieces in flight
+constexpr int WT_ROWS_F8 = 128;                         // rows of one launch over an FP8 cache (its rings need room)
+constexpr int WT_GROUP = 64;                            // threads that turn an FP8 piece into BF16
 constexpr int WT_THREADS = 384, WT_THREADS_F8 = 640;
 
 struct WeightsArgs {
   const uint16_t *q;
   int64_t qs[3];  // element strides (sequence, node, head)
-  const uint8_t *k8;
-  int64_t k8s[3];  // FP8 cache: byte strides (sequence, head, token)
   const int32_t *lengths;
   int64_t len_stride;
   const float *lse;
@@ -43,13 +43,13 @@ struct WeightsArgs {
   int64_t ws[3], os[3];  // (sequence, head, token)
   int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head; cols: rows up to 16s
   int32_t along[2];
-  int32_t stages;
+  int32_t stages;  // pieces of the ring
   float c2;
   uint32_t *status;
 };
 
 struct WeightsSmem {
-  uint64_t full[WT_STAGES], empty[WT_STAGES];
+  uint64_t full[WT_STAGES], empty[WT_STAGES], raw_full[WT_RAW], raw_empty[WT_RAW];
   uint64_t q_ready, q_free, acc_full[2], acc_free[2], drain;
   uint32_t tmem, abort;
   alignas(16) float lse2[2][WT_ROWS];  // log2(e) * lse, +inf for rows that do not count
@@ -65,18 +65,22 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   uint8_t *queries = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;  // [SUB][cols][128 bytes], swizzled
   uint8_t *ring = queries + SUB * a.cols * 128;
   uint8_t *raw = ring + a.stages * WT_PIECE;
-  WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(raw + (F8 ? WT_RAW * WT_PIECE / 2 : 0));
+  WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(raw + (F8 ? WT_RAW * (WT_PIECE / 2) : 0));
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int stages = a.stages;
   if (warp == 0) {
     tile_prefix<WT_KEYS>(a.lengths, a.len_stride, 0, a.t, a.batch, 0, s.len, s.pre);
-    if (lane == 0 && !F8) tma_prefetch_map(&map);
+    if (lane == 0) tma_prefetch_map(&map);
   } else if (warp == 1) {
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
     for (int i = 0; i < stages; ++i) {
-      bar_init(&s.full[i], F8 ? 8 : 1);
+      bar_init(&s.full[i], F8 ? WT_GROUP / 32 : 1);
       bar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < (F8 ? WT_RAW : 0); ++i) {
+      bar_init(&s.raw_full[i], 1);
+      bar_init(&s.raw_empty[i], WT_GROUP / 32);
     }
     bar_init(&s.q_ready, 8);
     bar_init(&s.q_free, 1);
@@ -99,28 +103,33 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   const long long g_begin = plan.begin(cta), g_end = plan.begin(cta + 1);
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
 
-  if (warp == 0 && !F8) {
-    // ---- loads
+  if (warp == 0) {
+    // ---- loads: BF16 pieces into the ring, FP8 pieces beside it
     const uint32_t one = elect_lane();
+    const int slots = F8 ? WT_RAW : stages;
+    uint64_t *const landed = F8 ? s.raw_full : s.full, *const freed = F8 ? s.raw_empty : s.empty;
     Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
     uint32_t seq = 0;
-    int stage = 0;
+    int slot = 0;
     uint32_t turn = 0;
     bool ok = true;
     while (ok && w.next())
       for (int i = 0; i < w.count && ok; ++i)
         for (int sub = 0; sub < SUB; ++sub) {
-          if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
-          tma_load(one, ring + stage * WT_PIECE, &map, (w.tile + i) * WT_KEYS, sub, w.unit * a.along[0],
-                   w.b * a.along[1], &s.full[stage], WT_PIECE);
+          if (!(ok = wait(&freed[slot], turn ^ 1))) break;
+          const int row = (w.tile + i) * WT_KEYS, y = w.unit * a.along[0], z = w.b * a.along[1];
+          if (F8)
+            tma_load_bytes(one, raw + slot * (WT_PIECE / 2), &map, sub * 64, row, y, z, &landed[slot], WT_PIECE / 2);
+          else
+            tma_load(one, ring + slot * WT_PIECE, &map, row, sub, y, z, &landed[slot], WT_PIECE);
           ++seq;
-          if (++stage == stages) stage = 0, turn ^= 1;
+          if (++slot == slots) slot = 0, turn ^= 1;
         }
     if (!ok)  // gave up: the copies in flight still land before the CTA ends
-      for (uint32_t back = 1; back <= (uint32_t)stages && back <= seq; ++back) {
+      for (uint32_t back = 1; back <= (uint32_t)slots && back <= seq; ++back) {
         const uint32_t q = seq - back;
         const unsigned long long t0 = timer_ns();
-        while (!bar_try(&s.full[q % stages], (q / stages) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+        while (!bar_try(&landed[q % slots], (q / slots) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
         }
       }
   } else if (warp == 1) {
@@ -180,25 +189,6 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
       const int h = w.unit;
       // the head's rows, once the tensor core is done with the ones before
       if (seg) wait(&s.q_free, (seg - 1) & 1);
-      constexpr int BATCH = 4;  // loads in flight per thread
-      for (int x0 = et; x0 < a.cols * (D / 8); x0 += 256 * BATCH) {
-        uint4 v[BATCH];
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const int x = x0 + 256 * j, r = x / (D / 8), row = a.row0 + r;
-          const int node = row / a.group, qh = h * a.group + row - node * a.group;
-          v[j] = make_uint4(0, 0, 0, 0);
-          if (r < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]]) &&
-              a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]] != -INFINITY)
-            v[j] = __ldg(reinterpret_cast<const uint4 *>(a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2]) + x % (D / 8));
-        }
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          const int x = x0 + 256 * j, r = x / (D / 8), c16 = x % (D / 8);
-          if (r < a.cols)
-            *reinterpret_cast<uint4 *>(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16) = v[j];
-        }
-      }
       if (et < a.cols) {
         float l2 = INFINITY;
         const int row = a.row0 + et, node = row / a.group, qh = h * a.group + row - node * a.group;
@@ -208,8 +198,19 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
         }
         s.lse2[seg & 1][et] = l2;
       }
-      async_fence();
       asm volatile("bar.sync 2, 256;" ::: "memory");
+      // asynchronous copies in a short loop: code that runs once per launch
+      // waits for its instructions, and unrolled loads took 20000 cycles here
+#pragma unroll 1
+      for (int x = et; x < a.cols * (D / 8); x += 256) {
+        const int r = x / (D / 8), c16 = x % (D / 8), row = a.row0 + min(r, a.rows - 1);
+        const int node = row / a.group, qh = h * a.group + row - node * a.group;
+        cp_async16(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16,
+                   a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2] + c16 * 8, s.lse2[seg & 1][r] != INFINITY);
+      }
+      cp_async_wait();
+      async_fence();
+      __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
       const float4 *lse2 = reinterpret_cast<const float4 *>(s.lse2[seg & 1]);
       const float *wrow = a.w + w.b * a.ws[0] + h * a.ws[1];
@@ -246,77 +247,49 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
       ++seg;
     }
   } else if (F8) {
-    // ---- FP8 caches: pieces copied ahead with cp.async, each thread its own
-    // 16 codes, turned into BF16 where TMA would have put a BF16 piece
-    constexpr int CHUNKS = WT_PIECE / 2 / 16 / 256;  // of one thread and piece
-    const int ct = tid - 384;
-    struct Items {
-      Walk w;
-      int tile = 0, sub = 0;
-      bool live;
-      __device__ Items(const Walk &x) : w(x) { live = w.next(); }
-      __device__ void step() {
-        if (++sub < SUB) return;
-        sub = 0;
-        if (++tile < w.count) return;
-        tile = 0;
-        live = w.next();
-      }
-    };
-    Items ahead(Walk(s.pre, a.batch, a.heads, 0, g_begin, g_end)), now = ahead;
-    auto issue = [&](const Items &it, int slot) {
-      if (it.live) {
-        const uint8_t *src = a.k8 + it.w.b * a.k8s[0] + it.w.unit * a.k8s[1] + it.sub * 64;
-        const int t0 = (it.w.tile + it.tile) * WT_KEYS, len = s.len[it.w.b];
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-          const int c = ct + j * 256, key = c / 4;
-          if (t0 + key < len) cp_async16(raw + slot * (WT_PIECE / 2) + c * 16, src + (t0 + key) * a.k8s[2] + (c % 4) * 16);
-        }
-      }
-      cp_async_commit();
-    };
-    for (int i = 0; i < WT_RAW; ++i) {
-      issue(ahead, i);
-      if (ahead.live) ahead.step();
-    }
-    int stage = 0, slot = 0;
-    uint32_t turn = 0;
-    while (now.live) {
-      const int left = s.len[now.w.b] - (now.w.tile + now.tile) * WT_KEYS;
-      uint4 v[CHUNKS];
-      cp_async_wait<WT_RAW - 1>();
-#pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) {
-        const int c = ct + j * 256;
-        v[j] = c / 4 < left ? *reinterpret_cast<const uint4 *>(raw + slot * (WT_PIECE / 2) + c * 16) : make_uint4(0, 0, 0, 0);
-      }
-      issue(ahead, slot);
-      if (ahead.live) ahead.step();
-      if (!wait(&s.empty[stage], turn ^ 1)) break;
-#pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) {
-        const int c = ct + j * 256, key = c / 4, c16 = 2 * (c % 4);
-        uint4 y[2];
+    // ---- FP8 caches: groups of WT_GROUP threads take the pieces in turn and
+    // turn their codes into BF16 where TMA puts a BF16 piece (skv_tree.cu)
+    constexpr int GROUPS = (WT_THREADS_F8 - WT_THREADS) / WT_GROUP, CHUNKS = WT_PIECE / 2 / 16 / WT_GROUP;
+    constexpr int STEP = WT_GROUP / 4;
+    static_assert(STEP % 8 == 0 && WT_RAW % GROUPS == 0, "one swizzle for all of a thread's keys; rings");
+    const int ct = (tid - WT_THREADS) % WT_GROUP, grp = (tid - WT_THREADS) / WT_GROUP;
+    const int key = ct / 4;
+    const uint32_t place = (2 * (ct % 4) ^ key) & 7;
+    Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
+    uint32_t base = 0;
+    bool ok = true;
+    while (ok && w.next()) {
+      const uint32_t end = base + w.count * SUB;
+      const int len = s.len[w.b];
+      for (uint32_t seq = base + (grp - base % GROUPS + GROUPS) % GROUPS; seq < end; seq += GROUPS) {
+        const int left = len - (w.tile + (int)((seq - base) / SUB)) * WT_KEYS - key;  // keys from this thread's first
+        // (both rings' lengths are multiples of GROUPS: a place in them belongs
+        // to one group, which sees its phases in turn)
+        const uint32_t slot = seq % WT_RAW, stage = seq % stages;
+        if (!(ok = wait(&s.raw_full[slot], (seq / WT_RAW) & 1))) break;
+        if (!(ok = wait(&s.empty[stage], ((seq / stages) & 1) ^ 1))) break;
+        const uint8_t *from = raw + slot * (WT_PIECE / 2) + ct * 16;
+        uint8_t *at = ring + stage * WT_PIECE + key * 128;
         uint32_t nan = 0;
-        e4m3_to_bf16(v[j], y[0], y[1], nan);
-        // (eight neighbouring threads are two keys, whose swizzles differ: all banks differ)
-        uint8_t *line = ring + stage * WT_PIECE + key * 128;
-        *reinterpret_cast<uint4 *>(line + (c16 ^ (key & 7)) * 16) = y[0];
-        *reinterpret_cast<uint4 *>(line + ((c16 + 1) ^ (key & 7)) * 16) = y[1];
-        if (nan & E4M3_NAN) {
-          e4m3_put_nan(reinterpret_cast<uint4 *>(line + (c16 ^ (key & 7)) * 16));
-          e4m3_put_nan(reinterpret_cast<uint4 *>(line + ((c16 + 1) ^ (key & 7)) * 16));
+#pragma unroll 2
+        for (int j = 0; j < CHUNKS; ++j) {
+          uint4 x = *reinterpret_cast<const uint4 *>(from + j * WT_GROUP * 16), y0, y1;
+          if (STEP * j >= left) x = make_uint4(0, 0, 0, 0);
+          e4m3_to_bf16(x, y0, y1, nan);
+          *reinterpret_cast<uint4 *>(at + j * STEP * 128 + place * 16) = y0;
+          *reinterpret_cast<uint4 *>(at + j * STEP * 128 + (place ^ 1) * 16) = y1;
         }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.raw_empty[slot]);
+        if (nan & E4M3_NAN)
+          for (int j = 0; j < CHUNKS; ++j)
+            for (int u = 0; u < 2; ++u) e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * STEP * 128 + (place ^ u) * 16));
+        async_fence();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&s.full[stage]);
       }
-      async_fence();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&s.full[stage]);
-      now.step();
-      if (++stage == stages) stage = 0, turn ^= 1;
-      if (++slot == WT_RAW) slot = 0;
+      base = end;
     }
-    cp_async_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -328,11 +301,16 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 
 template <int D, bool F8>
 int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, int device, cudaStream_t st) {
-  constexpr int most = 232448, fixed = 1024 + (int)sizeof(WeightsSmem) + (F8 ? WT_RAW * WT_PIECE / 2 : 0);
+  constexpr int most = 232448, fixed = 1024 + (int)sizeof(WeightsSmem);
+  constexpr int raw = F8 ? WT_RAW * (WT_PIECE / 2) : 0;
   const int rows = (D / 64) * a.cols * 128;
-  int stages = (most - fixed - rows) / WT_PIECE;
+  const int stages = (most - fixed - raw - rows) / WT_PIECE;
   a.stages = stages < WT_STAGES ? stages : WT_STAGES;
-  const int smem = fixed + rows + a.stages * WT_PIECE;
+  if (F8) a.stages &= ~3;  // (see the conversion)
+  const int smem = fixed + raw + rows + a.stages * WT_PIECE;
+  static_assert(most - fixed - WT_ROWS * 512 >= 4 * WT_PIECE && most - fixed - 2 * raw - WT_ROWS_F8 * 512 >= 0 &&
+                    most - fixed - raw - (F8 ? WT_ROWS_F8 : 0) * 512 >= 4 * WT_PIECE,
+                "rings beside the most queries");
   auto *kernel = &k_weights<D, F8>;
   static bool set[64];
   if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), most, device, set)) return rc;
@@ -391,7 +369,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   a.c2 = (float)(d->scale * 1.4426950408889634);
   a.len_stride = d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
-    a.qs[i] = qs[i], a.k8s[i] = kcs[i], a.ls[i] = ls[i];
+    a.qs[i] = qs[i], a.ls[i] = ls[i];
     a.os[i] = os[i];
   }
   op_strides(a.ts, d->rows_stride, of_q, 2);
@@ -406,20 +384,18 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
     a.take = d->rows ? static_cast<const uint8_t *>(d->rows) + b0 * a.ts[0] : nullptr;
     a.out = static_cast<float *>(d->weights_out) + b0 * a.os[0];
     CUtensorMap map{};
-    if (f8) {
-      a.k8 = static_cast<const uint8_t *>(d->k_cache) + b0 * a.k8s[0];
-    } else {
-      const int64_t step[3] = {kcs[2], kcs[1], kcs[0]};
-      if (int rc = make_map(&map, static_cast<const uint16_t *>(d->k_cache) + b0 * kcs[0], d->dim, d->tokens,
-                            d->kv_heads, nb, step, WT_KEYS, 1))
-        return rc;
-      a.along[0] = kcs[1] ? 1 : 0;
-      a.along[1] = nb > 1 && kcs[0] ? 1 : 0;
-    }
+    const int64_t step[3] = {kcs[2], kcs[1], kcs[0]};
+    const uint8_t *base = static_cast<const uint8_t *>(d->k_cache) + b0 * kcs[0] * (f8 ? 1 : 2);
+    if (int rc = f8 ? make_byte_map(&map, base, d->dim, d->tokens, d->kv_heads, nb, step, WT_KEYS, 64)
+                    : make_map(&map, base, d->dim, d->tokens, d->kv_heads, nb, step, WT_KEYS, 1))
+      return rc;
+    a.along[0] = kcs[1] ? 1 : 0;
+    a.along[1] = nb > 1 && kcs[0] ? 1 : 0;
     // more rows than the MMA's N: further launches add to what the first wrote
-    for (int64_t r0 = 0; r0 < rows; r0 += WT_ROWS) {
+    const int64_t most = f8 ? WT_ROWS_F8 : WT_ROWS;
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
       a.row0 = (int)r0;
-      a.rows = (int)(rows - r0 < WT_ROWS ? rows - r0 : WT_ROWS);
+      a.rows = (int)(rows - r0 < most ? rows - r0 : most);
       a.cols = (a.rows + 15) & ~15;
       if (r0 == 0) {
         a.w = static_cast<const float *>(d->weights) + b0 * ws[0];
