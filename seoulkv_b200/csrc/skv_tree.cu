@@ -126,8 +126,8 @@ struct TreeCfg {
   static constexpr int RAW = STAGE / 2;   // an FP8 stage before its conversion
   // (FP8: multiples of the converting groups, so that a place in either ring
   // belongs to one group, which sees its phases in turn)
-  static constexpr int NRAW = F8 ? (D == 256 ? 4 : 8) : 0;
-  static constexpr int NSTAGE = F8 ? 8 : D == 256 ? 10 : D == 128 ? 11 : 12;
+  static constexpr int NRAW = F8 ? (D == 256 ? 12 : 8) : 0;
+  static constexpr int NSTAGE = F8 ? (D == 256 ? 4 : 8) : D == 256 ? 10 : D == 128 ? 11 : 12;
   static constexpr int THREADS = F8 ? 576 : 384;  // FP8: warps 2, 3 and 12.. convert
   static constexpr int COL_S = 256;       // tensor memory columns: O, then two score tiles (P over S)
   static constexpr int QBYTES = TR_ROWS * D * 2;
