@@ -13,10 +13,17 @@ struct Plan {
   long long total;  // places in the list
   int items;        // ranges that are not empty
   __device__ Plan(long long total_, int items_) : total(total_), items((int)min((long long)items_, total_)) {}
-  __device__ long long begin(int i) const { return i < items ? total * i / items : total; }
+  __device__ long long begin(int i) const { return i < items ? quotient(total * i, items) : total; }
   // the item whose range holds place g
-  __device__ int owner(long long g) const { return (int)(((g + 1) * items - 1) / total); }
+  __device__ int owner(long long g) const { return (int)quotient((g + 1) * items - 1, total); }
+  // (a 64-bit division takes a few hundred cycles, and every role starts with some)
+  static __device__ long long quotient(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+  }
 };
+
+// n / d for 0 <= n < 2^18 by a multiplication with ceil(2^32 / d), d <= 2^12.
+__device__ __forceinline__ int by_inverse(int n, uint64_t inverse) { return (int)(((uint64_t)(uint32_t)n * inverse) >> 32); }
 
 // pre[b] (places of the sequences before b, one unit's worth) and len[b], by
 // one warp: KT cached tokens a tile, and `extra` places more.
@@ -69,7 +76,7 @@ struct Walk {
       while ((long long)pre[b + 1] * units <= g) ++b;
       const int places = pre[b + 1] - pre[b];
       const long long rel = g - (long long)pre[b] * units;
-      unit = (int)(rel / places);
+      unit = (int)Plan::quotient(rel, places);
       tile = (int)(rel - (long long)unit * places);
       start = g - tile;
       tiles = places - idle;

@@ -153,6 +153,7 @@ struct TreeArgs {
   float *lse;              // [sequence][node][query head]
   float2 *ml;              // partials: [slot][rows] (m in log2 units, l; l < 0: the row is unused)
   float *part;             // [slot][rows][D]
+  uint64_t by_group;       // (by_inverse)
   int32_t batch, n, heads, group, t, mtiles, rows;
   int32_t along[4][2];     // coordinate steps (head, sequence) of the four maps: 0 where one element stands for all
   float c2;                // scale * log2(e)
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     const int left = a.n * a.group - mt * TR_ROWS;  // rows of this part
     const bool warp_on = (row & ~31) < left, on = row < left;
     const int r = mt * TR_ROWS + row;  // row of the KV head
-    const int node = on ? r / a.group : 0, qg = on ? r - node * a.group : 0;
+    const int node = on ? by_inverse(r, a.by_group) : 0, qg = on ? r - node * a.group : 0;
     // rows that do not exist are zeros: a product of zeros draws no power,
     // and power is what the clock follows
     for (int x = st; x < (TR_ROWS - min(left, TR_ROWS)) * (D / 8); x += 256) {
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       const int total = min(left, TR_ROWS) * (D / 8);
 #pragma unroll 1
       for (int c = st; c < total; c += 256) {
-        const int at = c / (D / 8), c16 = c % (D / 8), rr = mt * TR_ROWS + at, nd = rr / a.group;
+        const int at = c / (D / 8), c16 = c % (D / 8), rr = mt * TR_ROWS + at, nd = by_inverse(rr, a.by_group);
         cp_async16(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16,
                    a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2] + c16 * 8, true);
       }
@@ -909,6 +910,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
   if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads), rows = (int)d->n * group;
   a.heads = (int)d->kv_heads, a.group = group, a.n = (int)d->n, a.t = (int)d->tokens;
+  a.by_group = ((1ull << 32) + group - 1) / group;
   a.mtiles = (rows + TR_ROWS - 1) / TR_ROWS;
   a.rows = rows < TR_ROWS ? rows : TR_ROWS;
   a.c2 = (float)(d->scale * 1.4426950408889634);

@@ -41,6 +41,7 @@ struct WeightsArgs {
   const float *w;
   float *out;
   int64_t ws[3], os[3];  // (sequence, head, token)
+  uint64_t by_group;  // (by_inverse)
   int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head; cols: rows up to 16s
   int32_t along[2];
   int32_t stages;  // pieces of the ring
@@ -53,6 +54,7 @@ struct WeightsSmem {
   uint64_t q_ready, q_free, acc_full[2], acc_free[2], drain;
   uint32_t tmem, abort;
   alignas(16) float lse2[2][WT_ROWS];  // log2(e) * lse, +inf for rows that do not count
+  int64_t q_at[WT_ROWS];               // element offsets of the rows in a head's queries
   int32_t len[PLAN_BATCH];
   int32_t pre[PLAN_BATCH + 1];
 };
@@ -190,23 +192,23 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
       // the head's rows, once the tensor core is done with the ones before
       if (seg) wait(&s.q_free, (seg - 1) & 1);
       if (et < a.cols) {
-        float l2 = INFINITY;
-        const int row = a.row0 + et, node = row / a.group, qh = h * a.group + row - node * a.group;
-        if (et < a.rows && (!a.take || a.take[w.b * a.ts[0] + node * a.ts[1]])) {
-          const float l = a.lse[w.b * a.ls[0] + node * a.ls[1] + qh * a.ls[2]];
-          if (l != -INFINITY) l2 = l * 1.4426950408889634f;  // (-inf: a row that saw nothing)
-        }
-        s.lse2[seg & 1][et] = l2;
+        const int row = a.row0 + min(et, a.rows - 1), node = by_inverse(row, a.by_group), g = row - node * a.group;
+        const float l = a.lse[w.b * a.ls[0] + node * a.ls[1] + (h * a.group + g) * a.ls[2]];
+        const uint8_t take = a.take ? a.take[w.b * a.ts[0] + node * a.ts[1]] : 1;
+        // (-inf: a row that saw nothing)
+        s.lse2[seg & 1][et] = et < a.rows && take && l != -INFINITY ? l * 1.4426950408889634f : INFINITY;
+        s.q_at[et] = node * a.qs[1] + g * a.qs[2];
       }
       asm volatile("bar.sync 2, 256;" ::: "memory");
       // asynchronous copies in a short loop: code that runs once per launch
       // waits for its instructions, and unrolled loads took 20000 cycles here
+      {
+        const int c16 = et % (D / 8);
+        const uint16_t *q = a.q + w.b * a.qs[0] + h * a.group * a.qs[2] + c16 * 8;
+        uint8_t *to = queries + (c16 / 8) * a.cols * 128;
 #pragma unroll 1
-      for (int x = et; x < a.cols * (D / 8); x += 256) {
-        const int r = x / (D / 8), c16 = x % (D / 8), row = a.row0 + min(r, a.rows - 1);
-        const int node = row / a.group, qh = h * a.group + row - node * a.group;
-        cp_async16(queries + (c16 / 8) * a.cols * 128 + r * 128 + ((c16 % 8) ^ (r & 7)) * 16,
-                   a.q + w.b * a.qs[0] + node * a.qs[1] + qh * a.qs[2] + c16 * 8, s.lse2[seg & 1][r] != INFINITY);
+        for (int r = et / (D / 8); r < a.cols; r += 256 / (D / 8))
+          cp_async16(to + r * 128 + ((c16 % 8) ^ (r & 7)) * 16, q + s.q_at[r], s.lse2[seg & 1][r] != INFINITY);
       }
       cp_async_wait();
       async_fence();
@@ -335,7 +337,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
   if (d->dim != 64 && d->dim != 128 && d->dim != 256) return op_fail(SKV_E_INVALID, "head size must be 64, 128 or 256");
   if (d->batch < 0 || d->n < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096 ||
-      d->n > (1 << 20) || d->batch > (1 << 20))
+      d->n * (d->heads / d->kv_heads) > (1 << 17) || d->batch > (1 << 20))
     return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, counts in range");
   if (d->tokens < 1 || d->tokens > (1 << 26)) return op_fail(SKV_E_INVALID, "tokens must be in [1, 2^26]");
   if (!(d->scale > 0.0) || !(d->scale < 1e30)) return op_fail(SKV_E_INVALID, "scale must be positive and finite");
@@ -366,6 +368,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads);
   a.heads = (int)d->kv_heads, a.group = group, a.t = (int)d->tokens;
+  a.by_group = ((1ull << 32) + group - 1) / group;
   a.c2 = (float)(d->scale * 1.4426950408889634);
   a.len_stride = d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
