@@ -178,7 +178,20 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
         const int b = p / a.heads, h = p - b * a.heads;
         const float *w = a.w + b * a.ws[0] + h * a.ws[1];
         float *o = a.out + b * a.os[0] + h * a.os[1];
-        for (int t = s.len[b] + (cta % share) * 64 + tid - 64; t < a.t; t += share * 64) o[t * a.os[2]] = w[t * a.ws[2]];
+        constexpr int BATCH = 8;  // (loads in flight: one at a time this copy outlasted the rest of the kernel)
+        for (int t0 = s.len[b] + (cta % share) * 64 + tid - 64; t0 < a.t; t0 += share * 64 * BATCH) {
+          float x[BATCH];
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j) {
+            const int t = t0 + share * 64 * j;
+            x[j] = t < a.t ? w[t * a.ws[2]] : 0.0f;
+          }
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j) {
+            const int t = t0 + share * 64 * j;
+            if (t < a.t) o[t * a.os[2]] = x[j];
+          }
+        }
       }
     }
   } else if (warp < 12) {
