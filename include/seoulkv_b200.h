@@ -435,6 +435,15 @@ typedef struct SkvTree {
 int skv_tree_attention(const SkvTree *desc, void *stream);
 int skv_tree_workspace(const SkvTree *desc, int64_t *bytes);
 
+/* skv_tree_attention over the engine's own cache: the FP8 records of every
+ * slot (batch = n_slots, 16 heads, 4 KV heads, dim 256), as many tokens as the
+ * slots hold when the kernel runs (appends ahead of it on the stream or in the
+ * graph included).  Of the descriptor, q, k, v, parents, out, lse, workspace
+ * and workspace_bytes (skv_tree_workspace with tokens = the engine's largest
+ * context), scale, n and the strides of q, k, v and parents are used.  The
+ * cache does not change: append the accepted nodes with skv_append. */
+int skv_run_tree(void *handle, const SkvTree *desc, void *stream);
+
 /* Attention weights accumulated per cached key:
  *   weights_out[b][h][t] = weights[b][h][t] + sum of exp(scale q_r.k_t - lse_r)
  * over the rows r (nodes i with rows[b][i] != 0, or all of them with rows

@@ -33,7 +33,7 @@ EXPORTS = (
     "skv_shard_outputs", "skv_shard_merge", "skv_shard_attention", "skv_shard_combine",
     "skv_shard_setup", "skv_shard_connect", "skv_shard_ipc_handle_bytes", "skv_shard_gids",
     "skv_append", "skv_context", "skv_set_l2_residency",
-    "skv_rotary", "skv_tree_attention", "skv_tree_workspace", "skv_accumulate_weights", "skv_evict", "skv_operator_status",
+    "skv_rotary", "skv_tree_attention", "skv_tree_workspace", "skv_run_tree", "skv_accumulate_weights", "skv_evict", "skv_operator_status",
 )
 
 SKV_FLAG_STAGED = 1
@@ -151,6 +151,7 @@ def load() -> ctypes.CDLL:
         # the stand-alone operators take their descriptors as packed bytes
         for name in ("skv_rotary", "skv_tree_attention", "skv_accumulate_weights", "skv_evict"):
             getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        lib.skv_run_tree.argtypes = [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p]
         lib.skv_tree_workspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
         lib.skv_operator_status.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint32)]
         _lib = lib

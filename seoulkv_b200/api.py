@@ -244,6 +244,31 @@ class SeoulKV4:
         else:
             self._context += m
 
+    def run_tree(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Exact attention of N <= 64 drafted tokens over the whole cache and their own ancestors.
+
+        Where ``run`` decodes one token with the sparse funnel, this scores a
+        tree of drafted tokens with every record of the cache (the FP8 K and V
+        that ``run`` attends with), for a verification step: BF16 Q
+        [1, N, 16, 256], the drafted tokens' own K and V [4, N, 256] as
+        ``append`` takes them, int32 ``parents`` [N] as in
+        ``seoulkv_b200.tree_attention`` (-1: follows the cache).  Returns CUDA
+        tensors: BF16 [1, N, 16, 256] and the rows' log-sum-exp, FP32
+        [1, N, 16].  Stream-ordered like ``run`` and ``append``, and may be
+        captured (CUDA inputs, instance already initialised); the cache does
+        not change: ``append`` the accepted tokens.
+        """
+        from seoulkv_b200.operators import run_tree
+
+        self._require_open()
+        if self._engine is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("initialise SeoulKV4 (run or append once) before capturing a tree")
+            self._engine = self._initialize()
+            self._host_kv = None
+        return run_tree(self._engine, (), q, k, v, parents, self._device_index)
+
     def _bind_query(self, q: torch.Tensor) -> None:
         self._validate_query(q)
         eng = self._require_initialized()

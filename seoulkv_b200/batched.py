@@ -189,6 +189,24 @@ class SeoulKV4Batch:
         _enqueue_append(self._engine, k, v, self._device_index, self._stream())
         self._context += m
 
+    def run_tree(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Exact attention of N <= 64 drafted tokens per cache over that whole cache and their own ancestors.
+
+        The contract of ``SeoulKV4.run_tree`` per cache: BF16 Q
+        [n, N, 16, 256], K and V [n, 4, N, 256], int32 parents [n, N]; returns
+        CUDA tensors BF16 [n, N, 16, 256] and FP32 [n, N, 16].
+        """
+        from seoulkv_b200.operators import run_tree
+
+        self._require_open()
+        if self._engine is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("initialise SeoulKV4Batch (run or append once) before capturing a tree")
+            self._engine = self._initialize()
+            self._caches = [(None, None, c[2]) for c in self._caches]
+        return run_tree(self._engine, (self.n,), q, k, v, parents, self._device_index)
+
     def synchronize(self) -> None:
         """Wait for the last run; raises RuntimeError if a live count left its range."""
         self._require_open()

@@ -19,6 +19,7 @@
 #include "skv_fused.cuh"
 #include "skv_kernels.cuh"
 #include "skv_shard.cuh"
+#include "skv_tree.cuh"
 
 using namespace skv;
 
@@ -121,6 +122,10 @@ struct Engine {
   uint32_t *rebuild_done = nullptr;    // CTAs of the running CSR rebuild that finished
   uint32_t *assign_done = nullptr;     // [cell] CTAs of the running assignment that finished
   size_t post_cap = 0;                 // postings a CSR set holds (largest over cells)
+  // K and V tensor maps of every cell's FP8 records (skv_run_tree), made with the records
+  CUtensorMap *record_maps = nullptr;
+  cudaEvent_t tree_done = nullptr;     // the last skv_run_tree outside a capture
+  bool tree_ran = false;
   uint16_t *kv_stage = nullptr;        // host-input staging [2][n_cells][APPEND_MAX][256]
   bool appends() const { return tmax > desc.context; }
 };
@@ -464,6 +469,7 @@ int skv_create(const SkvDesc *d, void **handle) {
   TRY(cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking) ? fail(SKV_E_CUDA, "stream") : 0);
   TRY(cudaEventCreateWithFlags(&e->q_copied, cudaEventDisableTiming) ? fail(SKV_E_CUDA, "event") : 0);
   TRY(cudaEventCreateWithFlags(&e->done, cudaEventDisableTiming) ? fail(SKV_E_CUDA, "event") : 0);
+  TRY(cudaEventCreateWithFlags(&e->tree_done, cudaEventDisableTiming) ? fail(SKV_E_CUDA, "event") : 0);
   TRY(cudaHostAlloc(reinterpret_cast<void **>(&e->q_pinned), (size_t)d->n_slots * 16 * D * 2,
                     cudaHostAllocMapped) ? fail(SKV_E_CUDA, "pinned query buffer") : 0);
   TRY(cudaHostGetDevicePointer(reinterpret_cast<void **>(&e->q_pinned_dev), e->q_pinned, 0)
@@ -544,6 +550,7 @@ int skv_create(const SkvDesc *d, void **handle) {
   TRY(dalloc(e, &w.arrive, C));
   TRY(dalloc(e, &w.hist, C * 4 * G * 4096));
   TRY(dalloc(e, &e->phase_ts, 2 * FUSED_MARKS));
+  TRY(dalloc(e, &e->record_maps, 2 * (size_t)e->n_cells));
   e->tmax = d->max_context ? d->max_context : d->context;
   e->t_host = d->context;
   {
@@ -586,6 +593,8 @@ void skv_destroy(void *handle) {
   cudaSetDevice(e->desc.device);
   if (e->stream) cudaStreamSynchronize(e->stream);
   if (e->ran && e->done) cudaEventSynchronize(e->done);
+  if (e->tree_ran) cudaEventSynchronize(e->tree_done);
+  if (e->tree_done) cudaEventDestroy(e->tree_done);
   for (void *p : e->link.opened)
     if (p) cudaIpcCloseMemHandle(p);
   for (auto &row : e->link.kv8)
@@ -795,6 +804,11 @@ int skv_upload_kv(void *handle, int32_t slot, const uint16_t *k, const uint16_t 
   if (smax) cudaFree(smax);
   if (stage) cudaFree(stage);
   if (rc) return rc;
+  CUtensorMap maps[2 * G];
+  for (int g = 0; g < G && !rc; ++g) rc = record_maps(&maps[2 * g], kv8[g], (int64_t)rows);
+  if (!rc && cudaMemcpy(e->record_maps + (size_t)slot * 2 * G, maps, sizeof maps, cudaMemcpyHostToDevice) != cudaSuccess)
+    rc = fail(SKV_E_CUDA, "record maps");
+  if (rc) return rc;
   for (int g = 0; g < G; ++g) {
     const int cell = slot * G + g;
     CellDev &c = e->hcells[cell];
@@ -816,6 +830,28 @@ int skv_upload_kv(void *handle, int32_t slot, const uint16_t *k, const uint16_t 
   }
   rc = refresh_cells(e);
   return rc ? rc : label_window(e, slot);
+}
+
+int skv_run_tree(void *handle, const SkvTree *desc, void *stream) {
+  Engine *e = as_engine(handle);
+  if (!e || !desc) return fail(SKV_E_INVALID, "null engine or descriptor");
+  if (e->link.region) return fail(SKV_E_STATE, "a shard of a group holds only its part of the cache");
+  int rc = ready(e);
+  if (rc) return rc;
+  SkvTree d = *desc;
+  d.device = e->desc.device;
+  d.cache_dtype = SKV_DTYPE_E4M3;
+  d.batch = e->desc.n_slots;
+  d.heads = 16, d.kv_heads = G, d.dim = D, d.tokens = e->tmax;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = tree_attention(&d, e->record_maps, e->tlen, 0, st))) return rc;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  CK(cudaStreamIsCapturing(st, &cap));
+  if (cap == cudaStreamCaptureStatusNone) {
+    CK(cudaEventRecord(e->tree_done, st));
+    e->tree_ran = true;
+  }
+  return SKV_OK;
 }
 
 int skv_bind_query(void *handle, const uint16_t *q, int32_t on_device, void *stream) {

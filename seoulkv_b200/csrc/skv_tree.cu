@@ -31,6 +31,7 @@
 #include "skv_ops.cuh"
 #include "skv_plan.cuh"
 #include "skv_tensor.cuh"
+#include "skv_tree.cuh"
 
 namespace skv {
 
@@ -865,9 +866,14 @@ int check_tree(const SkvTree *d) {
 
 }  // namespace
 
-// Attention over a cache given by `d`, or (cells != null: device array of the K
-// and V maps of every cell) over FP8 records with the context at `tlen` (null:
-// `context`).
+int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
+  const int64_t step[3] = {REC, 0, 0};
+  for (int i = 0; i < 2; ++i)
+    if (int rc = make_byte_map(two + i, records + i * D, D, rows, 1, 1, step, i ? TR_KEYS / (D / 64) : TR_KEYS, i ? D : 64))
+      return rc;
+  return SKV_OK;
+}
+
 int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
   if (int rc = check_tree(d)) return rc;
   if (d->batch == 0) return SKV_OK;

@@ -329,6 +329,40 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     return out, lse
 
 
+def run_tree(engine, lead: tuple, q, k, v, parents, device: int):
+    """Tree attention over an engine's FP8 records (``SeoulKV4.run_tree`` and
+    ``SeoulKV4Batch.run_tree``): K and V [*lead, 4, N, 256], parents [*lead, N]."""
+    slots = engine.n_slots
+    if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.dtype is not _BF16 or q.shape[0] != slots \
+            or q.shape[2:] != (16, 256) or not 1 <= q.shape[1] <= TREE_MAX_NODES:
+        raise ValueError(f"expected BF16 Q [{slots},N,16,256] with 1 <= N <= {TREE_MAX_NODES}")
+    n = q.shape[1]
+    dims = "".join(f"{x}," for x in lead)
+    for name, t in (("K", k), ("V", v)):
+        if not isinstance(t, torch.Tensor) or t.dtype is not _BF16 or tuple(t.shape) != (*lead, 4, n, 256):
+            raise ValueError(f"expected BF16 drafted {name} [{dims}4,{n},256]")
+    if not isinstance(parents, torch.Tensor) or parents.dtype is not _I32 or tuple(parents.shape) != (*lead, n):
+        raise ValueError(f"expected int32 parents [{dims}{n}]")
+    if _recorded(q, k, v):
+        raise ValueError("run_tree has no backward pass (detach the inputs, or use no_grad)")
+    q, k, v, parents = (t if t.get_device() == device else t.to(f"cuda:{device}") for t in (q, k, v, parents))
+    if not lead:
+        k, v, parents = k[None], v[None], parents[None]
+    out = q.new_empty((slots, n, 16, 256))
+    lse = q.new_empty((slots, n, 16), dtype=_F32)
+    size = _tree_workspace(device, slots, n, 16, 4, 256, engine.max_context)
+    work = q.new_empty(size, dtype=torch.uint8)
+    packed = _TREE.pack(
+        q.data_ptr(), 0, 0, 0, k.data_ptr(), v.data_ptr(), parents.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        work.data_ptr(), 0.0625, device, _DTYPE[_FP8], size, slots, n, 16, 4, 256, engine.max_context,
+        *q.stride(), *(8 * (0,)), *k.stride(), *v.stride(), *parents.stride(), 0)
+    rc = engine.lib.skv_run_tree(engine.handle, packed, _current_stream(device))
+    if rc == -1:
+        raise ValueError(f"run_tree: {engine.lib.skv_last_error().decode(errors='replace')}")
+    _native.check(rc, "skv_run_tree")
+    return out, lse
+
+
 @functools.lru_cache(maxsize=1024)
 def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: int) -> int:
     """Bytes of scratch that one call needs (a function of the sizes)."""

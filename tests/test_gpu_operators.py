@@ -659,3 +659,83 @@ def test_draft_verify_accumulate_evict(dtype):
                 x[:, :, :keep] = y
             evictions += 1
     assert evictions
+
+
+# ---------------------------------------------------------------- the engine's own cache
+
+
+@pytest.fixture(scope="module")
+def grown():
+    from tests.helpers import AppendCase
+
+    return AppendCase()  # built on 8192 tokens, grows to 8892
+
+
+def records(ac, t):
+    """The engine's FP8 records of the first t tokens, [4, t, 256] each."""
+    return [torch.stack([x[g][:t] for g in range(4)]).to(F8).cuda() for x in (ac.k_full, ac.v_full)]
+
+
+def drafted(seed, slots, n):
+    g, rng = gen(seed), random.Random(seed)
+    q = normal(g, slots, n, 16, 256)
+    k, v = normal(g, slots, 4, n, 256), normal(g, slots, 4, n, 256)
+    parents = torch.tensor([make_parents(rng, n, "tree") for _ in range(slots)], dtype=torch.int32, device="cuda")
+    return q, k, v, parents
+
+
+def test_run_tree_sees_the_engines_cache(grown, cuda):
+    """Exact attention over the FP8 records, before and after appends, on the
+    device and captured; equal to tree_attention over the same records."""
+    cfg = skv.SeoulKV4Config(max_context=grown.total)
+    q, k, v, parents = drafted(61, 1, 7)
+    with skv.SeoulKV4(device=cuda, k=grown.k, v=grown.v, index=grown.index,
+                      config=cfg) as attn:
+        t = grown.context
+
+        def check(out, lse, t):
+            kc, vc = records(grown, t)
+            n = torch.tensor([t], dtype=torch.int32, device="cuda")
+            want, wl, eo, el = R.tree(q, kc[None], vc[None], n, k, v, parents)
+            close(out, want, eo)
+            close(lse, wl, el)
+
+        check(*attn.run_tree(q, k[0], v[0], parents[0]), t)
+        host = attn.run_tree(q.cpu(), k[0].cpu(), v[0].cpu(), parents[0].cpu())
+        assert torch.equal(host[0], attn.run_tree(q, k[0], v[0], parents[0])[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = attn.run_tree(q, k[0], v[0], parents[0])
+        for m in (1, 300):
+            attn.append(*grown.appended(t, t + m))
+            t += m
+            check(*attn.run_tree(q, k[0], v[0], parents[0]), t)
+            graph.replay()
+            check(out, lse, t)
+        # run() and the tree share the cache without touching each other
+        y = attn.run(grown.query(t, seed=3)).to_torch()
+        attn.run_tree(q, k[0], v[0], parents[0])
+        assert torch.equal(attn.run(grown.query(t, seed=3)).to_torch(), y)
+        for bad in (dict(q=q[:, :, :4]), dict(q=q.float()), dict(k=k), dict(v=v[0, :, :3]), dict(parents=parents),
+                    dict(parents=parents[0].long()), dict(q=q.clone().requires_grad_())):
+            a = dict(q=q, k=k[0], v=v[0], parents=parents[0])
+            a.update(bad)
+            with pytest.raises(ValueError):
+                attn.run_tree(**a)
+    with pytest.raises(RuntimeError, match="closed"):
+        attn.run_tree(q, k[0], v[0], parents[0])
+
+
+def test_run_tree_batched(grown, cuda):
+    """Every cache's own tree, equal to one instance per cache."""
+    t = grown.context
+    kv = [(grown.k, grown.v, grown.index)] * 3
+    q, k, v, parents = drafted(62, 3, 5)
+    with skv.SeoulKV4Batch(device=cuda, caches=kv) as batch:
+        out, lse = batch.run_tree(q, k, v, parents)
+    with skv.SeoulKV4(device=cuda, k=grown.k, v=grown.v, index=grown.index) as attn:
+        for i in range(3):
+            one, l1 = attn.run_tree(q[i:i + 1], k[i], v[i], parents[i])
+            # (the same tiles joined at other places: three roundings of the weights apart)
+            assert float((one.double() - out[i:i + 1].double()).abs().max()) <= 3 * 2.0 ** -8 * float(one.abs().max())
+            assert float((l1 - lse[i:i + 1]).abs().max()) < 1e-4

@@ -150,6 +150,7 @@ def test_null_descriptors_are_refused():
         assert getattr(lib, name)(None, None) == -1
     assert lib.skv_tree_workspace(_tree(), None) == -1
     assert lib.skv_operator_status(0, None) == -1
+    assert lib.skv_run_tree(None, _tree(), None) == -1
 
 
 def test_empty_batches_need_no_gpu():
