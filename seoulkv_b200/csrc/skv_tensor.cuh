@@ -139,6 +139,27 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
+// FP32 accumulator, FP8 e4m3 operands, both K-major (a step is 32 codes).
+__host__ __device__ constexpr uint32_t mma_desc_f8(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// K-major operand in rows of 128 or 64 bytes, swizzled over as many.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr, int row_bytes) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(row_bytes * 8 >> 4) << 32) | (1ull << 46) |
+         ((row_bytes == 128 ? 2ull : 4ull) << 61);
+}
+// The 16-byte unit of a swizzled row that holds its unit c.
+__device__ __forceinline__ int swizzled(int c, int row, int row_bytes) {
+  return row_bytes == 128 ? c ^ (row & 7) : c ^ (row >> 1 & 3);
+}
+// By the elected lane: D (tensor memory) = A B (shared memory, FP8) [+ D], K = 32.
+__device__ __forceinline__ void mma_f8(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(one)
+      : "memory");
+}
 // By the elected lane: D (tensor memory) = A (tensor memory) B (shared memory) [+ D], K = 16.
 __device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
   asm volatile(
@@ -230,6 +251,55 @@ static __device__ __noinline__ void e4m3_put_nan(uint4 *at) {
     if ((y[i] & 0x7fff0000u) == 0x43f00000u) y[i] |= 0x7fff0000u;
   }
 }
+// ---- a BF16 row as the sum of two FP8 e4m3 rows
+//
+// A query q (8 significant bits) times 2^e, with e so that the row's largest
+// element lies in [128, 256), is hi + lo: hi the nearest e4m3 (4 bits), lo what
+// is left (a multiple of 2^-7 of hi's power of two, at most 2^-4 of it: 4 bits
+// again).  The sum is exact wherever lo is no smaller than e4m3's last place,
+// 2^-9: for elements above 2^-9 of the largest.  Below, it is off by half a
+// last place, at most 2^-17 of the largest.  K in FP8 then goes to the tensor
+// core as it is stored, twice (at twice the BF16 rate), instead of through
+// registers into BF16.
+//
+// 2^e of a row that `lanes` neighbouring threads hold in 16-byte pieces, as
+// the exponent field of a float (127: a row of zeros or not finite).
+__device__ __forceinline__ uint32_t split_exponent(const uint4 &v, int lanes) {
+  uint32_t top = 0;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+  for (int o = lanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int e = (int)(top >> 7);  // the exponent field of BF16 and of FP32
+  return top == 0 || e == 255 ? 127u : (uint32_t)min(261 - e, 253);
+}
+// Two elements (BF16 pair) times f: hi and lo codes, two bytes each.
+__device__ __forceinline__ void split_pair(uint32_t pair, float f, uint32_t &hi, uint32_t &lo) {
+  float x = __uint_as_float(pair << 16) * f, y = __uint_as_float(pair & 0xffff0000u) * f;
+  x = isinf(x) ? __uint_as_float(0x7fffffffu) : x;  // (e4m3 has no infinity: a row with one is not a number)
+  y = isinf(y) ? __uint_as_float(0x7fffffffu) : y;
+  uint16_t h, l;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(y), "f"(x));
+  uint32_t back;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(h));
+  float hx, hy;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(hx), "=f"(hy)
+      : "r"(back));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(l) : "f"(y - hy), "f"(x - hx));
+  hi = h;
+  lo = l;
+}
+// Eight elements: eight bytes of hi, eight of lo.
+__device__ __forceinline__ void split_eight(const uint4 &v, float f, uint2 &hi, uint2 &lo) {
+  uint32_t h[4], l[4];
+  split_pair(v.x, f, h[0], l[0]);
+  split_pair(v.y, f, h[1], l[1]);
+  split_pair(v.z, f, h[2], l[2]);
+  split_pair(v.w, f, h[3], l[3]);
+  hi = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  lo = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+}
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
   uint64_t y;
   asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
@@ -268,9 +338,10 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_al
 int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int64_t ny, int64_t nz,
              const int64_t *stride, int box_rows, int pieces);
 // Map of [z][y][rows][bytes] with byte strides {row, y, z}, boxes of box_rows
-// rows of box_bytes bytes one after the other.
+// rows of box_bytes bytes one after the other (`swizzle`: swizzled over a
+// row's 128 or 64 bytes).
 int make_byte_map(CUtensorMap *map, const void *base, int64_t bytes, int64_t rows, int64_t ny, int64_t nz,
-                  const int64_t *stride, int box_rows, int box_bytes);
+                  const int64_t *stride, int box_rows, int box_bytes, bool swizzle);
 // The device's status word (set by waits that gave up).
 int status_word(int device, uint32_t **word);
 

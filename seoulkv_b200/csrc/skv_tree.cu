@@ -91,7 +91,7 @@ int make_map(CUtensorMap *map, const void *base, int64_t dim, int64_t rows, int6
 }
 
 int make_byte_map(CUtensorMap *map, const void *base, int64_t bytes, int64_t rows, int64_t ny, int64_t nz,
-                  const int64_t *stride, int box_rows, int box_bytes) {
+                  const int64_t *stride, int box_rows, int box_bytes, bool swizzle) {
   const Encode encode = encoder();
   if (!encode) return op_fail(SKV_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
   const int64_t n[3] = {rows, ny, nz};
@@ -103,7 +103,10 @@ int make_byte_map(CUtensorMap *map, const void *base, int64_t bytes, int64_t row
   }
   const cuuint32_t box[4] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, 1, 1}, unit[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), size, step, box, unit,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            !swizzle           ? CU_TENSOR_MAP_SWIZZLE_NONE
+                            : box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                               : CU_TENSOR_MAP_SWIZZLE_64B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SKV_OK : op_fail(SKV_E_INVALID, "cuTensorMapEncodeTiled: error %d", (int)r);
 }
@@ -869,7 +872,7 @@ int check_tree(const SkvTree *d) {
 int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
   const int64_t step[3] = {REC, 0, 0};
   for (int i = 0; i < 2; ++i)
-    if (int rc = make_byte_map(two + i, records + i * D, D, rows, 1, 1, step, i ? TR_KEYS / (D / 64) : TR_KEYS, i ? D : 64))
+    if (int rc = make_byte_map(two + i, records + i * D, D, rows, 1, 1, step, i ? TR_KEYS / (D / 64) : TR_KEYS, i ? D : 64, false))
       return rc;
   return SKV_OK;
 }
@@ -966,7 +969,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
         const int64_t *at = i ? vcs : kcs, step[3] = {at[2], at[1], at[0]};
         const void *base = static_cast<const uint8_t *>(i ? d->v_cache : d->k_cache) + b0 * at[0];
         rc = make_byte_map(i ? &maps.v : &maps.k, base, d->dim, d->tokens, d->kv_heads, nb, step,
-                           i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : 64);
+                           i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : 64, false);
         a.along[i][0] = d->kv_heads > 1 && at[1] ? 1 : 0;
         a.along[i][1] = nb > 1 && at[0] ? 1 : 0;
       }

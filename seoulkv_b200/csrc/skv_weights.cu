@@ -8,10 +8,14 @@
 // The product runs on tcgen05 with the keys as M = 128 lanes and the rows as
 // N: every thread of the epilogue then holds one key's scores in its own lane
 // and sums their exponentials without a word to its neighbours, in a fixed
-// order.  A tile's K arrives as pieces of 128 keys x 64 dimensions (16 KB), so
+// order.  A tile's K arrives as pieces of 128 keys x 128 bytes (16 KB), so
 // that the ring stays deep beside up to 128 KB of queries in shared memory;
 // the accumulator (FP32, tensor memory) is double-buffered against two
 // epilogue groups.  CTAs take contiguous ranges of the list of all tiles.
+//
+// An FP8 cache goes to the tensor core as it is stored: the queries are split
+// into two FP8 rows whose sum they are (skv_tensor.cuh), with a power of two
+// per row that the epilogue takes out again.
 #include <cuda_bf16.h>
 
 #include "skv_ops.cuh"
@@ -24,10 +28,7 @@ namespace {
 constexpr int WT_KEYS = 128, WT_PIECE = WT_KEYS * 128;  // bytes of a piece
 constexpr int WT_ROWS = 256;                            // rows of one launch: the MMA's largest N
 constexpr int WT_STAGES = 12;
-constexpr int WT_RAW = 8;                               // FP8 pieces in flight
-constexpr int WT_ROWS_F8 = 128;                         // rows of one launch over an FP8 cache (its rings need room)
-constexpr int WT_GROUP = 64;                            // threads that turn an FP8 piece into BF16
-constexpr int WT_THREADS = 384, WT_THREADS_F8 = 640;
+constexpr int WT_THREADS = 384;
 
 struct WeightsArgs {
   const uint16_t *q;
@@ -50,24 +51,25 @@ struct WeightsArgs {
 };
 
 struct WeightsSmem {
-  uint64_t full[WT_STAGES], empty[WT_STAGES], raw_full[WT_RAW], raw_empty[WT_RAW];
+  uint64_t full[WT_STAGES], empty[WT_STAGES];
   uint64_t q_ready, q_free, acc_full[2], acc_free[2], drain;
   uint32_t tmem, abort;
   alignas(16) float lse2[2][WT_ROWS];  // log2(e) * lse, +inf for rows that do not count
+  alignas(16) float scale2[2][WT_ROWS];  // scale * log2(e), by the row's power of two over an FP8 cache
   int64_t q_at[WT_ROWS];               // element offsets of the rows in a head's queries
   int32_t len[PLAN_BATCH];
   int32_t pre[PLAN_BATCH + 1];
 };
 
 template <int D, bool F8>
-__global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
+__global__ void __launch_bounds__(WT_THREADS, 1)
     k_weights(const __grid_constant__ CUtensorMap map, const __grid_constant__ WeightsArgs a) {
-  constexpr int SUB = D / 64;
+  // bytes of a piece's rows, pieces of a tile; FP8 queries: hi's pieces, then lo's
+  constexpr int ROW = F8 && D == 64 ? 64 : 128, SUB = D * (F8 ? 1 : 2) / ROW, PIECE = WT_KEYS * ROW;
   extern __shared__ uint8_t smem_dyn[];
-  uint8_t *queries = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;  // [SUB][cols][128 bytes], swizzled
-  uint8_t *ring = queries + SUB * a.cols * 128;
-  uint8_t *raw = ring + a.stages * WT_PIECE;
-  WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(raw + (F8 ? WT_RAW * (WT_PIECE / 2) : 0));
+  uint8_t *queries = smem_dyn + (1024 - (s_addr(smem_dyn) & 1023)) % 1024;  // [piece][cols][ROW bytes], swizzled
+  uint8_t *ring = queries + a.cols * D * 2;
+  WeightsSmem &s = *reinterpret_cast<WeightsSmem *>(ring + a.stages * WT_PIECE);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int stages = a.stages;
   if (warp == 0) {
@@ -77,12 +79,8 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
     for (int i = 0; i < stages; ++i) {
-      bar_init(&s.full[i], F8 ? WT_GROUP / 32 : 1);
+      bar_init(&s.full[i], 1);
       bar_init(&s.empty[i], 1);
-    }
-    for (int i = 0; i < (F8 ? WT_RAW : 0); ++i) {
-      bar_init(&s.raw_full[i], 1);
-      bar_init(&s.raw_empty[i], WT_GROUP / 32);
     }
     bar_init(&s.q_ready, 8);
     bar_init(&s.q_free, 1);
@@ -106,39 +104,38 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
 
   if (warp == 0) {
-    // ---- loads: BF16 pieces into the ring, FP8 pieces beside it
+    // ---- loads
     const uint32_t one = elect_lane();
-    const int slots = F8 ? WT_RAW : stages;
-    uint64_t *const landed = F8 ? s.raw_full : s.full, *const freed = F8 ? s.raw_empty : s.empty;
     Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
     uint32_t seq = 0;
-    int slot = 0;
+    int stage = 0;
     uint32_t turn = 0;
     bool ok = true;
     while (ok && w.next())
       for (int i = 0; i < w.count && ok; ++i)
         for (int sub = 0; sub < SUB; ++sub) {
-          if (!(ok = wait(&freed[slot], turn ^ 1))) break;
+          if (!(ok = wait(&s.empty[stage], turn ^ 1))) break;
           const int row = (w.tile + i) * WT_KEYS, y = w.unit * a.along[0], z = w.b * a.along[1];
+          uint8_t *to = ring + stage * WT_PIECE;
           if (F8)
-            tma_load_bytes(one, raw + slot * (WT_PIECE / 2), &map, sub * 64, row, y, z, &landed[slot], WT_PIECE / 2);
+            tma_load_bytes(one, to, &map, sub * ROW, row, y, z, &s.full[stage], PIECE);
           else
-            tma_load(one, ring + slot * WT_PIECE, &map, row, sub, y, z, &landed[slot], WT_PIECE);
+            tma_load(one, to, &map, row, sub, y, z, &s.full[stage], PIECE);
           ++seq;
-          if (++slot == slots) slot = 0, turn ^= 1;
+          if (++stage == stages) stage = 0, turn ^= 1;
         }
     if (!ok)  // gave up: the copies in flight still land before the CTA ends
-      for (uint32_t back = 1; back <= (uint32_t)slots && back <= seq; ++back) {
+      for (uint32_t back = 1; back <= (uint32_t)stages && back <= seq; ++back) {
         const uint32_t q = seq - back;
         const unsigned long long t0 = timer_ns();
-        while (!bar_try(&landed[q % slots], (q / slots) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
+        while (!bar_try(&s.full[q % stages], (q / stages) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
         }
       }
   } else if (warp == 1) {
     // ---- tensor core
     const uint32_t one = elect_lane();
     Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
-    const uint32_t desc = mma_desc(WT_KEYS, a.cols, false);
+    const uint32_t desc = F8 ? mma_desc_f8(WT_KEYS, a.cols) : mma_desc(WT_KEYS, a.cols, false);
     const uint32_t q0 = s_addr(queries), ring0 = s_addr(ring);
     int stage = 0;
     uint32_t turn = 0, gt = 0, seg = 0;
@@ -151,10 +148,17 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) {
           wait(&s.full[stage], turn);
-          const uint32_t k0 = ring0 + stage * WT_PIECE, qs = q0 + sub * a.cols * 128;
+          const uint32_t k0 = ring0 + stage * WT_PIECE, qs = q0 + sub * a.cols * ROW, d = tmem + buf * WT_ROWS;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_ss(one, tmem + buf * WT_ROWS, smem_desc(k0 + ks * 32, 16), smem_desc(qs + ks * 32, 16), desc, sub + ks > 0);
+          for (int ks = 0; ks < ROW / 32; ++ks) {
+            const uint64_t kd = smem_desc_rows(k0 + ks * 32, ROW), qd = smem_desc_rows(qs + ks * 32, ROW);
+            if (F8) {
+              mma_f8(one, d, kd, qd, desc, sub + ks > 0);
+              mma_f8(one, d, kd, smem_desc_rows(qs + a.cols * D + ks * 32, ROW), desc, true);
+            } else {
+              mma_ss(one, d, kd, qd, desc, sub + ks > 0);
+            }
+          }
           mma_commit(one, &s.empty[stage]);
           if (++stage == stages) stage = 0, turn ^= 1;
         }
@@ -213,20 +217,39 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
         s.q_at[et] = node * a.qs[1] + g * a.qs[2];
       }
       asm volatile("bar.sync 2, 256;" ::: "memory");
-      // asynchronous copies in a short loop: code that runs once per launch
-      // waits for its instructions, and unrolled loads took 20000 cycles here
-      {
-        const int c16 = et % (D / 8);
-        const uint16_t *q = a.q + w.b * a.qs[0] + h * a.group * a.qs[2] + c16 * 8;
+      const int c16 = et % (D / 8);
+      const uint16_t *q = a.q + w.b * a.qs[0] + h * a.group * a.qs[2] + c16 * 8;
+      // (short loops: code that runs once per launch waits for its
+      // instructions, and unrolled loads took 20000 cycles here)
+      if (F8) {
+        uint4 v = make_uint4(0, 0, 0, 0), ahead = v;
+        auto fetch = [&](int r) { return r < a.cols && s.lse2[seg & 1][r] != INFINITY ? __ldg(reinterpret_cast<const uint4 *>(q + s.q_at[r])) : make_uint4(0, 0, 0, 0); };
+        ahead = fetch(et / (D / 8));
+#pragma unroll 1
+        for (int r = et / (D / 8); r < a.cols; r += 256 / (D / 8)) {
+          v = ahead;
+          ahead = fetch(r + 256 / (D / 8));
+          const uint32_t e = split_exponent(v, D / 8);
+          uint2 hi, lo;
+          split_eight(v, __uint_as_float(e << 23), hi, lo);
+          // 8 bytes at byte 8 c16 of the row
+          uint8_t *to = queries + (c16 * 8 / ROW) * a.cols * ROW + r * ROW + swizzled(c16 * 8 % ROW / 16, r, ROW) * 16 + c16 % 2 * 8;
+          *reinterpret_cast<uint2 *>(to) = hi;
+          *reinterpret_cast<uint2 *>(to + a.cols * D) = lo;
+          if (c16 == 0) s.scale2[seg & 1][r] = a.c2 * __uint_as_float((254 - e) << 23);
+        }
+      } else {
         uint8_t *to = queries + (c16 / 8) * a.cols * 128;
 #pragma unroll 1
         for (int r = et / (D / 8); r < a.cols; r += 256 / (D / 8))
           cp_async16(to + r * 128 + ((c16 % 8) ^ (r & 7)) * 16, q + s.q_at[r], s.lse2[seg & 1][r] != INFINITY);
+        cp_async_wait();
       }
-      cp_async_wait();
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
+      if (F8) asm volatile("bar.sync 2, 256;" ::: "memory");  // the rows' scales are there
+      const float4 *scale2 = reinterpret_cast<const float4 *>(s.scale2[seg & 1]);
       const float4 *lse2 = reinterpret_cast<const float4 *>(s.lse2[seg & 1]);
       const float *wrow = a.w + w.b * a.ws[0] + h * a.ws[1];
       float *orow = a.out + w.b * a.os[0] + h * a.os[1];
@@ -245,11 +268,11 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float4 l = lse2[c / 4 + j];
-            sum[0] += exp2_fast(fmaf(__uint_as_float(x[4 * j]), a.c2, -l.x));
-            sum[1] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 1]), a.c2, -l.y));
-            sum[2] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 2]), a.c2, -l.z));
-            sum[3] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 3]), a.c2, -l.w));
+            const float4 l = lse2[c / 4 + j], f = F8 ? scale2[c / 4 + j] : make_float4(a.c2, a.c2, a.c2, a.c2);
+            sum[0] += exp2_fast(fmaf(__uint_as_float(x[4 * j]), f.x, -l.x));
+            sum[1] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 1]), f.y, -l.y));
+            sum[2] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 2]), f.z, -l.z));
+            sum[3] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 3]), f.w, -l.w));
           }
         }
         tc_fence_before();
@@ -260,50 +283,6 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
         if (on) orow[t * a.os[2]] = before + add;
       }
       ++seg;
-    }
-  } else if (F8) {
-    // ---- FP8 caches: groups of WT_GROUP threads take the pieces in turn and
-    // turn their codes into BF16 where TMA puts a BF16 piece (skv_tree.cu)
-    constexpr int GROUPS = (WT_THREADS_F8 - WT_THREADS) / WT_GROUP, CHUNKS = WT_PIECE / 2 / 16 / WT_GROUP;
-    constexpr int STEP = WT_GROUP / 4;
-    static_assert(STEP % 8 == 0 && WT_RAW % GROUPS == 0, "one swizzle for all of a thread's keys; rings");
-    const int ct = (tid - WT_THREADS) % WT_GROUP, grp = (tid - WT_THREADS) / WT_GROUP;
-    const int key = ct / 4;
-    const uint32_t place = (2 * (ct % 4) ^ key) & 7;
-    Walk w(s.pre, a.batch, a.heads, 0, g_begin, g_end);
-    uint32_t base = 0;
-    bool ok = true;
-    while (ok && w.next()) {
-      const uint32_t end = base + w.count * SUB;
-      const int len = s.len[w.b];
-      for (uint32_t seq = base + (grp - base % GROUPS + GROUPS) % GROUPS; seq < end; seq += GROUPS) {
-        const int left = len - (w.tile + (int)((seq - base) / SUB)) * WT_KEYS - key;  // keys from this thread's first
-        // (both rings' lengths are multiples of GROUPS: a place in them belongs
-        // to one group, which sees its phases in turn)
-        const uint32_t slot = seq % WT_RAW, stage = seq % stages;
-        if (!(ok = wait(&s.raw_full[slot], (seq / WT_RAW) & 1))) break;
-        if (!(ok = wait(&s.empty[stage], ((seq / stages) & 1) ^ 1))) break;
-        const uint8_t *from = raw + slot * (WT_PIECE / 2) + ct * 16;
-        uint8_t *at = ring + stage * WT_PIECE + key * 128;
-        uint32_t nan = 0;
-#pragma unroll 2
-        for (int j = 0; j < CHUNKS; ++j) {
-          uint4 x = *reinterpret_cast<const uint4 *>(from + j * WT_GROUP * 16), y0, y1;
-          if (STEP * j >= left) x = make_uint4(0, 0, 0, 0);
-          e4m3_to_bf16(x, y0, y1, nan);
-          *reinterpret_cast<uint4 *>(at + j * STEP * 128 + place * 16) = y0;
-          *reinterpret_cast<uint4 *>(at + j * STEP * 128 + (place ^ 1) * 16) = y1;
-        }
-        __syncwarp();
-        if (lane == 0) bar_arrive(&s.raw_empty[slot]);
-        if (nan & E4M3_NAN)
-          for (int j = 0; j < CHUNKS; ++j)
-            for (int u = 0; u < 2; ++u) e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * STEP * 128 + (place ^ u) * 16));
-        async_fence();
-        __syncwarp();
-        if (lane == 0) bar_arrive(&s.full[stage]);
-      }
-      base = end;
     }
   }
   tc_fence_before();
@@ -317,21 +296,16 @@ __global__ void __launch_bounds__(F8 ? WT_THREADS_F8 : WT_THREADS, 1)
 template <int D, bool F8>
 int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, int device, cudaStream_t st) {
   constexpr int most = 232448, fixed = 1024 + (int)sizeof(WeightsSmem);
-  constexpr int raw = F8 ? WT_RAW * (WT_PIECE / 2) : 0;
-  const int rows = (D / 64) * a.cols * 128;
-  const int stages = (most - fixed - raw - rows) / WT_PIECE;
+  const int rows = a.cols * D * 2, stages = (most - fixed - rows) / WT_PIECE;
   a.stages = stages < WT_STAGES ? stages : WT_STAGES;
-  if (F8) a.stages &= ~3;  // (see the conversion)
-  const int smem = fixed + raw + rows + a.stages * WT_PIECE;
-  static_assert(most - fixed - WT_ROWS * 512 >= 4 * WT_PIECE && most - fixed - 2 * raw - WT_ROWS_F8 * 512 >= 0 &&
-                    most - fixed - raw - (F8 ? WT_ROWS_F8 : 0) * 512 >= 4 * WT_PIECE,
-                "rings beside the most queries");
+  const int smem = fixed + rows + a.stages * WT_PIECE;
+  static_assert(most - fixed - WT_ROWS * 512 >= 4 * WT_PIECE, "a ring beside the most queries");
   auto *kernel = &k_weights<D, F8>;
   static bool set[64];
   if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), most, device, set)) return rc;
   const int64_t tiles = (int64_t)a.batch * a.heads * ((a.t + WT_KEYS - 1) / WT_KEYS);
   const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
-  return op_cuda(op_launch(kernel, dim3(grid), dim3(F8 ? WT_THREADS_F8 : WT_THREADS), smem, st, false, 1, map, a),
+  return op_cuda(op_launch(kernel, dim3(grid), dim3(WT_THREADS), smem, st, false, 1, map, a),
                  "k_weights launch");
 }
 
@@ -402,16 +376,15 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
     CUtensorMap map{};
     const int64_t step[3] = {kcs[2], kcs[1], kcs[0]};
     const uint8_t *base = static_cast<const uint8_t *>(d->k_cache) + b0 * kcs[0] * (f8 ? 1 : 2);
-    if (int rc = f8 ? make_byte_map(&map, base, d->dim, d->tokens, d->kv_heads, nb, step, WT_KEYS, 64)
+    if (int rc = f8 ? make_byte_map(&map, base, d->dim, d->tokens, d->kv_heads, nb, step, WT_KEYS, d->dim == 64 ? 64 : 128, true)
                     : make_map(&map, base, d->dim, d->tokens, d->kv_heads, nb, step, WT_KEYS, 1))
       return rc;
     a.along[0] = kcs[1] ? 1 : 0;
     a.along[1] = nb > 1 && kcs[0] ? 1 : 0;
     // more rows than the MMA's N: further launches add to what the first wrote
-    const int64_t most = f8 ? WT_ROWS_F8 : WT_ROWS;
-    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    for (int64_t r0 = 0; r0 < rows; r0 += WT_ROWS) {
       a.row0 = (int)r0;
-      a.rows = (int)(rows - r0 < most ? rows - r0 : most);
+      a.rows = (int)(rows - r0 < WT_ROWS ? rows - r0 : WT_ROWS);
       a.cols = (a.rows + 15) & ~15;
       if (r0 == 0) {
         a.w = static_cast<const float *>(d->weights) + b0 * ws[0];

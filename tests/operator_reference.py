@@ -68,12 +68,23 @@ def visible(parents):
     return see
 
 
-def _score_slack(q, k, scale):
+def _score_slack(q, k, scale, fp8=False):
     """FP32 accumulation of D exact products in steps of 16: each step rounds
     (or cuts) by at most 2^-23 of a partial sum, the products inside a step as
-    often again; the bound is (D / 16 + 16) 2^-23 of sum |q k|."""
+    often again; the bound is (D / 16 + 16) 2^-23 of sum |q k|.
+
+    Over FP8 keys a query row is the sum of two e4m3 rows, hi + lo, after a
+    power of two that puts its largest element x into [128, 256).  hi rounds to
+    4 significant bits; what is left is a multiple of 2^-7 of hi's power of two
+    and at most 2^-4 of it, so it fits lo's 4 bits unless it is below e4m3's
+    last place of 2^-9.  There lo is off by at most half of that, 2^-10, which
+    is 2^-10 / 128 = 2^-17 of x at most.  The score is then off by at most
+    2^-17 max|q| sum |k|; and it is accumulated in twice as many steps."""
     d = q.shape[-1]
-    return scale * (q.abs() @ k.abs().T) * (d / 16 + 16) * 2.0 ** -23
+    slack = scale * (q.abs() @ k.abs().T) * (d / 16 + 16) * 2.0 ** -23
+    if fp8:
+        slack = 2 * slack + scale * 2.0 ** -17 * q.abs().amax(1, keepdim=True) * k.abs().sum(1)
+    return slack
 
 
 def tree(q, kc, vc, lengths, k, v, parents, scale=None):
@@ -102,7 +113,7 @@ def tree(q, kc, vc, lengths, k, v, parents, scale=None):
                 p = torch.softmax(z, 1)
                 out[i, j, h * g:(h + 1) * g] = p @ vals
                 lse[i, j, h * g:(h + 1) * g] = torch.logsumexp(z, 1)
-                dz = _score_slack(x, keys, scale).amax(1, keepdim=True) + z.abs().amax(1, keepdim=True) * 2.0 ** -22
+                dz = _score_slack(x, keys, scale, kc.dtype == torch.float8_e4m3fn).amax(1, keepdim=True) + z.abs().amax(1, keepdim=True) * 2.0 ** -22
                 rel = torch.expm1(2 * dz) + 2.0 ** -18
                 mass = p @ vals.abs()
                 eo[i, j, h * g:(h + 1) * g] = (rel + 2.0 ** -8) * mass + out[i, j, h * g:(h + 1) * g].abs() * 2.0 ** -8 \
@@ -134,7 +145,7 @@ def weights(q, kc, lengths, lse, w, rows=None, scale=None):
             keys = kc[i, h, :m].double()
             z = x @ keys.T * scale
             p = torch.exp(z - less)
-            dz = _score_slack(x, keys, scale) + (z.abs() + less.abs() + 1) * 2.0 ** -21
+            dz = _score_slack(x, keys, scale, kc.dtype == torch.float8_e4m3fn) + (z.abs() + less.abs() + 1) * 2.0 ** -21
             y[i, h, :m] += p.sum(0)
             e[i, h, :m] += (p * torch.expm1(dz)).sum(0) + p.sum(0) * (x.shape[0] + 4) * 2.0 ** -24
     return y, e + y.abs() * 2.0 ** -23
