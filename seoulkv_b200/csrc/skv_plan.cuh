@@ -5,7 +5,7 @@
 
 namespace skv {
 
-constexpr int PLAN_BATCH = 256;  // sequences of one launch (their tile counts are kept in shared memory)
+constexpr int PLAN_BATCH = 128;  // sequences of one launch (their tile counts are kept in shared memory)
 
 // The list: sequence after sequence, unit (KV head) after unit, tile after
 // tile; every unit ends with `idle` places that stand for its fixed cost.

@@ -124,18 +124,22 @@ struct TreeCfg {
   static constexpr int D = D_;
   static constexpr bool F8 = F8_;
   static constexpr int KT = TR_KEYS;
-  static constexpr int PIECES = D / 64;   // ring stages of a tile's K, and of its V
+  static constexpr int PIECES = D / 64;   // ring stages of a BF16 tile of K or V
   static constexpr int VROWS = KT / PIECES;  // keys of a V stage
   static constexpr int STAGE = KT * 128;  // bytes: K 128 keys x 64 dimensions, V VROWS keys x D
-  static constexpr int RAW = STAGE / 2;   // an FP8 stage before its conversion
-  // (FP8: multiples of the converting groups, so that a place in either ring
-  // belongs to one group, which sees its phases in turn)
-  static constexpr int NRAW = F8 ? (D == 256 ? 12 : 8) : 0;
-  static constexpr int NSTAGE = F8 ? (D == 256 ? 4 : 8) : D == 256 ? 10 : D == 128 ? 11 : 12;
+  // FP8: K tiles as they are stored in a ring of their own (128 or 64 bytes of
+  // every key a stage), V before its conversion in another.  The rings of V
+  // are multiples of the converting groups, so that a place in them belongs to
+  // one group, which sees its phases in turn.
+  static constexpr int ROW8 = D < 128 ? D : 128, PIECES8 = D / ROW8;
+  static constexpr int NK8 = F8 ? 4 : 0;
+  static constexpr int RAW = STAGE / 2;
+  static constexpr int NRAW = F8 ? (D == 256 ? 4 : 8) : 0;
+  static constexpr int NSTAGE = F8 ? 4 : D == 256 ? 10 : D == 128 ? 11 : 12;
   static constexpr int THREADS = F8 ? 576 : 384;  // FP8: warps 2, 3 and 12.. convert
   static constexpr int COL_S = 256;       // tensor memory columns: O, then two score tiles (P over S)
-  static constexpr int QBYTES = TR_ROWS * D * 2;
-  static constexpr int RING = QBYTES + NSTAGE * STAGE + NRAW * RAW;
+  static constexpr int QBYTES = TR_ROWS * D * 2;  // BF16, or both FP8 halves
+  static constexpr int RING = QBYTES + (NSTAGE + NK8) * STAGE + NRAW * RAW;
 };
 
 struct TreeMaps {
@@ -167,7 +171,9 @@ struct TreeArgs {
 template <class C>
 struct TreeSmem {
   uint64_t full[C::NSTAGE], empty[C::NSTAGE];
-  uint64_t raw_full[C::NRAW + 1], raw_empty[C::NRAW + 1];  // (+ 1: no empty arrays without FP8)
+  uint64_t raw_full[C::F8 ? C::NRAW : 1], raw_empty[C::F8 ? C::NRAW : 1];
+  uint64_t k8_full[C::F8 ? C::NK8 : 1], k8_empty[C::F8 ? C::NK8 : 1];
+  float scale2[C::F8 ? TR_ROWS : 1];  // of the split queries' rows: scale * log2(e), by the row's power of two
   uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;
   uint64_t anc[TR_NODES];      // nodes that node i sees (0: unused)
   unsigned long long bad;      // nodes with a value that is not finite
@@ -178,14 +184,17 @@ struct TreeSmem {
   int32_t pre[PLAN_BATCH + 1];  // places of the sequences before (one unit's worth)
 };
 
-// Order of a segment's 2n operand tiles in the ring: K0, K1, V0, K2, V1, ...,
-// V(n-1), the order in which the MMA thread needs them.
-__device__ __forceinline__ int pos_k(int i) { return i ? 2 * i - 1 : 0; }
+// Order of a segment's 2n operand tiles: K0, K1, V0, K2, V1, ..., V(n-1), the
+// order in which the tensor core needs them.
 __device__ __forceinline__ int pos_v(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 __device__ __forceinline__ void tile_at(int p, int n, bool &is_v, int &i) {
   is_v = p == 2 * n - 1 || (p > 0 && !(p & 1));
   i = p == 0 ? 0 : p == 2 * n - 1 ? n - 1 : is_v ? (p - 2) / 2 : (p + 1) / 2;
 }
+// Over an FP8 cache the BF16 ring has the V tiles and the nodes' K: a segment
+// with the nodes (in its last tile) has n + 1 tiles there, the nodes' K at
+// this place among them.
+__device__ __forceinline__ int nodes_k_place(int n) { return n > 1 ? n - 2 : 0; }
 
 __device__ __forceinline__ bool not_finite_bf16(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
 
@@ -198,7 +207,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_dyn[];
   uint8_t *queries = smem_dyn;  // [D / 64][128 rows][128 bytes], swizzled
   uint8_t *ring = queries + C::QBYTES;
-  uint8_t *raw = ring + C::NSTAGE * C::STAGE;
+  uint8_t *ring8 = ring + C::NSTAGE * C::STAGE, *raw = ring8 + C::NK8 * C::STAGE;
   TreeSmem<C> &s = *reinterpret_cast<TreeSmem<C> *>(smem_dyn + C::RING);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
@@ -224,6 +233,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     for (int i = 0; i < C::NRAW; ++i) {
       bar_init(&s.raw_full[i], 1);
       bar_init(&s.raw_empty[i], TR_GROUP / 32);
+    }
+    for (int i = 0; i < C::NK8; ++i) {
+      bar_init(&s.k8_full[i], 1);
+      bar_init(&s.k8_empty[i], 1);
     }
     bar_init(&s.q_ready, 8);
     bar_init(&s.drain, 1);
@@ -255,12 +268,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   };
 
   if (warp == 0) {
-    // ---- loads: BF16 stages into the ring, FP8 stages (cache tiles alone) beside it
+    // ---- loads: BF16 tiles into the ring; of FP8 caches K into its own, and V
+    // beside it to be converted
     const uint32_t one = elect_lane();
-    constexpr int SLOTS = C::F8 ? C::NRAW : C::NSTAGE;
-    uint64_t *const landed = C::F8 ? s.raw_full : s.full, *const freed = C::F8 ? s.raw_empty : s.empty;
     Walk w = walk;
-    uint32_t seq = 0;
+    uint32_t seq = 0, seq8 = 0;  // stages of the ring (or V stages before conversion), FP8 K stages
     bool ok = true;
     while (ok && w.next()) {
       for (int p = 0; ok && p < 2 * w.count; ++p) {
@@ -273,55 +285,93 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (C::F8 && a.cell_maps) map = a.cell_maps + 2 * ((int64_t)w.b * a.heads + w.unit) + is_v;
         const int row = nodes ? 0 : (w.tile + i) * KT;
         const int y = w.unit * a.along[which][0], z = w.b * a.along[which][1];
-        for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
-          const int slot = seq % SLOTS;
-          if (!(ok = wait(&freed[slot], ((seq / SLOTS) & 1) ^ 1))) break;
-          if (C::F8 && nodes) {  // (not FP8: copied by the converting warps; the place in the ring passes)
-            if (one) bar_arrive(&landed[slot]);
-          } else if (C::F8)
-            tma_load_bytes(one, raw + slot * C::RAW, map, is_v ? 0 : piece * 64, row + (is_v ? piece * C::VROWS : 0), y,
-                           z, &landed[slot], C::RAW);
-          else
+        if constexpr (C::F8) {
+          if (!nodes && !is_v) {
+            for (int piece = 0; piece < C::PIECES8; ++piece, ++seq8) {
+              const uint32_t slot = seq8 % C::NK8;
+              if (!(ok = wait(&s.k8_empty[slot], ((seq8 / C::NK8) & 1) ^ 1))) break;
+              tma_load_bytes(one, ring8 + slot * C::STAGE, map, piece * C::ROW8, row, y, z, &s.k8_full[slot], KT * C::ROW8);
+            }
+          } else {
+            for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
+              const uint32_t slot = seq % C::NRAW;
+              if (!(ok = wait(&s.raw_empty[slot], ((seq / C::NRAW) & 1) ^ 1))) break;
+              if (!nodes)
+                tma_load_bytes(one, raw + slot * C::RAW, map, 0, row + piece * C::VROWS, y, z, &s.raw_full[slot], C::RAW);
+              else if (one)  // (the converting warps copy the nodes: the place passes)
+                bar_arrive(&s.raw_full[slot]);
+            }
+          }
+        } else {
+          for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
+            const uint32_t slot = seq % C::NSTAGE;
+            if (!(ok = wait(&s.empty[slot], ((seq / C::NSTAGE) & 1) ^ 1))) break;
             tma_load(one, ring + slot * C::STAGE, map, row + (is_v ? piece * C::VROWS : 0), is_v ? 0 : piece, y, z,
-                     &landed[slot], C::STAGE);
+                     &s.full[slot], C::STAGE);
+          }
         }
       }
     }
-    if (!ok)  // gave up: the copies in flight still land before the CTA ends
-      for (uint32_t back = 1; back <= SLOTS && back <= seq; ++back) {
-        const uint32_t q = seq - back;
-        const unsigned long long t0 = timer_ns();
-        while (!bar_try(&landed[q % SLOTS], (q / SLOTS) & 1) && timer_ns() - t0 < WAIT_NS / 4) {
-        }
+    if (!ok) {  // gave up: the copies in flight still land before the CTA ends
+      const unsigned long long t0 = timer_ns();
+      auto landed = [&](uint64_t *bar, uint32_t slots, uint32_t n) {
+        for (uint32_t back = 1; back <= slots && back <= n; ++back)
+          while (!bar_try(&bar[(n - back) % slots], ((n - back) / slots) & 1) && timer_ns() - t0 < WAIT_NS / 2) {
+          }
+      };
+      if constexpr (C::F8) {
+        landed(s.raw_full, C::NRAW, seq);
+        landed(s.k8_full, C::NK8, seq8);
+      } else {
+        landed(s.full, C::NSTAGE, seq);
       }
+    }
   } else if (warp == 1) {
     // ---- tensor core
     const uint32_t one = elect_lane();
     Walk w = walk;
     constexpr uint32_t DESC_S = mma_desc(TR_ROWS, KT, false), DESC_O = mma_desc(TR_ROWS, D, true);
-    const uint32_t q0 = s_addr(queries), ring0 = s_addr(ring);
-    uint32_t seq = 0, gt = 0, seg = 0;
+    constexpr uint32_t DESC_S8 = mma_desc_f8(TR_ROWS, KT);
+    const uint32_t q0 = s_addr(queries), ring0 = s_addr(ring), ring80 = s_addr(ring8);
+    uint32_t seq = 0, seq8 = 0, gt = 0, loaded = 0;  // loaded: times that the queries were
     while (w.next()) {
       const int n = w.count;
-      auto scores = [&](uint32_t buf) {
+      auto scores = [&](int i, uint32_t buf) {
         const uint32_t d = tmem + C::COL_S + buf * KT;
+        if (C::F8 && w.tile + i < w.tiles - 1) {
 #pragma unroll
-        for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
-          const uint32_t stage = seq % C::NSTAGE;
-          wait(&s.full[stage], (seq / C::NSTAGE) & 1);
-          const uint32_t k0 = ring0 + stage * C::STAGE, qp = q0 + piece * TR_ROWS * 128;
+          for (int piece = 0; piece < C::PIECES8; ++piece, ++seq8) {
+            const uint32_t slot = seq8 % (C::F8 ? C::NK8 : 1);
+            wait(&s.k8_full[slot], (seq8 / (C::F8 ? C::NK8 : 1)) & 1);
+            const uint32_t k0 = ring80 + slot * C::STAGE, qp = q0 + piece * TR_ROWS * C::ROW8;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_ss(one, d, smem_desc(qp + ks * 32, 16), smem_desc(k0 + ks * 32, 16), DESC_S, piece + ks > 0);
-          mma_commit(one, &s.empty[stage]);
+            for (int ks = 0; ks < C::ROW8 / 32; ++ks) {
+              const uint64_t kd = smem_desc_rows(k0 + ks * 32, C::ROW8);
+              mma_f8(one, d, smem_desc_rows(qp + ks * 32, C::ROW8), kd, DESC_S8, piece + ks > 0);
+              mma_f8(one, d, smem_desc_rows(qp + TR_ROWS * D + ks * 32, C::ROW8), kd, DESC_S8, true);
+            }
+            mma_commit(one, &s.k8_empty[slot]);
+          }
+        } else {
+          if (C::F8 && i > 0) wait(&s.q_ready, loaded++ & 1);  // the queries in BF16
+#pragma unroll
+          for (int piece = 0; piece < C::PIECES; ++piece, ++seq) {
+            const uint32_t stage = seq % C::NSTAGE;
+            wait(&s.full[stage], (seq / C::NSTAGE) & 1);
+            const uint32_t k0 = ring0 + stage * C::STAGE, qp = q0 + piece * TR_ROWS * 128;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              mma_ss(one, d, smem_desc(qp + ks * 32, 16), smem_desc(k0 + ks * 32, 16), DESC_S, piece + ks > 0);
+            mma_commit(one, &s.empty[stage]);
+          }
         }
         mma_commit(one, &s.s_full[buf]);
       };
-      wait(&s.q_ready, seg & 1);
-      scores(gt & 1);
+      wait(&s.q_ready, loaded++ & 1);
+      scores(0, gt & 1);
       for (int i = 0; i < n; ++i, ++gt) {
         const uint32_t buf = gt & 1;
-        if (i + 1 < n) scores(buf ^ 1);
+        if (i + 1 < n) scores(i + 1, buf ^ 1);
         wait(&s.p_ready[buf], (gt >> 1) & 1);
         tc_fence_after();
 #pragma unroll
@@ -339,7 +389,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         }
         mma_commit(one, &s.o_done[buf]);
       }
-      ++seg;
     }
     if (*abort) {  // what was issued ends before tensor memory is given back
       mma_commit(one, &s.drain);
@@ -371,20 +420,51 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       __syncwarp();
       tc_fence_after();
     };
-    auto load_queries = [&](const Walk &x) {
-      // asynchronous copies in a short loop: code that runs once per segment
-      // waits for its instructions when it is unrolled
-      const int total = min(left, TR_ROWS) * (D / 8);
+    // The rows' queries of a unit: BF16, or (FP8 cache) split into two FP8 rows
+    // whose sum they are.  Short loops: code that runs once per segment waits
+    // for its instructions when it is unrolled.
+    const int total = min(left, TR_ROWS) * (D / 8);
+    auto row_at = [&](const Walk &x, int c) {  // the row that holds 16-byte piece c
+      const int rr = mt * TR_ROWS + c / (D / 8), nd = by_inverse(rr, a.by_group);
+      return a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2] + c % (D / 8) * 8;
+    };
+    auto load_bf16 = [&](const Walk &x) {
 #pragma unroll 1
       for (int c = st; c < total; c += 256) {
-        const int at = c / (D / 8), c16 = c % (D / 8), rr = mt * TR_ROWS + at, nd = by_inverse(rr, a.by_group);
-        cp_async16(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16,
-                   a.q + x.b * a.qs[0] + nd * a.qs[1] + (x.unit * a.group + rr - nd * a.group) * a.qs[2] + c16 * 8, true);
+        const int at = c / (D / 8), c16 = c % (D / 8);
+        cp_async16(queries + (c16 / 8) * TR_ROWS * 128 + at * 128 + ((c16 % 8) ^ (at & 7)) * 16, row_at(x, c), true);
       }
       cp_async_wait();
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
+    };
+    auto load_split = [&](const Walk &x) {
+      const int c16 = st % (D / 8);
+      auto fetch = [&](int c) { return c < total ? __ldg(reinterpret_cast<const uint4 *>(row_at(x, c))) : make_uint4(0, 0, 0, 0); };
+      // (whole warps, since a row's threads look at one another's)
+      const int whole_warps = (total + 31) & ~31;
+      uint4 ahead = fetch(st);
+#pragma unroll 1
+      for (int c = st; c < whole_warps; c += 256) {
+        const uint4 v = ahead;
+        ahead = fetch(c + 256);
+        const int at = c / (D / 8);
+        const uint32_t e = split_exponent(v, D / 8);
+        uint2 hi, lo;
+        split_eight(v, __uint_as_float(e << 23), hi, lo);
+        uint8_t *to = queries + (c16 * 8 / C::ROW8) * TR_ROWS * C::ROW8 + at * C::ROW8 +
+                      swizzled(c16 * 8 % C::ROW8 / 16, at, C::ROW8) * 16 + c16 % 2 * 8;
+        *reinterpret_cast<uint2 *>(to) = hi;
+        *reinterpret_cast<uint2 *>(to + TR_ROWS * D) = lo;
+        if (C::F8 && c16 == 0) s.scale2[at] = a.c2 * __uint_as_float((254 - e) << 23);
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&s.q_ready);
+    };
+    auto load_queries = [&](const Walk &x) {
+      if (C::F8 && x.tile < x.tiles - 1) load_split(x); else load_bf16(x);
     };
     bool live = w.next();
     if (live) load_queries(w);
@@ -394,6 +474,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       const int n = cur.count, h = cur.unit;
       const int len = length(cur.b);
       const bool has_nodes = cur.tile + n == cur.tiles;
+      float cache_c2 = a.c2;
+      if (C::F8 && cur.tile < cur.tiles - 1) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the split rows' scales are there ...
+        if (on) cache_c2 = s.scale2[row];
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // ... and read, before the next segment's
+      }
       int up = -2;  // the parent of node st, wanted at the segment's last tile
       if (has_nodes && st < a.n) up = a.parents[cur.b * a.ps[0] + st * a.ps[1]];
       uint64_t see = 0;  // the nodes that this row sees
@@ -430,7 +516,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const bool whole = valid == KT && !nodes;
         const int v64 = valid - 64 * half;
         const uint64_t keep = nodes ? (half ? 0 : see) : v64 >= 64 ? ~0ull : v64 > 0 ? (1ull << v64) - 1 : 0;
+        const float c2 = nodes ? a.c2 : cache_c2;
         done(s.s_full, gt + i);
+        // (FP8) the nodes' K is BF16: their scores need the queries as they are
+        if (C::F8 && has_nodes && i == n - 2) load_bf16(cur);
         if (warp_on) {
           // S stays in registers between the maximum and the exponentials
           // where there are enough of them, and is read again where not (FP8)
@@ -467,7 +556,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
           s.share[half][row] = top;
           asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-          top = fmaxf(top, s.share[half ^ 1][row]) * a.c2;
+          top = fmaxf(top, s.share[half ^ 1][row]) * c2;
           // the maximum moves only when it grows by more than 2^8: until then
           // weights up to 2^8 lose nothing in FP32 sums and BF16 products,
           // and the accumulator stays where it is
@@ -488,7 +577,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           }
           if (move) m = top;
           const float base2 = m == -INFINITY ? 0.0f : m;
-          const uint64_t scale2 = pack2(a.c2, a.c2), minus2 = pack2(-base2, -base2);
+          const uint64_t scale2 = pack2(c2, c2), minus2 = pack2(-base2, -base2);
           uint64_t sum = 0;  // two sums
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -527,7 +616,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           // them; the rows that do get them back below)
           // (the tile before is waited for so that a stage's parity names V(i)'s use of it)
           if (i > 0) done(s.o_done, gt + i - 1);
-          const uint32_t v0 = base + pos_v(i, n) * C::PIECES;
+          const uint32_t v0 = base + (C::F8 ? i + (has_nodes ? 1 : 0) : pos_v(i, n)) * C::PIECES;
           const int from = nodes ? 0 : valid, to = nodes ? a.n : KT;
           for (int piece = from / C::VROWS; piece * C::VROWS < to; ++piece) {
             const uint32_t stage = (v0 + piece) % C::NSTAGE;
@@ -619,84 +708,77 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       // all have read O, s.bad and s.anc before the next segment's products and nodes
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (has_nodes && st == 0) s.bad = 0;
-      base += 2 * n * C::PIECES;
+      base += (C::F8 ? n + (has_nodes ? 1 : 0) : 2 * n) * C::PIECES;
       gt += n;
     }
   } else if (C::F8 && (warp >= 12 || warp == 2 || warp == 3)) {
-    // ---- FP8 caches: groups of TR_GROUP threads take the stages in turn, turn
-    // their codes into BF16 and put them where TMA puts a BF16 stage.  The
-    // nodes' own K and V are BF16 and are copied.
+    // ---- FP8 caches: groups of TR_GROUP threads take the stages of V in turn,
+    // turn their codes into BF16 and put them where TMA puts a BF16 stage.
+    // The nodes' own K and V are BF16 and are copied.
     constexpr int GROUPS = 4, CHUNKS = C::RAW / 16 / TR_GROUP;  // 16-code pieces of one thread and stage
+    constexpr uint32_t SLOTS = C::F8 ? C::NRAW : 1;
     const int ct = tid % TR_GROUP, grp = warp < 4 ? 0 : (warp - 10) / 2;
     static_assert(TR_GROUP == 64 && GROUPS % C::PIECES == 0, "groups of two warps, one stage each");
     static_assert(!C::F8 || (C::NRAW % GROUPS == 0 && C::NSTAGE % GROUPS == 0), "places of one group");
-    // Piece j of this thread: K key ct / 4 + KSTEP j, dimensions 16 (ct % 4)..
-    // of the stage's 64 (KSTEP is a multiple of 8: one swizzle for all j); V
-    // key CHUNKS (ct / VPER) + j of the stage's, dimensions 16 (ct % VPER)...
-    constexpr int VPER = D / 16, KSTEP = TR_GROUP / 4;
-    static_assert(KSTEP % 8 == 0 && CHUNKS == 8, "swizzle of an FP8 stage's pieces");
-    const int key_k = ct / 4, key_v = ct / VPER * CHUNKS;
-    const int unit_k = 2 * (ct % 4), unit_v = 2 * (ct % VPER);  // the first of its two 16-byte places in a row
-    const int raw_k = ct * 16, raw_v = key_v * D + ct % VPER * 16;
-    const int to_v = (unit_v / 8) * C::VROWS * 128 + key_v * 128;
-    constexpr uint32_t SLOTS = C::F8 ? C::NRAW : 1;
+    // Piece j of this thread: key CHUNKS (ct / PER) + j of the stage's, dimensions 16 (ct % PER)...
+    constexpr int PER = D / 16;
+    static_assert(CHUNKS == 8, "a thread's keys cover a swizzle period");
+    const int key = ct / PER * CHUNKS, unit = 2 * (ct % PER);  // unit: the first of its two 16-byte places in a row
     const int piece = grp % C::PIECES;
     Walk w = walk;
-    uint32_t base = 0;  // stages of the segments before
+    uint32_t base = 0;  // tiles of the ring in the segments before
     bool ok = true;
     while (ok && w.next()) {
       const int n = w.count, len = length(w.b);
-      for (int p = (grp - base % GROUPS + GROUPS) % GROUPS / C::PIECES; p < 2 * n; p += GROUPS / C::PIECES) {
-        bool is_v;
-        int i;
-        tile_at(p, n, is_v, i);
-        const uint32_t seq = base + p * C::PIECES + piece, stage = seq % C::NSTAGE, slot = seq % SLOTS;
+      const bool has_nodes = w.tile + n == w.tiles;
+      const int tiles = n + (has_nodes ? 1 : 0), k_place = has_nodes ? nodes_k_place(n) : tiles;
+      for (int t = (grp / C::PIECES - base % (GROUPS / C::PIECES) + GROUPS) % (GROUPS / C::PIECES); t < tiles;
+           t += GROUPS / C::PIECES) {
+        const bool is_k = t == k_place;
+        const int i = is_k ? n - 1 : t - (t > k_place);  // the segment's tile
+        const uint32_t seq = (base + t) * C::PIECES + piece, stage = seq % C::NSTAGE, slot = seq % SLOTS;
         uint8_t *to = ring + stage * C::STAGE;
+        if (!(ok = wait(&s.raw_full[slot], (seq / SLOTS) & 1))) break;
+        if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
         if (w.tile + i < w.tiles - 1) {
-          if (!(ok = wait(&s.raw_full[slot], (seq / SLOTS) & 1))) break;
-          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
-          const int left = len - (w.tile + i) * KT - (is_v ? piece * C::VROWS + key_v : key_k);  // keys from this thread's first
-          const int gap = is_v ? 1 : KSTEP, turn = is_v ? 7 : 0;
-          const uint8_t *from = raw + slot * C::RAW + (is_v ? raw_v : raw_k);
-          uint8_t *at = to + (is_v ? to_v : key_k * 128);
-          const uint32_t first = is_v ? unit_v & 7 : (unit_k ^ key_k) & 7;
+          const int left = len - (w.tile + i) * KT - piece * C::VROWS - key;  // keys from this thread's first
+          const uint8_t *from = raw + slot * C::RAW + key * D + ct % PER * 16;
+          uint8_t *at = to + (unit / 8) * C::VROWS * 128 + key * 128;
           uint32_t nan = 0;
           // (a short body: straight-line code for all pieces would wait for its instructions)
 #pragma unroll 2
           for (int j = 0; j < CHUNKS; ++j) {
-            uint4 x = *reinterpret_cast<const uint4 *>(from + j * (is_v ? D : KSTEP * 64)), y0, y1;
-            if (gap * j >= left) x = make_uint4(0, 0, 0, 0);  // behind the length
+            uint4 x = *reinterpret_cast<const uint4 *>(from + j * D), y0, y1;
+            if (j >= left) x = make_uint4(0, 0, 0, 0);  // behind the length
             e4m3_to_bf16(x, y0, y1, nan);
-            const uint32_t place = first ^ (j & turn);
-            *reinterpret_cast<uint4 *>(at + j * gap * 128 + place * 16) = y0;
-            *reinterpret_cast<uint4 *>(at + j * gap * 128 + (place ^ 1) * 16) = y1;
+            const uint32_t place = (unit & 7) ^ j;
+            *reinterpret_cast<uint4 *>(at + j * 128 + place * 16) = y0;
+            *reinterpret_cast<uint4 *>(at + j * 128 + (place ^ 1) * 16) = y1;
           }
-          __syncwarp();
-          if (lane == 0) bar_arrive(&s.raw_empty[slot]);
           if (nan & E4M3_NAN)
             for (int j = 0; j < CHUNKS; ++j)
               for (int u = 0; u < 2; ++u)
-                e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * gap * 128 + ((first ^ (j & turn)) ^ u) * 16));
+                e4m3_put_nan(reinterpret_cast<uint4 *>(at + j * 128 + (((unit & 7) ^ j) ^ u) * 16));
         } else {
-          if (!(ok = wait(&s.raw_full[slot], (seq / SLOTS) & 1))) break;
-          if (lane == 0) bar_arrive(&s.raw_empty[slot]);
-          if (!(ok = wait(&s.empty[stage], ((seq / C::NSTAGE) & 1) ^ 1))) break;
-          const uint16_t *src = is_v ? a.vn + w.b * a.vns[0] + w.unit * a.vns[1] : a.kn + w.b * a.kns[0] + w.unit * a.kns[1];
-          const int64_t st = is_v ? a.vns[2] : a.kns[2];
-          const int rows = is_v ? C::VROWS : KT, per = is_v ? D / 8 : 8;  // 16-byte units of a key in this stage
+          const uint16_t *src = is_k ? a.kn + w.b * a.kns[0] + w.unit * a.kns[1] : a.vn + w.b * a.vns[0] + w.unit * a.vns[1];
+          const int64_t st = is_k ? a.kns[2] : a.vns[2];
+          const int rows = is_k ? KT : C::VROWS, per = is_k ? 8 : D / 8;  // 16-byte units of a key in this stage
 #pragma unroll 4
           for (int c = ct; c < C::STAGE / 16; c += TR_GROUP) {
-            const int key = c / per, c16 = c % per;
-            const int nd = is_v ? piece * C::VROWS + key : key, off = is_v ? c16 : piece * 8 + c16;
+            const int r = c / per, c16 = c % per;
+            const int nd = is_k ? r : piece * C::VROWS + r, off = is_k ? piece * 8 + c16 : c16;
             const uint4 y = nd < a.n ? __ldg(reinterpret_cast<const uint4 *>(src + nd * st) + off) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(to + (c16 / 8) * rows * 128 + key * 128 + ((c16 ^ key) & 7) * 16) = y;
+            *reinterpret_cast<uint4 *>(to + (c16 / 8) * rows * 128 + r * 128 + ((c16 ^ r) & 7) * 16) = y;
           }
         }
         async_fence();
         __syncwarp();
-        if (lane == 0) bar_arrive(&s.full[stage]);
+        if (lane == 0) {
+          bar_arrive(&s.raw_empty[slot]);
+          bar_arrive(&s.full[stage]);
+        }
       }
-      base += 2 * n * C::PIECES;
+      base += tiles;
     }
   }
   tc_fence_before();
@@ -872,7 +954,7 @@ int check_tree(const SkvTree *d) {
 int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
   const int64_t step[3] = {REC, 0, 0};
   for (int i = 0; i < 2; ++i)
-    if (int rc = make_byte_map(two + i, records + i * D, D, rows, 1, 1, step, i ? TR_KEYS / (D / 64) : TR_KEYS, i ? D : 64, false))
+    if (int rc = make_byte_map(two + i, records + i * D, D, rows, 1, 1, step, i ? TR_KEYS / (D / 64) : TR_KEYS, i ? D : 128, !i))
       return rc;
   return SKV_OK;
 }
@@ -969,7 +1051,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
         const int64_t *at = i ? vcs : kcs, step[3] = {at[2], at[1], at[0]};
         const void *base = static_cast<const uint8_t *>(i ? d->v_cache : d->k_cache) + b0 * at[0];
         rc = make_byte_map(i ? &maps.v : &maps.k, base, d->dim, d->tokens, d->kv_heads, nb, step,
-                           i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : 64, false);
+                           i ? TR_KEYS / ((int)d->dim / 64) : TR_KEYS, i ? (int)d->dim : d->dim == 64 ? 64 : 128, !i);
         a.along[i][0] = d->kv_heads > 1 && at[1] ? 1 : 0;
         a.along[i][1] = nb > 1 && at[0] ? 1 : 0;
       }
