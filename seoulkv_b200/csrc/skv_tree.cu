@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             maximum(0);
             maximum(1);
           } else {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 2; ++c) {
               load(c);
               tmem_wait_ld();
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const float base2 = m == -INFINITY ? 0.0f : m;
           const uint64_t scale2 = pack2(c2, c2), minus2 = pack2(-base2, -base2);
           uint64_t sum = 0;  // two sums
-#pragma unroll
+#pragma unroll(C::F8 ? 1 : 2)
           for (int c = 0; c < 2; ++c) {
             if (C::F8) {
               load(c);
