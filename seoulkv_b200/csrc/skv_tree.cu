@@ -523,16 +523,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (warp_on) {
           // S stays in registers between the maximum and the exponentials
           // where there are enough of them, and is read again where not (FP8)
-          constexpr bool REREAD = true;
-          constexpr int HELD = REREAD ? 32 : 64;
+          constexpr int HELD = C::F8 ? 32 : 64;
           uint32_t x[HELD];
           float top = -INFINITY;
           auto load = [&](int c) {
-            uint32_t(&z)[32] = *reinterpret_cast<uint32_t(*)[32]>(x + (REREAD ? 0 : 32 * c));
+            uint32_t(&z)[32] = *reinterpret_cast<uint32_t(*)[32]>(x + (C::F8 ? 0 : 32 * c));
             tmem_ld32(z, at + 64 * half + 32 * c);
           };
           auto maximum = [&](int c) {
-            const uint32_t *z = x + (REREAD ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
+            const uint32_t *z = x + (C::F8 ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
             if (whole) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(z[j]));
@@ -541,7 +540,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               for (int j = 0; j < 32; ++j) top = fmaxf(top, bits >> j & 1 ? __uint_as_float(z[j]) : -INFINITY);
             }
           };
-          if (!REREAD) {
+          if (!C::F8) {
             load(0);
             load(1);
             tmem_wait_ld();
@@ -580,13 +579,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const float base2 = m == -INFINITY ? 0.0f : m;
           const uint64_t scale2 = pack2(c2, c2), minus2 = pack2(-base2, -base2);
           uint64_t sum = 0;  // two sums
-#pragma unroll(REREAD ? 1 : 2)
+#pragma unroll(C::F8 ? 1 : 2)
           for (int c = 0; c < 2; ++c) {
-            if (REREAD) {
+            if (C::F8) {
               load(c);
               tmem_wait_ld();
             }
-            const uint32_t *z = x + (REREAD ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
+            const uint32_t *z = x + (C::F8 ? 0 : 32 * c), bits = (uint32_t)(keep >> (32 * c));
             uint32_t y[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
