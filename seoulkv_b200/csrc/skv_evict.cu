@@ -294,6 +294,8 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
     return op_fail(SKV_E_INVALID, "null input or output pointer");
   if (d->dim > 1 && (d->k_stride[3] != 1 || d->v_stride[3] != 1))
     return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
+  int sms = 0;
+  if (int rc = sm_count(d->device, &sms)) return rc;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -308,10 +310,9 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   a.out_w = static_cast<float *>(d->weights_out);
   a.heads = (int)d->kv_heads, a.t = (int)d->tokens, a.keep = (int)d->keep;
   a.sink = (int)d->sink, a.local = (int)d->local;
-  static bool set[64];
-  int sms = 0, rc = sm_count((int)d->device, &sms);  // (checks the ordinal)
-  static bool wide[64];
-  if (!rc && !__atomic_load_n(&wide[d->device], __ATOMIC_RELAXED)) {  // clusters of 16 are not portable
+  static bool set[64], wide[64];
+  int rc = SKV_OK;
+  if (!__atomic_load_n(&wide[d->device], __ATOMIC_RELAXED)) {  // clusters of 16 are not portable
     rc = op_cuda(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
     if (!rc) __atomic_store_n(&wide[d->device], true, __ATOMIC_RELAXED);
   }

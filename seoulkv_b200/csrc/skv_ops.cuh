@@ -64,12 +64,12 @@ inline void op_strides(int64_t *to, const int64_t *from, const int64_t *size, in
 }
 
 // SMs of a device, asked once.
-inline int sm_count(int device, int *sms) noexcept {
+inline int sm_count(int64_t device, int *sms) noexcept {
   static int known[64];
   if (device < 0 || device >= 64) return op_fail(SKV_E_INVALID, "device ordinal out of range");
   int n = __atomic_load_n(&known[device], __ATOMIC_RELAXED);
   if (!n) {
-    if (int rc = op_cuda(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "device attribute")) return rc;
+    if (int rc = op_cuda(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, (int)device), "device attribute")) return rc;
     __atomic_store_n(&known[device], n, __ATOMIC_RELAXED);
   }
   *sms = n;

@@ -183,6 +183,8 @@ extern "C" int skv_rotary(const SkvRotary *d, void *stream) {
     return op_fail(SKV_E_INVALID, "the innermost dimension must be contiguous");
   if (!d->q || !d->q_out || (has_k && (!d->k || !d->k_out)) || !d->positions || !d->phase)
     return op_fail(SKV_E_INVALID, "null input or output pointer");
+  int sms = 0;
+  if (int rc = sm_count(d->device, &sms)) return rc;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
   const bool half = d->layout == SKV_ROTARY_HALF;
@@ -230,8 +232,6 @@ extern "C" int skv_rotary(const SkvRotary *d, void *stream) {
     a.rot_chunks = 2 * a.pairs / v;
     a.chunks = a.dim / v;
   }
-  int sms = 0;
-  if (int rc = sm_count((int)d->device, &sms)) return rc;
   // few tokens: more threads share a token's heads (each computes its own
   // sines); many tokens: one thread per token and chunk, sines computed once
   const int total = a.heads[0] + a.heads[1];

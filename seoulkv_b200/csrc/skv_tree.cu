@@ -817,9 +817,11 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   const Plan plan((long long)s_pre[a.batch] * a.heads, groups);
   const long long g0 = (long long)s_pre[b] * a.heads + (long long)h * places;
   const int c0 = plan.owner(g0), c1 = plan.owner(g0 + places - TR_IDLE - 1);
-  if (c0 == c1) return;  // written by its one CTA
   const int shift = plan.begin(c0) < g0 ? 1 : 0;  // only its first item may hold a part of a unit before
+  // (blocks without work wait too: what follows this kernel on the stream
+  // must find the attention kernel's own rows written)
   grid_dependency_wait();
+  if (c0 == c1) return;  // written by its one CTA
   const int parts = c1 - c0 + 1, prow = r - mt * TR_ROWS;
   auto slot = [&](int i) { return (int64_t)(2 * ((c0 + i) * a.mtiles + mt) + (i == 0 ? shift : 0)) * a.rows + prow; };
   auto o_of = [&](int i) { return __ldcg(reinterpret_cast<const float4 *>(a.part + slot(i) * D) + d4); };
@@ -990,10 +992,10 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
     return op_fail(SKV_E_INVALID, "outputs must start on 16-byte boundaries");
   const int64_t *const qs = rows_of[0].stride, *const ks = rows_of[1].stride, *const vs = rows_of[2].stride,
                 *const kcs = rows_of[3].stride, *const vcs = rows_of[4].stride;
+  int sms = 0;
+  if (int rc = sm_count(d->device, &sms)) return rc;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
-  int sms = 0;
-  if (int rc = sm_count((int)d->device, &sms)) return rc;
   if (d->workspace_bytes < tree_workspace(sms, d))
     return op_fail(SKV_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
                    (long long)tree_workspace(sms, d));
@@ -1075,7 +1077,7 @@ int skv_tree_workspace(const SkvTree *d, int64_t *bytes) {
   if (!bytes) return op_fail(SKV_E_INVALID, "null result pointer");
   if (int rc = check_tree(d)) return rc;
   int sms = 0;
-  if (int rc = sm_count((int)d->device, &sms)) return rc;
+  if (int rc = sm_count(d->device, &sms)) return rc;
   *bytes = tree_workspace(sms, d);
   return SKV_OK;
 }

@@ -347,10 +347,10 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   for (int i = 0; i < 3; ++i) ok = ok && qs[i] >= 0 && qs[i] % 8 == 0 && kcs[i] >= 0 && kcs[i] % (f8 ? 16 : 8) == 0;
   if (!ok) return op_fail(SKV_E_INVALID, "rows must start on 16-byte boundaries");
   if (d->tokens > 1 && !kcs[2]) return op_fail(SKV_E_INVALID, "tokens must not share one row");
+  int sms = 0;
+  if (int rc = sm_count(d->device, &sms)) return rc;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
-  int sms = 0;
-  if (int rc = sm_count((int)d->device, &sms)) return rc;
   WeightsArgs a{};
   if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads);

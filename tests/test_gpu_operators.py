@@ -2,7 +2,10 @@
 bits with the bounds that tests/operator_reference.py derives."""
 
 import math
+import pathlib
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -342,6 +345,24 @@ def test_tree_attention_offsets_beyond_32_bits():
     assert (y[:-1] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F8])
+def test_tree_attention_units_of_one_cta_each(dtype):
+    """As many units as SMs: every row is written by the first of the two kernels, and what
+    follows the second must find it there."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    args = tree_case(16, [1000] * (sms // 2), 3, 4, 2, 128, 1000, dtype=dtype)
+    copies = []
+    for _ in range(8):
+        out, lse = skv.tree_attention(*args)
+        copies.append((out.clone(), lse.clone()))
+        out.zero_()
+    for out, lse in copies[1:]:
+        assert torch.equal(out, copies[0][0]) and torch.equal(lse, copies[0][1])
+    want, wl, eo, el = R.tree(*args)
+    close(copies[0][0], want, eo)
+    close(copies[0][1], wl, el)
+
+
 def test_tree_attention_graph_follows_the_cache():
     """A captured call replayed after lengths, queries and the cache changed; two graphs of one program."""
     args = list(tree_case(14, [50, 200], 4, 8, 2, 128, 400))
@@ -659,6 +680,56 @@ def test_draft_verify_accumulate_evict(dtype):
                 x[:, :, :keep] = y
             evictions += 1
     assert evictions
+
+
+CAPTURED = """
+import torch
+import seoulkv_b200 as skv
+
+b, n, hq, hkv, d, room, keep = 2, 6, 8, 2, 128, 700, 300
+g = torch.Generator(device="cuda").manual_seed(53)
+normal = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+q, k, v = normal(b, n, hq, d), normal(b, hkv, n, d), normal(b, hkv, n, d)
+caches = normal(b, hkv, room, d), normal(b, hkv, room, d)
+lengths = torch.tensor([690, 100], dtype=torch.int32, device="cuda")
+positions = lengths.long()[:, None] + torch.arange(n, device="cuda")
+parents = torch.tensor([[-1, 0, 0, 2, -1, 9]] * b, dtype=torch.int32, device="cuda")
+accepted = torch.ones(b, n, dtype=torch.bool, device="cuda")
+weights = torch.zeros(b, hkv, room, device="cuda")
+
+
+def step():
+    skv.rotary(q, k, positions, out=(q, k))
+    out, lse = skv.tree_attention(q, *caches, lengths, k, v, parents)
+    skv.accumulate_weights(q, caches[0], lengths, lse, weights, rows=accepted, out=weights)
+    return (out, lse, *skv.evict(*caches, weights, lengths, keep=keep, sink=4, local=16))
+
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = step()
+for turn in range(3):
+    lengths.fill_(turn * 300 + 7)
+    caches[0].mul_(0.75)
+    start = [x.clone() for x in (q, k, weights)]
+    graph.replay()
+    got = [x.clone() for x in (*captured, q, k, weights)]
+    for x, y in zip((q, k, weights), start):
+        x.copy_(y)
+    want = (*step(), q, k, weights)
+    for i, (x, y) in enumerate(zip(got, want)):
+        assert torch.equal(x.nan_to_num(nan=7.0), y.nan_to_num(nan=7.0)), (turn, i)
+skv.check_operators("cuda:0")
+"""
+
+
+def test_first_calls_captured_together():
+    """One graph of all operators, in place where they may be, as a process's first calls of them;
+    replayed with other contents it gives what eager calls give."""
+    done = subprocess.run([sys.executable, "-c", CAPTURED], capture_output=True, text=True, timeout=600,
+                          cwd=pathlib.Path(__file__).parents[1])
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 # ---------------------------------------------------------------- the engine's own cache

@@ -153,6 +153,16 @@ def test_null_descriptors_are_refused():
     assert lib.skv_run_tree(None, _tree(), None) == -1
 
 
+@pytest.mark.parametrize("device", [-1, 64, 1 << 32, (1 << 32) + 1])
+def test_devices_out_of_range_are_refused(device):
+    for name, packed in (("skv_rotary", _rotary(device=device)), ("skv_tree_attention", _tree(device=device)),
+                         ("skv_accumulate_weights", _weights(device=device)), ("skv_evict", _evict(device=device))):
+        rc, message = _refused(name, packed)
+        assert rc == -1 and "device" in message, name
+    size = ctypes.c_int64()
+    assert _native.load().skv_tree_workspace(_tree(device=device), ctypes.byref(size)) == -1
+
+
 def test_empty_batches_need_no_gpu():
     for name, packed in (("skv_rotary", _rotary(b=0)), ("skv_tree_attention", _tree(b=0)),
                          ("skv_accumulate_weights", _weights(b=0)), ("skv_evict", _evict(b=0))):
