@@ -419,7 +419,8 @@ int skv_evict(const SkvEvict *desc, void *stream);
  *   q BF16 [batch][n][heads][dim], k, v BF16 [batch][kv_heads][n][dim],
  *   k_cache, v_cache BF16 or FP8 e4m3 [batch][kv_heads][tokens][dim],
  *   out BF16 [batch][n][heads][dim] and lse FP32 [batch][n][heads] contiguous;
- *   workspace: skv_tree_workspace() bytes, not shared by calls that overlap.
+ *   workspace: skv_tree_workspace() bytes (0 for short caches, where it may be
+ *   null), not shared by calls that overlap.
  * dim is 64, 128 or 256, n at most SKV_TREE_MAX_NODES.  Rows start on 16-byte
  * boundaries.  Sequence and head strides may be 0 (a cache that all share). */
 #define SKV_TREE_MAX_NODES 64

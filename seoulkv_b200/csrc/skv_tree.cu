@@ -118,6 +118,7 @@ constexpr int TR_KEYS = 128;   // keys of a tile
 constexpr int TR_ROWS = 128;   // rows of a unit: the MMA's M
 constexpr int TR_GROUP = 64;   // threads that turn an FP8 stage into BF16
 constexpr int TR_IDLE = 1;     // what starting and ending a unit costs, in tiles
+constexpr int TR_JOIN = 5;     // what cutting units and joining their parts costs, in tiles
 
 template <int D_, bool F8_>
 struct TreeCfg {
@@ -163,6 +164,7 @@ struct TreeArgs {
   float *part;             // [slot][rows][D]
   uint64_t by_group;       // (by_inverse)
   int32_t batch, n, heads, group, t, mtiles, rows;
+  int32_t whole;           // an item is a unit, and nothing is left to join
   int32_t along[4][2];     // coordinate steps (head, sequence) of the four maps: 0 where one element stands for all
   float c2;                // scale * log2(e)
   uint32_t *status;
@@ -260,7 +262,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   // keys at the same time and HBM delivers them once
   const Plan plan((long long)s.pre[a.batch] * a.heads, (int)gridDim.x / a.mtiles);
   const int item = blockIdx.x / a.mtiles, mt = blockIdx.x % a.mtiles;
-  const Walk walk(s.pre, a.batch, a.heads, TR_IDLE, plan.begin(item), plan.begin(item + 1));
+  long long from = 0, to = 0;
+  if (a.whole) {
+    const int b = item / a.heads, places = s.pre[b + 1] - s.pre[b];
+    from = (long long)s.pre[b] * a.heads + (long long)(item - b * a.heads) * places, to = from + places;
+  } else {
+    from = plan.begin(item), to = plan.begin(item + 1);
+  }
+  const Walk walk(s.pre, a.batch, a.heads, TR_IDLE, from, to);
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
   auto length = [&](int b) {
     const int n = a.lengths ? a.lengths[b * a.len_stride] : a.context;
@@ -906,6 +915,7 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, c
   if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, false, 1, maps, a),
                        "k_tree_attention launch"))
     return rc;
+  if (a.whole) return SKV_OK;
   const unsigned rows = (unsigned)(a.batch * a.heads * a.n * a.group);
   const int items = ctas / a.mtiles;
   constexpr unsigned per = TC_THREADS / (C::D / 4);
@@ -923,6 +933,17 @@ int launch_tree_d(int d, const TreeMaps &maps, const TreeArgs &a, int ctas, int 
   return launch_tree<TreeCfg<256, F8>>(maps, a, ctas, device, st);
 }
 
+// Whether units are left whole: one CTA each, one launch and no workspace.
+// Cutting them shares their tiles among all SMs, tiles (1 - units / sms) less
+// for the longest, and costs the partials and a second kernel.  Measured (BF16,
+// a tile 1.2 us): 12 units, 128 tokens 8.7 us whole, 10.4 cut; 512, 12.3 and
+// 11.0 (and 4 us less on the host); 1152, 17.9 and 10.9.  128 units, 128
+// tokens 9.6 and 15.2; 2176, 30.7 and 35.9.
+bool tree_whole(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t t) {
+  const int64_t units = batch * heads * mtiles, tiles = (t + TR_KEYS - 1) / TR_KEYS + 1;
+  return units <= sms && tiles * (sms - units) <= TR_JOIN * sms;
+}
+
 // CTAs of a launch: one per SM, whole items (or fewer, the most places that the list can have).
 int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t t) {
   const int64_t most = batch * heads * ((t + TR_KEYS - 1) / TR_KEYS + 1 + TR_IDLE);
@@ -932,9 +953,14 @@ int64_t tree_ctas(int sms, int64_t batch, int64_t heads, int64_t mtiles, int64_t
 
 int64_t tree_workspace(int sms, const SkvTree *d) {
   const int64_t rows = d->n * (d->heads / d->kv_heads), per = rows < TR_ROWS ? rows : TR_ROWS;
-  const int64_t batch = d->batch < PLAN_BATCH ? d->batch : PLAN_BATCH;
-  const int64_t slots = 2 * tree_ctas(sms, batch, d->kv_heads, (rows + TR_ROWS - 1) / TR_ROWS, d->tokens);
-  return slots * per * (d->dim + 2) * 4;
+  const int64_t mtiles = (rows + TR_ROWS - 1) / TR_ROWS;
+  auto slots = [&](int64_t batch) {  // of a launch
+    return batch == 0 || tree_whole(sms, batch, d->kv_heads, mtiles, d->tokens)
+               ? 0
+               : 2 * tree_ctas(sms, batch, d->kv_heads, mtiles, d->tokens);
+  };
+  const int64_t full = slots(d->batch < PLAN_BATCH ? d->batch : PLAN_BATCH), last = slots(d->batch % PLAN_BATCH);
+  return (full > last ? full : last) * per * (d->dim + 2) * 4;
 }
 
 int check_tree(const SkvTree *d) {
@@ -964,9 +990,9 @@ int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
 int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
   if (int rc = check_tree(d)) return rc;
   if (d->batch == 0) return SKV_OK;
-  if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse || !d->workspace ||
+  if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse ||
       (!cells && (!d->k_cache || !d->v_cache || !d->lengths)))
-    return op_fail(SKV_E_INVALID, "null input, output or workspace pointer");
+    return op_fail(SKV_E_INVALID, "null input or output pointer");
   const bool f8 = d->cache_dtype == SKV_DTYPE_E4M3;
   const int64_t of_q[3] = {d->batch, d->n, d->heads}, of_cache[3] = {d->batch, d->kv_heads, d->tokens},
                 of_nodes[3] = {d->batch, d->kv_heads, d->n};
@@ -996,9 +1022,9 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
   if (int rc = sm_count(d->device, &sms)) return rc;
   DeviceScope scope((int)d->device);
   if (int rc = op_cuda(scope.error(), "selecting the device")) return rc;
-  if (d->workspace_bytes < tree_workspace(sms, d))
-    return op_fail(SKV_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes,
-                   (long long)tree_workspace(sms, d));
+  const int64_t scratch = tree_workspace(sms, d);
+  if (d->workspace_bytes < scratch || (scratch && !d->workspace))
+    return op_fail(SKV_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes, (long long)scratch);
   TreeArgs a{};
   if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads), rows = (int)d->n * group;
@@ -1025,7 +1051,8 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
     a.parents = static_cast<const int32_t *>(d->parents) + b0 * a.ps[0];
     a.out = static_cast<uint16_t *>(d->out) + b0 * d->n * d->heads * d->dim;
     a.lse = static_cast<float *>(d->lse) + b0 * d->n * d->heads;
-    const int ctas = (int)tree_ctas(sms, nb, a.heads, a.mtiles, d->tokens);
+    a.whole = tree_whole(sms, nb, a.heads, a.mtiles, d->tokens);
+    const int ctas = a.whole ? (int)(nb * a.heads * a.mtiles) : (int)tree_ctas(sms, nb, a.heads, a.mtiles, d->tokens);
     a.part = static_cast<float *>(d->workspace);
     a.ml = reinterpret_cast<float2 *>(a.part + 2 * (int64_t)ctas * a.rows * d->dim);
     TreeMaps maps{};

@@ -319,10 +319,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if not b:
         return out, lse
     size = _tree_workspace(dev, b, n, hq, hkv, d, t)
-    work = q.new_empty(size, dtype=torch.uint8)
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
     packed = _TREE.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), lengths.data_ptr(), k.data_ptr(), v.data_ptr(),
-        parents.data_ptr(), out.data_ptr(), lse.data_ptr(), work.data_ptr(),
+        parents.data_ptr(), out.data_ptr(), lse.data_ptr(), work.data_ptr() if size else 0,
         _ROOT[d] if scale is None else _scale(scale), dev, _DTYPE[kind], size, b, n, hq, hkv, d, t,
         *q.stride(), *k_cache.stride(), *v_cache.stride(), *k.stride(), *v.stride(), *parents.stride(), *lengths.stride())
     _run(_native.load().skv_tree_attention, packed, dev, "tree_attention")
@@ -351,10 +351,10 @@ def run_tree(engine, lead: tuple, q, k, v, parents, device: int):
     out = q.new_empty((slots, n, 16, 256))
     lse = q.new_empty((slots, n, 16), dtype=_F32)
     size = _tree_workspace(device, slots, n, 16, 4, 256, engine.max_context)
-    work = q.new_empty(size, dtype=torch.uint8)
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
     packed = _TREE.pack(
         q.data_ptr(), 0, 0, 0, k.data_ptr(), v.data_ptr(), parents.data_ptr(), out.data_ptr(), lse.data_ptr(),
-        work.data_ptr(), 0.0625, device, _DTYPE[_FP8], size, slots, n, 16, 4, 256, engine.max_context,
+        work.data_ptr() if size else 0, 0.0625, device, _DTYPE[_FP8], size, slots, n, 16, 4, 256, engine.max_context,
         *q.stride(), *(8 * (0,)), *k.stride(), *v.stride(), *parents.stride(), 0)
     rc = engine.lib.skv_run_tree(engine.handle, packed, _current_stream(device))
     if rc == -1:
@@ -365,11 +365,11 @@ def run_tree(engine, lead: tuple, q, k, v, parents, device: int):
 
 @functools.lru_cache(maxsize=1024)
 def _tree_workspace(device: int, b: int, n: int, hq: int, hkv: int, d: int, t: int) -> int:
-    """Bytes of scratch that one call needs (a function of the sizes)."""
+    """Bytes of scratch that one call needs (a function of the sizes; 0 for short caches)."""
     size = ctypes.c_int64()
     packed = _TREE.pack(*(10 * (0,)), 1.0, device, 0, 0, b, n, hq, hkv, d, t, *(23 * (0,)))
     _native.check(_native.load().skv_tree_workspace(packed, ctypes.byref(size)), "skv_tree_workspace")
-    return max(16, size.value)
+    return size.value
 
 
 # ---------------------------------------------------------------- accumulated weights

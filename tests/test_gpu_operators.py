@@ -346,11 +346,29 @@ def test_tree_attention_offsets_beyond_32_bits():
 
 
 @pytest.mark.parametrize("dtype", [BF, F8])
-def test_tree_attention_units_of_one_cta_each(dtype):
-    """As many units as SMs: every row is written by the first of the two kernels, and what
+@pytest.mark.parametrize("b,n,hkv,t", [(3, 5, 1, 511), (3, 5, 1, 513), (70, 2, 2, 900), (129, 1, 1, 800), (129, 40, 1, 700),
+                                       (148, 1, 1, 130), (149, 1, 1, 130), (9, 64, 4, 640)])
+def test_tree_attention_whole_and_cut_units(b, n, hkv, t, dtype):
+    """Both sides of the rule that leaves units whole, and launches of one call on different sides of it."""
+    rng = random.Random(t)
+    check_tree(tree_case(17, [rng.choice([0, 1, t // 2, t - 1, t]) for _ in range(b)], n, 4 * hkv, hkv, 64, t, dtype=dtype,
+                         kind="padded"))
+
+
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("lengths,n,hq,hkv,d", [([0, 1, 63, 64, 65], 1, 4, 1, 256), ([127, 128, 129, 0], 5, 6, 2, 128),
+                                                ([300, 7], 64, 4, 2, 64), ([20, 0, 70, 2600], 31, 4, 1, 256),
+                                                ([0], 64, 16, 4, 256), ([1], 1, 1, 1, 64)])
+def test_tree_attention_short_lengths_in_a_long_cache(lengths, n, hq, hkv, d, dtype):
+    check_tree(tree_case(18, lengths, n, hq, hkv, d, 2700, dtype=dtype, kind="padded"))
+
+
+@pytest.mark.parametrize("dtype", [BF, F8])
+def test_tree_attention_cut_between_units(dtype):
+    """Two units for every SM, cut where they end: every row is written by the first of the two kernels, and what
     follows the second must find it there."""
     sms = torch.cuda.get_device_properties(0).multi_processor_count
-    args = tree_case(16, [1000] * (sms // 2), 3, 4, 2, 128, 1000, dtype=dtype)
+    args = tree_case(16, [1000] * (sms // 2), 3, 8, 4, 128, 1000, dtype=dtype)
     copies = []
     for _ in range(8):
         out, lse = skv.tree_attention(*args)
