@@ -31,9 +31,9 @@ constexpr int EV_BINS = 256;
 // copies of the histogram, one per lane modulo 8: weights share exponents, so
 // a warp's counts fall on few bins and one copy would serialise them
 constexpr int EV_COPIES = 8;
-constexpr int EV_CACHED = 24576;  // keys a CTA holds in shared memory (96 KB); longer segments are read again
+constexpr int EV_CACHED = 49152;  // most keys that a CTA holds in shared memory (192 KB); longer segments are read again
 constexpr int EV_CLUSTER = 16;    // most CTAs of a row
-constexpr int EV_ROW = 8192;      // tokens of a row up to which one CTA is enough, and per CTA beyond
+constexpr int EV_ROW = 2048;      // tokens of a row up to which one CTA is enough, and per CTA beyond
 
 struct EvictArgs {
   const float *weights;
@@ -43,6 +43,7 @@ struct EvictArgs {
   int32_t *ids, *out_lengths;
   float *out_w;
   int heads, t, keep, sink, local;
+  int room;  // keys that fit into the launch's shared memory
 };
 
 struct SelectSmem {
@@ -52,8 +53,7 @@ struct SelectSmem {
   uint32_t tie[EV_WARPS];
   uint32_t found[3];   // bin, still wanted inside it, its count
   uint32_t total[2];   // this CTA's kept-above and tied counts
-  uint32_t key[EV_CACHED];
-};
+};  // (keys follow)
 
 // Larger weight, larger key; -0 equals +0, NaN is 0 (below -inf).
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
   const int warps = ranks * EV_WARPS;
   const int seg = ((n + warps - 1) / warps + 31) & ~31;
   const int begin = min(n, (rank * EV_WARPS + warp) * seg), end = min(n, begin + seg);
-  const bool cached = seg * EV_WARPS <= EV_CACHED;
-  uint32_t *mine = s.key + (cached ? warp * seg : 0);
+  const bool cached = seg * EV_WARPS <= a.room;
+  uint32_t *mine = reinterpret_cast<uint32_t *>(&s + 1) + (cached ? warp * seg : 0);
   const int lo = n <= a.keep ? n : a.sink, hi = n - a.local;  // the middle that competes: [lo, hi)
   auto key_at = [&](int i) { return cached ? mine[i - begin] : order_key(w[i * a.ws[2]]); };
   if (cached) {
@@ -316,14 +316,18 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
     rc = op_cuda(cudaFuncSetAttribute(k_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cluster size");
     if (!rc) __atomic_store_n(&wide[d->device], true, __ATOMIC_RELAXED);
   }
-  if (!rc) rc = op_shared_memory(reinterpret_cast<const void *>(&k_evict_select), (int)sizeof(SelectSmem), (int)d->device, set);
+  if (!rc) rc = op_shared_memory(reinterpret_cast<const void *>(&k_evict_select), (int)sizeof(SelectSmem) + EV_CACHED * 4, (int)d->device, set);
   if (rc) return rc;
   // CTAs of a row: as many as its length gives work to, while all rows fit on
-  // the device together (a 128K row: one CTA 60 us, sixteen 10 us)
+  // the device together.  Measured (with a gather of almost nothing), one CTA
+  // a row and up to sixteen: 4 rows of 4103 tokens 13.7 and 13.0 us, of 16384
+  // 23.0 and 15.8, of 131072 213 and 27.4.
   int ranks = 1;
   while (ranks < EV_CLUSTER && d->tokens > (int64_t)EV_ROW * ranks && d->batch * d->kv_heads * ranks * 2 <= sms) ranks *= 2;
+  const int64_t warps = (int64_t)ranks * EV_WARPS, keys = ((d->tokens + warps - 1) / warps + 31) / 32 * 32 * EV_WARPS;
+  a.room = keys <= EV_CACHED ? (int)keys : 0;
   rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
-                         sizeof(SelectSmem), st, false, (unsigned)ranks, a), "k_evict_select launch");
+                         sizeof(SelectSmem) + (size_t)a.room * 4, st, false, (unsigned)ranks, a), "k_evict_select launch");
   if (rc) return rc;
   GatherArgs g;
   g.x[0] = static_cast<const uint8_t *>(d->k), g.x[1] = static_cast<const uint8_t *>(d->v);

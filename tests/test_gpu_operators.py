@@ -609,6 +609,15 @@ def test_evict_types_rows_and_strides(dtype, d):
     check_evict(rec[..., :d], rec[..., d:], w, lengths, 20, 0, 0)
 
 
+@pytest.mark.parametrize("t", [524288, 786432, 786433, 1000003])
+def test_evict_long_rows(t):
+    """Rows of sixteen CTAs whose keys just fit into shared memory, and longer ones."""
+    g = gen(47)
+    k, v = (torch.randint(0, 120, (1, 2, t, 1), device="cuda", generator=g, dtype=torch.uint8).view(F8) for _ in range(2))
+    check_evict(k, v, torch.rand(1, 2, t, device="cuda", generator=g), torch.tensor([t - 3], dtype=torch.int32, device="cuda"),
+                t // 3, 4, 100)
+
+
 def test_evict_graph_and_offsets():
     g = gen(43)
     k, v, w = normal(g, 1, 2, 5000, 64), normal(g, 1, 2, 5000, 64), torch.rand(1, 2, 5000, device="cuda", generator=g)
