@@ -62,7 +62,10 @@ def _check(name: str, t, shape, dtypes, device: int | None = None) -> None:
 
 
 def _recorded(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    for t in tensors:
+        if t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -200,8 +203,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
         raise ValueError("layout must be 'half' or 'interleaved'")
     _, phase, m = _rotary_table(r, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor)
     if out is None:
-        qo = q.new_empty((b, n, hq, d))
-        ko = None if k is None else k.new_empty((b, hkv, n, d))
+        qo = q.new_empty(b, n, hq, d)
+        ko = None if k is None else k.new_empty(b, hkv, n, d)
     else:
         qo, ko = out
         _check_rotary_out(q, k, qo, ko, dev)
@@ -314,8 +317,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _check("k", k, node, (_BF16,), dev)
         _check("v", v, node, (_BF16,), dev)
         _check("parents", parents, (b, n), (_I32,), dev)
-    out = q.new_empty((b, n, hq, d))
-    lse = q.new_empty((b, n, hq), dtype=_F32)
+    out = q.new_empty(b, n, hq, d)
+    lse = q.new_empty(b, n, hq, dtype=_F32)
     if not b:
         return out, lse
     size = _tree_workspace(dev, b, n, hq, hkv, d, t)
@@ -348,8 +351,8 @@ def run_tree(engine, lead: tuple, q, k, v, parents, device: int):
     q, k, v, parents = (t if t.get_device() == device else t.to(f"cuda:{device}") for t in (q, k, v, parents))
     if not lead:
         k, v, parents = k[None], v[None], parents[None]
-    out = q.new_empty((slots, n, 16, 256))
-    lse = q.new_empty((slots, n, 16), dtype=_F32)
+    out = q.new_empty(slots, n, 16, 256)
+    lse = q.new_empty(slots, n, 16, dtype=_F32)
     size = _tree_workspace(device, slots, n, 16, 4, 256, engine.max_context)
     work = q.new_empty(size, dtype=torch.uint8) if size else None
     packed = _TREE.pack(
@@ -421,7 +424,7 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
                                  and rows.get_device() == dev):
         _check("rows", rows, (b, n), (torch.bool,), dev)
     if out is None:
-        out = weights.new_empty(held)
+        out = weights.new_empty(b, hkv, t)
     else:
         _check("out", out, held, (_F32,), dev)
         if any(x == 0 and size > 1 for x, size in zip(out.stride(), out.shape)):
@@ -483,11 +486,11 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, l
     if type(keep) is not int or type(sink) is not int or type(local) is not int or not 1 <= keep <= t \
             or sink < 0 or local < 0 or sink + local > keep:
         raise ValueError(f"keep must be in [1, {t}] and hold the sink and local tokens")
-    ko = k_cache.new_empty((b, h, keep, d))
+    ko = k_cache.new_empty(b, h, keep, d)
     vo = torch.empty_like(ko)
-    wo = weights.new_empty((b, h, keep))
+    wo = weights.new_empty(b, h, keep)
     ids = torch.empty_like(wo, dtype=_I32)
-    left = lengths.new_empty(b)
+    left = torch.empty_like(lengths)
     if not b:
         return ko, vo, wo, ids, left
     packed = _EVICT.pack(
