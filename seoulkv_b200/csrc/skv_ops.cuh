@@ -86,8 +86,12 @@ inline int op_shared_memory(const void *kernel, int bytes, int device, bool *set
 }
 
 // Launch; with `early` the kernel's blocks may be placed while the kernel
-// before it on the stream still runs (it calls grid_dependency_wait() before
-// it reads what that kernel wrote), which hides its launch.
+// before it on the stream still runs, which hides its launch and its prologue.
+// That holds once every block of the kernel before has called
+// grid_dependency_release() or ended; a kernel that never does (any that is
+// not of these operators) ends first.  Such a kernel's threads call
+// grid_dependency_wait() before they read or write global memory: it returns
+// when the kernel before has ended, and with it all that were before that.
 template <typename... P, typename... A>
 inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool early,
                              unsigned cluster, A &&...args) noexcept {

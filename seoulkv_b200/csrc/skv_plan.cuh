@@ -36,7 +36,7 @@ __device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stri
     const int b = b0 + lane;
     int n = 0, tiles = 0;
     if (b < batch) {
-      n = lengths ? lengths[b * stride] : context;
+      n = lengths ? __ldcg(lengths + b * stride) : context;  // (from L2: k_tree_combine reads before it waits)
       n = max(0, min(n, t));
       tiles = (n + KT - 1) / KT + extra;
     }

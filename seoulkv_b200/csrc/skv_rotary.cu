@@ -12,6 +12,11 @@
 // product with the integer position keeps the fraction of a turn modulo one
 // exactly, so there is no range reduction and the error is p * 2^-65 turns at
 // any position, negative ones included.  The top 32 bits go to sincospif.
+//
+// Measured (a copy moves 6437 GB/s): 65536 tokens, 16 + 4 heads of 256 in FP32,
+// 414 us for 2.68 GB, the copy rate: a token's sines are computed once for all
+// of its heads.  One token, or 64 x 13 drafted ones in BF16 (17 MB, 2.6 us of
+// traffic), 11.5 us a call: the host's time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -73,6 +78,8 @@ __global__ void __launch_bounds__(RT_THREADS) k_rotary(const __grid_constant__ R
   __shared__ uint64_t s_phase[RT_PAIRS];
   for (int i = threadIdx.x; i < a.pairs; i += RT_THREADS) s_phase[i] = a.phase[i];
   __syncthreads();
+  grid_dependency_wait();
+  grid_dependency_release();
   constexpr int NP = HALF ? V : (V + 1) / 2;  // pairs of one thread
   using W = Vec<T, V>;
   const int64_t items = a.tokens * a.split * a.chunks;
@@ -150,8 +157,8 @@ cudaError_t launch_rotary(const RotaryArgs &a, bool half, int sms, cudaStream_t 
   const int64_t items = a.tokens * a.split * a.chunks;
   const int64_t want = (items + RT_THREADS - 1) / RT_THREADS;
   const unsigned grid = (unsigned)(want < 16LL * sms ? want : 16LL * sms);
-  if (half) return op_launch(k_rotary<T, V, true>, dim3(grid), dim3(RT_THREADS), 0, st, false, 1, a);
-  return op_launch(k_rotary<T, V < 2 ? 2 : V, false>, dim3(grid), dim3(RT_THREADS), 0, st, false, 1, a);
+  if (half) return op_launch(k_rotary<T, V, true>, dim3(grid), dim3(RT_THREADS), 0, st, true, 1, a);
+  return op_launch(k_rotary<T, V < 2 ? 2 : V, false>, dim3(grid), dim3(RT_THREADS), 0, st, true, 1, a);
 }
 
 template <typename T>

@@ -195,13 +195,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&v)[16], uint32_t at) {
       : SKV_R8(v, 0), SKV_R8(v, 8)
       : "r"(at));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::SKV_W8(v, 0),
-      SKV_W8(v, 8), SKV_W8(v, 16), SKV_W8(v, 24), "r"(at)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::SKV_W8(

@@ -9,12 +9,20 @@
 // are FP32 (the accumulator in tensor memory).
 //
 // Both products run on tcgen05 with the rows as M = 128 lanes: S = Q K^T with
-// Q in tensor memory (loaded once per unit; from shared memory it would be
-// read again for every tile, at 192 bytes a cycle of the 128 there are) and
-// O += P V with P = exp(s - m) written back over S as BF16, rounded once (half
-// a step, 2^-9 of each weight, as the BF16 values it multiplies; the row sum
-// is taken before rounding).  K and V tiles arrive by TMA in a ring that keeps
-// 100 KB and more in flight per SM, which is what carries the HBM bandwidth.
+// Q in shared memory (64 KB at D = 256; tensor memory is full: O has 256
+// columns, two score tiles 128 each), and O += P V with P = exp(s - m) written
+// over S as BF16, rounded once (at most 2^-8 of each weight; the row sum is
+// taken before rounding).  Tiles are 128 keys: an MMA of N = 64 takes as long
+// as one of N = 128.  K and V arrive by TMA in a ring of 160 KB and more per
+// SM, which is what carries the HBM bandwidth.
+//
+// Two threads per row do the softmax, each half of a tile's columns.  The
+// scores of tile g + 1 are computed beside the softmax of tile g.  The maximum
+// moves only when it grows by more than 2^8, so that O is hardly ever scaled.
+//
+// Over an FP8 cache K goes to the tensor core as it is stored, against queries
+// split into two FP8 rows (skv_tensor.cuh); V is turned into BF16 by four
+// groups of two warps, since FP8 weights would lose the tail of a softmax.
 //
 // The tiles of all units (sequence, KV head, 128 rows) form one list that is
 // cut into equal contiguous ranges, one per CTA (one CTA per SM): ragged
@@ -22,7 +30,25 @@
 // once; of a unit cut across CTAs every CTA writes its partial (m, l, O) and
 // k_tree_combine joins them in order, so that results do not depend on timing.
 // The cut is worked out on the device from the lengths: no host wait, and a
-// captured graph follows its caches as they grow.
+// captured graph follows its caches as they grow.  (Ranges handed out as CTAs
+// become free were slower: 94 -> 99 us for the token below, 208 -> 212 for the
+// requests, since the fixed ranges already read at the copy rate.)  Short
+// caches are not cut at all (tree_whole).
+//
+// What bounds it, measured at 16 query heads on 4 KV heads of 256 (a copy
+// moves 6437 GB/s):
+//   one token, 131072 cached, BF16: 92 us, 537 MB = 91% of the copy rate (more
+//     tokens add bytes at 7.2 TB/s; starting and joining 148 partials are a
+//     fixed 14 us);
+//   64 nodes (256 rows a KV head): 162 us.  138 GFLOP would take 102 us at the
+//     1349 TFLOP/s that the clock under load sustains; the softmax of 268M
+//     scores runs beside it and is what keeps the tensor core waiting;
+//   16 requests of up to 32768, 12 nodes: 200 us, 1.08 GB = 84%;
+//   8 nodes over an FP8 cache of 131072: 84 us, 269 MB = 50% (more tokens add
+//     bytes at 4.7 TB/s: 3700 cycles a tile).  Shared memory is the nearest
+//     limit: per tile (64 KB) TMA writes 64 KB, the conversion of V reads 32
+//     and writes 64, the MMAs read 192: 2800 cycles at 128 bytes;
+//   3 ragged caches of up to 327, 5 nodes: 13 us a call, the host's time.
 #include <cuda_bf16.h>
 
 #include <mutex>
@@ -214,7 +240,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (warp == 0) {
-    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
     if (lane == 0) {
       if (!a.cell_maps) {
         tma_prefetch_map(&maps.k);
@@ -225,6 +250,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         tma_prefetch_map(&maps.vn);
       }
     }
+    grid_dependency_wait();
+    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
   } else if (warp == 1) {
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
@@ -251,6 +278,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     s.abort = 0;
     s.bad = 0;
   }
+  grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -816,11 +844,14 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   __shared__ float s_red[1][TC_THREADS / 32];
   __shared__ float4 s_o[FEW ? 1 : GROUPS][LANES];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = tid / LANES, d4 = tid % LANES;
+  grid_dependency_release();
+  // (the lengths are older than the attention kernel, which released this one
+  // after its own wait)
   if (warp == 0) tile_prefix<TR_KEYS>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
   __syncthreads();
   const int rows = a.n * a.group, all = rows * a.heads * a.batch;
   const int index = FEW ? blockIdx.x * GROUPS + group : blockIdx.x;
-  if (index >= all) return;  // (no barrier of the block below where FEW)
+  if (index >= all) return;  // (of the last block, where FEW: no barrier of the block below)
   const int r = index % rows, bh = index / rows, h = bh % a.heads, b = bh / a.heads;
   const int mt = r / TR_ROWS, places = s_pre[b + 1] - s_pre[b];
   const Plan plan((long long)s_pre[a.batch] * a.heads, groups);
@@ -912,7 +943,7 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, c
   auto *kernel = &k_tree_attention<C>;
   static bool set[64];
   if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), smem, device, set)) return rc;
-  if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, false, 1, maps, a),
+  if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, true, 1, maps, a),
                        "k_tree_attention launch"))
     return rc;
   if (a.whole) return SKV_OK;
