@@ -18,8 +18,8 @@
 // per row that the epilogue takes out again.
 //
 // What bounds it, measured at 16 query heads on 4 KV heads of 256 (a copy
-// moves 6437 GB/s): one token over 131072 cached, 44 us, 273 MB = 96%; the
-// last 32 tokens (128 rows) of four requests of up to 32768, 31.5 us, 139 MB =
+// moves 6437 GB/s): one token over 131072 cached, 43.7 us, 273 MB = 97%; the
+// last 32 tokens (128 rows) of four requests of up to 32768, 31.4 us, 139 MB =
 // 69%.  Longer caches add bytes at 6.7 TB/s, so what is left is a fixed 8 us:
 // lengths, queries and the first tile come one after the other, and the last
 // epilogue follows the last tile.
@@ -53,7 +53,7 @@ struct WeightsArgs {
   int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head; cols: rows up to 16s
   int32_t along[2];
   int32_t stages;  // pieces of the ring
-  float c2;
+  float scale;
   uint32_t *status;
 };
 
@@ -61,8 +61,8 @@ struct WeightsSmem {
   uint64_t full[WT_STAGES], empty[WT_STAGES];
   uint64_t q_ready, q_free, acc_full[2], acc_free[2], drain;
   uint32_t tmem, abort;
-  alignas(16) float lse2[2][WT_ROWS];  // log2(e) * lse, +inf for rows that do not count
-  alignas(16) float scale2[2][WT_ROWS];  // scale * log2(e), by the row's power of two over an FP8 cache
+  alignas(16) float lse[2][WT_ROWS];  // +inf for rows that do not count
+  alignas(16) float scale[2][WT_ROWS];  // over an FP8 cache: the scale, by the row's power of two
   int64_t q_at[WT_ROWS];               // element offsets of the rows in a head's queries
   int32_t len[PLAN_BATCH];
   int32_t pre[PLAN_BATCH + 1];
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
         const float l = a.lse[w.b * a.ls[0] + node * a.ls[1] + (h * a.group + g) * a.ls[2]];
         const uint8_t take = a.take ? a.take[w.b * a.ts[0] + node * a.ts[1]] : 1;
         // (-inf: a row that saw nothing)
-        s.lse2[seg & 1][et] = et < a.rows && take && l != -INFINITY ? l * 1.4426950408889634f : INFINITY;
+        s.lse[seg & 1][et] = et < a.rows && take && l != -INFINITY ? l : INFINITY;
         s.q_at[et] = node * a.qs[1] + g * a.qs[2];
       }
       asm volatile("bar.sync 2, 256;" ::: "memory");
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
       // instructions, and unrolled loads took 20000 cycles here)
       if (F8) {
         uint4 v = make_uint4(0, 0, 0, 0), ahead = v;
-        auto fetch = [&](int r) { return r < a.cols && s.lse2[seg & 1][r] != INFINITY ? __ldg(reinterpret_cast<const uint4 *>(q + s.q_at[r])) : make_uint4(0, 0, 0, 0); };
+        auto fetch = [&](int r) { return r < a.cols && s.lse[seg & 1][r] != INFINITY ? __ldg(reinterpret_cast<const uint4 *>(q + s.q_at[r])) : make_uint4(0, 0, 0, 0); };
         ahead = fetch(et / (D / 8));
 #pragma unroll 1
         for (int r = et / (D / 8); r < a.cols; r += 256 / (D / 8)) {
@@ -246,21 +246,21 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           uint8_t *to = queries + (c16 * 8 / ROW) * a.cols * ROW + r * ROW + swizzled(c16 * 8 % ROW / 16, r, ROW) * 16 + c16 % 2 * 8;
           *reinterpret_cast<uint2 *>(to) = hi;
           *reinterpret_cast<uint2 *>(to + a.cols * D) = lo;
-          if (c16 == 0) s.scale2[seg & 1][r] = a.c2 * __uint_as_float((254 - e) << 23);
+          if (c16 == 0) s.scale[seg & 1][r] = a.scale * __uint_as_float((254 - e) << 23);
         }
       } else {
         uint8_t *to = queries + (c16 / 8) * a.cols * 128;
 #pragma unroll 1
         for (int r = et / (D / 8); r < a.cols; r += 256 / (D / 8))
-          cp_async16(to + r * 128 + ((c16 % 8) ^ (r & 7)) * 16, q + s.q_at[r], s.lse2[seg & 1][r] != INFINITY);
+          cp_async16(to + r * 128 + ((c16 % 8) ^ (r & 7)) * 16, q + s.q_at[r], s.lse[seg & 1][r] != INFINITY);
         cp_async_wait();
       }
       async_fence();
       __syncwarp();
       if (lane == 0) bar_arrive(&s.q_ready);
       if (F8) asm volatile("bar.sync 2, 256;" ::: "memory");  // the rows' scales are there
-      const float4 *scale2 = reinterpret_cast<const float4 *>(s.scale2[seg & 1]);
-      const float4 *lse2 = reinterpret_cast<const float4 *>(s.lse2[seg & 1]);
+      const float4 *scale = reinterpret_cast<const float4 *>(s.scale[seg & 1]);
+      const float4 *lse = reinterpret_cast<const float4 *>(s.lse[seg & 1]);
       const float *wrow = a.w + w.b * a.ws[0] + h * a.ws[1];
       float *orow = a.out + w.b * a.os[0] + h * a.os[1];
       for (int i = 0; i < w.count; ++i, ++gt) {
@@ -278,17 +278,36 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float4 l = lse2[c / 4 + j], f = F8 ? scale2[c / 4 + j] : make_float4(a.c2, a.c2, a.c2, a.c2);
-            sum[0] += exp2_fast(fmaf(__uint_as_float(x[4 * j]), f.x, -l.x));
-            sum[1] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 1]), f.y, -l.y));
-            sum[2] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 2]), f.z, -l.z));
-            sum[3] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 3]), f.w, -l.w));
+            // (the difference first: rounded in log2 units, score and lse
+            // would each bring their own size's error into the exponent)
+            const float4 l = lse[c / 4 + j], f = F8 ? scale[c / 4 + j] : make_float4(a.scale, a.scale, a.scale, a.scale);
+            sum[0] += exp2_fast(fmaf(__uint_as_float(x[4 * j]), f.x, -l.x) * 1.4426950408889634f);
+            sum[1] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 1]), f.y, -l.y) * 1.4426950408889634f);
+            sum[2] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 2]), f.z, -l.z) * 1.4426950408889634f);
+            sum[3] += exp2_fast(fmaf(__uint_as_float(x[4 * j + 3]), f.w, -l.w) * 1.4426950408889634f);
           }
+        }
+        float add = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // a key with an infinity or a NaN: the zeros that stand for rows that
+        // do not count made NaNs with it, so they are left out one by one
+        if (__any_sync(0xffffffffu, add != add)) {
+          float again = 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < a.cols; c += 16) {
+            uint32_t x[16];
+            tmem_ld16(x, lanes + c);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float l = s.lse[seg & 1][c + j], f = F8 ? s.scale[seg & 1][c + j] : a.scale;
+              if (l != INFINITY) again += exp2_fast(fmaf(__uint_as_float(x[j]), f, -l) * 1.4426950408889634f);
+            }
+          }
+          if (add != add) add = again;
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&s.acc_free[half]);
-        float add = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (*abort) add = __uint_as_float(0x7fffffffu);
         if (on) orow[t * a.os[2]] = before + add;
       }
@@ -366,7 +385,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   const int group = (int)(d->heads / d->kv_heads);
   a.heads = (int)d->kv_heads, a.group = group, a.t = (int)d->tokens;
   a.by_group = ((1ull << 32) + group - 1) / group;
-  a.c2 = (float)(d->scale * 1.4426950408889634);
+  a.scale = (float)d->scale;
   a.len_stride = d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = qs[i], a.ls[i] = ls[i];

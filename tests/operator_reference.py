@@ -147,7 +147,8 @@ def weights(q, kc, lengths, lse, w, rows=None, scale=None):
             p = torch.exp(z - less)
             dz = _score_slack(x, keys, scale, kc.dtype == torch.float8_e4m3fn) + (z.abs() + less.abs() + 1) * 2.0 ** -21
             y[i, h, :m] += p.sum(0)
-            e[i, h, :m] += (p * torch.expm1(dz)).sum(0) + p.sum(0) * (x.shape[0] + 4) * 2.0 ** -24
+            # (a score of -inf is exact, whatever its bound: its weight is 0)
+            e[i, h, :m] += torch.where(p == 0, 0.0, p * torch.expm1(dz)).sum(0) + p.sum(0) * (x.shape[0] + 4) * 2.0 ** -24
     return y, e + y.abs() * 2.0 ** -23
 
 

@@ -512,6 +512,17 @@ def test_accumulate_weights_what_is_left_out_does_not_count(dtype):
     assert torch.equal(skv.accumulate_weights(q, kc, lengths, lse, w, rows=rows), w)
 
 
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("n,rows", [(1, [1]), (1, [0]), (3, [0, 1, 0]), (7, [1] * 7), (40, [0, 1] * 20), (40, [0] * 40)])
+def test_accumulate_weights_keys_that_are_not_finite(n, rows, dtype):
+    """Only the rows that count meet such a key, each with what exp() gives."""
+    q, kc, lengths, lse, w = weights_case(35, [300, 140], n, 8, 2, 128, 300, dtype=dtype)
+    for i, value in enumerate([NAN] if dtype is F8 else [NAN, INF, -INF]):  # (e4m3 has no infinity)
+        kc[:, :, 17 + 100 * i, 5 * i] = value
+    rows = torch.tensor([rows] * 2, device="cuda", dtype=torch.bool)
+    close(skv.accumulate_weights(q, kc, lengths, lse, w, rows=rows), *R.weights(q, kc, lengths, lse, w, rows))
+
+
 def test_accumulate_weights_sum_to_the_rows_over_the_cache():
     """With tree_attention's lse a row's weights over the cache and over its own line sum to one."""
     args = tree_case(34, [900, 300], 5, 8, 2, 128, 900, kind="chain")
