@@ -285,6 +285,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     other value marks an unused node (padding of a smaller tree): it and the
     nodes below it get zeros and an lse of -inf, and nothing sees them.
 
+    Over an FP8 cache the scores take the queries as sums of two FP8 rows: an
+    element is off by at most 2^-17 of its row's largest one, and a query with
+    an infinity gives NaN.
+
     Returns the attention output, BF16 [B, N, Hq, D], and the natural
     log-sum-exp of each row's scaled scores, FP32 [B, N, Hq].  ``scale``
     defaults to D**-0.5.  N = 1 with parent -1 is exact decode of one token.
