@@ -45,9 +45,11 @@
 //     scores runs beside it and is what keeps the tensor core waiting;
 //   16 requests of up to 32768, 12 nodes: 200 us, 1.08 GB = 84%;
 //   8 nodes over an FP8 cache of 131072: 84 us, 269 MB = 50% (more tokens add
-//     bytes at 4.7 TB/s: 3700 cycles a tile).  Shared memory is the nearest
-//     limit: per tile (64 KB) TMA writes 64 KB, the conversion of V reads 32
-//     and writes 64, the MMAs read 192: 2800 cycles at 128 bytes;
+//     bytes at 4.7 TB/s: 3700 cycles a tile).  The conversion of V takes 1900
+//     of them and its ring waits as long for the next load; without it a tile
+//     takes 3100.  The second half of the queries and the exponentials cost
+//     nothing; other ring lengths, 12 converting warps instead of 8 and stores
+//     without bank conflicts changed nothing;
 //   3 ragged caches of up to 327, 5 nodes: 13 us a call, the host's time.
 #include <cuda_bf16.h>
 
