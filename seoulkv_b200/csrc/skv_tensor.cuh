@@ -228,12 +228,15 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t x, uint32_t pick) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(bits), "r"(0x7b807b80u));
   return y;
 }
-// (nan: bits 7, 15, 23, 31 are raised where a code is not a number)
+// (nan: one of bits 7, 15, 23, 31 is raised where a code is not a number: one
+// more turns its sign bit, as the carry out of such a code may turn the next)
 __device__ __forceinline__ void e4m3_to_bf16(const uint4 &x, uint4 &lo, uint4 &hi, uint32_t &nan) {
   lo = make_uint4(e4m3_pair(x.x, 0x9180), e4m3_pair(x.x, 0xb3a2), e4m3_pair(x.y, 0x9180), e4m3_pair(x.y, 0xb3a2));
   hi = make_uint4(e4m3_pair(x.z, 0x9180), e4m3_pair(x.z, 0xb3a2), e4m3_pair(x.w, 0x9180), e4m3_pair(x.w, 0xb3a2));
-  nan |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u);
-  nan |= ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+  nan |= x.x ^ (x.x + 0x01010101u);
+  nan |= x.y ^ (x.y + 0x01010101u);
+  nan |= x.z ^ (x.z + 0x01010101u);
+  nan |= x.w ^ (x.w + 0x01010101u);
 }
 constexpr uint32_t E4M3_NAN = 0x80808080u;
 // 480 to NaN, in 16 bytes that e4m3_to_bf16 wrote.

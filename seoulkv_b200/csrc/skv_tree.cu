@@ -788,12 +788,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll 2
           for (int j = 0; j < CHUNKS; ++j) {
             uint4 x = *reinterpret_cast<const uint4 *>(from + j * D), y0, y1;
-            if (j >= left) x = make_uint4(0, 0, 0, 0);  // behind the length
             e4m3_to_bf16(x, y0, y1, nan);
             const uint32_t place = (unit & 7) ^ j;
             *reinterpret_cast<uint4 *>(at + j * 128 + place * 16) = y0;
             *reinterpret_cast<uint4 *>(at + j * 128 + (place ^ 1) * 16) = y1;
           }
+          for (int j = max(left, 0); j < CHUNKS; ++j)  // behind the length
+            for (int u = 0; u < 2; ++u) *reinterpret_cast<uint4 *>(at + j * 128 + (((unit & 7) ^ j) ^ u) * 16) = make_uint4(0, 0, 0, 0);
           if (nan & E4M3_NAN)
             for (int j = 0; j < CHUNKS; ++j)
               for (int u = 0; u < 2; ++u)
