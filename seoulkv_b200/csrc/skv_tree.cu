@@ -785,13 +785,19 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           uint8_t *at = to + (unit / 8) * C::VROWS * 128 + key * 128;
           uint32_t nan = 0;
           // (a short body: straight-line code for all pieces would wait for its instructions)
-#pragma unroll 2
-          for (int j = 0; j < CHUNKS; ++j) {
-            uint4 x = *reinterpret_cast<const uint4 *>(from + j * D), y0, y1;
-            e4m3_to_bf16(x, y0, y1, nan);
-            const uint32_t place = (unit & 7) ^ j;
-            *reinterpret_cast<uint4 *>(at + j * 128 + place * 16) = y0;
-            *reinterpret_cast<uint4 *>(at + j * 128 + (place ^ 1) * 16) = y1;
+#pragma unroll 1
+          for (int j = 0; j < CHUNKS; j += 2) {
+            // (an odd key has its two units the other way round)
+            uint8_t *y0 = at + j * 128 + ((unit & 7) ^ j) * 16, *y1 = at + j * 128 + ((unit & 7) ^ j ^ 1) * 16;
+            const uint4 x0 = *reinterpret_cast<const uint4 *>(from + j * D);
+            const uint4 x1 = *reinterpret_cast<const uint4 *>(from + j * D + D);
+            uint4 lo, hi;
+            e4m3_to_bf16(x0, lo, hi, nan);
+            *reinterpret_cast<uint4 *>(y0) = lo;
+            *reinterpret_cast<uint4 *>(y1) = hi;
+            e4m3_to_bf16(x1, lo, hi, nan);
+            *reinterpret_cast<uint4 *>(y1 + 128) = lo;
+            *reinterpret_cast<uint4 *>(y0 + 128) = hi;
           }
           for (int j = max(left, 0); j < CHUNKS; ++j)  // behind the length
             for (int u = 0; u < 2; ++u) *reinterpret_cast<uint4 *>(at + j * 128 + (((unit & 7) ^ j) ^ u) * 16) = make_uint4(0, 0, 0, 0);
