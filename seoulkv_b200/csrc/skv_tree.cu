@@ -44,10 +44,10 @@
 //     1349 TFLOP/s that the clock under load sustains; the softmax of 268M
 //     scores runs beside it and is what keeps the tensor core waiting;
 //   16 requests of up to 32768, 12 nodes: 200 us, 1.08 GB = 84%;
-//   8 nodes over an FP8 cache of 131072: 84 us, 269 MB = 50% (more tokens add
-//     bytes at 4.7 TB/s: 3700 cycles a tile).  The conversion of V takes 1900
-//     of them and its ring waits as long for the next load; without it a tile
-//     takes 3100.  The second half of the queries and the exponentials cost
+//   8 nodes over an FP8 cache of 131072: 82 us, 269 MB = 51% (more tokens add
+//     bytes at 4.8 TB/s).  The integer operations of V's conversion bound it:
+//     every one less per piece shows, and without the conversion a tile takes
+//     a sixth less.  The second half of the queries and the exponentials cost
 //     nothing; other ring lengths, 12 converting warps instead of 8 and stores
 //     without bank conflicts changed nothing;
 //   3 ragged caches of up to 327, 5 nodes: 13 us a call, the host's time.
