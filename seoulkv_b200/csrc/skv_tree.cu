@@ -56,6 +56,7 @@
 #include <mutex>
 
 #include "skv_device.cuh"
+#include "skv_exchange.cuh"
 #include "skv_ops.cuh"
 #include "skv_plan.cuh"
 #include "skv_tensor.cuh"
@@ -207,7 +208,7 @@ struct TreeSmem {
   uint64_t q_ready, s_full[2], p_ready[2], o_done[2], drain;
   uint64_t anc[TR_NODES];      // nodes that node i sees (0: unused)
   unsigned long long bad;      // nodes with a value that is not finite
-  float share[2][TR_ROWS];     // maxima and sums that the two threads of a row exchange
+  float share[2][TR_ROWS];     // maxima and sums that the two threads of a row exchange (exchange_slot)
   int8_t up[TR_NODES];         // the node before (-1: the cache, -2: none, unused)
   uint32_t tmem;
   uint32_t abort;
@@ -593,9 +594,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
               maximum(c);
             }
           }
-          s.share[half][row] = top;
+          s.share[exchange_slot(half, gt + i)][row] = top;
           asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-          top = fmaxf(top, s.share[half ^ 1][row]) * c2;
+          top = fmaxf(top, s.share[exchange_slot(half ^ 1, gt + i)][row]) * c2;
           // the maximum moves only when it grows by more than 2^8: until then
           // weights up to 2^8 lose nothing in FP32 sums and BF16 products,
           // and the accumulator stays where it is
@@ -701,9 +702,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       }
       const bool direct = n == cur.tiles;
       if (warp_on) {
-        s.share[half][row] = l;
+        // (the next write to either slot is behind the barrier that ends the segment)
+        s.share[exchange_slot(half, gt + n)][row] = l;
         asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-        l = s.share[0][row] + s.share[1][row];
+        const int first = exchange_slot(0, gt + n);
+        l = s.share[first][row] + s.share[first ^ 1][row];
         if (*abort) l = __uint_as_float(0x7fffffffu);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         const int64_t out_row = ((int64_t)cur.b * a.n + node) * (a.heads * a.group) + h * a.group + qg;

@@ -1,0 +1,42 @@
+"""Operators around a decode step on the B200: orders of execution, reports and
+arguments beside those of tests/test_gpu_operators.py, against the same 64-bit
+definitions and bounds."""
+
+import math
+
+import pytest
+import torch
+
+import seoulkv_b200 as skv
+from tests import operator_reference as R
+from tests.test_gpu_operators import BF, F8, INF, NAN, close, drafted, gen, grown, normal, records, tree_case  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_wait_gave_up(cuda):
+    yield
+    skv.check_operators(cuda)
+
+
+# ---------------------------------------------------------------- tree attention
+
+
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("n", [1, 9, 32])
+def test_tree_attention_maxima_of_the_two_halves_of_a_row(n, dtype):
+    """Scores of hundreds whose maximum changes sides of a tile from tile to
+    tile: both threads of a row need the same one, at every tile, every time."""
+    args = list(tree_case(71, [3000, 1500], n, 16, 4, 256, 3000, dtype=dtype, sharp=8.0))
+    t = torch.arange(3000, device="cuda")
+    # keys of one half of a tile outweigh the other's, tile by tile in turn, and grow along the cache
+    size = torch.where((t // 64 + t // 128) % 2 == 0, 1.0, 0.1) * (0.2 + t / 3000)
+    args[1] = (args[1].float() * size[:, None]).to(dtype)
+    out, lse = skv.tree_attention(*args)
+    want, wl, eo, el = R.tree(*args)
+    close(out, want, eo)
+    close(lse, wl, el)
+    for _ in range(20):
+        again = skv.tree_attention(*args)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
