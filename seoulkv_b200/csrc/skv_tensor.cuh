@@ -77,6 +77,17 @@ __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
+// By the elected lane, before it loads with a map in global memory: what the
+// host wrote there is what the load sees.  (A map that an earlier launch used
+// at the same address may still be held by the SM.  Maps that are kernel
+// parameters need none of this.)
+__device__ __forceinline__ void tma_acquire_map(uint32_t one, const CUtensorMap *map) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "@q fence.proxy.tensormap::generic.acquire.sys [%0], 128;\n\t}" ::"l"(map),
+      "r"(one)
+      : "memory");
+}
 // The elected lane announces `bytes` on `bar` and loads the box at (row,
 // piece, y, z) of a make_map() map.
 __device__ __forceinline__ void tma_load(uint32_t one, void *dst, const CUtensorMap *map, int row, int piece, int y,

@@ -315,6 +315,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     uint32_t seq = 0, seq8 = 0;  // stages of the ring (or V stages before conversion), FP8 K stages
     bool ok = true;
     while (ok && w.next()) {
+      const CUtensorMap *cell = C::F8 && a.cell_maps ? a.cell_maps + 2 * ((int64_t)w.b * a.heads + w.unit) : nullptr;
+      if (cell) {
+        tma_acquire_map(one, cell);
+        tma_acquire_map(one, cell + 1);
+      }
       for (int p = 0; ok && p < 2 * w.count; ++p) {
         bool is_v;
         int i;
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const bool nodes = w.tile + i == w.tiles - 1;
         const int which = (nodes ? 2 : 0) + (is_v ? 1 : 0);
         const CUtensorMap *map = nodes ? (is_v ? &maps.vn : &maps.kn) : (is_v ? &maps.v : &maps.k);
-        if (C::F8 && a.cell_maps) map = a.cell_maps + 2 * ((int64_t)w.b * a.heads + w.unit) + is_v;
+        if (cell) map = cell + is_v;
         const int row = nodes ? 0 : (w.tile + i) * KT;
         const int y = w.unit * a.along[which][0], z = w.b * a.along[which][1];
         if constexpr (C::F8) {

@@ -40,3 +40,33 @@ def test_tree_attention_maxima_of_the_two_halves_of_a_row(n, dtype):
     for _ in range(20):
         again = skv.tree_attention(*args)
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+# ---------------------------------------------------------------- the engine's own cache
+
+
+def _tree_over_records(q, k, v, parents, ac, values, t):
+    kc = torch.stack([ac.k_full[g][:t] for g in range(4)]).to(F8).cuda()
+    n = torch.tensor([t], dtype=torch.int32, device="cuda")
+    return R.tree(q, kc[None], values.to(F8).cuda()[None], n, k, v, parents)
+
+
+def test_run_tree_of_engines_that_follow_one_another(grown, cuda):  # noqa: F811
+    """Engines with other records in turn in one process: each one's tensor maps
+    and records may lie where a closed one's lay, and each call sees its own."""
+    q, k, v, parents = drafted(72, 1, 7)
+    t = grown.context
+    outs = []
+    for turn in range(4):
+        values = torch.roll(grown.v, 1000 * turn + 1, 1) * (1.0 + turn)
+        room = t if turn % 2 else grown.total
+        with skv.SeoulKV4(device=cuda, k=grown.k, v=values, index=grown.index,
+                          config=skv.SeoulKV4Config(max_context=room)) as attn:
+            out, lse = attn.run_tree(q, k[0], v[0], parents[0])
+            want, wl, eo, el = _tree_over_records(q, k, v, parents, grown, values, t)
+            close(out, want, eo)
+            close(lse, wl, el)
+            again = attn.run_tree(q, k[0], v[0], parents[0])
+            assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+            outs.append(out)
+    assert all(not torch.equal(outs[0], x) for x in outs[1:])

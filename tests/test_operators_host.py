@@ -66,3 +66,19 @@ def test_row_exchange_is_the_kernels():
     text = (CSRC / "skv_tree.cu").read_text()
     assert text.count("s.share[") == 5
     assert text.count("s.share[exchange_slot(") == 3 and "s.share[first][row] + s.share[first ^ 1][row]" in text
+
+
+# ---------------------------------------------------------------- tensor maps in global memory
+
+
+def test_maps_in_global_memory_are_acquired_before_their_first_load():
+    """The loader takes a cell's map pair from global memory in one place, and
+    acquires both there, before the segment's loop of loads."""
+    text = (CSRC / "skv_tree.cu").read_text()
+    kernel = text[text.index("k_tree_attention("):text.index("k_tree_combine(")]
+    take = kernel.index("a.cell_maps + ")
+    assert kernel.count("a.cell_maps + ") == 1
+    loop = kernel.index("p < 2 * w.count", take)
+    assert kernel[take:loop].count("tma_acquire_map(one, cell") == 2
+    tensor = (CSRC / "skv_tensor.cuh").read_text()
+    assert "fence.proxy.tensormap::generic.acquire.sys" in tensor
