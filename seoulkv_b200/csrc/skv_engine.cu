@@ -18,6 +18,7 @@
 #include "skv_device.cuh"
 #include "skv_fused.cuh"
 #include "skv_kernels.cuh"
+#include "skv_ops.cuh"
 #include "skv_shard.cuh"
 #include "skv_tree.cuh"
 
@@ -843,6 +844,9 @@ int skv_run_tree(void *handle, const SkvTree *desc, void *stream) {
   d.cache_dtype = SKV_DTYPE_E4M3;
   d.batch = e->desc.n_slots;
   d.heads = 16, d.kv_heads = G, d.dim = D, d.tokens = e->tmax;
+  // (a null stream is the current device's: the engine's, also for the event below)
+  DeviceScope scope(e->desc.device);
+  CK(scope.error());
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((rc = tree_attention(&d, e->record_maps, e->tlen, 0, st))) return rc;
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;

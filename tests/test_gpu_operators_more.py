@@ -70,3 +70,16 @@ def test_run_tree_of_engines_that_follow_one_another(grown, cuda):  # noqa: F811
             assert torch.equal(again[0], out) and torch.equal(again[1], lse)
             outs.append(out)
     assert all(not torch.equal(outs[0], x) for x in outs[1:])
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs 2+ GPUs")
+def test_run_tree_on_another_device_than_the_current_one(grown):  # noqa: F811
+    q, k, v, parents = drafted(73, 1, 5)
+    with skv.SeoulKV4(device="cuda:1", k=grown.k, v=grown.v, index=grown.index) as attn:
+        attn.run(grown.query(grown.context, seed=3)).to_torch()
+        torch.cuda.set_device(0)
+        out, lse = attn.run_tree(q, k[0], v[0], parents[0])
+        assert out.get_device() == 1 and torch.cuda.current_device() == 0
+        want, wl, eo, el = _tree_over_records(q, k, v, parents, grown, grown.v, grown.context)
+        close(out.cuda(0), want, eo)
+        close(lse.cuda(0), wl, el)

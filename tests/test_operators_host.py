@@ -82,3 +82,15 @@ def test_maps_in_global_memory_are_acquired_before_their_first_load():
     assert kernel[take:loop].count("tma_acquire_map(one, cell") == 2
     tensor = (CSRC / "skv_tensor.cuh").read_text()
     assert "fence.proxy.tensormap::generic.acquire.sys" in tensor
+
+
+# ---------------------------------------------------------------- the engine's device
+
+
+def test_run_tree_selects_the_engines_device_before_it_touches_the_stream():
+    """(The null stream and an event record belong to the device that is current.)"""
+    text = (CSRC / "skv_engine.cu").read_text()
+    body = text[text.index("int skv_run_tree("):]
+    body = body[:body.index("\n}\n")]
+    scope = body.index("DeviceScope scope(e->desc.device)")
+    assert all(body.index(x) > scope for x in ("tree_attention(", "cudaStreamIsCapturing(", "cudaEventRecord("))
