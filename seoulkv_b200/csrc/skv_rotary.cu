@@ -8,10 +8,12 @@
 // and dimensions R.. are copied.  One read and one write of q and k.
 //
 // The angle.  p * f_i in FP32 is useless far out (at p = 2^20 it is off by
-// 2^-4 rad).  f_i / 2 pi arrives as a 64-bit fraction of a turn; the 64-bit
-// product with the integer position keeps the fraction of a turn modulo one
-// exactly, so there is no range reduction and the error is p * 2^-65 turns at
-// any position, negative ones included.  The top 32 bits go to sincospif.
+// 2^-4 rad).  f_i / 2 pi arrives as a 64-bit fraction of a turn, rounded once
+// from more digits; the 64-bit product with the integer position keeps the
+// fraction of a turn modulo one exactly, so there is no range reduction and the
+// error is p * 2^-65 turns, negative positions included: below the rounding to
+// FP32 that follows (2^-26 turns) up to p = 2^39.  The top 32 bits go to
+// sincospif.
 //
 // Measured (a copy moves 6437 GB/s): 65536 tokens, 16 + 4 heads of 256 in FP32,
 // 414 us for 2.68 GB, the copy rate: a token's sines are computed once for all

@@ -24,6 +24,7 @@ gradients are recorded.
 from __future__ import annotations
 
 import ctypes
+import decimal
 import functools
 import math
 import struct
@@ -104,6 +105,20 @@ def check_operators(device) -> None:
 # ---------------------------------------------------------------- rotary positions
 
 
+def _pi(digits: int) -> decimal.Decimal:
+    """pi = 16 atan(1/5) - 4 atan(1/239) (Machin), in integers of 10^-(digits + 10)."""
+    one = 10 ** (digits + 10)
+
+    def atan_inverse(n):
+        term, total, i = one // n, 0, 0
+        while term:
+            total += (-1) ** i * (term // (2 * i + 1))
+            term, i = term // (n * n), i + 1
+        return total
+
+    return decimal.Decimal(16 * atan_inverse(5) - 4 * atan_inverse(239)).scaleb(-digits - 10)
+
+
 @functools.lru_cache(maxsize=64)
 def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
     """(turns per position * 2^64 of each pair as packed uint64, its address, factor on the rotated part)."""
@@ -115,14 +130,9 @@ def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fas
     if scaling not in ("none", "linear", "ntk", "yarn"):
         raise ValueError("scaling must be 'none', 'linear', 'ntk' or 'yarn'")
     pairs, r = rotary_dim // 2, float(rotary_dim)
-    base = theta
-    if scaling == "ntk" and rotary_dim > 2:
-        base = theta * factor ** (r / (r - 2.0))
-    freq = [base ** (-2.0 * i / r) for i in range(pairs)]
+    low = high = 0
     m = 1.0
-    if scaling == "linear":
-        freq = [f / factor for f in freq]
-    elif scaling == "yarn":
+    if scaling == "yarn":
         if original_context is None or original_context < 1:
             raise ValueError("yarn scaling needs original_context >= 1")
         if not beta_fast > beta_slow > 0.0:
@@ -133,15 +143,31 @@ def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fas
 
         low = max(math.floor(pair_of(beta_fast)), 0)
         high = min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
-        for i in range(pairs):
-            part = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
-            freq[i] = freq[i] * (1.0 - part) + freq[i] / factor * part
         m = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
     if attention_factor is not None:
         m = float(attention_factor)
     if not math.isfinite(m):
         raise ValueError("attention_factor must be finite")
-    turns = [int(round(f / (2.0 * math.pi) * 2.0 ** 64)) & (2 ** 64 - 1) for f in freq]
+    # The fractions need 64 places behind the point, which is more than a
+    # double has: 60 decimal digits, and as many more as the frequencies may
+    # have before the point.
+    with decimal.localcontext() as context:
+        context.prec = digits = 60 + math.ceil(3 * (abs(math.log10(theta)) + abs(math.log10(factor))))
+        base, stretch = decimal.Decimal(theta), decimal.Decimal(factor)
+        if scaling == "ntk" and rotary_dim > 2:
+            base *= stretch ** (decimal.Decimal(rotary_dim) / (rotary_dim - 2))
+        step = base ** (decimal.Decimal(-2) / rotary_dim)
+        places, f = 2 ** 64 / (2 * _pi(digits)), decimal.Decimal(1)
+        turns = []
+        for i in range(pairs):
+            x = f
+            if scaling == "linear":
+                x = f / stretch
+            elif scaling == "yarn":
+                part = min(1, max(0, (i - low) / max(decimal.Decimal(high - low), decimal.Decimal(1e-3))))
+                x = f * (1 - part) + f / stretch * part
+            turns.append(int((x * places).to_integral_value()) & (2 ** 64 - 1))
+            f *= step
     table = ctypes.create_string_buffer(struct.pack(f"{pairs}Q", *turns))
     return table, ctypes.addressof(table), m
 
@@ -156,9 +182,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
     """Rotary positions on queries [B, N, Hq, D] and keys [B, Hkv, N, D] (or None).
 
     BF16, FP16 or FP32, both alike, on one device.  ``positions`` int32 or
-    int64, [N] or [B, N]; angles are exact to an FP32 rounding at any position
-    (2^-65 turns each), negative ones turn back (the inverse rotation, and the
-    gradient's, for a factor of 1).  The first ``rotary_dim`` (even, at most
+    int64, [N] or [B, N]; the angle of position p is off by p * 2^-65 turns,
+    which is less than its FP32 rounding up to 2^39; negative positions turn
+    back (the inverse rotation, and the gradient's, for a factor of 1).  The first ``rotary_dim`` (even, at most
     512; all of D by default) dimensions turn, the others are copied.
     ``layout``: "half" pairs dimension i with i + rotary_dim/2,
     "interleaved" 2i with 2i + 1.

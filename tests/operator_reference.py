@@ -161,3 +161,26 @@ def kept(w, n, keep, sink, local):
     # NaN below every number; equal weights (0 and -0 alike): the lowest index first
     best = sorted(middle, key=lambda i: (w[i] != w[i], -w[i] if w[i] == w[i] else 0.0, i))[:keep - sink - local]
     return list(range(sink)) + sorted(best) + list(range(n - local, n))
+
+
+def exact_turns(r, positions, theta=10000.0, factor=1.0, scaling="none"):
+    """The fraction of a turn in [0, 1) of every (position, pair), as Decimal from
+    60 digits (scaling: "none", "linear" or "ntk"): position * theta^(-2i/r) / (2 pi) modulo 1."""
+    from decimal import Decimal, localcontext
+
+    with localcontext() as c:
+        c.prec = 60
+        # pi = 48 atan(1/18) + 32 atan(1/57) - 20 atan(1/239)  (Gauss)
+        def atan(x):
+            total, power, i = Decimal(0), Decimal(1) / x, 0
+            while abs(power) > Decimal(10) ** -62:
+                total += power / (2 * i + 1) * (-1) ** i
+                power, i = power / (x * x), i + 1
+            return total
+
+        turn = 2 * (48 * atan(18) + 32 * atan(57) - 20 * atan(239))
+        base = Decimal(theta)
+        if scaling == "ntk":
+            base *= (Decimal(factor).ln() * r / (r - 2)).exp()
+        f = [(base.ln() * (-2 * i) / r).exp() / (Decimal(factor) if scaling == "linear" else 1) for i in range(r // 2)]
+        return [[(p * x / turn) % 1 for x in f] for p in positions]

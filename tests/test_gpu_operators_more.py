@@ -83,3 +83,30 @@ def test_run_tree_on_another_device_than_the_current_one(grown):  # noqa: F811
         want, wl, eo, el = _tree_over_records(q, k, v, parents, grown, grown.v, grown.context)
         close(out.cuda(0), want, eo)
         close(lse.cuda(0), wl, el)
+
+
+# ---------------------------------------------------------------- rotary
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("linear", 6.5), ("ntk", 4.0)])
+def test_rotary_values_at_far_positions(scaling, factor, layout):
+    """Rotated values against angles of 60 digits, also where positions differ
+    above bit 31 alone.  Beside R.rotated()'s bound: a position p is off by
+    p 2^-65 turns, p 2^-65 2 pi of |a| + |b|."""
+    r, g = 64, gen(74)
+    positions = [7, 2 ** 24 + 1, 2 ** 31 + 5, 5, 2 ** 32 + 7, 2 ** 33 + 7, 2 ** 33 + 8, 2 ** 39 - 1, -7, -(2 ** 32) - 7, -(2 ** 38) - 3]
+    q = normal(g, 1, len(positions), 3, 96, dtype=torch.float32)
+    pos = torch.tensor(positions, device="cuda")
+    y, _ = skv.rotary(q, None, pos, rotary_dim=r, layout=layout, scaling=scaling, factor=factor)
+    turns = [[float(x) for x in row] for row in R.exact_turns(r, positions, 1e4, factor, scaling)]
+    ang = 2 * math.pi * torch.tensor(turns, dtype=torch.float64, device="cuda")[None, :, None]
+    ia = torch.arange(r // 2, device="cuda") * (1 if layout == "half" else 2)
+    ib = ia + (r // 2 if layout == "half" else 1)
+    x = q.double()
+    u, w = x[..., ia], x[..., ib]
+    size = u.abs() + w.abs()
+    bound = size * (2.0 ** -20 + 2.0 ** -64 * math.pi * pos.abs()[None, :, None, None]) + 2.0 ** -120
+    assert ((y[..., ia].double() - (u * ang.cos() - w * ang.sin())).abs() <= bound).all()
+    assert ((y[..., ib].double() - (u * ang.sin() + w * ang.cos())).abs() <= bound).all()
+    assert torch.equal(y[..., r:], q[..., r:])

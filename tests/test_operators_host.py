@@ -2,10 +2,14 @@
 accesses to shared memory, tables, refusals and reports."""
 
 import shutil
+import struct
 import subprocess
 from pathlib import Path
 
 import pytest
+
+from seoulkv_b200 import operators
+from tests import operator_reference as R
 
 CSRC = Path(__file__).resolve().parent.parent / "seoulkv_b200" / "csrc"
 
@@ -94,3 +98,21 @@ def test_run_tree_selects_the_engines_device_before_it_touches_the_stream():
     body = body[:body.index("\n}\n")]
     scope = body.index("DeviceScope scope(e->desc.device)")
     assert all(body.index(x) > scope for x in ("tree_attention(", "cudaStreamIsCapturing(", "cudaEventRecord("))
+
+
+# ---------------------------------------------------------------- rotary frequencies
+
+
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("linear", 6.5), ("ntk", 4.0)])
+@pytest.mark.parametrize("r,theta", [(64, 1e4), (128, 5e5), (256, 1e4), (2, 3.7)])
+def test_rotary_fractions_are_right_to_their_last_place(r, theta, scaling, factor):
+    """The 64-bit fractions of a turn per position, against 60 digits: the
+    rounding to 2^-64 is all that they may be off by (half a unit)."""
+    if scaling == "ntk" and r == 2:
+        pytest.skip("one pair alone has no slowest pair to divide")
+    buf, _, _ = operators._rotary_table(r, theta, scaling, factor, None, 32.0, 1.0, None)
+    got = struct.unpack(f"{r // 2}Q", buf.raw[:4 * r])
+    want = R.exact_turns(r, [1], theta, factor, scaling)[0]
+    for i, (a, b) in enumerate(zip(got, want)):
+        off = abs(a - b * 2 ** 64)
+        assert min(off, 2 ** 64 - off) <= 0.5000001, (i, float(off))
