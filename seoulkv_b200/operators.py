@@ -119,7 +119,23 @@ def _pi(digits: int) -> decimal.Decimal:
     return decimal.Decimal(16 * atan_inverse(5) - 4 * atan_inverse(239)).scaleb(-digits - 10)
 
 
-@functools.lru_cache(maxsize=64)
+def _by_value(table):
+    """Caches a table of a few numbers by their values: an argument that is an
+    object (a tensor) would be found again after its value has changed."""
+    cached = functools.lru_cache(maxsize=64)(table)
+
+    def number(x):
+        return x if x is None or type(x) is float else float(x)
+
+    @functools.wraps(table)
+    def call(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
+        return cached(rotary_dim, number(theta), scaling, number(factor), number(original_context), number(beta_fast),
+                      number(beta_slow), number(attention_factor))
+
+    return call
+
+
+@_by_value
 def _rotary_table(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
     """(turns per position * 2^64 of each pair as packed uint64, its address, factor on the rotated part)."""
     theta, factor, beta_fast, beta_slow = (float(x) for x in (theta, factor, beta_fast, beta_slow))

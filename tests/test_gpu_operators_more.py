@@ -110,3 +110,14 @@ def test_rotary_values_at_far_positions(scaling, factor, layout):
     assert ((y[..., ia].double() - (u * ang.cos() - w * ang.sin())).abs() <= bound).all()
     assert ((y[..., ib].double() - (u * ang.sin() + w * ang.cos())).abs() <= bound).all()
     assert torch.equal(y[..., r:], q[..., r:])
+
+
+def test_rotary_follows_the_value_of_its_settings():
+    """A setting given as a tensor counts by its value at the call, not as the object that an earlier call had."""
+    q, pos = normal(gen(81), 1, 5, 2, 64, dtype=torch.float32), torch.arange(5, device="cuda") + 9
+    theta, factor = torch.tensor(1e4), torch.tensor(2.0)
+    skv.rotary(q, None, pos, theta=theta, scaling="linear", factor=factor)
+    theta.fill_(5e5)
+    factor.fill_(4.0)
+    got = skv.rotary(q, None, pos, theta=theta, scaling="linear", factor=factor)[0]
+    assert torch.equal(got, skv.rotary(q, None, pos, theta=5e5, scaling="linear", factor=4.0)[0])

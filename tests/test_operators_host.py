@@ -7,6 +7,7 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
 from seoulkv_b200 import operators
 from tests import operator_reference as R
@@ -116,3 +117,21 @@ def test_rotary_fractions_are_right_to_their_last_place(r, theta, scaling, facto
     for i, (a, b) in enumerate(zip(got, want)):
         off = abs(a - b * 2 ** 64)
         assert min(off, 2 ** 64 - off) <= 0.5000001, (i, float(off))
+
+
+def test_rotary_table_goes_by_the_values_of_its_settings():
+    """A setting that is a tensor may change in place between two calls."""
+    theta, factor = torch.tensor(1e4), torch.tensor(2.0)
+
+    def fractions(*a):
+        return operators._rotary_table(64, *a, 8192, 32.0, 1.0, None)[0].raw
+
+    first = fractions(theta, "linear", factor)
+    assert first == fractions(1e4, "linear", 2)
+    theta.fill_(5e5)
+    factor.fill_(4.0)
+    assert fractions(theta, "linear", factor) == fractions(5e5, "linear", 4.0) != first
+    context = torch.tensor(4096)
+    first = operators._rotary_table(64, 1e4, "yarn", 4.0, context, 32.0, 1.0, None)[0].raw
+    context.fill_(8192)
+    assert operators._rotary_table(64, 1e4, "yarn", 4.0, context, 32.0, 1.0, None)[0].raw != first
