@@ -913,13 +913,12 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
     const float w = exp2_fast(ml.x - base);
     dead = dead || ml.y < 0.0f;
     l += w * ml.y;
-    // (a part without a visible key has weight 0 and zeros or, for an unused row, anything)
-    if (w != 0.0f) {
-      o.x = fmaf(w, v.x, o.x);
-      o.y = fmaf(w, v.y, o.y);
-      o.z = fmaf(w, v.z, o.z);
-      o.w = fmaf(w, v.w, o.w);
-    }
+    // (also where w is 0: a value that is not finite counts however small its
+    // weight is, as it does inside a part; an unused row's sums are not used)
+    o.x = fmaf(w, v.x, o.x);
+    o.y = fmaf(w, v.y, o.y);
+    o.z = fmaf(w, v.z, o.z);
+    o.w = fmaf(w, v.w, o.w);
   };
 #pragma unroll
   for (int k = 0; k < TC_BATCH; ++k)

@@ -42,6 +42,28 @@ def test_tree_attention_maxima_of_the_two_halves_of_a_row(n, dtype):
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
 
 
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("poison", [NAN, INF, -INF])
+def test_tree_attention_value_that_is_not_finite_in_a_part_of_no_weight(poison, dtype):
+    """A visible value that is not finite reaches the output however small its
+    weight is, also where the part of the cache that holds it was another CTA's:
+    scores of -128 against 0 leave it a weight below FP32's smallest number."""
+    if dtype is F8 and poison == poison:
+        pytest.skip("e4m3 has no infinity")
+    g, t, d = gen(75), 40000, 64
+    q = torch.full((1, 1, 2, d), 4.0, device="cuda", dtype=BF)
+    kc = torch.zeros(1, 1, t, d, device="cuda", dtype=BF)
+    kc[:, :, :600] = -4.0  # 4 * 4 * 64 / 8 = 128
+    vc = normal(g, 1, 1, t, d)
+    vc[0, 0, 10, 5] = poison
+    k, v = torch.zeros(1, 1, 1, d, device="cuda", dtype=BF), normal(g, 1, 1, 1, d)
+    one = torch.full((1, 1), -1, dtype=torch.int32, device="cuda")
+    out, lse = skv.tree_attention(q, kc.to(dtype), vc.to(dtype), torch.tensor([t], dtype=torch.int32, device="cuda"), k, v, one)
+    assert not torch.isfinite(out[..., 5]).any()
+    rest = [x for x in range(d) if x != 5]
+    assert torch.isfinite(out[..., rest]).all() and torch.isfinite(lse).all()
+
+
 # ---------------------------------------------------------------- the engine's own cache
 
 
