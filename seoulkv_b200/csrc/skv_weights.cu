@@ -50,7 +50,7 @@ struct WeightsArgs {
   float *out;
   int64_t ws[3], os[3];  // (sequence, head, token)
   uint64_t by_group;  // (by_inverse)
-  int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head; cols: rows up to 16s
+  int32_t batch, heads, group, t, row0, rows, cols;  // rows [row0, row0 + rows) of a head, counted from q's node; cols: rows up to 16s
   int32_t along[2];
   int32_t stages;  // pieces of the ring
   float scale;
@@ -352,9 +352,10 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   using namespace skv;
   if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
   if (d->dim != 64 && d->dim != 128 && d->dim != 256) return op_fail(SKV_E_INVALID, "head size must be 64, 128 or 256");
-  if (d->batch < 0 || d->n < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096 ||
-      d->n * (d->heads / d->kv_heads) > (1 << 17) || d->batch > (1 << 20))
-    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, counts in range");
+  if (d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096)
+    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, and at most 4096");
+  if (d->batch < 0 || d->batch > (1 << 20) || d->n < 1 || d->n > INT32_MAX)
+    return op_fail(SKV_E_INVALID, "batch must be in [0, 2^20], n in [1, 2^31)");
   if (d->tokens < 1 || d->tokens > (1 << 26)) return op_fail(SKV_E_INVALID, "tokens must be in [1, 2^26]");
   if (!(d->scale > 0.0) || !(d->scale < 1e30)) return op_fail(SKV_E_INVALID, "scale must be positive and finite");
   if (d->cache_dtype != SKV_DTYPE_BF16 && d->cache_dtype != SKV_DTYPE_E4M3)
@@ -397,10 +398,7 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
   for (int64_t b0 = 0; b0 < d->batch; b0 += PLAN_BATCH) {
     const int64_t nb = d->batch - b0 < PLAN_BATCH ? d->batch - b0 : PLAN_BATCH;
     a.batch = (int)nb;
-    a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0];
     a.lengths = static_cast<const int32_t *>(d->lengths) + b0 * a.len_stride;
-    a.lse = static_cast<const float *>(d->lse) + b0 * a.ls[0];
-    a.take = d->rows ? static_cast<const uint8_t *>(d->rows) + b0 * a.ts[0] : nullptr;
     a.out = static_cast<float *>(d->weights_out) + b0 * a.os[0];
     CUtensorMap map{};
     const int64_t step[3] = {kcs[2], kcs[1], kcs[0]};
@@ -412,7 +410,12 @@ extern "C" int skv_accumulate_weights(const SkvWeights *d, void *stream) {
     a.along[1] = nb > 1 && kcs[0] ? 1 : 0;
     // more rows than the MMA's N: further launches add to what the first wrote
     for (int64_t r0 = 0; r0 < rows; r0 += WT_ROWS) {
-      a.row0 = (int)r0;
+      // (from the node that holds row r0 on, so that the kernel's row numbers stay small)
+      const int64_t node0 = r0 / group;
+      a.q = static_cast<const uint16_t *>(d->q) + b0 * a.qs[0] + node0 * a.qs[1];
+      a.lse = static_cast<const float *>(d->lse) + b0 * a.ls[0] + node0 * a.ls[1];
+      a.take = d->rows ? static_cast<const uint8_t *>(d->rows) + b0 * a.ts[0] + node0 * a.ts[1] : nullptr;
+      a.row0 = (int)(r0 - node0 * group);
       a.rows = (int)(rows - r0 < WT_ROWS ? rows - r0 : WT_ROWS);
       a.cols = (a.rows + 15) & ~15;
       if (r0 == 0) {

@@ -143,3 +143,18 @@ def test_rotary_follows_the_value_of_its_settings():
     factor.fill_(4.0)
     got = skv.rotary(q, None, pos, theta=theta, scaling="linear", factor=factor)[0]
     assert torch.equal(got, skv.rotary(q, None, pos, theta=5e5, scaling="linear", factor=4.0)[0])
+
+
+# ---------------------------------------------------------------- accumulated weights
+
+
+@pytest.mark.parametrize("dtype", [BF, F8])
+@pytest.mark.parametrize("n,hq", [(40003, 4), (8195, 48)])
+def test_accumulate_weights_of_a_long_window(n, hq, dtype):
+    """More than 2^17 rows a KV head: the number of nodes is not limited."""
+    g, t, d = gen(76), 70, 64
+    q, kc = normal(g, 1, n, hq, d), normal(g, 1, 1, t, d).to(dtype)
+    lse = torch.randn(1, n, hq, device="cuda", generator=g) + 12.0
+    rows = torch.rand(1, n, device="cuda", generator=g) < 0.5
+    w, lengths = torch.rand(1, 1, t, device="cuda", generator=g), torch.tensor([t - 3], dtype=torch.int32, device="cuda")
+    close(skv.accumulate_weights(q, kc, lengths, lse, w, rows=rows), *R.weights(q, kc, lengths, lse, w, rows))
