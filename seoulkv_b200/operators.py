@@ -34,6 +34,9 @@ import torch
 from seoulkv_b200 import _native
 from seoulkv_b200.api import _current_stream
 
+# Tells autograd that a tensor was written to (one that backward has saved is then an error there).
+_changed = torch.autograd.graph.increment_version
+
 TREE_MAX_NODES = 64
 ROTARY_MAX_DIM = 512
 _BF16, _F32, _I32, _FP8 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
@@ -259,6 +262,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
         dev, _DTYPE[dtype], layout == "interleaved", positions.dtype is torch.int64, b, n, hq, hkv, d, r,
         *q.stride(), *kk.stride(), *qo.stride(), *kko.stride(), *((0, *pos) if len(pos) == 1 else pos))
     _run(_native.load().skv_rotary, packed, dev, "rotary")
+    if out is not None:
+        _changed(qo)
+        if ko is not None:
+            _changed(ko)
     return qo, ko
 
 
@@ -469,7 +476,8 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
     if rows is not None and not (isinstance(rows, torch.Tensor) and rows.dtype is torch.bool and rows.shape == (b, n)
                                  and rows.get_device() == dev):
         _check("rows", rows, (b, n), (torch.bool,), dev)
-    if out is None:
+    given = out is not None
+    if not given:
         out = weights.new_empty(b, hkv, t)
     else:
         _check("out", out, held, (_F32,), dev)
@@ -485,6 +493,8 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
         hkv, d, t, *q.stride(), *k_cache.stride(), *lse.stride(), *((0, 0) if rows is None else rows.stride()),
         *weights.stride(), *out.stride(), *lengths.stride())
     _run(_native.load().skv_accumulate_weights, packed, dev, "accumulate_weights")
+    if given:
+        _changed(out)
     return out
 
 

@@ -158,3 +158,29 @@ def test_accumulate_weights_of_a_long_window(n, hq, dtype):
     rows = torch.rand(1, n, device="cuda", generator=g) < 0.5
     w, lengths = torch.rand(1, 1, t, device="cuda", generator=g), torch.tensor([t - 3], dtype=torch.int32, device="cuda")
     close(skv.accumulate_weights(q, kc, lengths, lse, w, rows=rows), *R.weights(q, kc, lengths, lse, w, rows))
+
+
+# ---------------------------------------------------------------- autograd around the operators
+
+
+def test_outputs_given_to_an_operator_count_as_changed():
+    """A tensor that backward needs and that an operator then writes to: an error, not a wrong gradient."""
+    pos = torch.arange(3, device="cuda")
+    for name in ("q", "k", "w"):
+        q, k = normal(gen(77), 1, 3, 4, 64, dtype=torch.float32), normal(gen(78), 1, 2, 3, 64, dtype=torch.float32)
+        kc, w = normal(gen(79), 1, 2, 9, 64), torch.rand(1, 2, 9, device="cuda")
+        x = dict(q=q, k=k, w=w)[name]
+        factor = torch.ones_like(x, requires_grad=True)
+        y = (factor * x).sum()
+        before = x._version
+        if name == "w":
+            skv.accumulate_weights(q.to(BF), kc, torch.tensor([9], dtype=torch.int32, device="cuda"),
+                                   torch.full((1, 3, 4), 5.0, device="cuda"), w, out=w)
+        else:
+            skv.rotary(q, k, pos, out=(q, k))
+        assert x._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        q = torch.ones(1, 3, 4, 64, device="cuda")
+        skv.rotary(q, None, pos, out=(q, None))
