@@ -18,7 +18,7 @@ and every call may be captured into a CUDA graph.  Tensors may have any
 strides as long as the innermost dimension is contiguous and, for the
 attention operators, rows start on 16-byte boundaries; ValueError otherwise.
 They are for inference: a tensor that requires a gradient is refused while
-gradients are recorded.
+gradients are recorded, and so is one with a forward-mode tangent.
 """
 
 from __future__ import annotations
@@ -30,6 +30,7 @@ import math
 import struct
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from seoulkv_b200 import _native
 from seoulkv_b200.api import _current_stream
@@ -63,13 +64,20 @@ def _check(name: str, t, shape, dtypes, device: int | None = None) -> None:
         raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators have no backward pass (detach it, or use no_grad)")
+    if _tangent(t):
+        raise ValueError(f"{name} carries a forward-mode tangent: the operators have no derivatives (detach it)")
+
+
+def _tangent(t) -> bool:
+    return _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None
 
 
 def _recorded(*tensors) -> bool:
+    """Whether a derivative of one of them is wanted, in either mode."""
     for t in tensors:
-        if t.requires_grad:
-            return torch.is_grad_enabled()
-    return False
+        if t.requires_grad and torch.is_grad_enabled():
+            return True
+    return _forward._current_level >= 0 and any(_tangent(t) for t in tensors)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -400,7 +408,8 @@ def run_tree(engine, lead: tuple, q, k, v, parents, device: int):
     if not isinstance(parents, torch.Tensor) or parents.dtype is not _I32 or tuple(parents.shape) != (*lead, n):
         raise ValueError(f"expected int32 parents [{dims}{n}]")
     if _recorded(q, k, v):
-        raise ValueError("run_tree has no backward pass (detach the inputs, or use no_grad)")
+        raise ValueError("run_tree has no derivatives: an input requires a gradient or carries a tangent "
+                         "(detach it, or use no_grad)")
     q, k, v, parents = (t if t.get_device() == device else t.to(f"cuda:{device}") for t in (q, k, v, parents))
     if not lead:
         k, v, parents = k[None], v[None], parents[None]

@@ -184,3 +184,26 @@ def test_outputs_given_to_an_operator_count_as_changed():
     with torch.inference_mode():
         q = torch.ones(1, 3, 4, 64, device="cuda")
         skv.rotary(q, None, pos, out=(q, None))
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    args = tree_case(80, [9], 3, 4, 2, 64, 16)
+    q, kc, vc, lengths, k, v, parents = args
+    lse, w = torch.zeros(1, 3, 4, device="cuda"), torch.zeros(1, 2, 16, device="cuda")
+    with fwd.dual_level():
+        def dual(x):
+            return fwd.make_dual(x, torch.ones_like(x))
+
+        skv.tree_attention(*args)  # (without a tangent)
+        for call in (lambda: skv.rotary(dual(q), None, torch.arange(3, device="cuda")),
+                     lambda: skv.rotary(q, dual(k), torch.arange(3, device="cuda")),
+                     lambda: skv.tree_attention(dual(q), *args[1:]),
+                     lambda: skv.tree_attention(q, kc, dual(vc), lengths, k, v, parents),
+                     lambda: skv.tree_attention(q, kc, vc, lengths, k, dual(v), parents),
+                     lambda: skv.accumulate_weights(q, kc, lengths, dual(lse), w),
+                     lambda: skv.accumulate_weights(q, kc, lengths, lse, dual(w)),
+                     lambda: skv.evict(kc, dual(vc), w, lengths, keep=4, sink=0, local=0)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()

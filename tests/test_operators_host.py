@@ -135,3 +135,20 @@ def test_rotary_table_goes_by_the_values_of_its_settings():
     first = operators._rotary_table(64, 1e4, "yarn", 4.0, context, 32.0, 1.0, None)[0].raw
     context.fill_(8192)
     assert operators._rotary_table(64, 1e4, "yarn", 4.0, context, 32.0, 1.0, None)[0].raw != first
+
+
+# ---------------------------------------------------------------- derivatives
+
+
+def test_a_wanted_derivative_is_seen_in_either_mode():
+    import torch.autograd.forward_ad as fwd
+
+    x, g = torch.ones(3), torch.ones(3, requires_grad=True)
+    assert operators._recorded(x, g) and not operators._recorded(x)
+    with torch.no_grad():
+        assert not operators._recorded(x, g)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones(3))
+        assert operators._recorded(x, d) and operators._recorded(d) and not operators._recorded(x)
+        with torch.no_grad():  # (no_grad is about the backward pass alone)
+            assert operators._recorded(x, d) and not operators._recorded(g)
