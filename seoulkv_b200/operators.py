@@ -93,6 +93,54 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _reaches(total: int, terms: list) -> bool:
+    """Whether sum(s * t) == total for some integers lo <= t <= hi of each term (s, lo, hi), s > 0.
+    Largest s first: in a layout whose dimensions nest, one or two t are left for each."""
+    if not terms:
+        return total == 0
+    (s, lo, hi), rest = terms[0], terms[1:]
+    least, most = sum(x * a for x, a, _ in rest), sum(x * b for x, _, b in rest)
+    first, last = max(lo, -((most - total) // s)), min(hi, (total - least) // s)
+    return any(_reaches(total - s * t, rest) for t in range(first, last + 1))
+
+
+@functools.lru_cache(maxsize=256)
+def _layouts_meet(off: int, a: tuple, of_a: tuple, b: tuple, of_b: tuple) -> bool:
+    """Whether layouts (strides, sizes) share a place, the second one ``off`` elements behind the first."""
+    terms = {}
+    for s, n in zip(a, of_a):
+        lo, hi = terms.get(s, (0, 0))
+        terms[s] = lo, hi + n - 1
+    for s, n in zip(b, of_b):
+        lo, hi = terms.get(s, (0, 0))
+        terms[s] = lo - n + 1, hi
+    return _reaches(off, sorted(((s, *x) for s, x in terms.items() if s), reverse=True))
+
+
+@functools.lru_cache(maxsize=256)
+def _layout_folds(strides: tuple, sizes: tuple) -> bool:
+    """Whether two elements of a layout share one place."""
+    dims = sorted(((s, n - 1) for s, n in zip(strides, sizes) if n > 1), reverse=True)
+    if dims and dims[-1][0] == 0:
+        return True
+    terms = [(s, -n, n) for s, n in dims]
+    return any(_reaches(-s * i, terms[at + 1:]) for at, (s, n) in enumerate(dims)
+               for i in range(1, min(n, sum(x * m for x, m in dims[at + 1:]) // s) + 1))
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one element type share a place."""
+    if not _overlap(a, b):
+        return False
+    off, size = b.data_ptr() - a.data_ptr(), a.element_size()
+    return off % size != 0 or _layouts_meet(off // size, a.stride(), a.shape, b.stride(), b.shape)
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether two elements of a tensor share one place."""
+    return not t.is_contiguous() and t.numel() > 0 and _layout_folds(t.stride(), t.shape)
+
+
 def _run(entry, packed: bytes, device: int, what: str) -> None:
     rc = entry(packed, _current_stream(device))
     if rc:
@@ -287,13 +335,16 @@ def _check_rotary_out(q, k, qo, ko, dev: int) -> None:
         _check("out[1]", ko, tuple(k.shape), (q.dtype,), dev)
         pairs.append(("out[1]", ko, k))
     for name, y, x in pairs:
-        if any(s == 0 and size > 1 for s, size in zip(y.stride(), y.shape)):
+        if _folded(y):
             raise ValueError(f"{name}: two elements share one place")
         same = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
         if not same and _overlap(y, x):
             raise ValueError(f"{name} overlaps its input without being it")
-    if k is not None and not (qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr()):
+    if k is not None and qo.data_ptr() == q.data_ptr() and ko.data_ptr() == k.data_ptr():
         # (in place, q and k may be interleaved parts of one projection)
+        if _meet(qo, ko):
+            raise ValueError("out[1] overlaps out[0]: q and k share places")
+    elif k is not None:
         for name, y, x in (("out[0]", qo, k), ("out[1]", ko, q), ("out[1]", ko, qo)):
             if _overlap(y, x):
                 raise ValueError(f"{name} overlaps another tensor of the call")
@@ -490,7 +541,7 @@ def accumulate_weights(q: torch.Tensor, k_cache: torch.Tensor, lengths: torch.Te
         out = weights.new_empty(b, hkv, t)
     else:
         _check("out", out, held, (_F32,), dev)
-        if any(x == 0 and size > 1 for x, size in zip(out.stride(), out.shape)):
+        if _folded(out):
             raise ValueError("out: two elements share one place")
         if not (out.data_ptr() == weights.data_ptr() and out.stride() == weights.stride()) and _overlap(out, weights):
             raise ValueError("out overlaps weights without being it")

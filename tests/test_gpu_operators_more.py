@@ -207,3 +207,25 @@ def test_forward_mode_tangents_are_refused():
                      lambda: skv.evict(kc, dual(vc), w, lengths, keep=4, sink=0, local=0)):
             with pytest.raises(ValueError, match="tangent"):
                 call()
+
+
+def test_rotary_in_place_refuses_q_and_k_that_share_places():
+    """Each element would turn twice, in any order."""
+    pos = torch.arange(6, device="cuda")
+    x = normal(gen(82), 2, 6, 4, 64)
+    before = x.clone()
+    k = x.transpose(1, 2)
+    with pytest.raises(ValueError, match="share places"):
+        skv.rotary(x, k, pos, out=(x, k))
+    with pytest.raises(ValueError, match="share places"):
+        skv.rotary(x, k[:, 3:], pos, out=(x, k[:, 3:]))
+    with pytest.raises(ValueError, match="share one place"):
+        windows = torch.zeros(64 + 8 * 5, device="cuda", dtype=BF).unfold(0, 64, 8)[None, :, None]
+        skv.rotary(windows, None, pos, out=(windows, None))
+    assert torch.equal(x, before)
+    # parts side by side in every head turn as copies of them do
+    qkv = normal(gen(83), 2, 6, 4, 3, 64)
+    want = skv.rotary(qkv[:, :, :, 0].contiguous(), qkv[:, :, :, 1].transpose(1, 2).contiguous(), pos)
+    q, k, v = qkv[:, :, :, 0], qkv[:, :, :, 1].transpose(1, 2), qkv[:, :, :, 2].clone()
+    skv.rotary(q, k, pos, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(qkv[:, :, :, 2], v)

@@ -1,6 +1,7 @@
 """Parts of the operators that can be checked without a GPU: the order of
 accesses to shared memory, tables, refusals and reports."""
 
+import random
 import shutil
 import struct
 import subprocess
@@ -152,3 +153,45 @@ def test_a_wanted_derivative_is_seen_in_either_mode():
         assert operators._recorded(x, d) and operators._recorded(d) and not operators._recorded(x)
         with torch.no_grad():  # (no_grad is about the backward pass alone)
             assert operators._recorded(x, d) and not operators._recorded(g)
+
+
+# ---------------------------------------------------------------- outputs that share places
+
+
+def _places(t):
+    at = torch.zeros(t.shape, dtype=torch.int64)
+    for i, (n, s) in enumerate(zip(t.shape, t.stride())):
+        at += (torch.arange(n) * s).reshape([-1 if j == i else 1 for j in range(t.ndim)])
+    return (at + t.storage_offset()).flatten().tolist()
+
+
+def test_shared_places_are_found_exactly():
+    """Against the sets of places, over views of one buffer that nest, interleave, overlap and fold."""
+    rng = random.Random(1)
+    buffer = torch.zeros(4000)
+    met = folded = 0
+    for _ in range(1500):
+        views = []
+        for _ in range(2):
+            shape = [rng.choice([1, 2, 3, 5]) for _ in range(3)] + [rng.choice([1, 2, 4])]
+            stride = [rng.choice([0, 1, 2, 3, 4, 6, 8, 12, 20, 24, 40, 120]) for _ in range(3)] + [1]
+            views.append(torch.as_strided(buffer, shape, stride, rng.randrange(0, 60)))
+        a, b = (_places(x) for x in views)
+        assert operators._meet(*views) == bool(set(a) & set(b)), views
+        for x, p in zip(views, (a, b)):
+            assert operators._folded(x) == (len(set(p)) < len(p)), (x.shape, x.stride())
+            folded += len(set(p)) < len(p)
+        met += bool(set(a) & set(b))
+    assert met > 100 and folded > 100
+
+
+def test_query_and_key_parts_of_one_projection_do_not_meet():
+    b, n, hq, hkv, d = 2, 9, 4, 2, 64
+    blocks = torch.zeros(b, n, hq + 2 * hkv, d)
+    q, k = blocks[:, :, :hq], blocks[:, :, hq:hq + hkv].transpose(1, 2)
+    assert not operators._meet(q, k) and operators._meet(q, blocks[:, :, hq - 1:hq + 1].transpose(1, 2))
+    by_head = torch.zeros(b, n, hq, 3, d)  # each head's q, k and v side by side
+    q, k = by_head[:, :, :, 0], by_head[:, :, :, 1].transpose(1, 2)
+    assert not operators._meet(q, k) and operators._meet(q, q.transpose(1, 2))
+    assert not operators._folded(q) and not operators._folded(k)
+    assert operators._folded(torch.zeros(200).unfold(0, 64, 8)[None, :, None])
