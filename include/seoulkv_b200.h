@@ -159,7 +159,8 @@ int skv_step(void *handle, const uint16_t *q, int32_t on_device, void *stream);
 int skv_finish(void *handle, uint16_t *out, SkvStatus *status);
 
 /* Wait for all work of this engine, then check the device status words:
- * returns SKV_E_CAPACITY if any cell reported a live count out of range. */
+ * returns SKV_E_CAPACITY if any cell reported a live count out of range, and
+ * SKV_E_CUDA, once, if a wait of a skv_run_tree kernel gave up. */
 int skv_sync(void *handle);
 int skv_status(void *handle, SkvStatus *out);
 
@@ -464,9 +465,11 @@ typedef struct SkvWeights {
 } SkvWeights;
 int skv_accumulate_weights(const SkvWeights *desc, void *stream);
 
-/* Waits for the device and reads its operators' status word: bits
- * SKV_STATUS_* of bounded device waits that gave up since the library was
- * loaded (the results of such a call are NaN). */
+/* Waits for the device, reads its operators' status word and clears it: bits
+ * SKV_STATUS_* of bounded device waits that gave up since the last such call
+ * (the results of an operator whose wait gave up are NaN).  One word per
+ * device, for all callers of the process; the trees of an engine
+ * (skv_run_tree) report to its skv_sync instead. */
 int skv_operator_status(int32_t device, uint32_t *flags);
 
 #ifdef __cplusplus

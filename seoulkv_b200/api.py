@@ -280,7 +280,8 @@ class SeoulKV4:
             eng.bind_query(qh.data_ptr(), False, self._stream())
 
     def synchronize(self) -> None:
-        """Wait for the last run; raises RuntimeError if a live count left its range."""
+        """Wait for the last run and the last run_tree; raises RuntimeError if a live
+        count left its range, or (once) if a bounded wait of a tree gave up."""
         self._require_open()
         if self._engine is not None:
             try:

@@ -208,7 +208,8 @@ class SeoulKV4Batch:
         return run_tree(self._engine, (self.n,), q, k, v, parents, self._device_index)
 
     def synchronize(self) -> None:
-        """Wait for the last run; raises RuntimeError if a live count left its range."""
+        """Wait for the last run and the last run_tree; raises RuntimeError if a live
+        count left its range, or (once) if a bounded wait of a tree gave up."""
         self._require_open()
         if self._engine is not None:
             try:

@@ -127,6 +127,8 @@ struct Engine {
   CUtensorMap *record_maps = nullptr;
   cudaEvent_t tree_done = nullptr;     // the last skv_run_tree outside a capture
   bool tree_ran = false;
+  uint32_t *tree_status = nullptr;     // SKV_STATUS_* of this engine's trees, until skv_sync reports them
+  bool tree_used = false;              // also inside a capture
   uint16_t *kv_stage = nullptr;        // host-input staging [2][n_cells][APPEND_MAX][256]
   bool appends() const { return tmax > desc.context; }
 };
@@ -285,6 +287,25 @@ int sync_done(Engine *e) {
   if (e->ran) CK(cudaEventSynchronize(e->done));
   CK(cudaStreamSynchronize(e->stream));
   return SKV_OK;
+}
+
+// Also waits for the last tree, which may have run on another stream.
+int sync_trees(Engine *e) {
+  CK(cudaSetDevice(e->desc.device));
+  if (e->tree_ran) CK(cudaEventSynchronize(e->tree_done));
+  return SKV_OK;
+}
+
+// Whether a tree's wait gave up; reported once.
+int tree_error(Engine *e) {
+  if (!e->tree_used) return SKV_OK;
+  uint32_t flags = 0;
+  CK(cudaMemcpy(&flags, e->tree_status, sizeof flags, cudaMemcpyDeviceToHost));
+  if (!flags) return SKV_OK;
+  CK(cudaMemset(e->tree_status, 0, sizeof flags));
+  char msg[128];
+  std::snprintf(msg, sizeof msg, "a wait of a tree's kernel gave up (status 0x%x); that tree's results are NaN", flags);
+  return fail(SKV_E_CUDA, msg);
 }
 
 int read_counts(Engine *e, std::vector<int32_t> &c) {
@@ -552,6 +573,7 @@ int skv_create(const SkvDesc *d, void **handle) {
   TRY(dalloc(e, &w.hist, C * 4 * G * 4096));
   TRY(dalloc(e, &e->phase_ts, 2 * FUSED_MARKS));
   TRY(dalloc(e, &e->record_maps, 2 * (size_t)e->n_cells));
+  TRY(dalloc(e, &e->tree_status, 1));
   e->tmax = d->max_context ? d->max_context : d->context;
   e->t_host = d->context;
   {
@@ -748,6 +770,7 @@ int skv_upload_kv(void *handle, int32_t slot, const uint16_t *k, const uint16_t 
   if (!e || !k || !v) return fail(SKV_E_INVALID, "null engine or K/V");
   if (slot < 0 || slot >= e->desc.n_slots) return fail(SKV_E_INVALID, "slot out of range");
   if (e->appended) return fail(SKV_E_STATE, "the cache has grown by appends; uploads are closed");
+  if (int rs = sync_trees(e)) return rs;  // (they read the records and their maps)
   CK(cudaSetDevice(e->desc.device));
   CK(cudaStreamSynchronize(e->stream));
   const size_t T = e->desc.context, elems = (size_t)G * T * D;
@@ -848,7 +871,8 @@ int skv_run_tree(void *handle, const SkvTree *desc, void *stream) {
   DeviceScope scope(e->desc.device);
   CK(scope.error());
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((rc = tree_attention(&d, e->record_maps, e->tlen, 0, st))) return rc;
+  e->tree_used = true;
+  if ((rc = tree_attention(&d, e->record_maps, e->tlen, 0, e->tree_status, st))) return rc;
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   CK(cudaStreamIsCapturing(st, &cap));
   if (cap == cudaStreamCaptureStatusNone) {
@@ -1173,12 +1197,16 @@ int skv_status(void *handle, SkvStatus *out) {
 int skv_sync(void *handle) {
   Engine *e = as_engine(handle);
   if (!e) return fail(SKV_E_INVALID, "null engine");
-  if (!e->ran) return sync_done(e);
-  SkvStatus s;
-  int rc = skv_status(handle, &s);
+  int rc = sync_trees(e);
   if (rc) return rc;
+  if (!e->ran) {
+    rc = sync_done(e);
+    return rc ? rc : tree_error(e);
+  }
+  SkvStatus s;
+  if ((rc = skv_status(handle, &s))) return rc;
   if (s.flags) return status_error(e, s);
-  return SKV_OK;
+  return tree_error(e);
 }
 
 int skv_output(void *handle, void *out, int32_t to_host) {

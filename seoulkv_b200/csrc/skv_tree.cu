@@ -1034,7 +1034,8 @@ int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
   return SKV_OK;
 }
 
-int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, cudaStream_t st) {
+int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, uint32_t *status,
+                   cudaStream_t st) {
   if (int rc = check_tree(d)) return rc;
   if (d->batch == 0) return SKV_OK;
   if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse ||
@@ -1073,7 +1074,9 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
   if (d->workspace_bytes < scratch || (scratch && !d->workspace))
     return op_fail(SKV_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes, (long long)scratch);
   TreeArgs a{};
-  if (int rc = status_word((int)d->device, &a.status)) return rc;
+  a.status = status;
+  if (!status)
+    if (int rc = status_word((int)d->device, &a.status)) return rc;
   const int group = (int)(d->heads / d->kv_heads), rows = (int)d->n * group;
   a.heads = (int)d->kv_heads, a.group = group, a.n = (int)d->n, a.t = (int)d->tokens;
   a.by_group = ((1ull << 32) + group - 1) / group;
@@ -1143,7 +1146,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
 extern "C" {
 
 int skv_tree_attention(const SkvTree *d, void *stream) {
-  return skv::tree_attention(d, nullptr, nullptr, 0, static_cast<cudaStream_t>(stream));
+  return skv::tree_attention(d, nullptr, nullptr, 0, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 int skv_tree_workspace(const SkvTree *d, int64_t *bytes) {
@@ -1165,6 +1168,8 @@ int skv_operator_status(int32_t device, uint32_t *flags) {
   if (int rc = status_word(device, &word)) return rc;
   if (int rc = op_cuda(cudaDeviceSynchronize(), "waiting for the device")) return rc;
   if (int rc = op_cuda(cudaMemcpy(&got, word, sizeof got, cudaMemcpyDeviceToHost), "reading the status word")) return rc;
+  if (got)  // reported once: later calls are judged by themselves
+    if (int rc = op_cuda(cudaMemset(word, 0, sizeof got), "clearing the status word")) return rc;
   *flags = got;
   return SKV_OK;
 }

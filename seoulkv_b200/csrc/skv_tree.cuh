@@ -13,7 +13,9 @@ namespace skv {
 int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows);
 // Attention over a cache given by `d`, or (cells != null: device array of the K
 // and V maps of every cell) over FP8 records with the context at `tlen` (null:
-// `context`).
-int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, cudaStream_t st);
+// `context`).  `status` (null: the device's word) gets the bits of waits that
+// gave up.
+int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, uint32_t *status,
+                   cudaStream_t st);
 
 }  // namespace skv

@@ -152,7 +152,9 @@ def _run(entry, packed: bytes, device: int, what: str) -> None:
 
 def check_operators(device) -> None:
     """Wait for the device; RuntimeError if a bounded wait of an operator's kernel gave up on it
-    (the outputs of that call are NaN).  Not for the inner loop."""
+    since the last check (the outputs of that call are NaN).  One record per device, for all its
+    users in the process; ``run_tree`` reports to its instance's ``synchronize()`` instead.  Not
+    for the inner loop."""
     from seoulkv_b200.api import _cuda_index
 
     flags = ctypes.c_uint32()

@@ -229,3 +229,21 @@ def test_rotary_in_place_refuses_q_and_k_that_share_places():
     q, k, v = qkv[:, :, :, 0], qkv[:, :, :, 1].transpose(1, 2), qkv[:, :, :, 2].clone()
     skv.rotary(q, k, pos, out=(q, k))
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(qkv[:, :, :, 2], v)
+
+
+def test_synchronize_waits_for_the_last_tree(grown, cuda):  # noqa: F811
+    """Also for one on another stream than any run, before the first run and after it."""
+    q, k, v, parents = drafted(84, 1, 3)
+    side = torch.cuda.Stream()
+    with skv.SeoulKV4(device=cuda, k=grown.k, v=grown.v, index=grown.index) as attn:
+        attn.run_tree(q, k[0], v[0], parents[0])
+        for turn in range(2):
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(200_000_000)  # a tenth of a second
+                out, _ = attn.run_tree(q, k[0], v[0], parents[0])
+            assert not side.query()
+            attn.synchronize()
+            assert side.query()
+            assert torch.isfinite(out).all()
+            attn.run(grown.query(grown.context, seed=3)).to_torch()

@@ -2,6 +2,7 @@
 accesses to shared memory, tables, refusals and reports."""
 
 import random
+import re
 import shutil
 import struct
 import subprocess
@@ -195,3 +196,20 @@ def test_query_and_key_parts_of_one_projection_do_not_meet():
     assert not operators._meet(q, k) and operators._meet(q, q.transpose(1, 2))
     assert not operators._folded(q) and not operators._folded(k)
     assert operators._folded(torch.zeros(200).unfold(0, 64, 8)[None, :, None])
+
+
+# ---------------------------------------------------------------- reports of waits that gave up
+
+
+def test_reports_of_waits_that_gave_up_reach_their_reader_once():
+    """A tree of an engine writes the engine's word, which skv_sync reads on every way out and clears; the
+    device's word is cleared when it is read.  (No wait is made to give up here: what is checked is who reads.)"""
+    engine = (CSRC / "skv_engine.cu").read_text()
+    assert re.search(r"tree_attention\(&d, e->record_maps, .*e->tree_status, st\)", engine)
+    sync = engine[engine.index("int skv_sync("):]
+    sync = sync[:sync.index("\n}\n")]
+    assert sync.index("sync_trees(e)") < sync.index("e->ran") and sync.count("tree_error(e)") == 2
+    error = engine[engine.index("int tree_error("):]
+    assert "cudaMemset(e->tree_status" in error[:error.index("\n}\n")]
+    tree = (CSRC / "skv_tree.cu").read_text()
+    assert "cudaMemset(word" in tree[tree.index("int skv_operator_status("):]
