@@ -872,7 +872,7 @@ int skv_run_tree(void *handle, const SkvTree *desc, void *stream) {
   CK(scope.error());
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   e->tree_used = true;
-  if ((rc = tree_attention(&d, e->record_maps, e->tlen, 0, e->tree_status, st))) return rc;
+  if ((rc = tree_attention(&d, e->record_maps, e->tlen, e->tree_status, st))) return rc;
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   CK(cudaStreamIsCapturing(st, &cap));
   if (cap == cudaStreamCaptureStatusNone) {

@@ -278,7 +278,7 @@ cudaError_t launch_gather(const GatherArgs &g, cudaStream_t st) {
   const int per_row = g.row_bytes / (int)sizeof(C);
   const int group = EG_THREADS / (per_row < EG_THREADS ? per_row : EG_THREADS);
   const int64_t blocks = (g.rows + group * EG_ROWS - 1) / (group * EG_ROWS);
-  return op_launch(k_evict_gather<C>, dim3((unsigned)blocks), dim3(EG_THREADS), 0, st, true, 1, g);
+  return op_launch(k_evict_gather<C>, dim3((unsigned)blocks), dim3(EG_THREADS), 0, st, 1, g);
 }
 
 }  // namespace
@@ -333,7 +333,7 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   const int64_t warps = (int64_t)ranks * EV_WARPS, keys = ((d->tokens + warps - 1) / warps + 31) / 32 * 32 * EV_WARPS;
   a.room = keys <= EV_CACHED ? (int)keys : 0;
   rc = op_cuda(op_launch(k_evict_select, dim3((unsigned)(d->batch * d->kv_heads * ranks)), dim3(EV_THREADS),
-                         sizeof(SelectSmem) + (size_t)a.room * 4, st, true, (unsigned)ranks, a), "k_evict_select launch");
+                         sizeof(SelectSmem) + (size_t)a.room * 4, st, (unsigned)ranks, a), "k_evict_select launch");
   if (rc) return rc;
   GatherArgs g;
   g.x[0] = static_cast<const uint8_t *>(d->k), g.x[1] = static_cast<const uint8_t *>(d->v);

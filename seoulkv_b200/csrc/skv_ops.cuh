@@ -85,16 +85,16 @@ inline int op_shared_memory(const void *kernel, int bytes, int device, bool *set
   return SKV_OK;
 }
 
-// Launch; with `early` the kernel's blocks may be placed while the kernel
-// before it on the stream still runs, which hides its launch and its prologue.
+// Launch; the kernel's blocks may be placed while the kernel before it on the
+// stream still runs, which hides its launch and its prologue.
 // That holds once every block of the kernel before has called
 // grid_dependency_release() or ended; a kernel that never does (any that is
 // not of these operators) ends first.  Such a kernel's threads call
 // grid_dependency_wait() before they read or write global memory: it returns
 // when the kernel before has ended, and with it all that were before that.
 template <typename... P, typename... A>
-inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool early,
-                             unsigned cluster, A &&...args) noexcept {
+inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, unsigned cluster,
+                             A &&...args) noexcept {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -102,10 +102,8 @@ inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   unsigned n = 0;
-  if (early) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n++].val.programmaticStreamSerializationAllowed = 1;
   if (cluster > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = cluster;

@@ -28,15 +28,15 @@ __device__ __forceinline__ int by_inverse(int n, uint64_t inverse) { return (int
 // pre[b] (places of the sequences before b, one unit's worth) and len[b], by
 // one warp: KT cached tokens a tile, and `extra` places more.
 template <int KT>
-__device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stride, int context, int t, int batch,
-                                            int extra, int32_t *len, int32_t *pre) {
+__device__ __forceinline__ void tile_prefix(const int32_t *lengths, int64_t stride, int t, int batch, int extra,
+                                            int32_t *len, int32_t *pre) {
   const int lane = threadIdx.x & 31;
   int base = 0;
   for (int b0 = 0; b0 < batch; b0 += 32) {
     const int b = b0 + lane;
     int n = 0, tiles = 0;
     if (b < batch) {
-      n = lengths ? __ldcg(lengths + b * stride) : context;  // (from L2: k_tree_combine reads before it waits)
+      n = __ldcg(lengths + b * stride);  // (from L2: k_tree_combine reads before it waits)
       n = max(0, min(n, t));
       tiles = (n + KT - 1) / KT + extra;
     }

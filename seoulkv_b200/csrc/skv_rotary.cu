@@ -159,8 +159,8 @@ cudaError_t launch_rotary(const RotaryArgs &a, bool half, int sms, cudaStream_t 
   const int64_t items = a.tokens * a.split * a.chunks;
   const int64_t want = (items + RT_THREADS - 1) / RT_THREADS;
   const unsigned grid = (unsigned)(want < 16LL * sms ? want : 16LL * sms);
-  if (half) return op_launch(k_rotary<T, V, true>, dim3(grid), dim3(RT_THREADS), 0, st, true, 1, a);
-  return op_launch(k_rotary<T, V < 2 ? 2 : V, false>, dim3(grid), dim3(RT_THREADS), 0, st, true, 1, a);
+  if (half) return op_launch(k_rotary<T, V, true>, dim3(grid), dim3(RT_THREADS), 0, st, 1, a);
+  return op_launch(k_rotary<T, V < 2 ? 2 : V, false>, dim3(grid), dim3(RT_THREADS), 0, st, 1, a);
 }
 
 template <typename T>

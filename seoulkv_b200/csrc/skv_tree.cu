@@ -184,7 +184,6 @@ struct TreeArgs {
   int64_t kns[3], vns[3];  // element strides (sequence, head, node)
   const int32_t *lengths;
   int64_t len_stride;
-  int32_t context;         // length of every sequence without `lengths`
   const int32_t *parents;
   int64_t ps[2];           // element strides (sequence, node)
   uint16_t *out;           // [sequence][node][query head][D]
@@ -254,7 +253,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       }
     }
     grid_dependency_wait();
-    tile_prefix<KT>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
+    tile_prefix<KT>(a.lengths, a.len_stride, a.t, a.batch, 1 + TR_IDLE, nullptr, s.pre);
   } else if (warp == 1) {
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
@@ -302,10 +301,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   }
   const Walk walk(s.pre, a.batch, a.heads, TR_IDLE, from, to);
   auto wait = [&](uint64_t *bar, uint32_t parity) { return bar_wait(bar, parity, abort, a.status); };
-  auto length = [&](int b) {
-    const int n = a.lengths ? a.lengths[b * a.len_stride] : a.context;
-    return max(0, min(n, a.t));
-  };
+  auto length = [&](int b) { return max(0, min(a.lengths[b * a.len_stride], a.t)); };
 
   if (warp == 0) {
     // ---- loads: BF16 tiles into the ring; of FP8 caches K into its own, and V
@@ -864,7 +860,7 @@ __global__ void __launch_bounds__(TC_THREADS) k_tree_combine(const __grid_consta
   grid_dependency_release();
   // (the lengths are older than the attention kernel, which released this one
   // after its own wait)
-  if (warp == 0) tile_prefix<TR_KEYS>(a.lengths, a.len_stride, a.context, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
+  if (warp == 0) tile_prefix<TR_KEYS>(a.lengths, a.len_stride, a.t, a.batch, 1 + TR_IDLE, nullptr, s_pre);
   __syncthreads();
   const int rows = a.n * a.group, all = rows * a.heads * a.batch;
   const int index = FEW ? blockIdx.x * GROUPS + group : blockIdx.x;
@@ -959,7 +955,7 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, c
   auto *kernel = &k_tree_attention<C>;
   static bool set[64];
   if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), smem, device, set)) return rc;
-  if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, true, 1, maps, a),
+  if (int rc = op_cuda(op_launch(kernel, dim3(ctas), dim3(C::THREADS), smem, st, 1, maps, a),
                        "k_tree_attention launch"))
     return rc;
   if (a.whole) return SKV_OK;
@@ -968,8 +964,8 @@ int launch_tree(const TreeMaps &maps, const TreeArgs &a, int ctas, int device, c
   constexpr unsigned per = TC_THREADS / (C::D / 4);
   // (a unit has about items / units parts: more than one thread group's batch of them is shared)
   const bool few = items <= (TC_BATCH - 2) * a.batch * a.heads;
-  return op_cuda(few ? op_launch(k_tree_combine<C::D, true>, dim3((rows + per - 1) / per), dim3(TC_THREADS), 0, st, true, 1, a, items)
-                     : op_launch(k_tree_combine<C::D, false>, dim3(rows), dim3(TC_THREADS), 0, st, true, 1, a, items),
+  return op_cuda(few ? op_launch(k_tree_combine<C::D, true>, dim3((rows + per - 1) / per), dim3(TC_THREADS), 0, st, 1, a, items)
+                     : op_launch(k_tree_combine<C::D, false>, dim3(rows), dim3(TC_THREADS), 0, st, 1, a, items),
                  "k_tree_combine launch");
 }
 
@@ -1034,8 +1030,7 @@ int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows) {
   return SKV_OK;
 }
 
-int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, uint32_t *status,
-                   cudaStream_t st) {
+int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, uint32_t *status, cudaStream_t st) {
   if (int rc = check_tree(d)) return rc;
   if (d->batch == 0) return SKV_OK;
   if (!d->q || !d->k || !d->v || !d->parents || !d->out || !d->lse ||
@@ -1083,7 +1078,6 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
   a.mtiles = (rows + TR_ROWS - 1) / TR_ROWS;
   a.rows = rows < TR_ROWS ? rows : TR_ROWS;
   a.c2 = (float)(d->scale * 1.4426950408889634);
-  a.context = context;
   a.len_stride = cells || d->batch == 1 ? 0 : d->lengths_stride;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = qs[i];
@@ -1146,7 +1140,7 @@ int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tl
 extern "C" {
 
 int skv_tree_attention(const SkvTree *d, void *stream) {
-  return skv::tree_attention(d, nullptr, nullptr, 0, nullptr, static_cast<cudaStream_t>(stream));
+  return skv::tree_attention(d, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 int skv_tree_workspace(const SkvTree *d, int64_t *bytes) {

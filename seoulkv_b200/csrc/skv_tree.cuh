@@ -12,10 +12,9 @@ namespace skv {
 // The K and V maps of one cell's FP8 records [rows][512] (K | V).
 int record_maps(CUtensorMap *two, const uint8_t *records, int64_t rows);
 // Attention over a cache given by `d`, or (cells != null: device array of the K
-// and V maps of every cell) over FP8 records with the context at `tlen` (null:
-// `context`).  `status` (null: the device's word) gets the bits of waits that
+// and V maps of every cell) over FP8 records with the context at `tlen`.
+// `status` (null: the device's word) gets the bits of waits that
 // gave up.
-int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, int32_t context, uint32_t *status,
-                   cudaStream_t st);
+int tree_attention(const SkvTree *d, const CUtensorMap *cells, const int32_t *tlen, uint32_t *status, cudaStream_t st);
 
 }  // namespace skv

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1)
   if (warp == 0) {
     if (lane == 0) tma_prefetch_map(&map);
     grid_dependency_wait();
-    tile_prefix<WT_KEYS>(a.lengths, a.len_stride, 0, a.t, a.batch, 0, s.len, s.pre);
+    tile_prefix<WT_KEYS>(a.lengths, a.len_stride, a.t, a.batch, 0, s.len, s.pre);
   } else if (warp == 1) {
     tmem_alloc(&s.tmem, 512);
   } else if (warp == 2 && lane == 0) {
@@ -334,7 +334,7 @@ int launch_weights(const CUtensorMap &map, WeightsArgs &a, int sms, int device, 
   if (int rc = op_shared_memory(reinterpret_cast<const void *>(kernel), most, device, set)) return rc;
   const int64_t tiles = (int64_t)a.batch * a.heads * ((a.t + WT_KEYS - 1) / WT_KEYS);
   const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
-  return op_cuda(op_launch(kernel, dim3(grid), dim3(WT_THREADS), smem, st, true, 1, map, a),
+  return op_cuda(op_launch(kernel, dim3(grid), dim3(WT_THREADS), smem, st, 1, map, a),
                  "k_weights launch");
 }
 
