@@ -181,17 +181,23 @@ def _pi(digits: int) -> decimal.Decimal:
 
 
 def _by_value(table):
-    """Caches a table of a few numbers by their values: an argument that is an
-    object (a tensor) would be found again after its value has changed."""
-    cached = functools.lru_cache(maxsize=64)(table)
+    """Caches a table of a few numbers by their values.  An object (a tensor) would be found again after its
+    value has changed; nothing is kept of a call that raises, so no object ever enters the cache."""
 
-    def number(x):
-        return x if x is None or type(x) is float else float(x)
+    @functools.lru_cache(maxsize=64)
+    def cached(*settings):
+        if not all(x is None or isinstance(x, (int, float, str)) for x in settings):
+            raise TypeError
+        return table(*settings)
 
     @functools.wraps(table)
     def call(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor):
-        return cached(rotary_dim, number(theta), scaling, number(factor), number(original_context), number(beta_fast),
-                      number(beta_slow), number(attention_factor))
+        try:
+            return cached(rotary_dim, theta, scaling, factor, original_context, beta_fast, beta_slow, attention_factor)
+        except TypeError:
+            return cached(rotary_dim, float(theta), scaling, float(factor),
+                          None if original_context is None else float(original_context), float(beta_fast),
+                          float(beta_slow), None if attention_factor is None else float(attention_factor))
 
     return call
 
