@@ -1010,9 +1010,10 @@ int check_tree(const SkvTree *d) {
   if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
   if (d->dim != 64 && d->dim != 128 && d->dim != 256) return op_fail(SKV_E_INVALID, "head size must be 64, 128 or 256");
   if (d->n < 1 || d->n > TR_NODES) return op_fail(SKV_E_INVALID, "nodes must be in [1, %d]", TR_NODES);
-  if (d->batch < 0 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096 ||
-      d->batch * d->heads * d->n > INT32_MAX)
-    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, counts in range");
+  if (d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads || d->heads > 4096)
+    return op_fail(SKV_E_INVALID, "query heads must be a multiple of the KV heads, and at most 4096");
+  if (d->batch < 0 || d->batch > INT32_MAX / (d->heads * d->n))
+    return op_fail(SKV_E_INVALID, "batch * nodes * query heads must be below 2^31");
   if (d->tokens < 1 || d->tokens > (1 << 26)) return op_fail(SKV_E_INVALID, "tokens must be in [1, 2^26]");
   if (!(d->scale > 0.0) || !(d->scale < 1e30)) return op_fail(SKV_E_INVALID, "scale must be positive and finite");
   if (d->cache_dtype != SKV_DTYPE_BF16 && d->cache_dtype != SKV_DTYPE_E4M3)

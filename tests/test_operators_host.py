@@ -213,3 +213,16 @@ def test_reports_of_waits_that_gave_up_reach_their_reader_once():
     assert "cudaMemset(e->tree_status" in error[:error.index("\n}\n")]
     tree = (CSRC / "skv_tree.cu").read_text()
     assert "cudaMemset(word" in tree[tree.index("int skv_operator_status("):]
+
+
+# ---------------------------------------------------------------- limits
+
+
+@pytest.mark.parametrize("counts,word", [(dict(hq=5), "4096"), (dict(hq=8192), "4096"), (dict(b=1 << 30), "2^31"),
+                                         (dict(b=1 << 62), "2^31")])
+def test_tree_attention_names_the_limit_that_a_call_passes(counts, word):
+    """(b = 2^62 times 8 rows is 2^65: the product itself would wrap around to 0.)"""
+    from tests.test_operators import _refused, _tree
+
+    rc, message = _refused("skv_tree_attention", _tree(**counts))
+    assert rc == -1 and word in message
