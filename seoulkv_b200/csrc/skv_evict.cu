@@ -289,9 +289,9 @@ extern "C" int skv_evict(const SkvEvict *d, void *stream) {
   if (!d) return op_fail(SKV_E_INVALID, "null descriptor");
   if (d->batch < 0 || d->kv_heads < 1 || d->tokens < 1 || d->tokens > INT32_MAX / 2 || d->dim < 1 || d->dim > 65536 ||
       (d->element_bytes != 1 && d->element_bytes != 2 && d->element_bytes != 4) || d->batch > (1 << 24) ||
-      d->batch * d->kv_heads > (1 << 24))
+      d->kv_heads > (1 << 24) || d->batch * d->kv_heads > (1 << 24))
     return op_fail(SKV_E_INVALID, "batch, heads, tokens, dim or element_bytes out of range");
-  if (d->keep < 1 || d->keep > d->tokens || d->sink < 0 || d->local < 0 || d->sink + d->local > d->keep)
+  if (d->keep < 1 || d->keep > d->tokens || d->sink < 0 || d->local < 0 || d->sink > d->keep || d->local > d->keep - d->sink)
     return op_fail(SKV_E_INVALID, "keep must be in [1, tokens] and hold the sink and local tokens");
   const int64_t rows = d->batch * d->kv_heads * d->keep;
   if (rows > (int64_t)INT32_MAX * 8) return op_fail(SKV_E_INVALID, "too many kept rows");

@@ -226,3 +226,12 @@ def test_tree_attention_names_the_limit_that_a_call_passes(counts, word):
 
     rc, message = _refused("skv_tree_attention", _tree(**counts))
     assert rc == -1 and word in message
+
+
+@pytest.mark.parametrize("counts", [dict(sink=1 << 62, local=1 << 62), dict(sink=(1 << 63) - 1, local=1),
+                                    dict(b=1 << 24, hkv=1 << 40), dict(b=2, hkv=1 << 63 - 1)])
+def test_evict_refuses_counts_whose_sums_and_products_wrap_around(counts):
+    from tests.test_operators import _evict, _refused
+
+    rc, message = _refused("skv_evict", _evict(**counts))
+    assert rc == -1 and message
