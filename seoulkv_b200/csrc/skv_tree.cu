@@ -37,20 +37,25 @@
 //
 // What bounds it, measured at 16 query heads on 4 KV heads of 256 (a copy
 // moves 6437 GB/s):
-//   one token, 131072 cached, BF16: 92 us, 537 MB = 91% of the copy rate (more
-//     tokens add bytes at 7.2 TB/s; starting and joining 148 partials are a
-//     fixed 14 us);
-//   64 nodes (256 rows a KV head): 162 us.  138 GFLOP would take 102 us at the
-//     1349 TFLOP/s that the clock under load sustains; the softmax of 268M
-//     scores runs beside it and is what keeps the tensor core waiting;
-//   16 requests of up to 32768, 12 nodes: 200 us, 1.08 GB = 84%;
-//   8 nodes over an FP8 cache of 131072: 82 us, 269 MB = 51% (more tokens add
-//     bytes at 4.8 TB/s).  The integer operations of V's conversion bound it:
-//     every one less per piece shows, and without the conversion a tile takes
-//     a sixth less.  The second half of the queries and the exponentials cost
-//     nothing; other ring lengths, 12 converting warps instead of 8 and stores
-//     without bank conflicts changed nothing;
-//   3 ragged caches of up to 327, 5 nodes: 13 us a call, the host's time.
+// (in long loops, where the power cap lowers the clock to 1.1 to 1.6 GHz; in
+// brackets at 1965 MHz)
+//   one token, 131072 cached, BF16: 92 us (86), 537 MB = 91% of the copy rate
+//     (more tokens add bytes at 7.2 TB/s; starting and joining 148 partials are
+//     a fixed 14 us);
+//   64 nodes (256 rows a KV head): 163 us (141; one cache again and again 129).
+//     138 GFLOP would take 102 us at the 1349 TFLOP/s that the clock under load
+//     sustains; the tensor pipe is busy 70% of the active cycles, and the
+//     softmax of 268M scores beside it is what keeps it waiting;
+//   16 requests of up to 32768, 12 nodes: 200 us (190), 1.08 GB = 84%;
+//   8 nodes over an FP8 cache of 131072: 82 us (69), 269 MB = 51% (more tokens
+//     add bytes at 4.1 to 4.8 TB/s).  No pipe is half full: DRAM 43%, tensor
+//     43%, ALU 33%, shared memory 34%.  The chain of a V stage (load,
+//     conversion, product) bounds it, since a converting group has one place
+//     before and one behind its conversion at D = 256.  A shorter conversion
+//     shortens the chain; without any, a tile takes a sixth less.  The second
+//     half of the queries and the exponentials cost nothing;
+//   3 ragged caches of up to 327, 5 nodes: 13 us a call, the host's time (12 us
+//     on the device).
 #include <cuda_bf16.h>
 
 #include <mutex>

@@ -18,11 +18,13 @@
 // per row that the epilogue takes out again.
 //
 // What bounds it, measured at 16 query heads on 4 KV heads of 256 (a copy
-// moves 6437 GB/s): one token over 131072 cached, 43.7 us, 273 MB = 97%; the
-// last 32 tokens (128 rows) of four requests of up to 32768, 31.4 us, 139 MB =
-// 69%.  Longer caches add bytes at 6.7 TB/s, so what is left is a fixed 8 us:
-// lengths, queries and the first tile come one after the other, and the last
-// epilogue follows the last tile.
+// moves 6437 GB/s): one token over 131072 cached, 44.1 us, 273 MB = 96%; the
+// last 32 tokens (128 rows) of four requests of up to 32768, 31.7 us, 139 MB =
+// 68%.  Longer caches add bytes at 6.7 TB/s, so what is left is a fixed 8 us:
+// lengths, queries and the first tile come one after the other, the last
+// epilogue follows the last tile, and a CTA whose range passes from one head to
+// the next reloads its queries while its ring stands full.  Over FP8: one token
+// over 131072, 28.4 us, 138 MB = 76% (262144: 48.4 us, 89%).
 #include <cuda_bf16.h>
 
 #include "skv_ops.cuh"

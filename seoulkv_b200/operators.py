@@ -15,8 +15,10 @@ Every operator is a function of CUDA tensors of one device and returns new
 ones (``rotary`` and ``accumulate_weights`` also write into given ones).  The
 work is enqueued on the current PyTorch stream of that device; nothing waits,
 and every call may be captured into a CUDA graph.  Tensors may have any
-strides as long as the innermost dimension is contiguous and, for the
-attention operators, rows start on 16-byte boundaries; ValueError otherwise.
+strides as long as the innermost dimension is contiguous; for the attention
+operators rows have to start on 16-byte boundaries (and there are at most 4096
+query heads), and the pairs of an interleaved rotation on two elements.
+ValueError otherwise.
 They are for inference: a tensor that requires a gradient is refused while
 gradients are recorded, and so is one with a forward-mode tangent.
 """
@@ -276,8 +278,12 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
     frequency by ``factor``; "ntk" raises theta so that the slowest pair is
     divided by it; "yarn" (Peng et al., 2023) divides the pairs that turn less
     than ``beta_slow`` times in ``original_context`` tokens, keeps those above
-    ``beta_fast``, goes linearly between, and multiplies the rotated part by
-    0.1 ln(factor) + 1 (``attention_factor`` sets another multiplier).
+    ``beta_fast``, and multiplies the rotated part by 0.1 ln(factor) + 1
+    (``attention_factor`` sets another multiplier).  Between the two corner
+    pairs, rounded outwards to whole ones, the share of the division grows
+    linearly with the pair's index, the form in use (the paper's text has it
+    linear in the number of turns).  With "none" the factor and the settings of
+    "yarn" are not used, except for ``attention_factor``.
 
     Returns (q, k) in new tensors, or in ``out=(q_out, k_out)``, which may be
     the inputs themselves (otherwise they must not overlap them).
@@ -401,9 +407,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     other value marks an unused node (padding of a smaller tree): it and the
     nodes below it get zeros and an lse of -inf, and nothing sees them.
 
-    Over an FP8 cache the scores take the queries as sums of two FP8 rows: an
-    element is off by at most 2^-17 of its row's largest one, and a query with
-    an infinity gives NaN.
+    The weights are rounded to BF16 for the product with V (2^-8 of each at
+    most; their sum is not).  Over an FP8 cache the scores take the queries as
+    sums of two FP8 rows: an element is off by at most 2^-17 of its row's
+    largest one, and a query with an infinity gives NaN.
 
     Returns the attention output, BF16 [B, N, Hq, D], and the natural
     log-sum-exp of each row's scaled scores, FP32 [B, N, Hq].  ``scale``
