@@ -269,10 +269,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
     BF16, FP16 or FP32, both alike, on one device.  ``positions`` int32 or
     int64, [N] or [B, N]; the angle of position p is off by p * 2^-65 turns,
     which is less than its FP32 rounding up to 2^39; negative positions turn
-    back (the inverse rotation, and the gradient's, for a factor of 1).  The first ``rotary_dim`` (even, at most
-    512; all of D by default) dimensions turn, the others are copied.
-    ``layout``: "half" pairs dimension i with i + rotary_dim/2,
-    "interleaved" 2i with 2i + 1.
+    back (the inverse rotation, and the gradient's, for a factor of 1).  The
+    first ``rotary_dim`` (even, at most 512; all of D by default) dimensions
+    turn, the others are copied.  ``layout``: "half" pairs dimension i with
+    i + rotary_dim/2, "interleaved" 2i with 2i + 1.
 
     ``scaling`` for contexts beyond the trained one: "linear" divides every
     frequency by ``factor``; "ntk" raises theta so that the slowest pair is
@@ -286,7 +286,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *, 
     "yarn" are not used, except for ``attention_factor``.
 
     Returns (q, k) in new tensors, or in ``out=(q_out, k_out)``, which may be
-    the inputs themselves (otherwise they must not overlap them).
+    the inputs themselves (q and k may then be parts of one projection that
+    share no place; otherwise the outputs must not overlap the inputs).
     """
     if not isinstance(q, torch.Tensor) or q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("q: expected a BF16 or FP16 or FP32 tensor")
